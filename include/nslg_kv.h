@@ -36,6 +36,8 @@ typedef void* nslg_stream_t; /* a hipStream_t; NULL = the null stream */
 
 enum nslg_dtype { NSLG_F16 = 0, NSLG_BF16 = 1, NSLG_F32 = 2 };
 
+enum nslg_code { NSLG_E4M3 = 0, NSLG_INT8 = 1 }; /* code types of 8-bit pools */
+
 enum nslg_status {
   NSLG_OK = 0,
   NSLG_EINVAL = -1,      /* bad pointer / size / stride */
@@ -436,6 +438,97 @@ int nslg_paged_prefill_append(const void* q, int64_t q_stride, const int32_t* qo
                               void* out, int64_t out_stride,
                               void* workspace, size_t workspace_bytes,
                               nslg_stream_t stream);
+
+/*
+ * ---- 8-bit caches ----
+ *
+ * One layer is the codes k_pool, v_pool [num_pages, page_size, Hkv, D] (1 byte: OCP e4m3
+ * without infinities, or int8 in [-127, 127]) and the scales k_scale, v_scale, fp32
+ * [num_pages, nb, Hkv] with nb = ceil(page_size / 16): one scale for each block of 16 slots
+ * of a page (the last one may be shorter) and KV head. A stored value is code * scale.
+ * Scales are powers of two, or 0; the scale of a block whose first slot has not been
+ * written is not read.
+ *
+ * Pools 16-byte aligned, D in {64, 128, 256}, fewer than 2^31 slots. Rows, q and outputs
+ * are f16 or bf16 (dtype); code is an nslg_code.
+ */
+
+/*
+ * Write a forward's new K/V rows into an 8-bit cache layer. The new tokens of sequence b are
+ * its last n_b = qo_indptr[b+1] - qo_indptr[b] positions; their slots come from the block table
+ * (as in nslg_paged_prefill_append). Per block and head, with M = 448 (e4m3) or 127 (int8):
+ *   need = the smallest power of two s >= 2^-126 with |x| <= M s for the block's new rows, 0
+ *          where they are all zero;
+ *   the block's scale becomes `need` if its first slot is among the new ones, else the larger of its own
+ *   and `need`; where it grew, the codes of the block's earlier tokens are rounded to it;
+ *   a new code is x / scale, rounded to nearest even.
+ * So a stored value is within half a step of x for the rows written with the block's last scale,
+ * and within one step (of that scale) for the others. Slots after the last token are left as
+ * they are. A value that is not finite: e4m3 stores NaN for it; with int8 the block's scale
+ * becomes NaN, and stays so until the block is written from its first slot again.
+ *
+ *   k_new, v_new    rows of Hkv*D elements at element strides, 16-byte aligned: row
+ *                   qo_indptr[b] + t for token t of sequence b (total_q rows), or, with
+ *                   q_rows (int32[total_q]), row q_rows[qo_indptr[b]] + t of a grid of
+ *                   batch * grid_width rows
+ * A page may be written by one sequence of a call at most (as the copy-on-write rule gives);
+ * page ids outside the pool are skipped, and so are tokens past the block table.
+ */
+int nslg_q8_append_kv(const void* k_new, int64_t k_new_stride, const void* v_new, int64_t v_new_stride,
+                      const int32_t* qo_indptr, const int32_t* q_rows, int32_t grid_width, int64_t total_q,
+                      void* k_pool, void* v_pool, float* k_scale, float* v_scale, int64_t num_pages,
+                      int32_t page_size, const int32_t* kv_indptr, const int32_t* kv_indices,
+                      const int32_t* kv_last_page_len, int32_t batch, int32_t num_kv_heads, int32_t head_dim,
+                      int32_t dtype, int32_t code, nslg_stream_t stream);
+
+/*
+ * Read an 8-bit cache layer back: code * scale of every sequence's tokens as contiguous
+ * [batch, max_len, Hkv, D] K and V of `dtype` (f16, bf16 or f32; rounded once), zeros past each
+ * length, 16-byte aligned. batch <= 65535.
+ */
+int nslg_q8_gather_kv(const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
+                      int64_t num_pages, int32_t page_size, const int32_t* kv_indptr, const int32_t* kv_indices,
+                      const int32_t* kv_last_page_len, int32_t batch, int32_t max_len, int32_t num_kv_heads,
+                      int32_t head_dim, int32_t code, int32_t dtype, void* k_out, void* v_out,
+                      nslg_stream_t stream);
+
+/*
+ * Decode attention over an 8-bit cache layer, one query row per sequence: nslg_paged_decode,
+ * nslg_paged_decode_append (k_new, v_new given: each sequence's token L_b - 1 is first written, as
+ * nslg_q8_append_kv writes it), the same with the rotary embedding (positions and tables given too,
+ * as in nslg_paged_decode_rope_append) and their grouped forms (num_groups > 0, as in
+ * nslg_paged_decode_grouped), with their arguments, workspace rules, layout record and statuses.
+ * Null k_new, tables or num_groups 0: without. sm_scale positive and finite. Rows are written on
+ * pages of a multiple of 16 slots only (EUNSUPPORTED otherwise: nslg_q8_append_kv first).
+ */
+size_t nslg_q8_paged_decode_workspace_size(int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+                                           int32_t head_dim, int64_t total_pages, int32_t page_size,
+                                           int32_t dtype, int32_t code, int32_t num_groups);
+int nslg_q8_paged_decode(const void* q, int64_t q_stride, const void* k_new, int64_t k_new_stride,
+                         const void* v_new, int64_t v_new_stride, const int32_t* positions,
+                         const float* cos_table, const float* sin_table, int64_t table_stride,
+                         int64_t table_rows, void* k_pool, void* v_pool, float* k_scale, float* v_scale,
+                         int64_t num_pages, int32_t page_size, const int32_t* kv_indptr,
+                         const int32_t* kv_indices, const int32_t* kv_last_page_len, int64_t total_pages,
+                         int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
+                         float sm_scale, int32_t dtype, int32_t code, const int32_t* seq_group_slot,
+                         int32_t num_groups, const int32_t* group_prefix_pages, const int32_t* group_members,
+                         void* out, int64_t out_stride, void* workspace, size_t workspace_bytes,
+                         int64_t layout, nslg_stream_t stream);
+
+/*
+ * Causal prefill attention over an 8-bit cache layer that holds the new tokens too
+ * (nslg_q8_append_kv first): nslg_paged_prefill, or with q_rows nslg_paged_prefill_grid, with
+ * their arguments and workspace (nslg_paged_prefill_workspace_size).
+ */
+int nslg_q8_paged_prefill(const void* q, int64_t q_stride, const int32_t* qo_indptr, const int32_t* q_rows,
+                          int32_t grid_width, int64_t total_q, int32_t max_q, const void* k_pool,
+                          const void* v_pool, const float* k_scale, const float* v_scale, int64_t num_pages,
+                          int32_t page_size, const int32_t* kv_indptr, const int32_t* kv_indices,
+                          const int32_t* kv_last_page_len, int32_t batch, int32_t num_qo_heads,
+                          int32_t num_kv_heads, int32_t head_dim, float sm_scale, int32_t dtype, int32_t code,
+                          void* out, int64_t out_stride, void* workspace, size_t workspace_bytes,
+                          nslg_stream_t stream);
 
 /*
  * Device-side plan of one decode step in which every sequence gains one token:

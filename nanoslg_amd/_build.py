@@ -47,6 +47,7 @@ HIPCC_FLAGS = [
 # compiler drops the quieting copy it otherwise puts in front of every max.
 FILE_FLAGS = {
     "paged_prefill.hip": ["-fno-honor-nans"],
+    "q8_prefill.hip": ["-fno-honor-nans"],
 }
 
 

@@ -16,6 +16,7 @@ import torch  # noqa: F401  (loads torch's HIP runtime first, so the library bin
 LIB_PATH = Path(__file__).resolve().parent / "libnslg_kv.so"
 
 NSLG_F16, NSLG_BF16, NSLG_F32 = 0, 1, 2
+NSLG_E4M3, NSLG_INT8 = 0, 1  # code types of 8-bit pools
 NSLG_EWORKSPACE = -4
 NSLG_ECAPTURE = -5  # a variant's first use on a device inside a stream capture
 NSLG_NOALLOC_SCRATCH_BYTES = 16 << 20  # the static scratch of nslg_paged_decode_noalloc
@@ -104,6 +105,23 @@ SIGNATURES = {
                                             c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p,
                                             c_void_p, c_int32, c_int32, c_int32, c_int32, c_float, c_int32,
                                             c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
+    "nslg_q8_append_kv": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int64,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p,
+                                    c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p]),
+    "nslg_q8_gather_kv": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p,
+                                    c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p,
+                                    c_void_p, c_void_p]),
+    "nslg_q8_paged_decode_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int64, c_int32, c_int32,
+                                                       c_int32, c_int32]),
+    "nslg_q8_paged_decode": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                       c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                       c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32,
+                                       c_int32, c_float, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_void_p,
+                                       c_void_p, c_int64, c_void_p, c_size_t, c_int64, c_void_p]),
+    "nslg_q8_paged_prefill": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_void_p,
+                                        c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p,
+                                        c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_int32, c_void_p,
+                                        c_int64, c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None

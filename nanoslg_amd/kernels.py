@@ -1131,3 +1131,15 @@ def paged_prefill(q: torch.Tensor, qo_indptr: torch.Tensor, total_q: int, max_q:
                                 dtype_code(q.dtype), out.data_ptr(), out.stride(0), ws_ptr, ws_bytes, _stream(q))
     _lib.check(rc, "nslg_paged_prefill")
     return out
+
+
+# the 8-bit cache's calls (nanoslg_amd.kernels_q8, which uses the above) under this module's name too
+_Q8_CALLS = ("append_kv_q8", "gather_kv_q8", "paged_decode_q8", "paged_decode_append_q8", "paged_decode_rope_append_q8",
+             "paged_prefill_q8")
+
+
+def __getattr__(name: str):
+    if name in _Q8_CALLS:
+        from . import kernels_q8
+        return getattr(kernels_q8, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -1,0 +1,314 @@
+"""Tensor-level wrappers of the 8-bit KV cache kernels (nslg_q8_* of the C ABI).
+
+One layer of an 8-bit cache is four tensors: codes k_layer and v_layer [P, page_size, Hkv, D]
+(torch.float8_e4m3fn or torch.int8) and scales k_scale and v_scale [P, nb, Hkv] (float32, nb =
+ceil(page_size / 16)): one scale for each block of 16 slots of a page and KV head. A stored value is
+code * scale; scales are powers of two or 0, as append_kv_q8 writes them. Rows, queries and
+outputs are float16 or bfloat16. As in ``kernels``, everything is checked on the host, runs on the
+current stream of the tensors' device, and nothing is computed on the CPU.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .kernels import (_DTYPE_CODE, DecodeGroups, Workspace, _i32, _prefill_workspace, _require_gpu, _rope_tables, _rows,
+                      _stream, rope_append)
+
+BLOCK_TOKENS = 16  # slots of a page that share a scale
+CODE_DTYPES = {torch.float8_e4m3fn: _lib.NSLG_E4M3, torch.int8: _lib.NSLG_INT8}
+HEAD_DIMS_Q8 = (64, 128, 256)
+
+
+def blocks_per_page(page_size: int) -> int:
+    return -(-page_size // BLOCK_TOKENS)
+
+
+class _on_device:
+    """The tensors' device as the current one (the library launches on the current device)."""
+
+    def __init__(self, t: torch.Tensor):
+        self.index = t.get_device()
+        self.prev = torch.cuda.current_device()
+
+    def __enter__(self):
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+
+
+def _layer(what: str, k_layer, v_layer, k_scale, v_scale):
+    """(P, page_size, Hkv, D, code) of a cache layer."""
+    if k_layer.dim() != 4 or k_layer.shape != v_layer.shape or k_layer.dtype != v_layer.dtype:
+        raise ValueError(f"{what}: codes must be [P, page_size, Hkv, D] for both K and V")
+    code = CODE_DTYPES.get(k_layer.dtype)
+    if code is None:
+        raise TypeError(f"{what}: codes must be float8_e4m3fn or int8 (got {k_layer.dtype})")
+    P, ps, Hkv, D = k_layer.shape
+    shape = (P, blocks_per_page(ps), Hkv)
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise TypeError(f"{what}: scales must be float32")
+    if tuple(k_scale.shape) != shape or tuple(v_scale.shape) != shape:
+        raise ValueError(f"{what}: scales must be {list(shape)}, one for each block of {BLOCK_TOKENS} slots and head")
+    if not (k_layer.is_contiguous() and v_layer.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+        raise ValueError(f"{what}: the cache layer must be contiguous")
+    return P, ps, Hkv, D, code
+
+
+def _table(what: str, kv_indptr, kv_indices, kv_last_page_len) -> int:
+    """The batch size of a block table."""
+    _i32(kv_indptr, "kv_indptr")
+    _i32(kv_indices, "kv_indices")
+    _i32(kv_last_page_len, "kv_last_page_len")
+    B = kv_indptr.numel() - 1
+    if B < 0 or kv_last_page_len.numel() < B:
+        raise ValueError(f"{what}: kv_indptr must have B+1 entries and kv_last_page_len B")
+    return B
+
+
+def _row_type(what: str, *ts) -> int:
+    code = _DTYPE_CODE.get(ts[0].dtype)
+    if code not in (_lib.NSLG_F16, _lib.NSLG_BF16):
+        raise TypeError(f"{what}: float16 or bfloat16 rows (got {ts[0].dtype})")
+    if any(t.dtype != ts[0].dtype for t in ts):
+        raise TypeError(f"{what}: q, k_new and v_new must share one dtype")
+    return code
+
+
+def _new_rows(what: str, t: torch.Tensor, name: str, n: int, Hkv: int, D: int) -> Tuple[torch.Tensor, int]:
+    """The rows of k_new / v_new at one 16-byte stride (others are copied) and the stride."""
+    if t.dim() < 2 or tuple(t.shape[-2:]) != (Hkv, D):
+        raise ValueError(f"{what}: {name} must hold rows of [{Hkv}, {D}]")
+    rows, stride, _ = _rows(t, name)
+    if rows != n:
+        raise ValueError(f"{what}: {rows} rows of {name} for {n}")
+    if t.data_ptr() % 16 or stride % 8 or stride < Hkv * D:
+        t, stride = t.reshape(rows, Hkv, D).clone(memory_format=torch.contiguous_format), Hkv * D
+    return t, stride
+
+
+def append_kv_q8(k_new: torch.Tensor, v_new: torch.Tensor, qo_indptr: torch.Tensor, total_q: int, k_layer: torch.Tensor,
+                 v_layer: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, kv_indptr: torch.Tensor,
+                 kv_indices: torch.Tensor, kv_last_page_len: torch.Tensor, q_rows: Optional[torch.Tensor] = None,
+                 grid_width: int = 0) -> None:
+    """Write a forward's new K/V rows into an 8-bit cache layer (nslg_q8_append_kv).
+
+    The block table covers the new tokens: sequence b's are its last qo_indptr[b+1] -
+    qo_indptr[b] positions, rows qo_indptr[b] .. of k_new / v_new ([..., Hkv, D], total_q rows), or,
+    with q_rows (int32 [total_q]), rows q_rows[qo_indptr[b]] .. of a padded grid of B * grid_width.
+    Each block of 16 slots and head has one power-of-two scale: what the block's new rows need, or,
+    if the block holds earlier tokens, the larger of that and its own, to which their codes are then
+    rounded. Codes are rounded to nearest even. Values that are not finite: float8_e4m3fn
+    stores NaN; int8 makes the block's scale NaN until the block is written from its start."""
+    _require_gpu(k_new, v_new, qo_indptr, k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len)
+    P, ps, Hkv, D, code = _layer("append_kv_q8", k_layer, v_layer, k_scale, v_scale)
+    B = _table("append_kv_q8", kv_indptr, kv_indices, kv_last_page_len)
+    _i32(qo_indptr, "qo_indptr")
+    dt = _row_type("append_kv_q8", k_new, v_new)
+    if qo_indptr.numel() != B + 1:
+        raise ValueError("append_kv_q8: qo_indptr must have B+1 entries")
+    n = total_q = int(total_q)
+    if q_rows is not None:
+        _require_gpu(k_new, q_rows)
+        _i32(q_rows, "q_rows")
+        if q_rows.numel() < total_q or grid_width < 1:
+            raise ValueError("append_kv_q8: a grid of B x grid_width rows and one q_rows entry per token")
+        n = B * int(grid_width)
+    k_new, ks = _new_rows("append_kv_q8", k_new, "k_new", n, Hkv, D)
+    v_new, vs = _new_rows("append_kv_q8", v_new, "v_new", n, Hkv, D)
+    with _on_device(k_layer):
+        rc = _lib.load().nslg_q8_append_kv(
+            k_new.data_ptr(), ks, v_new.data_ptr(), vs, qo_indptr.data_ptr(), None if q_rows is None else q_rows.data_ptr(),
+            int(grid_width), total_q, k_layer.data_ptr(), v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, ps,
+            kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), B, Hkv, D, dt, code, _stream(k_layer))
+    _lib.check(rc, "nslg_q8_append_kv")
+
+
+def gather_kv_q8(k_layer: torch.Tensor, v_layer: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                 kv_indptr: torch.Tensor, kv_indices: torch.Tensor, kv_last_page_len: torch.Tensor, max_len: int,
+                 dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The cached tokens' values (code * scale, rounded once) as contiguous [B, max_len, Hkv, D] K
+    and V of `dtype` (float16, bfloat16 or float32), zeros past each length."""
+    _require_gpu(k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len)
+    P, ps, Hkv, D, code = _layer("gather_kv_q8", k_layer, v_layer, k_scale, v_scale)
+    B = _table("gather_kv_q8", kv_indptr, kv_indices, kv_last_page_len)
+    if dtype not in _DTYPE_CODE:
+        raise TypeError(f"gather_kv_q8: unsupported dtype {dtype}")
+    k_out = torch.empty((B, int(max_len), Hkv, D), dtype=dtype, device=k_layer.device)
+    v_out = torch.empty_like(k_out)
+    with _on_device(k_layer):
+        rc = _lib.load().nslg_q8_gather_kv(
+            k_layer.data_ptr(), v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, ps, kv_indptr.data_ptr(),
+            kv_indices.data_ptr(), kv_last_page_len.data_ptr(), B, int(max_len), Hkv, D, code, _DTYPE_CODE[dtype],
+            k_out.data_ptr(), v_out.data_ptr(), _stream(k_layer))
+    _lib.check(rc, "nslg_q8_gather_kv")
+    return k_out, v_out
+
+
+def paged_decode_q8(q: torch.Tensor, k_layer: torch.Tensor, v_layer: torch.Tensor, k_scale: torch.Tensor,
+                    v_scale: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
+                    kv_last_page_len: torch.Tensor, total_pages: int, sm_scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None, workspace: Optional[Workspace] = None,
+                    groups: Optional[DecodeGroups] = None, layout: int = 0) -> torch.Tensor:
+    """Decode attention over an 8-bit cache layer: ``kernels.paged_decode`` with its arguments
+    (q [B, Hq, D], rows may be strided; returns [B, Hq, D])."""
+    return _decode8("paged_decode_q8", q, None, None, None, k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices,
+                    kv_last_page_len, total_pages, sm_scale, out, workspace, groups, layout)
+
+
+def paged_decode_append_q8(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_layer: torch.Tensor,
+                           v_layer: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, kv_indptr: torch.Tensor,
+                           kv_indices: torch.Tensor, kv_last_page_len: torch.Tensor, total_pages: int,
+                           sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                           workspace: Optional[Workspace] = None, groups: Optional[DecodeGroups] = None,
+                           layout: int = 0) -> torch.Tensor:
+    """One decode step of a layer: row b of k_new / v_new ([B, ..., Hkv, D], rows may be strided)
+    written as sequence b's last token, then decode attention. Same result as append_kv_q8 of
+    one row a sequence followed by paged_decode_q8; in the decode launch itself where 16
+    divides the page size (a block then lies in one wave's work), with a launch of
+    its own ahead otherwise."""
+    return _decode8("paged_decode_append_q8", q, k_new, v_new, None, k_layer, v_layer, k_scale, v_scale, kv_indptr,
+                    kv_indices, kv_last_page_len, total_pages, sm_scale, out, workspace, groups, layout)
+
+
+def paged_decode_rope_append_q8(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, positions: torch.Tensor,
+                                cos: torch.Tensor, sin: torch.Tensor, k_layer: torch.Tensor, v_layer: torch.Tensor,
+                                k_scale: torch.Tensor, v_scale: torch.Tensor, kv_indptr: torch.Tensor,
+                                kv_indices: torch.Tensor, kv_last_page_len: torch.Tensor, total_pages: int,
+                                sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                                workspace: Optional[Workspace] = None, groups: Optional[DecodeGroups] = None,
+                                layout: int = 0) -> torch.Tensor:
+    """paged_decode_append_q8 of q and k_new rotated at each sequence's `positions` entry (int32 [B]) with
+    the model's [max_positions, >= D] cos / sin tables, as in ``kernels.paged_decode_rope_append``."""
+    _require_gpu(positions, cos, sin)
+    _i32(positions, "positions")
+    if positions.numel() != q.shape[0]:
+        raise ValueError("paged_decode_rope_append_q8: one position per sequence")
+    return _decode8("paged_decode_rope_append_q8", q, k_new, v_new, (positions, *_rope_tables(cos, sin, q.shape[-1])),
+                    k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len, total_pages, sm_scale, out,
+                    workspace, groups, layout)
+
+
+def rotate_rows(q, k_new, v_new, positions, cos, sin):
+    """q and k_new ([..., H, D] rows, `positions` int32 one a row) rotated, as new contiguous rows
+    (``kernels.rope_append`` into rows of its own)."""
+    Hkv, D = k_new.shape[-2], k_new.shape[-1]
+    n = positions.numel()
+    k_rot = torch.empty((n, 1, Hkv, D), dtype=k_new.dtype, device=k_new.device)
+    slots = torch.arange(n, dtype=torch.int32, device=k_new.device)
+    q_rot = rope_append(q, k_new, v_new, positions, slots, cos, sin, k_rot, torch.empty_like(k_rot))
+    return q_rot, k_rot.view(n, Hkv, D)
+
+
+def _decode8(what, q, k_new, v_new, rope, k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len,
+             total_pages, sm_scale, out, workspace, groups, layout):
+    _require_gpu(q, k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len)
+    P, ps, Hkv, D, code = _layer(what, k_layer, v_layer, k_scale, v_scale)
+    B = _table(what, kv_indptr, kv_indices, kv_last_page_len)
+    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != D or q.stride(2) != 1 or q.stride(1) != D:
+        raise ValueError(f"{what}: q must be [{B}, Hq, {D}] with a contiguous [Hq, D] block")
+    Hq = q.shape[1]
+    if Hq % Hkv:
+        raise ValueError(f"{what}: Hq={Hq} is not a multiple of Hkv={Hkv}")
+    if out is None:
+        out = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
+    elif (out.shape != (B, Hq, D) or out.stride(2) != 1 or out.stride(1) != D or out.dtype != q.dtype
+          or out.get_device() != q.get_device()):
+        raise ValueError(f"{what}: bad out tensor")
+    rows = (None, 0, None, 0)
+    tables = (None, None, None, 0, 0)
+    if k_new is None:
+        dt = _row_type(what, q)
+    else:
+        _require_gpu(q, k_new, v_new)
+        dt = _row_type(what, q, k_new, v_new)
+        if ps % BLOCK_TOKENS:
+            # a block may lie in two waves' work: the rows go in ahead
+            if rope is not None:
+                q, k_new = rotate_rows(q, k_new, v_new, *rope)
+                rope = None
+            append_kv_q8(k_new, v_new, torch.arange(B + 1, dtype=torch.int32, device=q.device), B, k_layer, v_layer,
+                         k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len)
+        else:
+            k_new, ks = _new_rows(what, k_new, "k_new", B, Hkv, D)
+            v_new, vs = _new_rows(what, v_new, "v_new", B, Hkv, D)
+            rows = (k_new.data_ptr(), ks, v_new.data_ptr(), vs)
+            if rope is not None:
+                pos, cos, sin = rope
+                if cos.data_ptr() % 16 or sin.data_ptr() % 16 or cos.stride(0) % 4:
+                    cos, sin = (t[:, :D].clone(memory_format=torch.contiguous_format) for t in (cos, sin))
+                tables = (pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0])
+    grp = (None, 0, None, None)
+    if groups is not None:
+        _require_gpu(q, groups.seq_group_slot)
+        _i32(groups.seq_group_slot, "seq_group_slot")
+        if groups.seq_group_slot.numel() != B:
+            raise ValueError(f"{what}: one group slot per sequence")
+        grp = (groups.seq_group_slot.data_ptr(), groups.num_groups, groups.prefix_pages_np.ctypes.data,
+               groups.members_np.ctypes.data)
+    lib = _lib.load()
+    scale = (1.0 / math.sqrt(D)) if sm_scale is None else float(sm_scale)
+    with _on_device(q):
+        need = int(lib.nslg_q8_paged_decode_workspace_size(B, Hq, Hkv, D, int(total_pages), ps, dt, code, grp[1]))
+        if groups is not None and need == 0:
+            raise ValueError(f"{what}: unsupported grouped decode shape")
+        ws = (workspace or Workspace(q.device)).get(need)
+        rc = lib.nslg_q8_paged_decode(
+            q.data_ptr(), q.stride(0), *rows, *tables, k_layer.data_ptr(), v_layer.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), P, ps, kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(),
+            int(total_pages), B, Hq, Hkv, D, scale, dt, code, *grp, out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
+            layout, _stream(q))
+    _lib.check(rc, "nslg_q8_paged_decode")
+    return out
+
+
+def paged_prefill_q8(q: torch.Tensor, qo_indptr: torch.Tensor, total_q: int, max_q: int, k_layer: torch.Tensor,
+                     v_layer: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, kv_indptr: torch.Tensor,
+                     kv_indices: torch.Tensor, kv_last_page_len: torch.Tensor, sm_scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None, workspace: Optional[Workspace] = None,
+                     q_rows: Optional[torch.Tensor] = None, grid_width: int = 0,
+                     max_kv: Optional[int] = None) -> torch.Tensor:
+    """Causal (bottom-right) prefill attention over an 8-bit cache layer that holds the new tokens too
+    (append_kv_q8 first): ``kernels.paged_prefill`` with its arguments. max_kv: the longest
+    sequence's keys, where the caller knows it (it decides whether keys are cut into runs)."""
+    _require_gpu(q, qo_indptr, k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len)
+    P, ps, Hkv, D, code = _layer("paged_prefill_q8", k_layer, v_layer, k_scale, v_scale)
+    B = _table("paged_prefill_q8", kv_indptr, kv_indices, kv_last_page_len)
+    _i32(qo_indptr, "qo_indptr")
+    dt = _row_type("paged_prefill_q8", q)
+    total_q = int(total_q)
+    if q.dim() != 3 or q.shape[2] != D or q.stride(2) != 1 or q.stride(1) != D:
+        raise ValueError(f"paged_prefill_q8: q must be [T, Hq, {D}] with a contiguous [Hq, D] block")
+    T, Hq, _ = q.shape
+    if Hq % Hkv:
+        raise ValueError(f"paged_prefill_q8: Hq={Hq} is not a multiple of Hkv={Hkv}")
+    if qo_indptr.numel() != B + 1 or T < total_q:
+        raise ValueError("paged_prefill_q8: qo_indptr must have B+1 entries and q at least total_q rows")
+    if q_rows is not None:
+        _require_gpu(q, q_rows)
+        _i32(q_rows, "q_rows")
+        if q_rows.numel() < total_q or grid_width < 1 or T != B * grid_width:
+            raise ValueError("paged_prefill_q8: a grid of B x grid_width rows of q and one q_rows entry per token")
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+    elif (out.shape != (T, Hq, D) or out.stride(2) != 1 or out.stride(1) != D or out.dtype != q.dtype
+          or out.get_device() != q.get_device()):
+        raise ValueError("paged_prefill_q8: out must be shaped like q")
+    if max_kv is None:  # the average sequence's table stands for the longest one (its length is on the device)
+        max_kv = kv_indices.numel() * ps // max(B, 1)
+    scale = (1.0 / math.sqrt(D)) if sm_scale is None else float(sm_scale)
+    with _on_device(q):
+        ws, ws_ptr, ws_bytes = _prefill_workspace(q, B, Hq, D, total_q, int(max_q), max_kv, workspace)
+        rc = _lib.load().nslg_q8_paged_prefill(
+            q.data_ptr(), q.stride(0), qo_indptr.data_ptr(), None if q_rows is None else q_rows.data_ptr(), int(grid_width),
+            total_q, int(max_q), k_layer.data_ptr(), v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, ps,
+            kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), B, Hq, Hkv, D, scale, dt, code,
+            out.data_ptr(), out.stride(0), ws_ptr, ws_bytes, _stream(q))
+    _lib.check(rc, "nslg_q8_paged_prefill")
+    return out

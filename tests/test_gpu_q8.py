@@ -1,0 +1,421 @@
+"""8-bit cache kernels against plain 64-bit arithmetic: the write (codes and scales, exactly), the
+read-back (exactly) and attention (within bounds derived in the oracle from the roundings)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import q8_oracle as Q
+
+pytestmark = pytest.mark.gpu
+
+DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
+CODE = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+DEV = "cuda:0"
+
+
+def K():
+    from nanoslg_amd import kernels
+    return kernels
+
+
+def i32(x):
+    return torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)
+
+
+class Cache:
+    """A layer on the GPU and its oracle twin, with sequences in scattered pages. Every slot starts as written."""
+
+    def __init__(self, seed, code, page, hkv, d, lens, dtype="fp16", extra_pages=3, spread=1.5, stale_nan=False):
+        self.g = g = np.random.default_rng(seed)
+        self.code, self.page, self.hkv, self.d, self.lens, self.dtype = code, page, hkv, d, list(lens), dtype
+        npg = [-(-n // page) for n in lens]
+        P = self.P = sum(npg) + extra_pages + 1
+        nb = -(-page // 16)
+        order = g.permutation(np.arange(1, P))
+        at = np.concatenate([[0], np.cumsum(npg)])
+        self.tables = [order[a:b].tolist() for a, b in zip(at[:-1], at[1:])]
+        self.side = {}
+        for name in "kv":
+            s = np.ldexp(1.0, g.integers(-6, 3, (P, nb, hkv)))
+            lim = Q.MOST[code]
+            v = Q.round_code(np.clip(g.standard_normal((P, page, hkv, d)) * lim / 4 * spread, -lim, lim), code)
+            v *= g.random((P, page, hkv, 1)) < 0.97  # some rows of zeros
+            if stale_nan and code == "e4m3":  # slots past every sequence hold NaN
+                for tab, n in zip(self.tables, lens):
+                    if n % page:
+                        v[tab[-1], n % page:] = np.nan
+                v[order[at[-1]:]] = np.nan
+            lay = Q.Layer(v, s, code)
+            t = torch.from_numpy(v).float()
+            t = t.to(CODE[code]) if code == "e4m3" else t.to(torch.int8)
+            self.side[name] = (lay, t.to(DEV).contiguous(), torch.from_numpy(s).float().to(DEV).contiguous())
+        self.indptr, self.indices = i32(at), i32(np.concatenate([*self.tables, [0]]).astype(np.int64)[:max(1, at[-1])])
+        self.last = i32([n - (p - 1) * page if p else 0 for n, p in zip(lens, npg)])
+        self.total_pages = int(at[-1])
+
+    @property
+    def layer(self):
+        return (self.side["k"][1], self.side["v"][1], self.side["k"][2], self.side["v"][2])
+
+    @property
+    def table(self):
+        return (self.indptr, self.indices, self.last)
+
+    def rows(self, n, scale=1.0):
+        x = self.g.standard_normal((n, self.hkv, self.d)) * scale * np.exp(self.g.standard_normal((n, 1, 1)))
+        return torch.from_numpy(x).to(DT[self.dtype])
+
+    def values(self, name, b):
+        return self.side[name][0].read(self.tables[b], self.lens[b])
+
+    def same(self):
+        for name in "kv":
+            lay, codes, scale = self.side[name]
+            np.testing.assert_array_equal(scale.cpu().double().numpy(), lay.scale, err_msg=name + " scales")
+            np.testing.assert_array_equal(codes.cpu().float().double().numpy(), lay.values, err_msg=name + " codes")
+
+
+def append(c, new, kn, vn, grid=0, offs=None):
+    """The forward's rows through the kernel and the oracle: new[b] last tokens of each sequence."""
+    qo = np.concatenate([[0], np.cumsum(new)])
+    kw = {}
+    rows = [list(range(qo[b], qo[b + 1])) for b in range(len(new))]
+    if grid:
+        rows = [[b * grid + offs[b] + t for t in range(n)] for b, n in enumerate(new)]
+        kw = dict(q_rows=i32(sum(rows, []) or [0]), grid_width=grid)
+    K().append_kv_q8(kn, vn, i32(qo), int(qo[-1]), *c.layer, *c.table, **kw)
+    for name, x in (("k", kn), ("v", vn)):
+        x = x.reshape(-1, c.hkv, c.d).cpu().double().numpy()
+        for b, n in enumerate(new):
+            c.side[name][0].write(c.tables[b], c.lens[b] - n, x[rows[b]])
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("page,d,hkv,dtype,lens,new", [
+    (16, 128, 8, "fp16", [1, 16, 17, 40, 100, 3], [1, 16, 1, 24, 37, 0]),
+    (16, 128, 8, "bf16", [33, 64], [1, 1]),
+    (32, 64, 3, "bf16", [31, 97, 5], [14, 66, 5]),
+    (64, 256, 2, "fp16", [130, 64], [67, 1]),
+    (20, 128, 4, "fp16", [45, 20, 19, 81], [30, 4, 1, 81]),
+    (5, 64, 8, "bf16", [23, 4], [9, 2]),
+    (1, 128, 2, "fp16", [7, 2], [7, 1]),
+    (48, 128, 1, "fp16", [500], [411]),
+])
+def test_append_codes_and_scales(code, page, d, hkv, dtype, lens, new):
+    c = Cache(1, code, page, hkv, d, lens, dtype)
+    T = sum(new)
+    append(c, new, c.rows(T).to(DEV), c.rows(T, 30.0).to(DEV))
+    c.same()
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_append_padded_grid_and_strided_rows(code):
+    c = Cache(2, code, 16, 4, 128, [50, 7, 20], "bf16")
+    new, W = [9, 7, 1], 12
+    offs = [W - n for n in new]
+    kv = torch.randn(3, W, 2, 4, 128, device=DEV).bfloat16()  # K and V as halves of one projection output
+    append(c, new, kv[:, :, 0], kv[:, :, 1], grid=W, offs=offs)
+    c.same()
+
+
+@pytest.mark.parametrize("shift", [1, 4])
+def test_append_rows_off_16_byte_alignment(shift):
+    c = Cache(3, "e4m3", 16, 2, 64, [20, 18])
+    flat = torch.randn(2 * 3 * 128 + 8, device=DEV).half()
+    kn = flat[shift:shift + 3 * 128].view(3, 2, 64)
+    append(c, [2, 1], kn, kn.clone())
+    c.same()
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_append_extremes(code, dtype):
+    """The largest and smallest values, values at and just past MOST * 2^k, zero rows, a scale that grows by far."""
+    lim = Q.MOST[code]
+    big = 65504.0 if dtype == "fp16" else 3.3e38
+    tiny = 2.0 ** -24 if dtype == "fp16" else 2.0 ** -133
+    amax = [lim, lim * 2.0 ** -5, lim + (0.5 if code == "int8" else 1.0), big, tiny, 0.0, 1e-30, lim * 2 - 1]
+    c = Cache(4, code, 16, 1, 64, [16 + i % 5 + 1 for i in range(len(amax))], dtype)
+    rows = []
+    for i, a in enumerate(amax):
+        n = i % 5 + 1
+        x = c.rows(n)
+        x = x / x.abs().max().float().clamp(min=1) * 0.7 if a == 0 else (x.float() / x.float().abs().max() * a).to(DT[dtype])
+        if a == 0:
+            x = torch.zeros_like(x)
+        elif math.isfinite(a):
+            x[n // 2, 0, 5] = a
+        rows.append(x)
+    x = torch.cat(rows).to(DEV)
+    append(c, [i % 5 + 1 for i in range(len(amax))], x, -x)
+    c.same()
+    # one more token each: blocks that hold tokens, scales growing and not
+    c2 = Cache(5, code, 16, 1, 64, [18] * 6, dtype)
+    y = c2.rows(6).float() * torch.tensor([1e-3, 1.0, 1e2, 1e4, 0.0, 6e4]).view(6, 1, 1)
+    y = y.clamp(-big, big).to(DT[dtype]).to(DEV)
+    append(c2, [1] * 6, y, y.flip(0))
+    c2.same()
+    append(c2, [1] * 6, y.flip(0), y)  # the same slots once more
+    c2.same()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_append_values_that_are_not_finite(code, bad):
+    c = Cache(6, code, 16, 2, 64, [20, 33, 20], "bf16")
+    x = c.rows(9)
+    x[1, 0, 3] = bad   # sequence 0: token 17, head 0
+    x[8, 1, 63] = bad  # sequence 2: its only new token, head 1
+    append(c, [4, 4, 1], x.to(DEV), c.rows(9).to(DEV))
+    c.same()
+    k, _ = K().gather_kv_q8(*c.layer, *c.table, 33, torch.float32)
+    want = [c.values("k", b) for b in range(3)]
+    for b in range(3):
+        np.testing.assert_array_equal(k[b, :c.lens[b]].cpu().double().numpy(), want[b])
+    assert np.isnan(want[0]).any() and not np.isnan(want[1]).any()
+    # the block written from its first slot again is whole again
+    append(c, [20, 33, 20], c.rows(73).to(DEV), c.rows(73).to(DEV))
+    c.same()
+    assert not torch.isnan(K().gather_kv_q8(*c.layer, *c.table, 33, torch.float32)[0]).any()
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_append_skips_bad_pages_and_writes_nothing_else(code):
+    c = Cache(7, code, 16, 2, 64, [40, 20, 5])
+    before = [t.clone() for t in c.layer]
+    idx = c.indices.clone()
+    idx[1], idx[3] = -1, c.P  # sequence 0's second page, sequence 1's first
+    c.indices = idx
+    T = 40 + 20
+    kn = c.rows(T)
+    qo = i32([0, 40, 60, 60])
+    K().append_kv_q8(kn.to(DEV), kn.to(DEV), qo, T, *c.layer, *c.table)
+    x = kn.double().numpy()
+    for name in "kv":
+        lay = c.side[name][0]
+        for b, (a, n) in enumerate(((0, 40), (40, 20))):
+            for p in range(-(-n // 16)):
+                pid = int(idx[(0, 3)[b] + p])
+                if 0 <= pid < c.P:
+                    lay.write({p: pid}, 16 * p, x[a + 16 * p:a + min(n, 16 * p + 16)])
+    c.same()
+    assert len(before) == 4
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("out", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("page,d", [(16, 128), (20, 64), (64, 256), (3, 64)])
+def test_gather(code, out, page, d):
+    c = Cache(8, code, page, 3, d, [37, 0, 1, 64], stale_nan=True)
+    k, v = K().gather_kv_q8(*c.layer, *c.table, 66, out)
+    for name, got in (("k", k), ("v", v)):
+        for b, n in enumerate(c.lens):
+            want = torch.from_numpy(c.values(name, b)).float().to(out)
+            assert torch.equal(got[b, :n].cpu(), want), (name, b)
+            assert not got[b, n:].any()
+
+
+def check(c, out, q, b, new=1, scale=None):
+    """Sequence b's output rows against the oracle's."""
+    want, mag, big, low = Q.attend(q.cpu().double().numpy(), c.values("k", b), c.values("v", b), scale, c.dtype)
+    bound = Q.attention_bound(want, mag, big, low, c.lens[b], c.dtype)
+    off = np.abs(out.cpu().double().numpy() - want)
+    assert (off <= bound).all(), (b, float((off / bound).max()))
+
+
+DECODE = [  # page, d, hkv, group, lens
+    (16, 128, 8, 4, [1, 16, 17, 100, 0, 700]),
+    (16, 128, 1, 16, [33, 2500]),
+    (16, 64, 2, 1, [15, 31, 300]),
+    (32, 256, 4, 4, [1, 64, 65, 900]),
+    (64, 128, 3, 7, [129, 5000]),
+    (48, 64, 5, 8, [47, 48, 49, 1]),
+    (20, 128, 4, 4, [1, 39, 40, 41, 777]),
+    (8, 256, 2, 2, [9, 250]),
+    (1, 64, 2, 3, [1, 50]),
+]
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("page,d,hkv,group,lens", DECODE)
+def test_decode(code, dtype, page, d, hkv, group, lens):
+    c = Cache(9, code, page, hkv, d, lens, dtype, stale_nan=True)
+    wide = torch.randn(len(lens), hkv * group + 2, d, device=DEV).to(DT[dtype])
+    q = wide[:, 1:-1]  # strided rows
+    out = K().paged_decode_q8(q, *c.layer, *c.table, c.total_pages)
+    for b, n in enumerate(lens):
+        if n:
+            check(c, out[b:b + 1], q[b:b + 1], b)
+        else:
+            assert not out[b].any()
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("page,d,hkv,group,lens", [x for x in DECODE if 0 not in x[4]])
+def test_decode_append(code, dtype, page, d, hkv, group, lens):
+    """The step's rows written (codes and scales, exactly) and attended, in one call; a second step behind it."""
+    c = Cache(10, code, page, hkv, d, lens, dtype)
+    B = len(lens)
+    q = torch.randn(B, hkv * group, d, device=DEV).to(DT[dtype])
+    for scale in (1.0, 40.0):
+        kn, vn = c.rows(B, scale), c.rows(B, scale)
+        out = K().paged_decode_append_q8(q, kn.to(DEV)[:, None], vn.to(DEV)[:, None], *c.layer, *c.table, c.total_pages)
+        for b in range(B):
+            c.side["k"][0].write(c.tables[b], lens[b] - 1, kn[b:b + 1].double().numpy())
+            c.side["v"][0].write(c.tables[b], lens[b] - 1, vn[b:b + 1].double().numpy())
+        c.same()
+        for b in range(B):
+            check(c, out[b:b + 1], q[b:b + 1], b)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 32), (256, 16), (128, 20)])
+def test_decode_rope_append(dtype, d, page):
+    """Bit for bit rope_append into rows of its own, then the decode of the rotated rows."""
+    lens, hkv, G = [5, 40, 257], 2, 4
+    c = Cache(11, "e4m3", page, hkv, d, lens, dtype)
+    twin = [t.clone() for t in c.layer]
+    B = len(lens)
+    q = torch.randn(B, hkv * G, d, device=DEV).to(DT[dtype])
+    kn, vn = c.rows(B, 5).to(DEV), c.rows(B, 5).to(DEV)
+    a = torch.outer(torch.arange(300, dtype=torch.float64), 1e4 ** (-torch.arange(0, d, 2) / d))
+    a = torch.cat([a, a], 1)
+    cos, sin = a.cos().float().to(DEV), a.sin().float().to(DEV)
+    pos = i32([n - 1 for n in lens])
+    out = K().paged_decode_rope_append_q8(q, kn, vn, pos, cos, sin, *c.layer, *c.table, c.total_pages)
+    kr, vr = torch.empty(B, 1, hkv, d, device=DEV, dtype=DT[dtype]), torch.empty(B, 1, hkv, d, device=DEV, dtype=DT[dtype])
+    qr = K().rope_append(q, kn, vn, pos, i32(range(B)), cos, sin, kr, vr)
+    K().append_kv_q8(kr[:, 0], vn, i32(range(B + 1)), B, *twin, *c.table)
+    for x, y in zip(c.layer, twin):
+        assert torch.equal(x.view(torch.int8) if x.element_size() == 1 else x, y.view(torch.int8) if y.element_size() == 1 else y)
+    assert torch.equal(out, K().paged_decode_q8(qr, *twin, *c.table, c.total_pages))
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_decode_groups(code):
+    """Sequences on one prefix of pages, read once for the group: the same result within the bounds."""
+    c = Cache(12, code, 16, 2, 128, [200, 161, 170, 33], "fp16")
+    for b in (1, 2):  # their first 8 pages are sequence 0's
+        c.tables[b][:8] = c.tables[0][:8]
+    c.indices = i32(sum(c.tables, []))
+    grp = K().DecodeGroups(4, [[0, 1, 2]], [8], torch.device(DEV))
+    q = torch.randn(4, 8, 128, device=DEV).half()
+    kn, vn = c.rows(4, 20), c.rows(4, 20)
+    out = K().paged_decode_append_q8(q, kn.to(DEV), vn.to(DEV), *c.layer, *c.table, c.total_pages, groups=grp)
+    for b in range(4):
+        c.side["k"][0].write(c.tables[b], c.lens[b] - 1, kn[b:b + 1].double().numpy())
+        c.side["v"][0].write(c.tables[b], c.lens[b] - 1, vn[b:b + 1].double().numpy())
+    c.same()
+    for b in range(4):
+        check(c, out[b:b + 1], q[b:b + 1], b)
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_decode_of_a_block_that_is_not_finite(code):
+    """What reads such a block is NaN; other heads and sequences are not touched."""
+    c = Cache(13, code, 16, 2, 64, [40, 40], "fp16")
+    x = c.rows(2)
+    x[0, 0, 7] = math.nan
+    q = torch.randn(2, 4, 64, device=DEV).half()
+    out = K().paged_decode_append_q8(q, x.to(DEV), c.rows(2).to(DEV), *c.layer, *c.table, c.total_pages)
+    assert torch.isnan(out[0, :2]).all()
+    assert torch.isfinite(out[0, 2:]).all() and torch.isfinite(out[1]).all()
+
+
+PREFILL = [  # page, d, hkv, group, lens, new
+    (16, 128, 8, 4, [1, 40, 300, 17], [1, 40, 60, 0]),
+    (16, 128, 1, 16, [900], [70]),
+    (64, 64, 2, 3, [129, 64, 500], [129, 1, 200]),
+    (32, 256, 2, 4, [70, 400], [33, 150]),
+    (20, 128, 4, 1, [41, 39, 300], [41, 3, 120]),
+    (5, 64, 2, 4, [23], [23]),
+    (16, 128, 2, 4, [2300], [16]),
+]
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("page,d,hkv,group,lens,new", PREFILL)
+def test_prefill(code, dtype, page, d, hkv, group, lens, new):
+    c = Cache(14, code, page, hkv, d, lens, dtype, stale_nan=True)
+    qo = np.concatenate([[0], np.cumsum(new)])
+    T, hq = int(qo[-1]), hkv * group
+    q = torch.randn(T, hq + 1, d, device=DEV).to(DT[dtype])[:, :hq]
+    ws = K().Workspace(torch.device(DEV))
+    out = K().paged_prefill_q8(q, i32(qo), T, max(new), *c.layer, *c.table, workspace=ws)
+    whole = K().paged_prefill_q8(q, i32(qo), T, max(new), *c.layer, *c.table, max_kv=0)  # keys in one run
+    W = max(new) + 3
+    offs = [W - n for n in new]
+    rows = [b * W + offs[b] + t for b, n in enumerate(new) for t in range(n)]
+    grid = torch.zeros(len(lens) * W, hq, d, device=DEV, dtype=DT[dtype])
+    grid[rows] = q
+    padded = K().paged_prefill_q8(grid, i32(qo), T, max(new), *c.layer, *c.table, workspace=ws, q_rows=i32(rows), grid_width=W)
+    pad = torch.ones(len(lens) * W, dtype=torch.bool)
+    pad[rows] = False
+    assert not padded[pad.to(DEV)].any()
+    assert torch.equal(padded[rows], out)
+    for b in range(len(lens)):
+        if new[b]:
+            check(c, out[qo[b]:qo[b + 1]], q[qo[b]:qo[b + 1]], b)
+            check(c, whole[qo[b]:qo[b + 1]], q[qo[b]:qo[b + 1]], b)
+
+
+def test_write_then_attend_as_a_forward_does():
+    """A prompt in two chunks and three decode steps, each call on what the calls before left."""
+    c = Cache(15, "e4m3", 16, 2, 128, [90, 57], "bf16")
+    full = c.lens
+    kn, vn = [c.rows(95, 3) for _ in full], [c.rows(95, 3) for _ in full]
+    ws = K().Workspace(torch.device(DEV))
+    done = [0, 0]
+    c.tables[0].append(0 + c.P - 1)
+    for step in ([50, 17], [39, 39], [1, 1], [1, 1], [1, 1]):
+        now = [a + n for a, n in zip(done, step)]
+        c.lens = now
+        npg = [-(-n // 16) for n in now]
+        c.indptr, c.indices = i32([0, npg[0], sum(npg)]), i32(c.tables[0][:npg[0]] + c.tables[1][:npg[1]])
+        c.last = i32([n - 16 * (p - 1) for n, p in zip(now, npg)])
+        ks = torch.cat([x[a:n] for x, a, n in zip(kn, done, now)]).to(DEV)
+        vs = torch.cat([x[a:n] for x, a, n in zip(vn, done, now)]).to(DEV)
+        qo = np.concatenate([[0], np.cumsum(step)])
+        q = torch.randn(int(qo[-1]), 8, 128, device=DEV).bfloat16()
+        if step == [1, 1]:
+            out = K().paged_decode_append_q8(q, ks, vs, *c.layer, *c.table, sum(npg), workspace=ws)
+        else:
+            K().append_kv_q8(ks, vs, i32(qo), int(qo[-1]), *c.layer, *c.table)
+            out = K().paged_prefill_q8(q, i32(qo), int(qo[-1]), max(step), *c.layer, *c.table, workspace=ws)
+        for b in range(2):
+            c.side["k"][0].write(c.tables[b], done[b], kn[b][done[b]:now[b]].double().numpy())
+            c.side["v"][0].write(c.tables[b], done[b], vn[b][done[b]:now[b]].double().numpy())
+        c.same()
+        for b in range(2):
+            check(c, out[qo[b]:qo[b + 1]], q[qo[b]:qo[b + 1]], b)
+        done = now
+
+
+def test_side_stream_and_graph_replays():
+    """The step captured into a graph and replayed between eager work: every replay gives the eager bits."""
+    c = Cache(16, "e4m3", 16, 4, 128, [300, 77, 1000], "fp16")
+    q = torch.randn(3, 16, 128, device=DEV).half()
+    kn, vn = c.rows(3).to(DEV), c.rows(3).to(DEV)
+    ws, ws2 = K().Workspace(torch.device(DEV)), K().Workspace(torch.device(DEV))
+    want = K().paged_decode_append_q8(q, kn, vn, *c.layer, *c.table, c.total_pages, workspace=ws)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = K().paged_decode_append_q8(q, kn, vn, *c.layer, *c.table, c.total_pages, workspace=ws2)
+    side.synchronize()
+    assert torch.equal(out, want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        static = K().paged_decode_append_q8(q, kn, vn, *c.layer, *c.table, c.total_pages, workspace=ws2)
+    for i in range(4):
+        static.zero_()
+        g.replay()
+        assert torch.equal(static, want)
+        assert torch.equal(K().paged_decode_q8(q, *c.layer, *c.table, c.total_pages, workspace=ws), want)
+        torch.cuda.synchronize()

@@ -1,0 +1,153 @@
+"""8-bit cache: the C entry points' checks of arguments (no device work), the wrappers' refusal of CPU
+tensors, and the oracle's format against torch's own float8 conversion."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import q8_oracle as Q
+
+A = 4096  # an aligned stand-in for a device address: every call below ends in a host check
+
+
+def _lib():
+    from nanoslg_amd import _lib
+    return _lib
+
+
+def append_args(**kw):
+    a = dict(k=A, ks=1024, v=A, vs=1024, qo=A, rows=None, width=0, T=4, kp=A, vp=A, ksc=A, vsc=A, P=100, ps=16, ip=A, ix=A,
+             ll=A, B=2, hkv=8, d=128, dt=0, code=0, stream=None)
+    a.update(kw)
+    return list(a.values())
+
+
+def gather_args(**kw):
+    a = dict(kp=A, vp=A, ksc=A, vsc=A, P=100, ps=16, ip=A, ix=A, ll=A, B=2, n=64, hkv=8, d=128, code=0, dt=0, ko=A, vo=A,
+             stream=None)
+    a.update(kw)
+    return list(a.values())
+
+
+def decode_args(**kw):
+    a = dict(q=A, qs=4096, k=None, ks=0, v=None, vs=0, pos=None, cos=None, sin=None, ts=0, tr=0, kp=A, vp=A, ksc=A, vsc=A,
+             P=100, ps=16, ip=A, ix=A, ll=A, tp=10, B=2, hq=32, hkv=8, d=128, scale=0.1, dt=0, code=0, slot=None, ng=0,
+             pre=None, mem=None, out=A, os=4096, ws=None, wsn=0, layout=0, stream=None)
+    a.update(kw)
+    return list(a.values())
+
+
+def prefill_args(**kw):
+    a = dict(q=A, qs=4096, qo=A, rows=None, width=0, T=4, mq=4, kp=A, vp=A, ksc=A, vsc=A, P=100, ps=16, ip=A, ix=A, ll=A, B=2,
+             hq=32, hkv=8, d=128, scale=0.1, dt=0, code=0, out=A, os=4096, ws=None, wsn=0, stream=None)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(code=2), -1), (dict(code=-1), -1), (dict(d=96), -2), (dict(d=0), -1), (dict(dt=2), -2), (dict(dt=7), -2),
+    (dict(ps=0), -1), (dict(P=0), -1), (dict(P=1 << 28, ps=16), -2), (dict(B=-1), -1), (dict(T=-1), -1), (dict(k=None), -1),
+    (dict(qo=None), -1), (dict(ksc=None), -1), (dict(vsc=A + 2), -1), (dict(kp=A + 8), -1), (dict(k=A + 2), -1),
+    (dict(ks=1028), -1), (dict(ks=512), -1), (dict(vs=0), -1), (dict(rows=A, width=0), -1), (dict(rows=A, width=1, T=3), -1),
+    (dict(hkv=70000, ks=70000 * 128, vs=70000 * 128), -2), (dict(T=1 << 33), -1),
+])
+def test_append_refusals(bad, status):
+    L = _lib()
+    assert L.load().nslg_q8_append_kv(*append_args(**bad)) == status
+    assert L.last_error()
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(code=5), -1), (dict(d=80), -2), (dict(dt=9), -1), (dict(n=-1), -1), (dict(B=70000), -1), (dict(ko=None), -1),
+    (dict(vo=A + 4), -1), (dict(ix=None), -1),
+])
+def test_gather_refusals(bad, status):
+    assert _lib().load().nslg_q8_gather_kv(*gather_args(**bad)) == status
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(code=2), -1), (dict(dt=2), -2), (dict(dt=3), -2), (dict(d=96), -2), (dict(hq=30), -1), (dict(hq=136), -2),
+    (dict(scale=0.0), -1), (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(ksc=None), -1),
+    (dict(ksc=A + 1), -1), (dict(kp=A + 8), -1), (dict(qs=4095), -1), (dict(qs=4097), -1), (dict(k=A, v=None, ks=1024), -1),
+    (dict(k=A, v=A, ks=1024, vs=1024, ps=20), -2),  # a block may lie in two waves' work
+    (dict(k=A, v=A, ks=1024, vs=1023), -1), (dict(k=A + 2, v=A, ks=1024, vs=1024), -1),
+    (dict(cos=A, sin=A, pos=A, ts=128, tr=10), -1),  # tables without rows to rotate
+    (dict(ng=33, slot=A, pre=A, mem=A), -2), (dict(ng=1, slot=None, pre=A, mem=A), -1), (dict(ng=-1), -2), (dict(tp=-1), -1),
+    (dict(tp=1 << 28), -2), (dict(), -4),  # no workspace
+])
+def test_decode_refusals(bad, status):
+    assert _lib().load().nslg_q8_paged_decode(*decode_args(**bad)) == status
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(code=2), -1), (dict(dt=2), -2), (dict(d=96), -2), (dict(hq=30), -1), (dict(hq=136), -2), (dict(scale=-1.0), -1),
+    (dict(vsc=None), -1), (dict(vsc=A + 2), -1), (dict(qs=64), -1), (dict(rows=A, width=0), -1), (dict(T=-1), -1),
+])
+def test_prefill_refusals(bad, status):
+    assert _lib().load().nslg_q8_paged_prefill(*prefill_args(**bad)) == status
+
+
+def test_empty_calls_do_nothing():
+    lib = _lib().load()
+    assert lib.nslg_q8_append_kv(*append_args(B=0, T=0)) == 0
+    assert lib.nslg_q8_append_kv(*append_args(T=0, k=None, v=None)) == 0
+    assert lib.nslg_q8_gather_kv(*gather_args(B=0)) == 0
+    assert lib.nslg_q8_gather_kv(*gather_args(n=0, ko=None, vo=None)) == 0
+    assert lib.nslg_q8_paged_decode(*decode_args(B=0)) == 0
+    assert lib.nslg_q8_paged_prefill(*prefill_args(B=0)) == 0
+    assert lib.nslg_q8_paged_prefill(*prefill_args(T=0)) == 0
+
+
+def test_workspace_size():
+    f = _lib().load().nslg_q8_paged_decode_workspace_size
+    one = f(4, 32, 8, 128, 1000, 16, 0, 0, 0)
+    assert one > 0 and f(4, 32, 8, 128, 1000, 16, 1, 1, 0) > 0
+    assert f(4, 32, 8, 128, 1000, 16, 0, 0, 2) > one  # groups hold their members' partials
+    for bad in ((4, 32, 8, 96, 1000, 16, 0, 0, 0), (4, 32, 8, 128, 1000, 16, 2, 0, 0), (4, 32, 8, 128, 1000, 16, 0, 2, 0),
+                (4, 32, 8, 128, 1000, 16, 0, 0, 33), (4, 136, 8, 128, 1000, 16, 0, 0, 0), (0, 32, 8, 128, 10, 16, 0, 0, 0)):
+        assert f(*bad) == 0
+
+
+def test_wrappers_refuse_cpu_tensors():
+    from nanoslg_amd import kernels as K
+    x, s = torch.zeros(2, 16, 1, 64, dtype=torch.int8), torch.zeros(2, 1, 1)
+    i = torch.zeros(2, dtype=torch.int32)
+    rows = torch.zeros(1, 1, 64, dtype=torch.float16)
+    for call in (lambda: K.append_kv_q8(rows, rows, i, 1, x, x, s, s, i, i, i), lambda: K.gather_kv_q8(x, x, s, s, i, i, i, 16),
+                 lambda: K.paged_decode_q8(rows, x, x, s, s, i, i, i, 1),
+                 lambda: K.paged_decode_append_q8(rows, rows, rows, x, x, s, s, i, i, i, 1),
+                 lambda: K.paged_prefill_q8(rows, i, 1, 1, x, x, s, s, i, i, i)):
+        with pytest.raises(ValueError, match="device tensors"):
+            call()
+    with pytest.raises(AttributeError):
+        K.no_such_call
+
+
+def test_oracle_rounds_e4m3_as_torch_does():
+    x = np.concatenate([np.linspace(-448, 448, 20011), np.ldexp(np.linspace(-1, 1, 4001), -5)]).astype(np.float32)
+    want = torch.from_numpy(x).to(torch.float8_e4m3fn).double().numpy()
+    np.testing.assert_array_equal(Q.round_code(x, "e4m3"), want)
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_oracle_scale(code):
+    M = Q.MOST[code]
+    for e in (-126, -20, 0, 3, 100):
+        assert Q.need_scale(M * 2.0 ** e, code) == 2.0 ** e
+        assert Q.need_scale(M * 2.0 ** e * (1 + 2 ** -30), code) == 2.0 ** (e + 1)
+    assert Q.need_scale(1e-45, code) == 2.0 ** -126 and Q.need_scale(0.0, code) == 0.0
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_oracle_error_of_written_rows(code):
+    """A value read back is within half a step of the row written with the block's last scale, and within
+    one step where the scale grew after it."""
+    g = np.random.default_rng(0)
+    lay = Q.Layer(np.zeros((2, 16, 1, 64)), np.zeros((2, 1, 1)), code)
+    x = g.standard_normal((16, 1, 64)) * np.exp(2 * g.standard_normal((16, 1, 1)))
+    for t in range(16):
+        lay.write([1], t, x[t:t + 1])
+    s = lay.scale[1, 0, 0]
+    step = np.full_like(x, s) if code == "int8" else np.maximum(np.ldexp(1.0, np.frexp(np.abs(x))[1] - 4), s * 2.0 ** -9)
+    off = np.abs(lay.read([1], 16) - x)
+    assert (off <= step).all()
+    assert (off[-1] <= step[-1] / 2 * (1 + 1e-12)).all()
