@@ -1135,7 +1135,7 @@ def paged_prefill(q: torch.Tensor, qo_indptr: torch.Tensor, total_q: int, max_q:
 
 # the 8-bit cache's calls (nanoslg_amd.kernels_q8, which uses the above) under this module's name too
 _Q8_CALLS = ("append_kv_q8", "gather_kv_q8", "paged_decode_q8", "paged_decode_append_q8", "paged_decode_rope_append_q8",
-             "paged_prefill_q8")
+             "paged_prefill_q8", "rotate_rows", "DecodeLaunchQ8")
 
 
 def __getattr__(name: str):

@@ -15,8 +15,8 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .kernels import (_DTYPE_CODE, DecodeGroups, Workspace, _i32, _prefill_workspace, _require_gpu, _rope_tables, _rows,
-                      _stream, rope_append)
+from .kernels import (_DTYPE_CODE, _LAYOUT_TAGS, DecodeGroups, DecodeLaunch, Workspace, _i32, _prefill_workspace,
+                      _require_gpu, _rope_tables, _rows, _stream, rope_append)
 
 BLOCK_TOKENS = 16  # slots of a page that share a scale
 CODE_DTYPES = {torch.float8_e4m3fn: _lib.NSLG_E4M3, torch.int8: _lib.NSLG_INT8}
@@ -312,3 +312,131 @@ def paged_prefill_q8(q: torch.Tensor, qo_indptr: torch.Tensor, total_q: int, max
             out.data_ptr(), out.stride(0), ws_ptr, ws_bytes, _stream(q))
     _lib.check(rc, "nslg_q8_paged_prefill")
     return out
+
+
+class DecodeLaunchQ8(DecodeLaunch):
+    """Append + decode for every layer of one decode forward over an 8-bit cache: what
+    ``kernels.DecodeLaunch`` does over 16-bit pools, with its interface. The step's rows go in
+    in the decode launch (nslg_q8_paged_decode with new rows; on pages that 16 does not divide
+    nslg_q8_append_kv goes ahead), with RoPE rotated there too. The forward's first call
+    records its chunk layout for the other layers'."""
+
+    def __init__(self, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                 slot_mapping: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
+                 kv_last_page_len: torch.Tensor, total_pages: int, num_qo_heads: int,
+                 workspace: Optional[Workspace] = None, sm_scale: Optional[float] = None,
+                 groups: Optional[DecodeGroups] = None):
+        _require_gpu(k_pool, v_pool, k_scale, v_scale)
+        if k_pool.dim() != 5 or k_scale.dim() != 4:
+            raise ValueError("DecodeLaunchQ8: pools must be [L, P, page_size, Hkv, D] and scales [L, P, nb, Hkv]")
+        self.L = k_pool.shape[0]
+        if not (v_pool.dim() == 5 and v_scale.dim() == 4 and v_pool.shape[0] == k_scale.shape[0] == v_scale.shape[0] == self.L):
+            raise ValueError("DecodeLaunchQ8: pools and scales of as many layers")
+        self.P, self.ps, self.Hkv, self.D, self.q8 = _layer("DecodeLaunchQ8", k_pool[0], v_pool[0], k_scale[0], v_scale[0])
+        if not all(t.is_contiguous() for t in (k_pool, v_pool, k_scale, v_scale)):
+            raise ValueError("DecodeLaunchQ8: pools and scales must be contiguous")
+        if num_qo_heads % self.Hkv:
+            raise ValueError(f"DecodeLaunchQ8: Hq={num_qo_heads} is not a multiple of Hkv={self.Hkv}")
+        self.lib = _lib.load()
+        self.device, self.dev_index, self.dtype = k_pool.device, k_pool.get_device(), k_pool.dtype
+        self.Hq = num_qo_heads
+        self.kp0, self.vp0, self.ksp0, self.vsp0 = (t.data_ptr() for t in (k_pool, v_pool, k_scale, v_scale))
+        self.layer_bytes = k_pool[0].numel()
+        self.scale_bytes = 4 * k_scale[0].numel()
+        self.pools = (k_pool, v_pool, k_scale, v_scale)
+        self.workspace = workspace or Workspace(self.device)
+        self.scale = (1.0 / math.sqrt(self.D)) if sm_scale is None else float(sm_scale)
+        self.B = kv_indptr.numel() - 1
+        self.groups, self._ws_pages = None, -1
+        self.rebind(slot_mapping, kv_indptr, kv_indices, kv_last_page_len, total_pages, groups, check=True)
+
+    def rebind(self, slot_mapping: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
+               kv_last_page_len: torch.Tensor, total_pages: int, groups: Optional[DecodeGroups] = None,
+               check: bool = True) -> "DecodeLaunchQ8":
+        """Point the launcher at another forward's plan of the same batch size (slot_mapping is not used: the
+        slots come from the block table)."""
+        B = self.B
+        self._layout = 0
+        if check:
+            _require_gpu(self.pools[0], kv_indptr, kv_indices, kv_last_page_len)
+            if _table("DecodeLaunchQ8", kv_indptr, kv_indices, kv_last_page_len) != B:
+                raise ValueError(f"DecodeLaunchQ8: a plan of {B} sequences")
+            if groups is not None:
+                _require_gpu(self.pools[0], groups.seq_group_slot)
+                _i32(groups.seq_group_slot, "seq_group_slot")
+                if groups.seq_group_slot.numel() != B:
+                    raise ValueError("DecodeLaunchQ8: one group slot per sequence")
+        self.table = (kv_indptr, kv_indices, kv_last_page_len)
+        self.table_ptrs = (kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr())
+        self.total_pages = int(total_pages)
+        if groups is self.groups and self.total_pages <= self._ws_pages:
+            return self
+        self.groups = groups
+        self.grp = (None, 0, None, None)
+        if groups is not None:
+            self.grp = (groups.seq_group_slot.data_ptr(), groups.num_groups, groups.prefix_pages_np.ctypes.data,
+                        groups.members_np.ctypes.data)
+        # sized for some headroom, as in DecodeLaunch; f16 and bf16 calls may both come
+        bound = self.total_pages + max(self.total_pages // 4, 1024)
+        with _on_device(self.pools[0]):
+            need = max(int(self.lib.nslg_q8_paged_decode_workspace_size(B, self.Hq, self.Hkv, self.D, bound, self.ps, dt,
+                                                                        self.q8, self.grp[1]))
+                       for dt in (_lib.NSLG_F16, _lib.NSLG_BF16))
+        if groups is not None and need == 0:
+            raise ValueError("DecodeLaunchQ8: unsupported grouped decode shape")
+        self.ws = self.workspace.get(need)
+        self._ws_pages = bound
+        return self
+
+    def __call__(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
+                 rope: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
+        """As DecodeLaunch: q [B, Hq, D] or [B, 1, Hq, D], k_new / v_new [B, ..., Hkv, D] rows of one token each,
+        float16 or bfloat16; rope = (cos, sin, positions int32 [B])."""
+        if not 0 <= layer < self.L:
+            raise IndexError(f"layer {layer} out of range [0, {self.L})")
+        B, Hq, Hkv, D, di = self.B, self.Hq, self.Hkv, self.D, self.dev_index
+        if q.get_device() != di or k_new.get_device() != di or v_new.get_device() != di:
+            raise ValueError(f"DecodeLaunchQ8: tensors must be on {self.device}")
+        dt = _row_type("DecodeLaunchQ8", q, k_new, v_new)
+        out_shape = (B, Hq, D)
+        if q.dim() == 4 and q.shape[1] == 1:
+            q, out_shape = q[:, 0], (B, 1, Hq * D)
+        if q.shape != (B, Hq, D) or q.stride(2) != 1 or q.stride(1) != D:
+            raise ValueError(f"DecodeLaunchQ8: q must be [{B}, {Hq}, {D}] with a contiguous [Hq, D] block")
+        if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(0) < Hq * D:
+            q = q.clone(memory_format=torch.contiguous_format)
+        tables = (None, None, None, 0, 0)
+        if rope is not None:
+            cos, sin, pos = rope
+            _require_gpu(self.pools[0], cos, sin, pos)
+            _i32(pos, "positions")
+            if pos.numel() != B:
+                raise ValueError("DecodeLaunchQ8: one position per sequence")
+            cos, sin = _rope_tables(cos, sin, D)
+        rows = (None, 0, None, 0)
+        if self.ps % BLOCK_TOKENS:
+            if rope is not None:
+                q, k_new = rotate_rows(q, k_new, v_new, pos, cos, sin)
+            append_kv_q8(k_new, v_new, torch.arange(B + 1, dtype=torch.int32, device=self.device), B,
+                         *(t[layer] for t in self.pools), *self.table)
+        else:
+            k_new, ks = _new_rows("DecodeLaunchQ8", k_new, "k_new", B, Hkv, D)
+            v_new, vs = _new_rows("DecodeLaunchQ8", v_new, "v_new", B, Hkv, D)
+            rows = (k_new.data_ptr(), ks, v_new.data_ptr(), vs)
+            if rope is not None:
+                if cos.data_ptr() % 16 or sin.data_ptr() % 16 or cos.stride(0) % 4:
+                    cos, sin = (t[:, :D].clone(memory_format=torch.contiguous_format) for t in (cos, sin))
+                tables = (pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0])
+        out = torch.empty(out_shape, dtype=q.dtype, device=self.device)
+        lay = self._layout  # < 0: read the layout recorded under tag -lay
+        if lay == 0:  # the first call on this plan records its chunk layout
+            lay = next(_LAYOUT_TAGS)
+            self._layout = -lay
+        off, soff = layer * self.layer_bytes, layer * self.scale_bytes
+        with _on_device(q):
+            rc = self.lib.nslg_q8_paged_decode(
+                q.data_ptr(), q.stride(0), *rows, *tables, self.kp0 + off, self.vp0 + off, self.ksp0 + soff, self.vsp0 + soff,
+                self.P, self.ps, *self.table_ptrs, self.total_pages, B, Hq, Hkv, D, self.scale, dt, self.q8, *self.grp,
+                out.data_ptr(), Hq * D, self.ws.data_ptr(), self.ws.numel(), lay, _stream(q))
+        _lib.check(rc, "nslg_q8_paged_decode")
+        return out

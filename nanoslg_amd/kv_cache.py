@@ -37,6 +37,11 @@ import torch
 
 _BACKENDS = ("paged", "contiguous")
 
+# names of the cache types besides the model's own (None, "auto")
+_CACHE_DTYPES = {"fp8": torch.float8_e4m3fn, "fp8_e4m3": torch.float8_e4m3fn, "float8_e4m3fn": torch.float8_e4m3fn,
+                 "int8": torch.int8}
+_SCALE_BLOCK = 16  # slots of a page that share one scale per KV head in an 8-bit cache
+
 
 def _check_head_dim(cfg: "KVCacheConfig", kernels) -> None:
     """A cache is only built for a (dtype, head_dim) every kernel it uses supports,
@@ -93,8 +98,25 @@ class KVCacheConfig:
     # prompts shorter than a page are matched too, and a prefix ending inside a page
     # shares that page; the first write into it copies it (copy-on-write).
     share_partial_pages: bool = True
+    # What the pool holds: None (or "auto"), the model's dtype; torch.float8_e4m3fn ("fp8") or
+    # torch.int8 ("int8"), 8-bit codes with one power-of-two scale for each block of 16 slots of a
+    # page and KV head, K and V apart (fp16 and bf16 models). Half the bytes of a 16-bit cache.
+    cache_dtype: Optional[torch.dtype] = None
 
     def __post_init__(self):
+        if isinstance(self.cache_dtype, str):
+            if self.cache_dtype not in _CACHE_DTYPES and self.cache_dtype != "auto":
+                raise ValueError(f"unknown KV cache type {self.cache_dtype!r}; use auto|{'|'.join(_CACHE_DTYPES)}")
+            self.cache_dtype = _CACHE_DTYPES.get(self.cache_dtype)
+        if self.cache_dtype == self.dtype:
+            self.cache_dtype = None
+        if self.cache_dtype is not None:
+            if self.cache_dtype not in _CACHE_DTYPES.values():
+                raise ValueError(f"KV cache type {self.cache_dtype}: the model's dtype, float8_e4m3fn or int8")
+            if self.dtype not in (torch.float16, torch.bfloat16):
+                raise ValueError(f"an 8-bit KV cache is for float16 and bfloat16 models (dtype {self.dtype})")
+            if self.head_dim % 64:
+                raise ValueError(f"an 8-bit KV cache needs a head_dim of 64, 128 or 256 (got {self.head_dim})")
         if self.backend in ("auto", "flashinfer"):
             self.backend = "paged"
         if self.backend not in _BACKENDS:
@@ -106,7 +128,13 @@ class KVCacheConfig:
         if self.backend == "contiguous":
             self._auto_seq_len()
 
+    def scale_blocks(self, page_size: int) -> int:
+        """Scales per page and KV head of an 8-bit pool."""
+        return -(-page_size // _SCALE_BLOCK)
+
     def _elem_bytes(self) -> int:
+        if self.cache_dtype is not None:
+            return 1
         return {torch.float16: 2, torch.bfloat16: 2, torch.float32: 4}.get(self.dtype, 2)
 
     def _device_mem(self) -> Optional[Tuple[int, int]]:
@@ -127,6 +155,8 @@ class KVCacheConfig:
         budget = int(max(0, free - headroom) * self.memory_fraction)
         per_page = (2 * self.num_layers * self.page_size * self.num_kv_heads * self.head_dim
                     * self._elem_bytes())
+        if self.cache_dtype is not None:
+            per_page += 2 * self.num_layers * self.scale_blocks(self.page_size) * self.num_kv_heads * 4
         return max(64, min(budget // max(per_page, 1), self.max_pages_cap))
 
     def _auto_seq_len(self):
@@ -137,6 +167,8 @@ class KVCacheConfig:
         free, _ = mem
         budget = int(free * self.memory_fraction * 0.5)
         per_tok = 2 * self.num_layers * self.num_kv_heads * self.head_dim * self._elem_bytes()
+        if self.cache_dtype is not None:  # and its share of the scales
+            per_tok += -(-2 * self.num_layers * self.num_kv_heads * 4 // _SCALE_BLOCK)
         cap = budget // max(per_tok, 1) // max(self.max_batch_size, 1)
         self.max_seq_len = min(self.max_seq_len, max(512, cap))
 
@@ -498,8 +530,63 @@ def _get_positions(plan: _ForwardPlan, batch: int, iw: int, S: int) -> torch.Ten
 # --------------------------------------------------------------------------------------
 
 
-class PagePool:
-    """K and V pools [L, P, page_size, Hkv, D] on the device; page 0 is the permanent
+class _Pools:
+    """The K and V memory of a cache: pools [L, pages, page_size, Hkv, D] of the cache's type and, for
+    an 8-bit cache, the scales [L, pages, ceil(page_size / 16), Hkv] of each (a block's
+    scale has a meaning once its first slot is written; zero-on-alloc leaves it).
+
+    k_words / v_words: the pools as the page-moving kernels and the planners take them, in
+    16-bit words where they hold 8-bit codes."""
+
+    def __init__(self, cfg: KVCacheConfig, pages: int, page_size: int, device: torch.device):
+        shape = (cfg.num_layers, pages, page_size, cfg.num_kv_heads, cfg.head_dim)
+        dtype = cfg.cache_dtype or cfg.dtype
+        self.k = torch.zeros(shape, dtype=dtype, device=device)
+        self.v = torch.zeros(shape, dtype=dtype, device=device)
+        self.k_words, self.v_words = self.k, self.v
+        self.k_scale = self.v_scale = None
+        if cfg.cache_dtype is not None:
+            self.k_words, self.v_words = self.k.view(torch.float16), self.v.view(torch.float16)
+            shape = (cfg.num_layers, pages, cfg.scale_blocks(page_size), cfg.num_kv_heads)
+            self.k_scale = torch.zeros(shape, dtype=torch.float32, device=device)
+            self.v_scale = torch.zeros(shape, dtype=torch.float32, device=device)
+        self._layers8: List[Tuple[torch.Tensor, ...]] = []
+
+    def layer8(self, i: int) -> Tuple[torch.Tensor, ...]:
+        """Layer i of an 8-bit cache: codes of K and V, scales of K and V."""
+        if not self._layers8:
+            self._layers8 = list(zip(*(t.unbind(0) for t in (self.k, self.v, self.k_scale, self.v_scale))))
+        return self._layers8[i]
+
+    def decode_launch(self, kern, *args, **kw):
+        """The decode launcher over these pools (kernels.DecodeLaunch, or its 8-bit form)."""
+        if self.k_scale is None:
+            return kern.DecodeLaunch(self.k, self.v, *args, **kw)
+        return kern.DecodeLaunchQ8(self.k, self.v, self.k_scale, self.v_scale, *args, **kw)
+
+    def copy_pages(self, kern, src_ids: torch.Tensor, dst_ids: torch.Tensor) -> None:
+        """pool[:, dst] <- pool[:, src] on the device, scales included."""
+        kern.copy_pages(self.k_words, self.v_words, src_ids, dst_ids)
+        if self.k_scale is not None:
+            kern.copy_pages(self.k_scale.unsqueeze(-1), self.v_scale.unsqueeze(-1), src_ids, dst_ids)
+
+
+def _attend8(kern, ctx, layer, q, k_new, v_new):
+    """A multi-token forward of one layer of an 8-bit cache: its rows written, then attended.
+    layer: _Pools.layer8; ctx: the forward's context (its plan, widths and longest sequence)."""
+    plan = ctx._plan
+    B, S, Hq, D = q.shape
+    grid = {} if ctx._uniform_rows and S == ctx._iw else {"q_rows": plan.rows_for(S), "grid_width": S}
+    table = (plan.indptr, plan.indices, plan.lpl)
+    kern.append_kv_q8(k_new, v_new, plan.qo_indptr, plan.total_q, *layer, *table, **grid)
+    # (scratch from the caching allocator, as in the caches' 16-bit prefills: forwards may run on several streams)
+    o = kern.paged_prefill_q8(q.reshape(B * S, Hq, D), plan.qo_indptr, plan.total_q, ctx._max_q, *layer, *table,
+                              max_kv=ctx.max_kv_len, **grid)
+    return o.view(B, S, Hq * D)
+
+
+class PagePool(_Pools):
+    """K and V pools [L, P, page_size, Hkv, D] on the device (_Pools); page 0 is the permanent
     null/sink page. Host state: int32 refcounts and tokens_used, a LIFO free stack
     (lowest ids first on a fresh pool). Zero-on-alloc and copy-on-write are batched
     device launches."""
@@ -510,11 +597,9 @@ class PagePool:
         P = cfg.max_pages
         if P < 2:
             raise ValueError("max_pages must be >= 2 (page 0 is reserved)")
-        shape = (cfg.num_layers, P, cfg.page_size, cfg.num_kv_heads, cfg.head_dim)
         dev = torch.device(cfg.device) if cfg.device is not None else torch.device("cpu")
         self.device = dev
-        self.k = torch.zeros(shape, dtype=cfg.dtype, device=dev)
-        self.v = torch.zeros(shape, dtype=cfg.dtype, device=dev)
+        super().__init__(cfg, P, cfg.page_size, dev)
         self.ref_count = np.zeros(P, np.int64)
         self.tokens_used = np.zeros(P, np.int64)
         self.ref_count[0] = 1
@@ -568,7 +653,7 @@ class PagePool:
         if not page_ids:
             return
         (ids,) = _upload_i32([np.asarray(page_ids, np.int32)], self.device)
-        self.kernels.zero_pages(self.k, self.v, ids)
+        self.kernels.zero_pages(self.k_words, self.v_words, ids)
 
     def release(self, pid: int) -> None:
         if pid <= 0:
@@ -624,7 +709,7 @@ class PagePool:
         if len(src_ids) == 0:
             return
         src, dst = _upload_i32([np.asarray(src_ids, np.int32), np.asarray(dst_ids, np.int32)], self.device)
-        self.kernels.copy_pages(self.k, self.v, src, dst)
+        self.copy_pages(self.kernels, src, dst)
 
     def cow(self, pid: int) -> Optional[int]:
         """Single-page copy-on-write: allocate, copy all layers and slots, return the id."""
@@ -1033,7 +1118,7 @@ class PagedCacheContext(CacheContext):
                             self._plan.groups = kern.DecodeGroups(B, groups[0], groups[1], pool.device,
                                                                   seq_group_slot=slot)
                     if nz:  # zero-on-alloc of the pages this forward's extensions took
-                        cache.kernels.zero_pages(pool.k, pool.v, self._plan.zero_ids)
+                        cache.kernels.zero_pages(pool.k_words, pool.v_words, self._plan.zero_ids)
                     if self._is_decode and iw == 1:
                         cache._record_decode_plan(self.seq_ids, self._plan, self.seq_lens)
                     return
@@ -1169,9 +1254,9 @@ class PagedCacheContext(CacheContext):
                 self._plan.groups = kern.DecodeGroups(B, groups[0], groups[1], pool.device,
                                                       seq_group_slot=views[9])
         if zero.size:  # zero-on-alloc of the pages this forward's extensions took
-            kern.zero_pages(pool.k, pool.v, self._plan.zero_ids)
+            kern.zero_pages(pool.k_words, pool.v_words, self._plan.zero_ids)
         if cow_src:
-            kern.copy_pages(pool.k, pool.v, self._plan.cow_src, self._plan.cow_dst)
+            pool.copy_pages(kern, self._plan.cow_src, self._plan.cow_dst)
         if self._is_decode and iw == 1:
             cache._record_decode_plan(self.seq_ids, self._plan, self.seq_lens)
 
@@ -1196,6 +1281,8 @@ class PagedCacheContext(CacheContext):
             if launch is None or launch.bound_plan is not plan:
                 launch = self._decode_launch = cache._decode_launcher(plan, q.shape[2])
             return launch(layer_idx, q, k_new, v_new)
+        if pool.k_scale is not None:
+            return _attend8(kern, self, pool.layer8(layer_idx), q, k_new, v_new)
         k_layer, v_layer = pool.layer(layer_idx)
         o = self._prefill(q, k_layer, v_layer, k_new, v_new)  # the write and the attention in one launch
         if o is not None:
@@ -1221,6 +1308,9 @@ class PagedCacheContext(CacheContext):
             if launch is None or launch.bound_plan is not plan:
                 launch = self._decode_launch = cache._decode_launcher(plan, q.shape[2])
             return launch(layer_idx, q, k_new, v_new, rope=(cos, sin, pos))
+        if pool.k_scale is not None:
+            q, k_new = kern.rotate_rows(q, k_new, v_new, pos, cos, sin)
+            return _attend8(kern, self, pool.layer8(layer_idx), q, k_new, v_new)
         k_layer, v_layer = pool.layer(layer_idx)
         q_rot = kern.rope_append(q, k_new, v_new, pos, plan.slots_for(S), cos, sin, k_layer, v_layer)
         return self._prefill(q_rot, k_layer, v_layer)
@@ -1400,8 +1490,8 @@ class PagedKVCache(KVCacheManager):
             prev.bound_plan = plan
             return prev
         pool = self.pool
-        launch = kern.DecodeLaunch(pool.k, pool.v, plan.slot, plan.indptr, plan.indices, plan.lpl,
-                                   plan.total_pages, num_qo_heads, workspace=self.workspace, groups=plan.groups)
+        launch = pool.decode_launch(kern, plan.slot, plan.indptr, plan.indices, plan.lpl, plan.total_pages, num_qo_heads,
+                                    workspace=self.workspace, groups=plan.groups)
         launch.bound_plan = plan
         self._launcher = launch
         return launch
@@ -1547,14 +1637,14 @@ class PagedKVCache(KVCacheManager):
         fast = getattr(kern, "_decode_plan_step", None)
         if fast is not None:  # inputs are the previous plan's outputs: no argument checks
             if self._pool_args is None:
-                L, P, _, Hkv, D = pool.k.shape
-                self._pool_args = (pool.k.data_ptr(), pool.v.data_ptr(), L, P, Hkv, D, kern.dtype_code(pool.k.dtype))
+                L, P, _, Hkv, D = pool.k_words.shape
+                self._pool_args = (pool.k.data_ptr(), pool.v.data_ptr(), L, P, Hkv, D, kern.dtype_code(pool.k_words.dtype))
             dst = self._plan_buffers(B, plan.total_pages + n_new)
             indptr, indices, lpl, slot, pos, new = fast(plan.indptr, plan.indices, plan.lpl, new_page, ps, n_new,
                                                         self._pool_args, out=dst, new_page_ptr=new_page_ptr)
         else:
             indptr, indices, lpl, slot, pos, new = kern.decode_plan_step(plan.indptr, plan.indices, plan.lpl,
-                                                                        new_page, ps, n_new, pool.k, pool.v)
+                                                                        new_page, ps, n_new, pool.k_words, pool.v_words)
         rows = self._decode_rows.get(B)
         if rows is None:
             qo, qr = _upload_i32([np.arange(B + 1, dtype=np.int32), np.arange(B, dtype=np.int32)], pool.device)
@@ -1844,6 +1934,8 @@ class ContiguousCacheContext(CacheContext):
             launch = self._decode(q)
             if launch is not None:
                 return launch(layer_idx if layer_idx >= 0 else layer_idx + cache.cfg.num_layers, q, k_new, v_new)
+        if cache.pools.k_scale is not None:
+            return _attend8(cache.kernels, self, cache.pools.layer8(layer_idx), q, k_new, v_new)
         k_layer, v_layer = cache.paged_view(layer_idx)
         if not (self._is_decode and S == 1):
             # the write and the attention in one launch (a sequence's slot is its one page)
@@ -1874,6 +1966,9 @@ class ContiguousCacheContext(CacheContext):
             if launch is not None:
                 return launch(layer_idx if layer_idx >= 0 else layer_idx + cache.cfg.num_layers, q, k_new, v_new,
                               rope=(cos, sin, plan.pos_for(S)))
+        if cache.pools.k_scale is not None:
+            q, k_new = cache.kernels.rotate_rows(q, k_new, v_new, plan.pos_for(S), cos, sin)
+            return _attend8(cache.kernels, self, cache.pools.layer8(layer_idx), q, k_new, v_new)
         k_layer, v_layer = cache.paged_view(layer_idx)
         q_rot = cache.kernels.rope_append(q, k_new, v_new, plan.pos_for(S), plan.slots_for(S), cos, sin,
                                           k_layer, v_layer)
@@ -1906,7 +2001,7 @@ class ContiguousCacheContext(CacheContext):
                     and (prev.Hq, prev.kp0, prev.vp0) == of):
                 launch = prev.bound_to(*args)
             else:
-                launch = kern.DecodeLaunch(cache.k, cache.v, *args, q.shape[2], workspace=cache.workspace)
+                launch = cache.pools.decode_launch(kern, *args, q.shape[2], workspace=cache.workspace)
             cache._launcher = launch
             self._decode_launch = got = (of, launch)
         return got[1]
@@ -1939,9 +2034,8 @@ class ContiguousKVCache(KVCacheManager):
         self.kernels = kernels or _default_kernels()
         _check_head_dim(cfg, self.kernels)
         self.device = torch.device(cfg.device) if cfg.device is not None else torch.device("cpu")
-        shape = (cfg.num_layers, cfg.max_batch_size, cfg.max_seq_len, cfg.num_kv_heads, cfg.head_dim)
-        self.k = torch.zeros(shape, dtype=cfg.dtype, device=self.device)
-        self.v = torch.zeros(shape, dtype=cfg.dtype, device=self.device)
+        self.pools = _Pools(cfg, cfg.max_batch_size, cfg.max_seq_len, self.device)  # a slot is a page of max_seq_len
+        self.k, self.v = self.pools.k, self.pools.v
         self.states: Dict[str, _ContigSeqState] = {}
         self._slot = 0
         self.workspace = self.kernels.Workspace(self.device, 16 << 20)
@@ -1955,7 +2049,7 @@ class ContiguousKVCache(KVCacheManager):
         self._slot += 1
         assert s < self.cfg.max_batch_size, "Exceeded max_batch_size"
         (ids,) = _upload_i32([np.asarray([s], np.int32)], self.device)
-        self.kernels.zero_pages(self.k, self.v, ids)
+        self.kernels.zero_pages(self.pools.k_words, self.pools.v_words, ids)
         st = _ContigSeqState(seq_id, s)
         if token_ids:
             st.token_ids = list(token_ids)
@@ -2016,6 +2110,7 @@ def create_cache_manager(hf_config, parallel_config, device, dtype, model_config
         enable_prefix_caching=getattr(model_config, "enable_prefix_caching", True),
         share_partial_pages=getattr(model_config, "share_partial_pages", True),
         backend=backend,
+        cache_dtype=getattr(model_config, "kv_cache_dtype", None),
     )
     if kv_cfg.backend == "paged":
         return PagedKVCache(kv_cfg)
@@ -2157,12 +2252,12 @@ class DecodeGraph:
         self.dev_index = dev.index if dev.index is not None else torch.cuda.current_device()
         self.used = [False, False]
         L, P = cfg.num_layers, cfg.max_pages
-        self.pool_args = (pool.k.data_ptr(), pool.v.data_ptr(), L, P, cfg.num_kv_heads, cfg.head_dim,
-                          kern.dtype_code(pool.k.dtype))
+        self.pool_args = (pool.k.data_ptr(), pool.v.data_ptr(), L, P, cfg.num_kv_heads, pool.k_words.shape[-1],
+                          kern.dtype_code(pool.k_words.dtype))
         # The launch is captured once, so it is sized for the pool (P pages) rather than
         # this step's page count; the kernel derives its chunk length from the lengths.
-        launches = [kern.DecodeLaunch(pool.k, pool.v, p.slot, p.indptr, p.indices, p.lpl, P, cfg.num_qo_heads,
-                                      workspace=cache.workspace, groups=p.groups) for p in self.plans]
+        launches = [pool.decode_launch(kern, p.slot, p.indptr, p.indices, p.lpl, P, cfg.num_qo_heads,
+                                       workspace=cache.workspace, groups=p.groups) for p in self.plans]
         self.ctxs = [_GraphDecodeContext(self, self.plans[(i + 1) % 2], launches[(i + 1) % 2]) for i in range(2)]
         self.graphs, self.outputs = [], []
         side = torch.cuda.Stream(dev)

@@ -151,3 +151,38 @@ def test_oracle_error_of_written_rows(code):
     off = np.abs(lay.read([1], 16) - x)
     assert (off <= step).all()
     assert (off[-1] <= step[-1] / 2 * (1 + 1e-12)).all()
+
+
+def test_config_of_the_cache_type():
+    from nanoslg_amd import KVCacheConfig
+    base = dict(num_layers=2, num_kv_heads=2, num_qo_heads=4, head_dim=64, max_pages=8)
+    for name, t in (("fp8", torch.float8_e4m3fn), ("fp8_e4m3", torch.float8_e4m3fn), ("int8", torch.int8), ("auto", None),
+                    (None, None), (torch.int8, torch.int8), (torch.bfloat16, None)):
+        assert KVCacheConfig(**base, cache_dtype=name).cache_dtype == t
+    for bad in ("fp4", torch.float16, torch.float8_e5m2, torch.uint8):
+        with pytest.raises(ValueError):
+            KVCacheConfig(**base, cache_dtype=bad)
+    with pytest.raises(ValueError, match="float16 and bfloat16"):
+        KVCacheConfig(**base, dtype=torch.float32, cache_dtype="fp8")
+    with pytest.raises(ValueError, match="head_dim"):
+        KVCacheConfig(**{**base, "head_dim": 80}, cache_dtype="int8")
+
+
+def test_pool_of_an_8_bit_cache():
+    """Codes, their 16-bit words and the scales of the paged and the contiguous pool (host memory: no kernels)."""
+    import fake_kernels
+    from nanoslg_amd import ContiguousKVCache, KVCacheConfig, PagePool
+    cfg = KVCacheConfig(num_layers=3, num_kv_heads=2, num_qo_heads=4, head_dim=64, page_size=20, max_pages=8, cache_dtype="int8")
+    p = PagePool(cfg, kernels=fake_kernels)
+    assert p.k.dtype == torch.int8 and p.k.shape == (3, 8, 20, 2, 64) and p.k_scale.shape == (3, 8, 2, 2)
+    assert p.k_words.shape == (3, 8, 20, 2, 32) and p.k_words.data_ptr() == p.k.data_ptr()
+    assert [t.data_ptr() for t in p.layer8(1)] == [t[1].data_ptr() for t in (p.k, p.v, p.k_scale, p.v_scale)]
+    p.k.random_(-127, 128), p.v.random_(-127, 128), p.k_scale.uniform_(), p.v_scale.uniform_()
+    src, dst = p.alloc(1, zero=False)[0], p.cow(1)
+    for t in (p.k, p.v, p.k_scale, p.v_scale):  # copy-on-write takes the scales along
+        assert torch.equal(t[:, src], t[:, dst])
+    p.zero([src])
+    assert not p.k[:, src].any() and not p.v[:, src].any() and p.k[:, dst].any()
+    c = ContiguousKVCache(KVCacheConfig(num_layers=1, num_kv_heads=2, num_qo_heads=4, head_dim=64, max_batch_size=2, max_seq_len=100,
+                                        backend="contiguous", cache_dtype="fp8"), kernels=fake_kernels)
+    assert c.k.dtype == torch.float8_e4m3fn and c.pools.v_scale.shape == (1, 2, 7, 2)
