@@ -22,6 +22,8 @@ LIB_PATH = PKG_DIR / "libnslg_kv.so"
 # the CPython fast-call binding of the per-step entry points (links libnslg_kv.so)
 FAST_SRC = CSRC / "fastcall.c"
 FAST_PATH = PKG_DIR / ("_nslg_fast" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+FAST_Q8_SRC = CSRC / "fastcall_q8.c"  # the same of the 8-bit cache's entry points
+FAST_Q8_PATH = PKG_DIR / ("_nslg_fast_q8" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 # the host-side forward planner (plain C over the CPython API, no GPU code)
 HOST_SRC = CSRC / "host_plan.c"
 HOST_PATH = PKG_DIR / ("_nslg_host" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
@@ -89,7 +91,8 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
     _build_fast()
     _build_host()
     if verbose:
-        print(f"[nanoslg_amd] built {LIB_PATH} from {len(srcs)} sources, {FAST_PATH.name} and {HOST_PATH.name}",
+        print(f"[nanoslg_amd] built {LIB_PATH} from {len(srcs)} sources, {FAST_PATH.name}, "
+              f"{FAST_Q8_PATH.name} and {HOST_PATH.name}",
               file=sys.stderr)
     return LIB_PATH
 
@@ -112,9 +115,10 @@ def _build_ext(src: Path, out: Path, link: list[str]) -> None:
 
 
 def _build_fast() -> None:
-    """Compile the fast-call binding (host C, the system compiler) against the
-    library just linked; it finds the library next to itself at run time."""
-    _build_ext(FAST_SRC, FAST_PATH, [f"-L{PKG_DIR}", "-lnslg_kv", "-Wl,-rpath,$ORIGIN"])
+    """Compile the fast-call bindings (host C, the system compiler) against the
+    library just linked; they find the library next to themselves at run time."""
+    for src, out in ((FAST_SRC, FAST_PATH), (FAST_Q8_SRC, FAST_Q8_PATH)):
+        _build_ext(src, out, [f"-L{PKG_DIR}", "-lnslg_kv", "-Wl,-rpath,$ORIGIN"])
 
 
 def _build_host() -> None:

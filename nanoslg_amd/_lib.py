@@ -174,6 +174,24 @@ def fast():
     return _fast
 
 
+_fast_q8 = None
+
+
+def fast_q8():
+    """The fast-call binding of the 8-bit cache's entry points, as fast() is of the others."""
+    global _fast_q8
+    if _fast_q8 is not None:
+        return _fast_q8
+    load()
+    try:
+        from . import _nslg_fast_q8
+    except ImportError as e:
+        raise KernelLibraryError(f"the fast-call binding of {LIB_PATH} is not built or does not load ({e}); "
+                                 "run `python -m nanoslg_amd._build` (or __graft_entry__.build()) first") from e
+    _fast_q8 = _nslg_fast_q8
+    return _fast_q8
+
+
 _host = None
 
 

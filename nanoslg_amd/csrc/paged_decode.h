@@ -510,20 +510,21 @@ __device__ inline void write_new_row8(const DecodeParams& p, int b, int h, int p
   const int64_t blk = scale_index(pid, slot, p.blocks_per_page, p.num_kv_heads, h);
   const uint16_t* ksrc = p.k_new + (int64_t)b * p.k_new_stride + (int64_t)h * D;
   const uint16_t* vsrc = p.v_new + (int64_t)b * p.v_new_stride + (int64_t)h * D;
-  write_block<T, F, D>(reinterpret_cast<char*>(const_cast<uint16_t*>(p.k_pool)) + at, row_bytes, p.k_scale + blk, a, 1,
-                       [&](int, int e) {
-                         u16x8 x = *reinterpret_cast<const u16x8*>(ksrc + e);
-                         if (p.rope_cos != nullptr) {  // rotated at the token's position
-                           const bool lo = e < D / 2;
-                           const u16x8 y = *reinterpret_cast<const u16x8*>(ksrc + e + (lo ? D / 2 : -D / 2));
-                           const float *crow, *srow;
-                           rope_rows_of(p, b, crow, srow);
-                           x = rope8<T>(x, y, crow, srow, e, lo);
-                         }
-                         return x;
-                       });
-  write_block<T, F, D>(reinterpret_cast<char*>(const_cast<uint16_t*>(p.v_pool)) + at, row_bytes, p.v_scale + blk, a, 1,
-                       [&](int, int e) { return *reinterpret_cast<const u16x8*>(vsrc + e); });
+  BlockRows<D> krow, vrow;
+  load_block_rows<D>(krow, a, 1, [&](int, int e) {
+    u16x8 x = *reinterpret_cast<const u16x8*>(ksrc + e);
+    if (p.rope_cos != nullptr) {  // rotated at the token's position
+      const bool lo = e < D / 2;
+      const u16x8 y = *reinterpret_cast<const u16x8*>(ksrc + e + (lo ? D / 2 : -D / 2));
+      const float *crow, *srow;
+      rope_rows_of(p, b, crow, srow);
+      x = rope8<T>(x, y, crow, srow, e, lo);
+    }
+    return x;
+  });
+  load_block_rows<D>(vrow, a, 1, [&](int, int e) { return *reinterpret_cast<const u16x8*>(vsrc + e); });
+  write_block<T, F, D>(krow, reinterpret_cast<char*>(const_cast<uint16_t*>(p.k_pool)) + at, row_bytes, p.k_scale + blk, a, 1);
+  write_block<T, F, D>(vrow, reinterpret_cast<char*>(const_cast<uint16_t*>(p.v_pool)) + at, row_bytes, p.v_scale + blk, a, 1);
 }
 
 template <typename T, int D, bool kTileInPage, int kDepth, bool kGrouped, typename F>

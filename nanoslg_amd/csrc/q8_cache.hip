@@ -91,7 +91,6 @@ __global__ void __launch_bounds__(256) append_q8_kernel(Append8Params p) {
   if (!locate_block(p, blockIdx.x, t)) return;
   const int page = t.blk / p.blocks_per_page, i = t.blk - page * p.blocks_per_page;
   const int pid = p.indices[p.indptr[t.seq] + page];
-  if (pid < 0 || (int64_t)pid >= p.num_pages) return;
   const int base = page * p.page_size + kBlockToks * i;  // position of the block's row 0
   const int end = min(t.len, page * p.page_size + min(p.page_size, kBlockToks * (i + 1)));
   const int a = max(t.start - base, 0), cnt = end - base - a;
@@ -103,18 +102,24 @@ __global__ void __launch_bounds__(256) append_q8_kernel(Append8Params p) {
   if (cnt < 1 || r0 < 0 || r0 + cnt > p.num_rows) return;
   const bool is_v = c & 1;
   const int h = c >> 1;
-  const uint16_t* src = (is_v ? p.v_new : p.k_new) + r0 * (is_v ? p.v_stride : p.k_stride) + (int64_t)h * D;
   const int64_t stride = is_v ? p.v_stride : p.k_stride;
+  const uint16_t* src = (is_v ? p.v_new : p.k_new) + r0 * stride + (int64_t)h * D;
+  BlockRows<D> rows;  // (loaded before the page id is waited for)
+  load_block_rows<D>(rows, a, cnt, [&](int r, int e) { return *reinterpret_cast<const u16x8*>(src + (r - a) * stride + e); });
+  if (pid < 0 || (int64_t)pid >= p.num_pages) return;
   const int64_t row_bytes = (int64_t)p.num_kv_heads * D;
   char* codes = (is_v ? p.v_pool : p.k_pool) + ((int64_t)pid * p.page_size + kBlockToks * i) * row_bytes + (int64_t)h * D;
   float* scale = (is_v ? p.v_scale : p.k_scale) + ((int64_t)pid * p.blocks_per_page + i) * p.num_kv_heads + h;
-  write_block<T, F, D>(codes, row_bytes, scale, a, cnt,
-                       [&](int r, int e) { return *reinterpret_cast<const u16x8*>(src + (r - a) * stride + e); });
+  write_block<T, F, D>(rows, codes, row_bytes, scale, a, cnt);
 }
 
 // ---- gather: the cached tokens as contiguous rows ----------------------------------
-// A thread per 16 codes of a row (blockIdx.y: sequence, blockIdx.z: K or V): 16 bytes and a
-// scale in, 32 or 64 bytes out. HBM-bound on what it writes.
+// A workgroup takes kGatherToks tokens of a sequence (blockIdx.y: sequence, blockIdx.z: K or V), a thread
+// 8 codes of a row at a time: 8 bytes and a scale in, 16 (or 32) bytes out, both whole lines over a wave,
+// kGatherUnroll of them in flight. HBM-bound on what it writes: 16 conversations of 2k to 16k tokens, int8 to
+// fp16, NNN us for 693 MB.
+constexpr int kGatherToks = 16;
+constexpr int kGatherUnroll = 4;
 struct Gather8Params {
   const char* k_pool;
   const char* v_pool;
@@ -144,39 +149,53 @@ struct Out16 {
 
 template <typename O, typename F, int D>
 __global__ void __launch_bounds__(256) gather_q8_kernel(Gather8Params p) {
-  constexpr int kChunks = D / 16;  // of one head's row
+  constexpr int kChunks = D / 8;  // of one head's row
+  typedef typename O::Elem E;
+  typedef E E8 __attribute__((ext_vector_type(8)));
   const int per_row = p.num_kv_heads * kChunks;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (int64_t)p.max_len * per_row) return;
-  const int t = (int)(i / per_row), c = (int)(i - (int64_t)t * per_row);
   const int b = blockIdx.y;
   const bool is_v = blockIdx.z != 0;
   const int p0 = p.indptr[b], np = p.indptr[b + 1] - p0;
   int lpl = p.last_len[b];
   lpl = lpl < 1 ? 1 : (lpl > p.page_size ? p.page_size : lpl);
   const int64_t len = np > 0 ? (int64_t)(np - 1) * p.page_size + lpl : 0;
-  typedef typename O::Elem E;
-  typedef E E8 __attribute__((ext_vector_type(8)));
-  E8 out[2] = {};
-  if (t < len) {
-    const int page = t / p.page_size, slot = t - page * p.page_size;
-    int pid = p.indices[p0 + page];
-    if (pid < 0 || (int64_t)pid >= p.num_pages) pid = 0;
-    const int h = c / kChunks;
-    const float s = (is_v ? p.v_scale : p.k_scale)[scale_index(pid, slot, p.blocks_per_page, p.num_kv_heads, h)];
-    const u32x4 w = *reinterpret_cast<const u32x4*>((is_v ? p.v_pool : p.k_pool) +
-                                                    (((int64_t)pid * p.page_size + slot) * per_row + c) * 16);
+  const int t0 = blockIdx.x * kGatherToks;
+  const int items = min(kGatherToks, p.max_len - t0) * per_row;
+  E8* dst = reinterpret_cast<E8*>(is_v ? p.v_out : p.k_out) + ((int64_t)b * p.max_len + t0) * per_row;
+  const float* scales = is_v ? p.v_scale : p.k_scale;
+  const char* pool = is_v ? p.v_pool : p.k_pool;
+  for (int j0 = threadIdx.x; j0 < items; j0 += 256 * kGatherUnroll) {
+    u32x2 w[kGatherUnroll];
+    float s[kGatherUnroll];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float f[4];
-      F::decode4(w[k], f);
+    for (int u = 0; u < kGatherUnroll; ++u) {
+      const int j = j0 + 256 * u;
+      w[u] = u32x2{0u, 0u};
+      s[u] = 0.f;
+      const int r = j / per_row, t = t0 + r, c = j - r * per_row;
+      if (j < items && t < len) {
+        const int page = t / p.page_size, slot = t - page * p.page_size;
+        int pid = p.indices[p0 + page];
+        if (pid < 0 || (int64_t)pid >= p.num_pages) pid = 0;
+        s[u] = scales[scale_index(pid, slot, p.blocks_per_page, p.num_kv_heads, c / kChunks)];
+        w[u] = *reinterpret_cast<const u32x2*>(pool + (((int64_t)pid * p.page_size + slot) * per_row + c) * 8);
+      }
+    }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) out[k / 2][4 * (k % 2) + j] = O::of(f[j] * s);
+    for (int u = 0; u < kGatherUnroll; ++u) {
+      const int j = j0 + 256 * u;
+      if (j >= items) break;
+      E8 out;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float f[4];
+        F::decode4(w[u][k], f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[4 * k + e] = O::of(f[e] * s[u]);
+      }
+      dst[j] = out;
     }
   }
-  E8* dst = reinterpret_cast<E8*>(is_v ? p.v_out : p.k_out) + 2 * ((int64_t)b * p.max_len * per_row + i);
-  dst[0] = out[0];
-  dst[1] = out[1];
 }
 
 template <typename T, typename F>
@@ -292,8 +311,7 @@ extern "C" int nslg_q8_gather_kv(const void* k_pool, const void* v_pool, const f
   if (batch == 0 || max_len == 0) return NSLG_OK;
   if (!k_out || !v_out) return fail(NSLG_EINVAL, "q8_gather_kv: null pointer");
   if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) return fail(NSLG_EINVAL, "q8_gather_kv: outputs must be 16-byte aligned");
-  const int64_t work = ((int64_t)max_len * num_kv_heads * (head_dim / 16) + 255) / 256;
-  if (work > 0x7fffffff) return fail(NSLG_EUNSUPPORTED, "q8_gather_kv: too many rows");
+  const int64_t work = ((int64_t)max_len + kGatherToks - 1) / kGatherToks;
   Gather8Params p;
   p.k_pool = (const char*)k_pool;
   p.v_pool = (const char*)v_pool;

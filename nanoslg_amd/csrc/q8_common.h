@@ -132,30 +132,43 @@ __device__ inline void transpose4x4(const uint32_t (&r)[4], uint32_t (&c)[4]) {
 // Largest of the lanes' values (bit patterns of non-negative floats), and whether any lane's flag is set.
 __device__ inline uint32_t wave_max_bits(uint32_t x) { return (uint32_t)wave_max_i32((int)x); }
 
-// One wave writes rows a .. a + cnt - 1 (1 <= cnt, a + cnt <= 16) of one block of one KV head
-// and sets the block's scale. row(i, e) gives elements e .. e + 7 of the block's row i (a u16x8
-// of T), for new rows only. `codes`: the block's row 0 at this head, rows row_bytes apart.
+// A wave's new rows of one block of one KV head: each lane holds 8 elements of one row, 512 / D rows a
+// step. They stay in registers between the maximum and the rounding, so they are read once.
+template <int D>
+struct BlockRows {
+  static constexpr int kLanes = D / 8;
+  static constexpr int kRows = 64 / kLanes;
+  static constexpr int kIters = kBlockToks / kRows;
+  u16x8 x[kIters];
+};
+
+// row(i, e) gives elements e .. e + 7 of the block's row i (a u16x8 of T), for new rows only.
+template <int D, typename Row>
+__device__ inline void load_block_rows(BlockRows<D>& b, int a, int cnt, Row row) {
+  const int lane = threadIdx.x & 63;
+  const int i0 = lane / b.kLanes, e = 8 * (lane % b.kLanes);
+#pragma unroll
+  for (int it = 0; it < b.kIters; ++it) {
+    const int i = b.kRows * it + i0;
+    b.x[it] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    if (i >= a && i < a + cnt) b.x[it] = row(i, e);
+  }
+}
+
+// One wave writes its rows a .. a + cnt - 1 (1 <= cnt, a + cnt <= 16) of one block of one KV head
+// and sets the block's scale. `codes`: the block's row 0 at this head, rows row_bytes apart.
 //
 // A block written from its first row takes the scale its new rows need. Otherwise the scale
 // is the larger of its own and that one, and where it grew the rows 0 .. a - 1 are rounded
 // to it; rows past a + cnt - 1 (of no token) are left as they are.
-// Each lane holds 8 elements of one row, 512 / D rows a step; the rows stay in registers
-// between the maximum and the rounding, so they are read once.
-template <typename T, typename F, int D, typename Row>
-__device__ inline void write_block(char* codes, int64_t row_bytes, float* scale_ptr, int a, int cnt, Row row) {
-  constexpr int kLanes = D / 8;
-  constexpr int kRows = 64 / kLanes;
-  constexpr int kIters = kBlockToks / kRows;
+template <typename T, typename F, int D>
+__device__ inline void write_block(const BlockRows<D>& rows, char* codes, int64_t row_bytes, float* scale_ptr, int a,
+                                   int cnt) {
+  constexpr int kLanes = BlockRows<D>::kLanes, kRows = BlockRows<D>::kRows, kIters = BlockRows<D>::kIters;
   const int lane = threadIdx.x & 63;
   const int i0 = lane / kLanes, e = 8 * (lane % kLanes);
   const float old = a > 0 ? *scale_ptr : 0.f;
-  u16x8 x[kIters];
-#pragma unroll
-  for (int it = 0; it < kIters; ++it) {
-    const int i = kRows * it + i0;
-    x[it] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
-    if (i >= a && i < a + cnt) x[it] = row(i, e);
-  }
+  const auto& x = rows.x;
   uint32_t amax = 0;
   bool bad = false;
 #pragma unroll
@@ -206,7 +219,7 @@ __device__ inline void write_block(char* codes, int64_t row_bytes, float* scale_
   if (lane == 0) *scale_ptr = scale;
 }
 
-// Token `pos` of a page run: its block's scale index within the sequence's page `pos / ps`.
+// Index of the scale of slot `slot` of page pid at head h.
 __device__ inline int64_t scale_index(int64_t pid, int slot, int nb, int num_kv_heads, int h) {
   return (pid * nb + slot / kBlockToks) * num_kv_heads + h;
 }

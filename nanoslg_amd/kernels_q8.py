@@ -23,24 +23,24 @@ CODE_DTYPES = {torch.float8_e4m3fn: _lib.NSLG_E4M3, torch.int8: _lib.NSLG_INT8}
 HEAD_DIMS_Q8 = (64, 128, 256)
 
 
-def blocks_per_page(page_size: int) -> int:
-    return -(-page_size // BLOCK_TOKENS)
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-class _on_device:
-    """The tensors' device as the current one (the library launches on the current device)."""
+def _one_device(*ts: torch.Tensor) -> int:
+    """The index of the one GPU that all tensors are on."""
+    d = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != d or d < 0:
+            _require_gpu(*ts)  # raises its error
+    return d
 
-    def __init__(self, t: torch.Tensor):
-        self.index = t.get_device()
-        self.prev = torch.cuda.current_device()
 
-    def __enter__(self):
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.prev != self.index:
-            torch.cuda.set_device(self.prev)
+def _call(device: int, fn, *args) -> int:
+    """An entry point with the tensors' device as the current one (the library launches on the current device)."""
+    if _CURRENT_DEVICE() == device:
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
 
 
 def _layer(what: str, k_layer, v_layer, k_scale, v_scale):
@@ -51,10 +51,10 @@ def _layer(what: str, k_layer, v_layer, k_scale, v_scale):
     if code is None:
         raise TypeError(f"{what}: codes must be float8_e4m3fn or int8 (got {k_layer.dtype})")
     P, ps, Hkv, D = k_layer.shape
-    shape = (P, blocks_per_page(ps), Hkv)
+    shape = (P, -(-ps // BLOCK_TOKENS), Hkv)
     if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
         raise TypeError(f"{what}: scales must be float32")
-    if tuple(k_scale.shape) != shape or tuple(v_scale.shape) != shape:
+    if k_scale.shape != shape or v_scale.shape != shape:
         raise ValueError(f"{what}: scales must be {list(shape)}, one for each block of {BLOCK_TOKENS} slots and head")
     if not (k_layer.is_contiguous() and v_layer.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
         raise ValueError(f"{what}: the cache layer must be contiguous")
@@ -83,9 +83,14 @@ def _row_type(what: str, *ts) -> int:
 
 def _new_rows(what: str, t: torch.Tensor, name: str, n: int, Hkv: int, D: int) -> Tuple[torch.Tensor, int]:
     """The rows of k_new / v_new at one 16-byte stride (others are copied) and the stride."""
-    if t.dim() < 2 or tuple(t.shape[-2:]) != (Hkv, D):
+    shape = t.shape
+    if len(shape) < 2 or shape[-1] != D or shape[-2] != Hkv:
         raise ValueError(f"{what}: {name} must hold rows of [{Hkv}, {D}]")
-    rows, stride, _ = _rows(t, name)
+    if t.is_contiguous():  # a model's own rows
+        stride = Hkv * D
+        rows = t.numel() // stride
+    else:
+        rows, stride, _ = _rows(t, name)
     if rows != n:
         raise ValueError(f"{what}: {rows} rows of {name} for {n}")
     if t.data_ptr() % 16 or stride % 8 or stride < Hkv * D:
@@ -106,7 +111,7 @@ def append_kv_q8(k_new: torch.Tensor, v_new: torch.Tensor, qo_indptr: torch.Tens
     if the block holds earlier tokens, the larger of that and its own, to which their codes are then
     rounded. Codes are rounded to nearest even. Values that are not finite: float8_e4m3fn
     stores NaN; int8 makes the block's scale NaN until the block is written from its start."""
-    _require_gpu(k_new, v_new, qo_indptr, k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len)
+    dev = _one_device(k_layer, v_layer, k_scale, v_scale, k_new, v_new, qo_indptr, kv_indptr, kv_indices, kv_last_page_len)
     P, ps, Hkv, D, code = _layer("append_kv_q8", k_layer, v_layer, k_scale, v_scale)
     B = _table("append_kv_q8", kv_indptr, kv_indices, kv_last_page_len)
     _i32(qo_indptr, "qo_indptr")
@@ -122,11 +127,10 @@ def append_kv_q8(k_new: torch.Tensor, v_new: torch.Tensor, qo_indptr: torch.Tens
         n = B * int(grid_width)
     k_new, ks = _new_rows("append_kv_q8", k_new, "k_new", n, Hkv, D)
     v_new, vs = _new_rows("append_kv_q8", v_new, "v_new", n, Hkv, D)
-    with _on_device(k_layer):
-        rc = _lib.load().nslg_q8_append_kv(
-            k_new.data_ptr(), ks, v_new.data_ptr(), vs, qo_indptr.data_ptr(), None if q_rows is None else q_rows.data_ptr(),
-            int(grid_width), total_q, k_layer.data_ptr(), v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, ps,
-            kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), B, Hkv, D, dt, code, _stream(k_layer))
+    rc = _call(dev, _lib.fast_q8().append_kv, k_new.data_ptr(), ks, v_new.data_ptr(), vs, qo_indptr.data_ptr(),
+               None if q_rows is None else q_rows.data_ptr(), int(grid_width), total_q, k_layer.data_ptr(),
+               v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, ps, kv_indptr.data_ptr(),
+               kv_indices.data_ptr(), kv_last_page_len.data_ptr(), B, Hkv, D, dt, code, _stream(k_layer))
     _lib.check(rc, "nslg_q8_append_kv")
 
 
@@ -135,18 +139,16 @@ def gather_kv_q8(k_layer: torch.Tensor, v_layer: torch.Tensor, k_scale: torch.Te
                  dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
     """The cached tokens' values (code * scale, rounded once) as contiguous [B, max_len, Hkv, D] K
     and V of `dtype` (float16, bfloat16 or float32), zeros past each length."""
-    _require_gpu(k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len)
+    dev = _one_device(k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len)
     P, ps, Hkv, D, code = _layer("gather_kv_q8", k_layer, v_layer, k_scale, v_scale)
     B = _table("gather_kv_q8", kv_indptr, kv_indices, kv_last_page_len)
     if dtype not in _DTYPE_CODE:
         raise TypeError(f"gather_kv_q8: unsupported dtype {dtype}")
     k_out = torch.empty((B, int(max_len), Hkv, D), dtype=dtype, device=k_layer.device)
     v_out = torch.empty_like(k_out)
-    with _on_device(k_layer):
-        rc = _lib.load().nslg_q8_gather_kv(
-            k_layer.data_ptr(), v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, ps, kv_indptr.data_ptr(),
-            kv_indices.data_ptr(), kv_last_page_len.data_ptr(), B, int(max_len), Hkv, D, code, _DTYPE_CODE[dtype],
-            k_out.data_ptr(), v_out.data_ptr(), _stream(k_layer))
+    rc = _call(dev, _lib.fast_q8().gather_kv, k_layer.data_ptr(), v_layer.data_ptr(), k_scale.data_ptr(),
+               v_scale.data_ptr(), P, ps, kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), B,
+               int(max_len), Hkv, D, code, _DTYPE_CODE[dtype], k_out.data_ptr(), v_out.data_ptr(), _stream(k_layer))
     _lib.check(rc, "nslg_q8_gather_kv")
     return k_out, v_out
 
@@ -208,7 +210,7 @@ def rotate_rows(q, k_new, v_new, positions, cos, sin):
 
 def _decode8(what, q, k_new, v_new, rope, k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len,
              total_pages, sm_scale, out, workspace, groups, layout):
-    _require_gpu(q, k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len)
+    dev = _one_device(q, k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len)
     P, ps, Hkv, D, code = _layer(what, k_layer, v_layer, k_scale, v_scale)
     B = _table(what, kv_indptr, kv_indices, kv_last_page_len)
     if q.dim() != 3 or q.shape[0] != B or q.shape[2] != D or q.stride(2) != 1 or q.stride(1) != D:
@@ -226,7 +228,7 @@ def _decode8(what, q, k_new, v_new, rope, k_layer, v_layer, k_scale, v_scale, kv
     if k_new is None:
         dt = _row_type(what, q)
     else:
-        _require_gpu(q, k_new, v_new)
+        _one_device(q, k_new, v_new)
         dt = _row_type(what, q, k_new, v_new)
         if ps % BLOCK_TOKENS:
             # a block may lie in two waves' work: the rows go in ahead
@@ -252,18 +254,22 @@ def _decode8(what, q, k_new, v_new, rope, k_layer, v_layer, k_scale, v_scale, kv
             raise ValueError(f"{what}: one group slot per sequence")
         grp = (groups.seq_group_slot.data_ptr(), groups.num_groups, groups.prefix_pages_np.ctypes.data,
                groups.members_np.ctypes.data)
-    lib = _lib.load()
     scale = (1.0 / math.sqrt(D)) if sm_scale is None else float(sm_scale)
-    with _on_device(q):
-        need = int(lib.nslg_q8_paged_decode_workspace_size(B, Hq, Hkv, D, int(total_pages), ps, dt, code, grp[1]))
-        if groups is not None and need == 0:
-            raise ValueError(f"{what}: unsupported grouped decode shape")
-        ws = (workspace or Workspace(q.device)).get(need)
-        rc = lib.nslg_q8_paged_decode(
-            q.data_ptr(), q.stride(0), *rows, *tables, k_layer.data_ptr(), v_layer.data_ptr(), k_scale.data_ptr(),
+    total_pages = int(total_pages)
+    args = (q.data_ptr(), q.stride(0), *rows, *tables, k_layer.data_ptr(), v_layer.data_ptr(), k_scale.data_ptr(),
             v_scale.data_ptr(), P, ps, kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(),
-            int(total_pages), B, Hq, Hkv, D, scale, dt, code, *grp, out.data_ptr(), out.stride(0), ws.data_ptr(), ws.numel(),
-            layout, _stream(q))
+            total_pages, B, Hq, Hkv, D, scale, dt, code, *grp, out.data_ptr(), out.stride(0))
+    stream = _stream(q)
+    fn = _lib.fast_q8().paged_decode
+    rc = _lib.NSLG_EWORKSPACE
+    if workspace is not None:  # a kept workspace mostly suffices: the call itself says if it does not
+        ws = workspace.buf
+        rc = _call(dev, fn, *args, ws.data_ptr(), ws.numel(), layout, stream)
+    if rc == _lib.NSLG_EWORKSPACE:
+        need = int(_call(dev, _lib.load().nslg_q8_paged_decode_workspace_size, B, Hq, Hkv, D, total_pages, ps, dt, code,
+                         grp[1]))
+        ws = (workspace or Workspace(q.device)).get(need)
+        rc = _call(dev, fn, *args, ws.data_ptr(), ws.numel(), layout, stream)
     _lib.check(rc, "nslg_q8_paged_decode")
     return out
 
@@ -277,7 +283,7 @@ def paged_prefill_q8(q: torch.Tensor, qo_indptr: torch.Tensor, total_q: int, max
     """Causal (bottom-right) prefill attention over an 8-bit cache layer that holds the new tokens too
     (append_kv_q8 first): ``kernels.paged_prefill`` with its arguments. max_kv: the longest
     sequence's keys, where the caller knows it (it decides whether keys are cut into runs)."""
-    _require_gpu(q, qo_indptr, k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len)
+    dev = _one_device(q, qo_indptr, k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len)
     P, ps, Hkv, D, code = _layer("paged_prefill_q8", k_layer, v_layer, k_scale, v_scale)
     B = _table("paged_prefill_q8", kv_indptr, kv_indices, kv_last_page_len)
     _i32(qo_indptr, "qo_indptr")
@@ -303,13 +309,12 @@ def paged_prefill_q8(q: torch.Tensor, qo_indptr: torch.Tensor, total_q: int, max
     if max_kv is None:  # the average sequence's table stands for the longest one (its length is on the device)
         max_kv = kv_indices.numel() * ps // max(B, 1)
     scale = (1.0 / math.sqrt(D)) if sm_scale is None else float(sm_scale)
-    with _on_device(q):
-        ws, ws_ptr, ws_bytes = _prefill_workspace(q, B, Hq, D, total_q, int(max_q), max_kv, workspace)
-        rc = _lib.load().nslg_q8_paged_prefill(
-            q.data_ptr(), q.stride(0), qo_indptr.data_ptr(), None if q_rows is None else q_rows.data_ptr(), int(grid_width),
-            total_q, int(max_q), k_layer.data_ptr(), v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, ps,
-            kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), B, Hq, Hkv, D, scale, dt, code,
-            out.data_ptr(), out.stride(0), ws_ptr, ws_bytes, _stream(q))
+    ws, ws_ptr, ws_bytes = _prefill_workspace(q, B, Hq, D, total_q, int(max_q), max_kv, workspace)
+    rc = _call(dev, _lib.fast_q8().paged_prefill, q.data_ptr(), q.stride(0), qo_indptr.data_ptr(),
+               None if q_rows is None else q_rows.data_ptr(), int(grid_width), total_q, int(max_q), k_layer.data_ptr(),
+               v_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, ps, kv_indptr.data_ptr(),
+               kv_indices.data_ptr(), kv_last_page_len.data_ptr(), B, Hq, Hkv, D, scale, dt, code, out.data_ptr(),
+               out.stride(0), ws_ptr, ws_bytes, _stream(q))
     _lib.check(rc, "nslg_q8_paged_prefill")
     return out
 
@@ -338,6 +343,7 @@ class DecodeLaunchQ8(DecodeLaunch):
         if num_qo_heads % self.Hkv:
             raise ValueError(f"DecodeLaunchQ8: Hq={num_qo_heads} is not a multiple of Hkv={self.Hkv}")
         self.lib = _lib.load()
+        self._f_decode8 = _lib.fast_q8().paged_decode
         self.device, self.dev_index, self.dtype = k_pool.device, k_pool.get_device(), k_pool.dtype
         self.Hq = num_qo_heads
         self.kp0, self.vp0, self.ksp0, self.vsp0 = (t.data_ptr() for t in (k_pool, v_pool, k_scale, v_scale))
@@ -378,10 +384,8 @@ class DecodeLaunchQ8(DecodeLaunch):
                         groups.members_np.ctypes.data)
         # sized for some headroom, as in DecodeLaunch; f16 and bf16 calls may both come
         bound = self.total_pages + max(self.total_pages // 4, 1024)
-        with _on_device(self.pools[0]):
-            need = max(int(self.lib.nslg_q8_paged_decode_workspace_size(B, self.Hq, self.Hkv, self.D, bound, self.ps, dt,
-                                                                        self.q8, self.grp[1]))
-                       for dt in (_lib.NSLG_F16, _lib.NSLG_BF16))
+        need = max(int(_call(self.dev_index, self.lib.nslg_q8_paged_decode_workspace_size, B, self.Hq, self.Hkv, self.D, bound,
+                             self.ps, dt, self.q8, self.grp[1])) for dt in (_lib.NSLG_F16, _lib.NSLG_BF16))
         if groups is not None and need == 0:
             raise ValueError("DecodeLaunchQ8: unsupported grouped decode shape")
         self.ws = self.workspace.get(need)
@@ -433,10 +437,9 @@ class DecodeLaunchQ8(DecodeLaunch):
             lay = next(_LAYOUT_TAGS)
             self._layout = -lay
         off, soff = layer * self.layer_bytes, layer * self.scale_bytes
-        with _on_device(q):
-            rc = self.lib.nslg_q8_paged_decode(
-                q.data_ptr(), q.stride(0), *rows, *tables, self.kp0 + off, self.vp0 + off, self.ksp0 + soff, self.vsp0 + soff,
-                self.P, self.ps, *self.table_ptrs, self.total_pages, B, Hq, Hkv, D, self.scale, dt, self.q8, *self.grp,
-                out.data_ptr(), Hq * D, self.ws.data_ptr(), self.ws.numel(), lay, _stream(q))
+        rc = _call(di, self._f_decode8, q.data_ptr(), q.stride(0), *rows, *tables, self.kp0 + off, self.vp0 + off,
+                   self.ksp0 + soff, self.vsp0 + soff, self.P, self.ps, *self.table_ptrs, self.total_pages, B, Hq, Hkv, D,
+                   self.scale, dt, self.q8, *self.grp, out.data_ptr(), Hq * D, self.ws.data_ptr(), self.ws.numel(), lay,
+                   _stream(q))
         _lib.check(rc, "nslg_q8_paged_decode")
         return out

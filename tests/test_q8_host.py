@@ -186,3 +186,23 @@ def test_pool_of_an_8_bit_cache():
     c = ContiguousKVCache(KVCacheConfig(num_layers=1, num_kv_heads=2, num_qo_heads=4, head_dim=64, max_batch_size=2, max_seq_len=100,
                                         backend="contiguous", cache_dtype="fp8"), kernels=fake_kernels)
     assert c.k.dtype == torch.float8_e4m3fn and c.pools.v_scale.shape == (1, 2, 7, 2)
+
+
+def test_fast_binding_of_the_8_bit_entry_points():
+    """_nslg_fast_q8 calls the same C functions as ctypes, with the types of their declarations."""
+    import re
+    from ctypes import c_float, c_int32, c_int64, c_size_t, c_void_p
+    from pathlib import Path
+    L = _lib()
+    lib, fast = L.load(), L.fast_q8()
+    assert fast.append_kv(*append_args(code=2)) == lib.nslg_q8_append_kv(*append_args(code=2)) == -1
+    assert fast.gather_kv(*gather_args(d=80)) == -2 and fast.paged_prefill(*prefill_args(dt=2)) == -2
+    assert fast.paged_decode(*decode_args()) == L.NSLG_EWORKSPACE
+    with pytest.raises(TypeError):
+        fast.append_kv(*append_args()[:-1])
+    code = {c_void_p: "p", c_int64: "q", c_int32: "i", c_size_t: "z", c_float: "f"}
+    src = (Path(__file__).resolve().parent.parent / "nanoslg_amd" / "csrc" / "fastcall_q8.c").read_text()
+    found = re.findall(r'parse\("(\w+)", "(\w+)"', src)
+    assert len(found) == 4
+    for fn, sig in found:
+        assert sig == "".join(code[t] for t in L.SIGNATURES["nslg_" + fn][1]), fn
