@@ -30,17 +30,19 @@
 //
 // HBM traffic per (token, kv head): 2*D*2 bytes (K and V, read once).
 //
-// 8-bit pools (F = E4M3, Int8): the same work units, softmax and merge; a tile's codes become
-// 16-bit operands in registers.
-//   K: lane l loads token l%16, 16 codes at d = 64 i + 16 (l/16): the 32-wide steps 2i and 2i + 1 of
-//     QK take d = 64 i + 16 (l/16) + 0..7 and + 8..15, an order of the contraction that the Q
-//     operand is loaded in too, so no lane needs another lane's codes. The codes are operands
-//     as they are (exact in 16 bits); the block's scale multiplies the fp32 scores.
-//   V: lane l loads tokens 4(l/16)+j, D/16 codes each, as above; 4 x 4 bytes are transposed (8
-//     byte permutes) into one word per output tile, then converted with half the block's scale
-//     (a value may round up to 65536, past half's range) and the result is doubled at the end.
-//   On pages that are multiples of 16 a tile is one block: its two scales are scalars, from a
-//   window of 64 tiles' page ids and scales held one per lane.
+// 8-bit pools (F = E4M3, Int8): the same work units, softmax and merge; codes become 16-bit operands in
+// registers. On pages that are multiples of 16 a tile is one block, and two tiles are taken at once (32
+// tokens: half the softmax reductions, and P.V on the full-rate 16x16x32 MFMA):
+//   K: loaded as whole rows (16 codes a lane) and turned through the wave's LDS stage, so that lane l holds
+//     token l%16, 16 codes at d = 64 i + 16 (l/16): the 32-wide steps 2i and 2i + 1 of QK take d = 64 i + 16
+//     (l/16) + 0..7 and + 8..15, an order of the contraction that the Q operand is loaded in too. The codes are
+//     operands as they are (exact in 16 bits); the block's scale multiplies the fp32 scores.
+//   V: lane l loads tokens 4(l/16)+j of each tile, D/16 codes each, as above; 4 x 4 bytes are transposed (8
+//     byte permutes) into one word per output tile, then converted with half the block's scale (a
+//     value may round up to 65536, past half's range) and the result is doubled at the end.
+//   The two scales of a block are scalars, from a window of 64 tiles' page ids and scales held one per lane;
+//   row offsets are lane constants but for the chunk's last tile.
+// Other page sizes take 16 tokens at a time, each lane resolving its tokens' pages and scales.
 #pragma once
 
 #include "nslg_common.h"
@@ -433,14 +435,15 @@ struct WordsOf<64> {
   };
 };
 
-// 16 tokens of one block: K as operands need it, V as D/16 codes of 4 tokens per lane.
+// 16 tokens of one block: K as whole rows (D = 64: as the operands need it, which is whole rows too), V as
+// D/16 codes of 4 tokens per lane.
 template <int D>
 struct Tile8 {
   u32x4 k[D / 64];
   typename WordsOf<D>::type v[4];
   float ks, vs;  // wave-uniform
 };
-// 16 tokens of any blocks: the scales of tokens 4 (l/16) + j.
+// 16 tokens of any blocks: K as the operands need it; the scales of tokens 4 (l/16) + j.
 template <int D>
 struct Tile8Any {
   u32x4 k[D / 64];
@@ -456,20 +459,63 @@ __device__ inline typename WordsOf<D>::type v8_load(const char* p) {
     return kv_load<typename WordsOf<D>::type, kStream>(p);
 }
 
-// Rows of a tile that lies in one page; rows past `last` repeat row `last`.
-template <int D, bool kStream>
-__device__ inline void load_tile8_rows(const char* kbase, const char* vbase, int row_bytes, int last, Tile8<D>& t) {
+// Loads of one tile, whose rows are consecutive in one page, from the tile's first row (wave-uniform) and
+// the lane's offsets ko, vo (offsets8). All 16 rows are read: those past the chunk's end are the page's, and
+// are masked (K) or zeroed (V) where they are used.
+//   K, D >= 128: load i takes tokens (1024 / D) i + l / (D/16), 16 codes at d = 16 (l % (D/16))
+//   K, D = 64:   token l%16, 16 codes at d = 16 (l/16)
+//   V:           tokens 4 (l/16) + j, D/16 codes at d = (D/16) (l%16)
+template <int D>
+__device__ inline void offsets8(int row_bytes, uint32_t& ko, uint32_t& vo) {
   const int lane = threadIdx.x & 63;
-  const int r = lane & 15;
-  const int gq = lane >> 4;
-  const char* kp = kbase + (r < last ? r : last) * row_bytes + 16 * gq;
+  constexpr int kLanesPerTok = D / 16;
+  ko = D == 64 ? (lane & 15) * row_bytes + 16 * (lane >> 4)
+               : lane / kLanesPerTok * row_bytes + 16 * (lane % kLanesPerTok);
+  vo = 4 * (lane >> 4) * row_bytes + D / 16 * (lane & 15);
+}
+
+template <int D, bool kStream>
+__device__ inline void load_tile8_rows(const char* kbase, const char* vbase, uint32_t row_bytes, uint32_t ko, uint32_t vo,
+                                       Tile8<D>& t) {
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) t.k[i] = kv_load<u32x4, kStream>(kp + 64 * i);
+  for (int i = 0; i < D / 64; ++i)
+    t.k[i] = kv_load<u32x4, kStream>(kbase + (uint64_t)(i * (1024 / D) * row_bytes) + ko);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int vr = 4 * gq + j;
-    t.v[j] = v8_load<D, kStream>(vbase + (vr < last ? vr : last) * row_bytes + D / 16 * r);
+  for (int j = 0; j < 4; ++j) t.v[j] = v8_load<D, kStream>(vbase + (uint64_t)(j * row_bytes) + vo);
+}
+
+// Per-wave LDS stage of the K codes of two tiles (rows padded by 16 bytes: the 16-byte reads of 16 tokens hit
+// distinct banks).
+template <int D>
+struct KStage8 {
+  static constexpr int kPitch = D + 16;
+  char c[32 * kPitch];
+};
+
+// The K rows of two tiles into the stage; k8_operand then gives token l%16 of tile u, d = 64 i + 16 (l/16) .. + 15.
+template <int D>
+__device__ inline void k8_stage(KStage8<D>& st, const Tile8<D> (&t)[2]) {
+  if constexpr (D > 64) {
+    constexpr int kLanesPerTok = D / 16, kTokPerLoad = 1024 / D, kPitch = KStage8<D>::kPitch;
+    const int lane = threadIdx.x & 63;
+    const int w = lane / kLanesPerTok * kPitch + 16 * (lane % kLanesPerTok);
+    // (one wave's LDS operations complete in order; the fences are for the compiler, as in k_operands_from_rows)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i)
+        *reinterpret_cast<u32x4*>(&st.c[(16 * u + kTokPerLoad * i) * kPitch + w]) = t[u].k[i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
+}
+
+template <int D>
+__device__ inline u32x4 k8_operand(const KStage8<D>& st, const Tile8<D> (&t)[2], int u, int i) {
+  if constexpr (D == 64) return t[u].k[0];
+  const int lane = threadIdx.x & 63;
+  constexpr int kPitch = KStage8<D>::kPitch;
+  return *reinterpret_cast<const u32x4*>(&st.c[(16 * u + (lane & 15)) * kPitch + 16 * (lane >> 4) + 64 * i]);
 }
 
 // Each lane resolving its own tokens' pages and blocks (page sizes that 16 does not divide).
@@ -527,8 +573,13 @@ __device__ inline void write_new_row8(const DecodeParams& p, int b, int h, int p
   write_block<T, F, D>(vrow, reinterpret_cast<char*>(const_cast<uint16_t*>(p.v_pool)) + at, row_bytes, p.v_scale + blk, a, 1);
 }
 
+// Waves per SIMD that the registers are held to: what the tile buffers and accumulators of the 8-bit kernels
+// leave room for (without it the compiler widens codes early and loses a wave).
+template <int D, typename F>
+constexpr int kMinWaves = !F::kQ8 ? 1 : D == 64 ? 4 : D == 128 ? 3 : 2;
+
 template <typename T, int D, bool kTileInPage, int kDepth, bool kGrouped, typename F>
-__global__ void __launch_bounds__(64 * kMaxWaves)
+__global__ void __launch_bounds__(64 * kMaxWaves, (kMinWaves<D, F>))
 paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
   constexpr int kSteps = D / 32;
   constexpr int NT = D / 16;
@@ -759,9 +810,8 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
   // K tiles of the page-aligned path arrive as rows (head dims up to 128) and are
   // turned into operands in LDS
   __shared__ KStage<D> k_stage[kTileInPage && kKRows<D> && !F::kQ8 ? kMaxWaves : 1];
-  // Probabilities of one tile from its scores (log2 units): the running maximum and sum.
-  auto softmax_tile = [&](const float (&sv)[4], u16x4& pb, u16x4& pb_lo) {
-    float mx = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
+  // The running maximum raised to take in mx, the largest of a lane's new scores (log2 units).
+  auto raise_max = [&](float mx) {
     mx = rows_max(mx);
     if (__ballot(mx > m_run + kRescaleSlack)) {
       const float m_new = fmaxf(m_run, mx);
@@ -771,6 +821,10 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
       for (int n = 0; n < NT; ++n) o[n] *= alpha;
       m_run = m_new;
     }
+  };
+  // Probabilities of one tile from its scores: the running maximum and sum.
+  auto softmax_tile = [&](const float (&sv)[4], u16x4& pb, u16x4& pb_lo) {
+    raise_max(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])));
     float pj[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) pj[j] = fast_exp2(sv[j] - m_run);
@@ -810,46 +864,111 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
       if constexpr (kSplitP) o[n] = T::mma_k16(a, pb_lo, o[n]);
     }
   };
-  // The same on 8-bit codes (Tile8 or Tile8Any).
-  auto process8 = [&](const auto& cur, int t0) {
+  // The same on 8-bit codes of any blocks.
+  auto process_any8 = [&](const auto& cur, int t0) {  // (Tile8Any; generic: only compiled where it is called)
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < D / 64; ++i)
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
-        s = T::mma_k32(codes_to16<T, F>(u32x2{cur.k[i][2 * hh], cur.k[i][2 * hh + 1]}, 1.f), qb[2 * i + hh], s);
+        s = T::mma_k32(codes_as16<T, F>(u32x2{cur.k[i][2 * hh], cur.k[i][2 * hh + 1]}), qb[2 * i + hh], s);
     float sv[4];
-    const bool whole = t0 + 16 <= t_end;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (kTileInPage)
-        sv[j] = s[j] * (p.scale_log2 * cur.ks);
-      else
-        sv[j] = s[j] * (p.scale_log2 * cur.ks[j]);
-      if (!whole && t0 + 4 * gq + j >= t_end) sv[j] = -INFINITY;
-    }
+    for (int j = 0; j < 4; ++j) sv[j] = (t0 + 4 * gq + j < t_end) ? s[j] * (p.scale_log2 * cur.ks[j]) : -INFINITY;
     u16x4 pb, pb_lo;
     softmax_tile(sv, pb, pb_lo);
 #pragma unroll
     for (int m = 0; m < D / 64; ++m) {
-      u16x4 a[4];
-      if constexpr (kTileInPage) {
-        const uint32_t w[4] = {cur.v[0][m], cur.v[1][m], cur.v[2][m], cur.v[3][m]};
-        uint32_t c[4];
-        transpose4x4(w, c);
+      u16x4 x[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) a[n] = codes_to16<T, F>(c[n], 0.5f * cur.vs);
-      } else {
-        u16x4 x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = codes_to16<T, F>((uint32_t)cur.v[j][m], 0.5f * cur.vs[j]);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) a[n] = u16x4{x[0][n], x[1][n], x[2][n], x[3][n]};
+      for (int j = 0; j < 4; ++j) {
+        const u16x8 two = codes_to16<T, F>(u32x2{cur.v[j][m], 0u}, 0.5f * cur.vs[j]);
+        x[j] = __builtin_shufflevector(two, two, 0, 1, 2, 3);
       }
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        o[4 * m + n] = T::mma_k16(a[n], pb, o[4 * m + n]);
-        if constexpr (kSplitP) o[4 * m + n] = T::mma_k16(a[n], pb_lo, o[4 * m + n]);
+        const u16x4 a = {x[0][n], x[1][n], x[2][n], x[3][n]};
+        o[4 * m + n] = T::mma_k16(a, pb, o[4 * m + n]);
+        if constexpr (kSplitP) o[4 * m + n] = T::mma_k16(a, pb_lo, o[4 * m + n]);
+      }
+    }
+  };
+  // Two tiles of one block each, tokens t0 .. t0 + 31: lane l has tokens 4(l/16) + j of both.
+  __shared__ __attribute__((aligned(16))) KStage8<D> k_stage8[kTileInPage && F::kQ8 && D > 64 ? kMaxWaves : 1];
+  auto process8 = [&](auto& cur, int t0) {  // (Tile8[2])
+    KStage8<D>& st = k_stage8[D > 64 ? wave : 0];
+    k8_stage<D>(st, cur);
+    f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const u32x4 ka[2] = {k8_operand<D>(st, cur, 0, i), k8_operand<D>(st, cur, 1, i)};
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          s[u] = T::mma_k32(codes_as16<T, F>(u32x2{ka[u][2 * hh], ka[u][2 * hh + 1]}), qb[2 * i + hh], s[u]);
+      if constexpr (D == 256) __builtin_amdgcn_sched_barrier(0);  // the operands of one step at a time: registers
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");  // the stage's reads before the next pair's writes
+    float sv[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sv[4 * u + j] = s[u][j] * (p.scale_log2 * cur[u].ks);
+    if (t0 + 32 > t_end) {  // the chunk's last tiles: no score, and no code that might be NaN, past its end
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (t0 + 16 * (j >> 2) + 4 * gq + (j & 3) >= t_end) {
+          sv[j] = -INFINITY;
+          cur[j >> 2].v[j & 3] = {};
+        }
+    }
+    raise_max(fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7]))));
+    float pj[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) pj[j] = fast_exp2(sv[j] - m_run);
+    l_run += ((pj[0] + pj[1]) + (pj[2] + pj[3])) + ((pj[4] + pj[5]) + (pj[6] + pj[7]));
+    // V's scales (halved): in its codes' conversion, but for int8 in bf16, where the conversion has no product
+    // to put them in, on the probabilities (bf16 has fp32's range); for int8 in half a scale under
+    // 2^-24, which is no half, in both (the probabilities then lose 2^-25 of what is under 127 * 2^-24)
+    constexpr bool kScaleP = F::kNanScale && T::kDtype == NSLG_BF16;
+    float vs[2] = {0.5f * cur[0].vs, 0.5f * cur[1].vs};
+    if constexpr (kScaleP) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pj[j] *= vs[j >> 2];
+    } else if constexpr (F::kNanScale) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (vs[u] < 0x1p-24f) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) pj[4 * u + j] *= vs[u] * 0x1p24f;
+          vs[u] = 0x1p-24f;
+        }
+    }
+    u16x8 pb, pb_lo;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) pb[j] = T::from_f32(pj[j]);
+    if constexpr (kSplitP) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pb_lo[j] = T::from_f32(pj[j] - T::to_f32(pb[j]));
+    }
+#pragma unroll
+    for (int m = 0; m < D / 64; ++m) {
+      uint32_t c[2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t w[4] = {cur[u].v[0][m], cur[u].v[1][m], cur[u].v[2][m], cur[u].v[3][m]};
+        transpose4x4(w, c[u]);
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        u16x4 half[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          half[u] = kScaleP ? codes_as16<T, F>(c[u][n]) : codes_to16<T, F>(c[u][n], vs[u]);
+        const u16x8 a = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        o[4 * m + n] = T::mma_k32(a, pb, o[4 * m + n]);
+        if constexpr (kSplitP) o[4 * m + n] = T::mma_k32(a, pb_lo, o[4 * m + n]);
       }
     }
   };
@@ -861,11 +980,10 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
   const int n_tiles = (t_end - t_begin + 15) >> 4;
   auto pipeline = [&](auto stream_tag) {
     constexpr bool kStream = decltype(stream_tag)::value;
-    typename std::conditional<!F::kQ8, Tile<D>,
-                              typename std::conditional<kTileInPage, Tile8<D>, Tile8Any<D>>::type>::type buf[kDepth];
     if constexpr (F::kQ8 && kTileInPage) {
       // Every tile is one block of one page. The page ids and scales of a window of 64 tiles
       // sit one per lane; each tile's are broadcast to scalar registers (readlane).
+      Tile8<D> buf[kDepth][2];
       const int ps = p.page_size;
       const int tpp = ps >> 4;  // tiles (blocks) per page
       const int row_bytes = p.num_kv_heads * D;
@@ -888,7 +1006,8 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
       int sub = first % tpp;  // block of the next tile within its page
       const char* kb = kpool;
       const char* vb = vpool;
-      int last = 0;
+      uint32_t ko, vo, more = ~0u;
+      offsets8<D>(row_bytes, ko, vo);
       auto issue = [&](Tile8<D>& dst) {
         if (ld_tile < n_tiles) {
           if (ld_tile - win_base == 64) {
@@ -902,26 +1021,32 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
           const int64_t row0 = (int64_t)pid * ps + 16 * sub;
           kb = kpool + row0 * row_bytes;
           vb = vpool + row0 * row_bytes;
-          last = min(15, t_last - (t_begin + 16 * ld_tile));
           if (++sub == tpp) sub = 0;
           ++ld_tile;
         } else {
-          last = 0;  // past the chunk's end, as below
+          more = 0;  // past the chunk's end, as below: the last tile's first bytes, by every lane
+          dst.ks = dst.vs = 0.f;
         }
-        load_tile8_rows<D, kStream>(kb, vb, row_bytes, last, dst);
+        load_tile8_rows<D, kStream>(kb, vb, row_bytes & more, ko & more, vo & more, dst);
       };
+      auto issue2 = [&](Tile8<D> (&dst)[2]) {
+        issue(dst[0]);
+        issue(dst[1]);
+      };
+      const int n_pairs = (n_tiles + 1) >> 1;
 #pragma unroll
-      for (int j = 0; j < kDepth - 1; ++j) issue(buf[j]);
-      for (int i = 0; i < n_tiles; i += kDepth) {
+      for (int j = 0; j < kDepth - 1; ++j) issue2(buf[j]);
+      for (int i = 0; i < n_pairs; i += kDepth) {
 #pragma unroll
         for (int j = 0; j < kDepth; ++j) {
-          if (i + j >= n_tiles) break;
-          issue(buf[(j + kDepth - 1) % kDepth]);
+          if (i + j >= n_pairs) break;
+          issue2(buf[(j + kDepth - 1) % kDepth]);
           __builtin_amdgcn_sched_barrier(0);
-          process8(buf[j], t_begin + 16 * (i + j));
+          process8(buf[j], t_begin + 32 * (i + j));
         }
       }
     } else if constexpr (F::kQ8) {
+      Tile8Any<D> buf[kDepth];
       auto issue_any = [&](int tile, Tile8Any<D>& dst) {
         load_tile8_any<D, kStream>(p, idx, h, t_begin + 16 * min(tile, n_tiles - 1), t_last, dst);
       };
@@ -933,10 +1058,11 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
           if (i + j >= n_tiles) break;
           issue_any(i + j + kDepth - 1, buf[(j + kDepth - 1) % kDepth]);
           __builtin_amdgcn_sched_barrier(0);
-          process8(buf[j], t_begin + 16 * (i + j));
+          process_any8(buf[j], t_begin + 16 * (i + j));
         }
       }
     } else if constexpr (kTileInPage) {
+      Tile<D> buf[kDepth];
       // Every tile lies inside one page. The ids of a window of 128 pages sit one per
       // lane in two registers and each tile's id is broadcast to a scalar register
       // (readlane), so page lookups never wait behind the K/V loads in flight; a chunk
@@ -1002,6 +1128,7 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
         }
       }
     } else {
+      Tile<D> buf[kDepth];
       const int head_off = h * D;
       auto issue_any = [&](int tile, Tile<D>& dst) {
         load_tile_any<D, kStream>(p, idx, head_off, t_begin + 16 * min(tile, n_tiles - 1), t_last, dst);
@@ -1264,10 +1391,10 @@ constexpr int64_t kStreamBytes = (int64_t)128 << 20;
 // The first call of a variant on a device queries the device (attribute and
 // occupancy); a call whose stream is being captured into a graph must not make
 // those queries, so it returns 0 (refused) when the figure is not cached yet.
-// Tiles in flight per wave and one computed: 16-bit tiles of 16 tokens are 8 KB of K and V at
-// D = 128, 8-bit ones half of that.
+// Buffers of tiles: one computed, the others in flight. (16-bit tiles of 16 tokens and pairs of 8-bit ones
+// are 8 KB of K and V at D = 128.)
 template <typename F, bool kTileInPage>
-constexpr int kTileDepth = F::kQ8 && kTileInPage ? 4 : 2;
+constexpr int kTileDepth = 2;
 
 template <typename T, int D, bool kTileInPage, bool kGrouped, typename F>
 int decode_wg_slots(int waves, const CaptureCheck& cc) {

@@ -17,6 +17,7 @@ constexpr int kBlockToks = 16;  // tokens of a block (the last block of a page m
 // The pool holds the 16-bit elements themselves.
 struct Raw16 {
   static constexpr bool kQ8 = false;
+  static constexpr bool kNanScale = false;
   static constexpr int kBytes = 2;  // of an element
 };
 
@@ -78,9 +79,42 @@ struct Int8 {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-// Four codes times `scale` (a power of two) as 16-bit elements of type T. Every product is
-// exact in T where it is a normal number of T.
+// Four codes as 16-bit elements of type T, exactly.
 template <typename T, typename F>
+__device__ inline u16x4 codes_as16(uint32_t w) {
+  u32x2 r;
+  if constexpr (!F::kNanScale && T::kDtype == NSLG_F16) {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true));
+  } else if constexpr (!F::kNanScale) {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true));
+  } else if constexpr (T::kDtype == NSLG_F16) {
+    // 0x6400 | u is the half 1024 + u: with u = code + 128, minus 1152 gives the code
+    const uint32_t u = w ^ 0x80808080u;
+    const f16x2 off = {(_Float16)1152.f, (_Float16)1152.f};
+    const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u));
+    const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
+    r[0] = __builtin_bit_cast(uint32_t, a - off);
+    r[1] = __builtin_bit_cast(uint32_t, b - off);
+  } else {  // 8 significant bits hold a code: the upper half of its fp32 value is exact
+    float f[4];
+    F::decode4(w, f);
+    r[0] = __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302u);
+    r[1] = __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x07060302u);
+  }
+  return __builtin_bit_cast(u16x4, r);
+}
+
+template <typename T, typename F>
+__device__ inline u16x8 codes_as16(u32x2 w) {
+  const u16x4 a = codes_as16<T, F>(w[0]), b = codes_as16<T, F>(w[1]);
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Four codes times `scale` (a power of two; NaN gives NaN) as 16-bit elements of type T, exact wherever the
+// product is a normal number of T. kSmall: int8 codes in half with a scale under 2^-24, which is no half.
+template <typename T, typename F, bool kSmall = false>
 __device__ inline u16x4 codes_to16(uint32_t w, float scale) {
   u32x2 r;
   if constexpr (T::kDtype == NSLG_F16 && !F::kNanScale) {
@@ -89,33 +123,38 @@ __device__ inline u16x4 codes_to16(uint32_t w, float scale) {
   } else if constexpr (T::kDtype == NSLG_BF16 && !F::kNanScale) {
     r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
     r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true));
-  } else if (T::kDtype == NSLG_F16 && !(scale < 0x1p-24f)) {
-    // 0x6400 | u is the half 1024 + u: with u = code + 128, minus 1152 gives the code
-    const uint32_t u = w ^ 0x80808080u;
+  } else if constexpr (T::kDtype == NSLG_F16 && !kSmall) {
     const _Float16 s = (_Float16)scale;
-    const f16x2 off = {(_Float16)1152.f, (_Float16)1152.f}, ss = {s, s};
-    const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u));
-    const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
-    r[0] = __builtin_bit_cast(uint32_t, (a - off) * ss);
-    r[1] = __builtin_bit_cast(uint32_t, (b - off) * ss);
+    const f16x2 ss = {s, s};
+    const u16x4 c = codes_as16<T, F>(w);
+    const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_shufflevector(c, c, 0, 1));
+    const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_shufflevector(c, c, 2, 3));
+    r[0] = __builtin_bit_cast(uint32_t, lo * ss);
+    r[1] = __builtin_bit_cast(uint32_t, hi * ss);
   } else {
-    const uint32_t u = w ^ 0x80808080u;
     float f[4];
+    F::decode4(w, f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = fmaf((float)((u >> (8 * i)) & 0xffu), scale, -128.f * scale);
-    if constexpr (T::kDtype == NSLG_BF16) {  // 8 significant bits hold the product: its upper half is exact
+    for (int i = 0; i < 4; ++i) f[i] *= scale;
+    if constexpr (T::kDtype == NSLG_BF16) {
       r[0] = __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302u);
       r[1] = __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x07060302u);
-    } else {  // below half's range: rounded into its subnormals
+    } else {  // rounded into half's subnormals
       return u16x4{T::from_f32(f[0]), T::from_f32(f[1]), T::from_f32(f[2]), T::from_f32(f[3])};
     }
   }
   return __builtin_bit_cast(u16x4, r);
 }
 
+// Eight codes, any power of two as the scale.
 template <typename T, typename F>
 __device__ inline u16x8 codes_to16(u32x2 w, float scale) {
-  const u16x4 a = codes_to16<T, F>(w[0], scale), b = codes_to16<T, F>(w[1], scale);
+  u16x4 a, b;
+  if (F::kNanScale && T::kDtype == NSLG_F16 && scale < 0x1p-24f) {
+    a = codes_to16<T, F, true>(w[0], scale), b = codes_to16<T, F, true>(w[1], scale);
+  } else {
+    a = codes_to16<T, F>(w[0], scale), b = codes_to16<T, F>(w[1], scale);
+  }
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 

@@ -419,3 +419,36 @@ def test_side_stream_and_graph_replays():
         assert torch.equal(static, want)
         assert torch.equal(K().paged_decode_q8(q, *c.layer, *c.table, c.total_pages, workspace=ws), want)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("page", [16, 20])
+def test_attention_at_the_ends_of_the_scales(code, dtype, page):
+    """Blocks with scales from under half's range to its largest values (a code may stand for 65536), next to each
+    other; and bf16's."""
+    c = Cache(17, code, page, 2, 128, [70, 33, 200], dtype)
+    top = 65504.0 if dtype == "fp16" else 1e30
+    for name in "kv":
+        lay, codes, scale = c.side[name]
+        # K small enough for finite scores; V anything
+        exps = np.array([-40, -33, -26, -24, -20, -10, 0, 5] if name == "v" else [-40, -30, -24, -9])
+        s = np.ldexp(1.0, c.g.choice(exps, lay.scale.shape))
+        if name == "v":
+            big = c.g.random(s.shape) < 0.25
+            s = np.where(big, Q.need_scale(top, code), s)
+        lay.scale[:] = s
+        scale.copy_(torch.from_numpy(s).float())
+    if dtype == "fp16":  # the largest half rounds up to 65536 in e4m3 and int8
+        for lay, codes, _ in (c.side["v"],):
+            x = np.minimum(np.abs(lay.values * lay.scale.repeat(16, 1)[:, :page, :, None]), 65536) / lay.scale.repeat(
+                16, 1)[:, :page, :, None] * np.sign(lay.values)
+            lay.values[:] = Q.round_code(x, code)
+            codes.copy_(torch.from_numpy(lay.values).float().to(CODE[code]))
+    B = len(c.lens)
+    q = torch.randn(B, 8, 128, device=DEV).to(DT[dtype])
+    out = K().paged_decode_q8(q, *c.layer, *c.table, c.total_pages)
+    pre = K().paged_prefill_q8(q, i32(range(B + 1)), B, 1, *c.layer, *c.table)
+    for b in range(B):
+        for o in (out, pre):
+            check(c, o[b:b + 1], q[b:b + 1], b)
