@@ -651,9 +651,13 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
       // Grouped calls merge each member's own partials with its group prefix's, so
       // longer chunks pay there sooner: t_all / 64 (16 requests on a 2040-token
       // prefix: 25.0 -> 22.4 us per call; t_all / 48 the same as / 64).
-      constexpr int64_t kLoDiv = kGrouped ? 64 : 96;
+      // 8-bit pools, half the bytes a token: t_all / 128, at most 192 tokens (with / 96 and 256: 32
+      // sequences of 1k-3k tokens 35.1 -> 38.8 us, 16 of 700-6000 at D = 256 29.9 -> 32.0, 4 of 1k-4k 15.2 ->
+      // 16.1, 16 of 256-8191 28.2 -> 27.8; at most 160: 35.4, 34.7, 15.3, 30.1).
+      constexpr int64_t kLoDiv = kGrouped ? 64 : F::kQ8 ? 128 : 96;
+      constexpr int64_t kLoMax = F::kQ8 && !kGrouped ? 192 : 256;
       int64_t lo = ((t_all / kLoDiv + 15) / 16) * 16;
-      lo = lo < 64 ? 64 : (lo > 256 ? 256 : lo);
+      lo = lo < 64 ? 64 : (lo > kLoMax ? kLoMax : lo);
       hi = hi < lo ? lo : (hi > ((int64_t)1 << 30) ? ((int64_t)1 << 30) : hi);
       ct = fit_chunk_tokens<kGrouped>(p, ga, lens, (int)lo, (int)hi, p.chunk_budget);
     }
@@ -893,6 +897,14 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
       }
     }
   };
+  // (D = 256: the Q operand, 32 registers, is read back from LDS step by step; held, the loop spilled: 36 us a call of
+  // 16 conversations of 700 to 6000 tokens, 42 with spills)
+  constexpr bool kQInLds = F::kQ8 && kTileInPage && D == 256;
+  __shared__ u16x8 q_stage[kQInLds ? kMaxWaves : 1][kQInLds ? kSteps : 1][kQInLds ? 64 : 1];
+  if constexpr (kQInLds) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) q_stage[wave][s][lane] = qb[s];  // (each lane reads its own)
+  }
   // Two tiles of one block each, tokens t0 .. t0 + 31: lane l has tokens 4(l/16) + j of both.
   __shared__ __attribute__((aligned(16))) KStage8<D> k_stage8[kTileInPage && F::kQ8 && D > 64 ? kMaxWaves : 1];
   auto process8 = [&](auto& cur, int t0) {  // (Tile8[2])
@@ -903,10 +915,16 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
     for (int i = 0; i < D / 64; ++i) {
       const u32x4 ka[2] = {k8_operand<D>(st, cur, 0, i), k8_operand<D>(st, cur, 1, i)};
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh)
+      for (int hh = 0; hh < 2; ++hh) {
+        u16x8 qs;
+        if constexpr (kQInLds)
+          qs = q_stage[wave][2 * i + hh][lane];
+        else
+          qs = qb[2 * i + hh];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-          s[u] = T::mma_k32(codes_as16<T, F>(u32x2{ka[u][2 * hh], ka[u][2 * hh + 1]}), qb[2 * i + hh], s[u]);
+          s[u] = T::mma_k32(codes_as16<T, F>(u32x2{ka[u][2 * hh], ka[u][2 * hh + 1]}), qs, s[u]);
+      }
       if constexpr (D == 256) __builtin_amdgcn_sched_barrier(0);  // the operands of one step at a time: registers
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");  // the stage's reads before the next pair's writes
