@@ -307,12 +307,15 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
   // Each half (kKeys / 2 keys) is fetched into registers and stashed into the next LDS
   // stage at its own point of the current tile, so only one half's staging registers
   // are live at a time.
-  constexpr int kChunks = D / 8;                             // 16 B chunks per row
+  // (8-bit pools at D >= 128: a thread moves 16 codes, so that the page, slot and scale of a key are found by
+  // half as many threads: 8 x 512 tokens over 3584, e4m3, NNN -> MMM us)
+  constexpr int kElems = F::kQ8 && D > 64 ? 16 : 8;          // elements of a row that a thread moves at a time
+  constexpr int kChunks = D / kElems;
   constexpr int kHalf = kKeys / 2;
   constexpr int kPerThreadH = kHalf * kChunks / kThreads;    // D=128: 2 (8 waves) or 4 (4 waves)
-  typedef typename std::conditional<F::kQ8, u32x2, u32x4>::type Staged;  // 8 elements of a row
+  typedef typename std::conditional<F::kQ8 && kElems == 8, u32x2, u32x4>::type Staged;
   Staged kreg[kPerThreadH], vreg[kPerThreadH];
-  float kscale[kPerThreadH], vscale[kPerThreadH];  // 8-bit pools: half the keys' scales
+  float kscale[kPerThreadH], vscale[kPerThreadH];  // 8-bit pools: the keys' scales
   int win_base = -1;
 
   auto load_pages = [&](int first_key) {
@@ -330,8 +333,9 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
     }
     win_base = pg0;
   };
-  // thread tid moves 16-byte chunk tid % kChunks of keys tid / kChunks + (kThreads / kChunks) i
-  const int f_ch16 = (tid % kChunks) * 16;
+  // thread tid moves chunk tid % kChunks (at byte f_ch16 of a row in 16 bits) of keys tid / kChunks +
+  // (kThreads / kChunks) i
+  const int f_ch16 = (tid % kChunks) * 2 * kElems;
   const int f_key = tid / kChunks;
   const bool ps_pow2 = (ps & (ps - 1)) == 0;
   const int ps_shift = __builtin_ctz((unsigned)ps);
@@ -352,9 +356,11 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
       kreg[i] = *reinterpret_cast<const Staged*>(kpool + off);
       vreg[i] = *reinterpret_cast<const Staged*>(vpool + off);
       if constexpr (F::kQ8) {
-        const int64_t at = scale_index(pid, slot, p.blocks_per_page, p.num_kv_heads, h);
-        kscale[i] = 0.5f * p.k_scale[at];
-        vscale[i] = 0.5f * p.v_scale[at];
+        // (pid * blocks + block is below 2^31, checked by the host)
+        const uint64_t at = (uint64_t)(pid * (uint32_t)p.blocks_per_page + (uint32_t)slot / kBlockToks) *
+                                (uint32_t)p.num_kv_heads + (uint32_t)h;
+        kscale[i] = p.k_scale[at];
+        vscale[i] = p.v_scale[at];
       }
   };
   auto fetch_half = [&](int kt, int half) {
@@ -389,8 +395,15 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
     for (int i = 0; i < kPerThreadH; ++i) {
       const int key = half * kHalf + f_key + (kThreads / kChunks) * i;
       if constexpr (F::kQ8) {
-        *reinterpret_cast<u16x8*>(&k_lds[stage][key * kPitch + f_ch16 / 2]) = codes_to16<T, F>(kreg[i], kscale[i]);
-        *reinterpret_cast<u16x8*>(&v_lds[stage][key * kVPitch + f_ch16 / 2]) = codes_to16<T, F>(vreg[i], vscale[i]);
+        uint16_t* kd = &k_lds[stage][key * kPitch + f_ch16 / 2];
+        uint16_t* vd = &v_lds[stage][key * kVPitch + f_ch16 / 2];
+        const float ks = 0.5f * kscale[i], vs = 0.5f * vscale[i];
+#pragma unroll
+        for (int e = 0; e < kElems / 8; ++e) {
+          const u32x2 kw = {kreg[i][2 * e], kreg[i][2 * e + 1]}, vw = {vreg[i][2 * e], vreg[i][2 * e + 1]};
+          *reinterpret_cast<u16x8*>(kd + 8 * e) = codes_to16<T, F>(kw, ks);
+          *reinterpret_cast<u16x8*>(vd + 8 * e) = codes_to16<T, F>(vw, vs);
+        }
       } else {
         *reinterpret_cast<u32x4*>(&k_lds[stage][key * kPitch + f_ch16 / 2]) = kreg[i];
         *reinterpret_cast<u32x4*>(&v_lds[stage][key * kVPitch + f_ch16 / 2]) = vreg[i];
@@ -664,7 +677,7 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
     }
     // this tile's own keys go out after the next tile's loads have been waited for (the
     // wait counter covers stores too), under the page-id window of this tile
-    const bool own_tile = kt * kKeys + kKeys > own_lo && kt * kKeys < own_hi;  // uniform
+    const bool own_tile = !F::kQ8 && kt * kKeys + kKeys > own_lo && kt * kKeys < own_hi;  // uniform
     if (staged) {
       if (!half1_done) {
         stash_half(stage ^ 1, 0);
