@@ -116,10 +116,11 @@ __global__ void __launch_bounds__(256) append_q8_kernel(Append8Params p) {
 // ---- gather: the cached tokens as contiguous rows ----------------------------------
 // A workgroup takes kGatherToks tokens of a sequence (blockIdx.y: sequence, blockIdx.z: K or V), a thread
 // 8 codes of a row at a time: 8 bytes and a scale in, 16 (or 32) bytes out, both whole lines over a wave,
-// kGatherUnroll of them in flight. HBM-bound on what it writes: 16 conversations of 2k to 16k tokens, int8 to
-// fp16, NNN us for 693 MB.
+// kGatherUnroll of them in flight (2 or 8: the same). HBM-bound: 16 conversations of 2k to 16k tokens, int8 to fp16,
+// 232 MB of codes in and 727 MB out (past the lengths too), 174 us.
 constexpr int kGatherToks = 16;
 constexpr int kGatherUnroll = 4;
+constexpr int64_t kGatherStreamBytes = (int64_t)128 << 20;  // larger outputs go out past the caches: 188 -> 174 us
 struct Gather8Params {
   const char* k_pool;
   const char* v_pool;
@@ -147,7 +148,7 @@ struct Out16 {
   __device__ static inline unsigned short of(float x) { return T::from_f32(x); }
 };
 
-template <typename O, typename F, int D>
+template <typename O, typename F, int D, bool kStream>
 __global__ void __launch_bounds__(256) gather_q8_kernel(Gather8Params p) {
   constexpr int kChunks = D / 8;  // of one head's row
   typedef typename O::Elem E;
@@ -193,7 +194,10 @@ __global__ void __launch_bounds__(256) gather_q8_kernel(Gather8Params p) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[4 * k + e] = O::of(f[e] * s[u]);
       }
-      dst[j] = out;
+      if constexpr (kStream)
+        stream_store(dst + j, out);
+      else
+        dst[j] = out;
     }
   }
 }
@@ -207,12 +211,20 @@ void launch_append(const Append8Params& p, int head_dim, dim3 grid, hipStream_t 
   }
 }
 
+template <typename O, typename F, int D>
+void launch_gather_d(const Gather8Params& p, int64_t out_bytes, dim3 grid, hipStream_t s) {
+  if (out_bytes > kGatherStreamBytes)
+    gather_q8_kernel<O, F, D, true><<<grid, 256, 0, s>>>(p);
+  else
+    gather_q8_kernel<O, F, D, false><<<grid, 256, 0, s>>>(p);
+}
+
 template <typename O, typename F>
-void launch_gather(const Gather8Params& p, int head_dim, dim3 grid, hipStream_t s) {
+void launch_gather(const Gather8Params& p, int head_dim, int64_t out_bytes, dim3 grid, hipStream_t s) {
   switch (head_dim) {
-    case 64: gather_q8_kernel<O, F, 64><<<grid, 256, 0, s>>>(p); break;
-    case 128: gather_q8_kernel<O, F, 128><<<grid, 256, 0, s>>>(p); break;
-    default: gather_q8_kernel<O, F, 256><<<grid, 256, 0, s>>>(p); break;
+    case 64: return launch_gather_d<O, F, 64>(p, out_bytes, grid, s);
+    case 128: return launch_gather_d<O, F, 128>(p, out_bytes, grid, s);
+    default: return launch_gather_d<O, F, 256>(p, out_bytes, grid, s);
   }
 }
 
@@ -327,15 +339,16 @@ extern "C" int nslg_q8_gather_kv(const void* k_pool, const void* v_pool, const f
   p.num_kv_heads = num_kv_heads;
   p.k_out = k_out;
   p.v_out = v_out;
+  const int64_t out_bytes = 2 * (int64_t)batch * max_len * num_kv_heads * head_dim * elem_bytes(dtype);
   const dim3 grid((unsigned)work, (unsigned)batch, 2);
   hipStream_t s = as_stream(stream);
   if (dtype == NSLG_F16)
-    code == NSLG_E4M3 ? launch_gather<Out16<F16>, E4M3>(p, head_dim, grid, s)
-                      : launch_gather<Out16<F16>, Int8>(p, head_dim, grid, s);
+    code == NSLG_E4M3 ? launch_gather<Out16<F16>, E4M3>(p, head_dim, out_bytes, grid, s)
+                      : launch_gather<Out16<F16>, Int8>(p, head_dim, out_bytes, grid, s);
   else if (dtype == NSLG_BF16)
-    code == NSLG_E4M3 ? launch_gather<Out16<BF16>, E4M3>(p, head_dim, grid, s)
-                      : launch_gather<Out16<BF16>, Int8>(p, head_dim, grid, s);
+    code == NSLG_E4M3 ? launch_gather<Out16<BF16>, E4M3>(p, head_dim, out_bytes, grid, s)
+                      : launch_gather<Out16<BF16>, Int8>(p, head_dim, out_bytes, grid, s);
   else
-    code == NSLG_E4M3 ? launch_gather<OutF32, E4M3>(p, head_dim, grid, s) : launch_gather<OutF32, Int8>(p, head_dim, grid, s);
+    code == NSLG_E4M3 ? launch_gather<OutF32, E4M3>(p, head_dim, out_bytes, grid, s) : launch_gather<OutF32, Int8>(p, head_dim, out_bytes, grid, s);
   return check_launch("q8_gather_kv");
 }

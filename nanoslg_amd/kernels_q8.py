@@ -29,9 +29,13 @@ _CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.curre
 def _one_device(*ts: torch.Tensor) -> int:
     """The index of the one GPU that all tensors are on."""
     d = ts[0].get_device()
-    for t in ts:
-        if t.get_device() != d or d < 0:
-            _require_gpu(*ts)  # raises its error
+    if d >= 0:
+        for t in ts:
+            if t.get_device() != d:
+                break
+        else:
+            return d
+    _require_gpu(*ts)  # raises its error
     return d
 
 
@@ -45,17 +49,18 @@ def _call(device: int, fn, *args) -> int:
 
 def _layer(what: str, k_layer, v_layer, k_scale, v_scale):
     """(P, page_size, Hkv, D, code) of a cache layer."""
-    if k_layer.dim() != 4 or k_layer.shape != v_layer.shape or k_layer.dtype != v_layer.dtype:
+    shape, dtype = k_layer.shape, k_layer.dtype
+    if len(shape) != 4 or shape != v_layer.shape or dtype != v_layer.dtype:
         raise ValueError(f"{what}: codes must be [P, page_size, Hkv, D] for both K and V")
-    code = CODE_DTYPES.get(k_layer.dtype)
+    code = CODE_DTYPES.get(dtype)
     if code is None:
-        raise TypeError(f"{what}: codes must be float8_e4m3fn or int8 (got {k_layer.dtype})")
-    P, ps, Hkv, D = k_layer.shape
-    shape = (P, -(-ps // BLOCK_TOKENS), Hkv)
+        raise TypeError(f"{what}: codes must be float8_e4m3fn or int8 (got {dtype})")
+    P, ps, Hkv, D = shape
+    scales = (P, -(-ps // BLOCK_TOKENS), Hkv)
     if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
         raise TypeError(f"{what}: scales must be float32")
-    if k_scale.shape != shape or v_scale.shape != shape:
-        raise ValueError(f"{what}: scales must be {list(shape)}, one for each block of {BLOCK_TOKENS} slots and head")
+    if k_scale.shape != scales or v_scale.shape != scales:
+        raise ValueError(f"{what}: scales must be {list(scales)}, one for each block of {BLOCK_TOKENS} slots and head")
     if not (k_layer.is_contiguous() and v_layer.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
         raise ValueError(f"{what}: the cache layer must be contiguous")
     return P, ps, Hkv, D, code
@@ -63,20 +68,26 @@ def _layer(what: str, k_layer, v_layer, k_scale, v_scale):
 
 def _table(what: str, kv_indptr, kv_indices, kv_last_page_len) -> int:
     """The batch size of a block table."""
-    _i32(kv_indptr, "kv_indptr")
-    _i32(kv_indices, "kv_indices")
-    _i32(kv_last_page_len, "kv_last_page_len")
+    i32 = torch.int32
+    if not (kv_indptr.dtype is i32 and kv_indices.dtype is i32 and kv_last_page_len.dtype is i32 and kv_indptr.is_contiguous()
+            and kv_indices.is_contiguous() and kv_last_page_len.is_contiguous()):
+        for t, n in ((kv_indptr, "kv_indptr"), (kv_indices, "kv_indices"), (kv_last_page_len, "kv_last_page_len")):
+            _i32(t, n)
     B = kv_indptr.numel() - 1
     if B < 0 or kv_last_page_len.numel() < B:
         raise ValueError(f"{what}: kv_indptr must have B+1 entries and kv_last_page_len B")
     return B
 
 
-def _row_type(what: str, *ts) -> int:
-    code = _DTYPE_CODE.get(ts[0].dtype)
-    if code not in (_lib.NSLG_F16, _lib.NSLG_BF16):
-        raise TypeError(f"{what}: float16 or bfloat16 rows (got {ts[0].dtype})")
-    if any(t.dtype != ts[0].dtype for t in ts):
+_ROW_TYPES = {torch.float16: _lib.NSLG_F16, torch.bfloat16: _lib.NSLG_BF16}
+
+
+def _row_type(what: str, q, k_new=None, v_new=None) -> int:
+    dtype = q.dtype
+    code = _ROW_TYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"{what}: float16 or bfloat16 rows (got {dtype})")
+    if (k_new is not None and k_new.dtype is not dtype) or (v_new is not None and v_new.dtype is not dtype):
         raise TypeError(f"{what}: q, k_new and v_new must share one dtype")
     return code
 
@@ -144,8 +155,7 @@ def gather_kv_q8(k_layer: torch.Tensor, v_layer: torch.Tensor, k_scale: torch.Te
     B = _table("gather_kv_q8", kv_indptr, kv_indices, kv_last_page_len)
     if dtype not in _DTYPE_CODE:
         raise TypeError(f"gather_kv_q8: unsupported dtype {dtype}")
-    k_out = torch.empty((B, int(max_len), Hkv, D), dtype=dtype, device=k_layer.device)
-    v_out = torch.empty_like(k_out)
+    k_out, v_out = torch.empty((2, B, int(max_len), Hkv, D), dtype=dtype, device=k_layer.device).unbind(0)
     rc = _call(dev, _lib.fast_q8().gather_kv, k_layer.data_ptr(), v_layer.data_ptr(), k_scale.data_ptr(),
                v_scale.data_ptr(), P, ps, kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), B,
                int(max_len), Hkv, D, code, _DTYPE_CODE[dtype], k_out.data_ptr(), v_out.data_ptr(), _stream(k_layer))
@@ -219,7 +229,7 @@ def _decode8(what, q, k_new, v_new, rope, k_layer, v_layer, k_scale, v_scale, kv
     if Hq % Hkv:
         raise ValueError(f"{what}: Hq={Hq} is not a multiple of Hkv={Hkv}")
     if out is None:
-        out = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
+        out = q.new_empty((B, Hq, D))
     elif (out.shape != (B, Hq, D) or out.stride(2) != 1 or out.stride(1) != D or out.dtype != q.dtype
           or out.get_device() != q.get_device()):
         raise ValueError(f"{what}: bad out tensor")
@@ -260,7 +270,7 @@ def _decode8(what, q, k_new, v_new, rope, k_layer, v_layer, k_scale, v_scale, kv
             v_scale.data_ptr(), P, ps, kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(),
             total_pages, B, Hq, Hkv, D, scale, dt, code, *grp, out.data_ptr(), out.stride(0))
     stream = _stream(q)
-    fn = _lib.fast_q8().paged_decode
+    fn = (_lib._fast_q8 or _lib.fast_q8()).paged_decode
     rc = _lib.NSLG_EWORKSPACE
     if workspace is not None:  # a kept workspace mostly suffices: the call itself says if it does not
         ws = workspace.buf
@@ -302,7 +312,7 @@ def paged_prefill_q8(q: torch.Tensor, qo_indptr: torch.Tensor, total_q: int, max
         if q_rows.numel() < total_q or grid_width < 1 or T != B * grid_width:
             raise ValueError("paged_prefill_q8: a grid of B x grid_width rows of q and one q_rows entry per token")
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+        out = q.new_empty((T, Hq, D))
     elif (out.shape != (T, Hq, D) or out.stride(2) != 1 or out.stride(1) != D or out.dtype != q.dtype
           or out.get_device() != q.get_device()):
         raise ValueError("paged_prefill_q8: out must be shaped like q")
@@ -431,7 +441,7 @@ class DecodeLaunchQ8(DecodeLaunch):
                 if cos.data_ptr() % 16 or sin.data_ptr() % 16 or cos.stride(0) % 4:
                     cos, sin = (t[:, :D].clone(memory_format=torch.contiguous_format) for t in (cos, sin))
                 tables = (pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0])
-        out = torch.empty(out_shape, dtype=q.dtype, device=self.device)
+        out = q.new_empty(out_shape)
         lay = self._layout  # < 0: read the layout recorded under tag -lay
         if lay == 0:  # the first call on this plan records its chunk layout
             lay = next(_LAYOUT_TAGS)
