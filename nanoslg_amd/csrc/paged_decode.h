@@ -947,8 +947,9 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
     for (int j = 0; j < 8; ++j) pj[j] = fast_exp2(sv[j] - m_run);
     l_run += ((pj[0] + pj[1]) + (pj[2] + pj[3])) + ((pj[4] + pj[5]) + (pj[6] + pj[7]));
     // V's scales (halved): in its codes' conversion, but for int8 in bf16, where the conversion has no product
-    // to put them in, on the probabilities (bf16 has fp32's range); for int8 in half a scale under
-    // 2^-24, which is no half, in both (the probabilities then lose 2^-25 of what is under 127 * 2^-24)
+    // to put them in, on the probabilities (bf16 has fp32's range); for int8 in half what is past the
+    // conversion's scales on the probabilities too (at most 2^4; or, under 2^-24, where values are under 127 *
+    // 2^-24 and a probability's lost 2^-25 is nothing)
     constexpr bool kScaleP = F::kNanScale && T::kDtype == NSLG_BF16;
     float vs[2] = {0.5f * cur[0].vs, 0.5f * cur[1].vs};
     if constexpr (kScaleP) {
@@ -957,10 +958,11 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
     } else if constexpr (F::kNanScale) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        if (vs[u] < 0x1p-24f) {
+        if (vs[u] < kHalfScaleMin || vs[u] > kHalfScaleMax) {
+          const float to = vs[u] < kHalfScaleMin ? kHalfScaleMin : kHalfScaleMax;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) pj[4 * u + j] *= vs[u] * 0x1p24f;
-          vs[u] = 0x1p-24f;
+          for (int j = 0; j < 4; ++j) pj[4 * u + j] *= vs[u] / to;
+          vs[u] = to;
         }
     }
     u16x8 pb, pb_lo;

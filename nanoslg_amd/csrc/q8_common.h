@@ -112,9 +112,12 @@ __device__ inline u16x8 codes_as16(u32x2 w) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// Scales that codes_to16 takes as they are for int8 codes in half: a half themselves, and 1152 times them too.
+constexpr float kHalfScaleMin = 0x1p-24f, kHalfScaleMax = 32.f;
+
 // Four codes times `scale` (a power of two; NaN gives NaN) as 16-bit elements of type T, exact wherever the
-// product is a normal number of T. kSmall: int8 codes in half with a scale under 2^-24, which is no half.
-template <typename T, typename F, bool kSmall = false>
+// product is a normal number of T. kWide: int8 codes in half with a scale past the two above.
+template <typename T, typename F, bool kWide = false>
 __device__ inline u16x4 codes_to16(uint32_t w, float scale) {
   u32x2 r;
   if constexpr (T::kDtype == NSLG_F16 && !F::kNanScale) {
@@ -123,14 +126,15 @@ __device__ inline u16x4 codes_to16(uint32_t w, float scale) {
   } else if constexpr (T::kDtype == NSLG_BF16 && !F::kNanScale) {
     r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
     r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true));
-  } else if constexpr (T::kDtype == NSLG_F16 && !kSmall) {
-    const _Float16 s = (_Float16)scale;
-    const f16x2 ss = {s, s};
-    const u16x4 c = codes_as16<T, F>(w);
-    const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_shufflevector(c, c, 0, 1));
-    const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_shufflevector(c, c, 2, 3));
-    r[0] = __builtin_bit_cast(uint32_t, lo * ss);
-    r[1] = __builtin_bit_cast(uint32_t, hi * ss);
+  } else if constexpr (T::kDtype == NSLG_F16 && !kWide) {
+    // as in codes_as16: (1152 + code) * scale - 1152 * scale, every step exact
+    const uint32_t u = w ^ 0x80808080u;
+    const _Float16 s = (_Float16)scale, n = (_Float16)(-1152.f * scale);
+    const f16x2 ss = {s, s}, nn = {n, n};
+    const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u));
+    const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(a, ss, nn));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(b, ss, nn));
   } else {
     float f[4];
     F::decode4(w, f);
@@ -150,7 +154,7 @@ __device__ inline u16x4 codes_to16(uint32_t w, float scale) {
 template <typename T, typename F>
 __device__ inline u16x8 codes_to16(u32x2 w, float scale) {
   u16x4 a, b;
-  if (F::kNanScale && T::kDtype == NSLG_F16 && scale < 0x1p-24f) {
+  if (F::kNanScale && T::kDtype == NSLG_F16 && (scale < kHalfScaleMin || scale > kHalfScaleMax)) {
     a = codes_to16<T, F, true>(w[0], scale), b = codes_to16<T, F, true>(w[1], scale);
   } else {
     a = codes_to16<T, F>(w[0], scale), b = codes_to16<T, F>(w[1], scale);
