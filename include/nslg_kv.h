@@ -464,8 +464,10 @@ int nslg_paged_prefill_append(const void* q, int64_t q_stride, const int32_t* qo
  *   a new code is x / scale, rounded to nearest even.
  * So a stored value is within half a step of x for the rows written with the block's last scale,
  * and within one step (of that scale) for the others. Slots after the last token are left as
- * they are. A value that is not finite: e4m3 stores NaN for it; with int8 the block's scale
- * becomes NaN, and stays so until the block is written from its first slot again.
+ * they are. A token's value that is not finite, in K or in V, makes K NaN: with e4m3 codes of
+ * the token's row; with int8 the scale of the block's K, until the block is written from its
+ * first slot again. Queries that see the token (int8: a token of the block) then answer NaN, and
+ * no other does: V, whose weight 0 would not keep a NaN out, holds 0 in its place.
  *
  *   k_new, v_new    rows of Hkv*D elements at element strides, 16-byte aligned: row
  *                   qo_indptr[b] + t for token t of sequence b (total_q rows), or, with

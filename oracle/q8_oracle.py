@@ -13,6 +13,12 @@ BLOCK = 16
 MOST = {"e4m3": 448.0, "int8": 127.0}
 
 
+def write_kv(k, v, table, start, k_rows, v_rows):
+    """A sequence's new rows into layers k and v."""
+    k.write(table, start, k_rows, v_rows)
+    v.write(table, start, v_rows)
+
+
 def need_scale(amax: float, code: str) -> float:
     """Smallest power of two s >= 2^-126 with amax <= MOST * s; 0 for amax 0."""
     if amax == 0:
@@ -41,8 +47,11 @@ class Layer:
         self.values, self.scale, self.code = np.array(values, np.float64), np.array(scale, np.float64), code
         self.page = self.values.shape[1]
 
-    def write(self, table, start, rows):
-        """rows [n, Hkv, D] as the tokens at positions start .. start + n - 1 of a sequence with page table `table`."""
+    def write(self, table, start, rows, twin=None):
+        """rows [n, Hkv, D] as the tokens at positions start .. start + n - 1 of a sequence with page table `table`.
+        K is given V's rows as `twin`: a value that is not finite, in either, is K's to show (chunk by chunk of 8 elements
+        for V's); in V it is 0."""
+        is_k = twin is not None
         t, n = start, len(rows)
         while t < start + n:
             pid, slot = table[t // self.page], t % self.page
@@ -51,10 +60,14 @@ class Layer:
             for h in range(self.values.shape[2]):
                 x = np.asarray(rows[t - start:stop - start, h], np.float64)
                 fin = np.isfinite(x)
+                spoilt = np.zeros_like(fin)
+                if is_k:
+                    bad = ~np.isfinite(np.asarray(twin[t - start:stop - start, h], np.float64))
+                    spoilt = np.repeat(bad.reshape(len(x), -1, 8).any(2), 8, 1)
                 need = need_scale(float(np.abs(np.where(fin, x, 0)).max()), self.code)
                 old = float(self.scale[pid, blk, h]) if slot % BLOCK else 0.0
                 new = max(need, old)
-                if self.code == "int8" and (not fin.all() or math.isnan(old)):
+                if self.code == "int8" and is_k and (not fin.all() or spoilt.any() or math.isnan(old)):
                     new = math.nan
                 held = self.values[pid, BLOCK * blk:slot, h]
                 if slot % BLOCK and new > old:
@@ -64,8 +77,8 @@ class Layer:
                 else:
                     y = np.where(fin, x, 0) / new
                 y = round_code(y, self.code)
-                if self.code == "e4m3":
-                    y = np.where(fin, y, np.nan)
+                if self.code == "e4m3" and is_k:
+                    y = np.where(fin & ~spoilt, y, np.nan)
                 self.values[pid, slot:slot + stop - t, h] = y
                 self.scale[pid, blk, h] = new
             t = stop

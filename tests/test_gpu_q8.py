@@ -86,10 +86,9 @@ def append(c, new, kn, vn, grid=0, offs=None):
         rows = [[b * grid + offs[b] + t for t in range(n)] for b, n in enumerate(new)]
         kw = dict(q_rows=i32(sum(rows, []) or [0]), grid_width=grid)
     K().append_kv_q8(kn, vn, i32(qo), int(qo[-1]), *c.layer, *c.table, **kw)
-    for name, x in (("k", kn), ("v", vn)):
-        x = x.reshape(-1, c.hkv, c.d).cpu().double().numpy()
-        for b, n in enumerate(new):
-            c.side[name][0].write(c.tables[b], c.lens[b] - n, x[rows[b]])
+    k, v = (x.reshape(-1, c.hkv, c.d).cpu().double().numpy() for x in (kn, vn))
+    for b, n in enumerate(new):
+        Q.write_kv(c.side["k"][0], c.side["v"][0], c.tables[b], c.lens[b] - n, k[rows[b]], v[rows[b]])
 
 
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
@@ -165,20 +164,47 @@ def test_append_extremes(code, dtype):
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
 def test_append_values_that_are_not_finite(code, bad):
     c = Cache(6, code, 16, 2, 64, [20, 33, 20], "bf16")
-    x = c.rows(9)
-    x[1, 0, 3] = bad   # sequence 0: token 17, head 0
+    x, y = c.rows(9), c.rows(9)
+    x[1, 0, 3] = bad   # sequence 0: K of token 17, head 0
+    y[3, 1, 40] = bad  # V of token 19, head 1
     x[8, 1, 63] = bad  # sequence 2: its only new token, head 1
-    append(c, [4, 4, 1], x.to(DEV), c.rows(9).to(DEV))
+    append(c, [4, 4, 1], x.to(DEV), y.to(DEV))
     c.same()
-    k, _ = K().gather_kv_q8(*c.layer, *c.table, 33, torch.float32)
+    k, v = K().gather_kv_q8(*c.layer, *c.table, 33, torch.float32)
     want = [c.values("k", b) for b in range(3)]
     for b in range(3):
         np.testing.assert_array_equal(k[b, :c.lens[b]].cpu().double().numpy(), want[b])
-    assert np.isnan(want[0]).any() and not np.isnan(want[1]).any()
+    assert np.isnan(want[0][17, 0]).any() and np.isnan(want[0][19, 1]).any() and not np.isnan(want[1]).any()
+    assert not torch.isnan(v).any()
     # the block written from its first slot again is whole again
     append(c, [20, 33, 20], c.rows(73).to(DEV), c.rows(73).to(DEV))
     c.same()
     assert not torch.isnan(K().gather_kv_q8(*c.layer, *c.table, 33, torch.float32)[0]).any()
+
+
+@pytest.mark.parametrize("in_v", [False, True])
+@pytest.mark.parametrize("page", [16, 20])
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_only_queries_that_see_it_get_what_is_not_finite(code, page, in_v):
+    """A token that is not finite, in K or V: NaN for its own and later queries of that KV head, nothing for those before it
+    (int8: before its block)."""
+    n, at = 70, 50
+    c = Cache(18, code, page, 2, 128, [n, 40], "fp16")
+    kn, vn = c.rows(n), c.rows(n)
+    (vn if in_v else kn)[at, 1, 77] = math.inf
+    append(c, [n, 0], kn.to(DEV), vn.to(DEV))
+    c.same()
+    q = torch.randn(n, 8, 128, device=DEV).half()
+    out = K().paged_prefill_q8(q, i32([0, n, n]), n, n, *c.layer, *c.table)
+    first = at if code == "e4m3" else at - at % page % 16
+    assert torch.isnan(out[at:, 4:]).all()
+    assert torch.isfinite(out[:first, 4:]).all() and torch.isfinite(out[:, :4]).all()
+    c.side["k"][0].values[np.isnan(c.side["k"][0].values)] = 0
+    c.side["k"][0].scale[np.isnan(c.side["k"][0].scale)] = 0
+    want = Q.attend(q.cpu().double().numpy(), c.values("k", 0), c.values("v", 0), None, "fp16")
+    bound = Q.attention_bound(*want, n, "fp16")
+    off = np.abs(out.cpu().double().numpy() - want[0])
+    assert (off <= bound)[:first].all() and (off <= bound)[:, :4].all()
 
 
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
@@ -193,13 +219,12 @@ def test_append_skips_bad_pages_and_writes_nothing_else(code):
     qo = i32([0, 40, 60, 60])
     K().append_kv_q8(kn.to(DEV), kn.to(DEV), qo, T, *c.layer, *c.table)
     x = kn.double().numpy()
-    for name in "kv":
-        lay = c.side[name][0]
-        for b, (a, n) in enumerate(((0, 40), (40, 20))):
-            for p in range(-(-n // 16)):
-                pid = int(idx[(0, 3)[b] + p])
-                if 0 <= pid < c.P:
-                    lay.write({p: pid}, 16 * p, x[a + 16 * p:a + min(n, 16 * p + 16)])
+    for b, (a, n) in enumerate(((0, 40), (40, 20))):
+        for p in range(-(-n // 16)):
+            pid = int(idx[(0, 3)[b] + p])
+            if 0 <= pid < c.P:
+                r = x[a + 16 * p:a + min(n, 16 * p + 16)]
+                Q.write_kv(c.side["k"][0], c.side["v"][0], {p: pid}, 16 * p, r, r)
     c.same()
     assert len(before) == 4
 
@@ -265,8 +290,7 @@ def test_decode_append(code, dtype, page, d, hkv, group, lens):
         kn, vn = c.rows(B, scale), c.rows(B, scale)
         out = K().paged_decode_append_q8(q, kn.to(DEV)[:, None], vn.to(DEV)[:, None], *c.layer, *c.table, c.total_pages)
         for b in range(B):
-            c.side["k"][0].write(c.tables[b], lens[b] - 1, kn[b:b + 1].double().numpy())
-            c.side["v"][0].write(c.tables[b], lens[b] - 1, vn[b:b + 1].double().numpy())
+            Q.write_kv(c.side["k"][0], c.side["v"][0], c.tables[b], lens[b] - 1, kn[b:b + 1].double().numpy(), vn[b:b + 1].double().numpy())
         c.same()
         for b in range(B):
             check(c, out[b:b + 1], q[b:b + 1], b)
@@ -307,8 +331,7 @@ def test_decode_groups(code):
     kn, vn = c.rows(4, 20), c.rows(4, 20)
     out = K().paged_decode_append_q8(q, kn.to(DEV), vn.to(DEV), *c.layer, *c.table, c.total_pages, groups=grp)
     for b in range(4):
-        c.side["k"][0].write(c.tables[b], c.lens[b] - 1, kn[b:b + 1].double().numpy())
-        c.side["v"][0].write(c.tables[b], c.lens[b] - 1, vn[b:b + 1].double().numpy())
+        Q.write_kv(c.side["k"][0], c.side["v"][0], c.tables[b], c.lens[b] - 1, kn[b:b + 1].double().numpy(), vn[b:b + 1].double().numpy())
     c.same()
     for b in range(4):
         check(c, out[b:b + 1], q[b:b + 1], b)
@@ -388,8 +411,7 @@ def test_write_then_attend_as_a_forward_does():
             K().append_kv_q8(ks, vs, i32(qo), int(qo[-1]), *c.layer, *c.table)
             out = K().paged_prefill_q8(q, i32(qo), int(qo[-1]), max(step), *c.layer, *c.table, workspace=ws)
         for b in range(2):
-            c.side["k"][0].write(c.tables[b], done[b], kn[b][done[b]:now[b]].double().numpy())
-            c.side["v"][0].write(c.tables[b], done[b], vn[b][done[b]:now[b]].double().numpy())
+            Q.write_kv(c.side["k"][0], c.side["v"][0], c.tables[b], done[b], kn[b][done[b]:now[b]].double().numpy(), vn[b][done[b]:now[b]].double().numpy())
         c.same()
         for b in range(2):
             check(c, out[qo[b]:qo[b + 1]], q[qo[b]:qo[b + 1]], b)

@@ -57,8 +57,7 @@ def forward(mgr, twins, ids, new, g, dtype, offs=None, rope=None, spread=1.0, ch
         o = o.view(B, S, HQ, D).cpu().double().numpy()
         for b, sid in enumerate(ids):
             t, r = twins[sid], slice(offs[b], offs[b] + new[b])
-            for lay, x in zip(t.side[layer], (k, v)):
-                lay.write(t.table, t.len, x[b, r].double().numpy())
+            Q.write_kv(*t.side[layer], t.table, t.len, k[b, r].double().numpy(), v[b, r].double().numpy())
             pad = np.ones(S, bool)
             pad[r] = False
             assert not o[b, pad].any()
