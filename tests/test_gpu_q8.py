@@ -47,6 +47,11 @@ class Cache:
                     if n % page:
                         v[tab[-1], n % page:] = np.nan
                 v[order[at[-1]:]] = np.nan
+            if stale_nan:  # and so do the scales of blocks without a token
+                for tab, n in zip(self.tables, lens):
+                    if n % page:
+                        s[tab[-1], -(-(n % page) // 16):] = np.nan
+                s[order[at[-1]:]] = np.nan
             lay = Q.Layer(v, s, code)
             t = torch.from_numpy(v).float()
             t = t.to(CODE[code]) if code == "e4m3" else t.to(torch.int8)
@@ -474,3 +479,88 @@ def test_attention_at_the_ends_of_the_scales(code, dtype, page):
     for b in range(B):
         for o in (out, pre):
             check(c, o[b:b + 1], q[b:b + 1], b)
+
+
+def test_offsets_past_32_bits():
+    """Pages behind the first 2^32 bytes of a pool: what a small pool with the same pages gives, bit for bit."""
+    page, hkv, d, lens, new = 16, 8, 128, [50, 7, 200], [20, 1, 3]
+    far = 2 ** 32 // (page * hkv * d) + 40
+    g = torch.Generator().manual_seed(31)
+    npg = [-(-n // page) for n in lens]
+    n_pages = sum(npg)
+    near = torch.randperm(n_pages, generator=g)
+    indptr, last = i32(np.concatenate([[0], np.cumsum(npg)])), i32([n - page * (p - 1) for n, p in zip(lens, npg)])
+    codes = torch.randint(-127, 128, (2, n_pages, page, hkv, d), generator=g).to(torch.int8)
+    scales = torch.ldexp(torch.ones(2, n_pages, 1, hkv), torch.randint(-8, -3, (2, n_pages, 1, hkv), generator=g))
+    total = sum(new)
+    x = torch.randn(2, total, hkv, d, generator=g).half().to(DEV)
+    q = torch.randn(total, 2 * hkv, d, generator=g).half().to(DEV)
+    qo = i32(np.concatenate([[0], np.cumsum(new)]))
+    got = []
+    for base, size in ((0, n_pages), (far - n_pages, far)):
+        ids = near + base
+        layer = [torch.zeros(size, page, hkv, d, dtype=torch.int8, device=DEV) for _ in "kv"]
+        layer += [torch.zeros(size, 1, hkv, device=DEV) for _ in "kv"]
+        for i in range(2):
+            layer[i][base:] = codes[i].to(DEV)
+            layer[2 + i][base:] = scales[i].to(DEV)
+        table = (indptr, i32(ids), last)
+        K().append_kv_q8(x[0], x[1], qo, total, *layer, *table)
+        outs = [K().paged_prefill_q8(q, qo, total, max(new), *layer, *table),
+                K().paged_decode_append_q8(q[:3], x[0, :3], x[1, :3], *layer, *table, n_pages),
+                K().paged_decode_q8(q[:3], *layer, *table, n_pages),
+                *K().gather_kv_q8(*layer, *table, 210), *(t[base:].clone() for t in layer)]
+        if base:
+            assert not any(t[:base].any() for t in layer)
+        got.append(outs)
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("out", [torch.float16, torch.float32])
+def test_gather_of_a_large_output(out):
+    """An output past 128 MiB (stored past the caches): the values of the small calls that make it up."""
+    c = Cache(32, "e4m3", 16, 8, 128, [700, 16, 0, 33])
+    rows = 2 ** 27 // (2 * 4 * 8 * 128 * 2) + 1  # a little more at 2 bytes an element
+    k, v = K().gather_kv_q8(*c.layer, *c.table, rows, out)
+    small = K().gather_kv_q8(*c.layer, *c.table, 710, out)
+    for x, y in zip((k, v), small):
+        assert torch.equal(x[:, :710], y) and not x[:, 710:].any()
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("grouped", [False, True])
+def test_decode_by_a_recorded_layout(code, grouped):
+    """A call that records its chunk layout and the calls of other layers that read it: the bits of calls without."""
+    c = Cache(33, code, 16, 2, 128, [400, 161, 170, 33], "bf16")
+    grp = None
+    if grouped:
+        for b in (1, 2):
+            c.tables[b][:8] = c.tables[0][:8]
+        c.indices = i32(sum(c.tables, []))
+        grp = K().DecodeGroups(4, [[0, 1, 2]], [8], torch.device(DEV))
+    ws = K().Workspace(torch.device(DEV))
+    qs = [torch.randn(4, 8, 128, device=DEV).bfloat16() for _ in range(3)]
+    want = [K().paged_decode_q8(q, *c.layer, *c.table, c.total_pages, groups=grp) for q in qs]
+    K().paged_decode_q8(qs[0], *c.layer, *c.table, c.total_pages, workspace=ws, groups=grp)  # (sizes the workspace)
+    for q, w, layout in zip(qs, want, (4242, -4242, -4242)):
+        out = K().paged_decode_q8(q, *c.layer, *c.table, c.total_pages, workspace=ws, groups=grp, layout=layout)
+        assert torch.equal(out, w)
+
+
+@pytest.mark.parametrize("grid", [False, True])
+def test_prefill_rows_of_no_token(grid):
+    """Rows of the output that no token has keep what they held; the padding of a grid becomes 0, as over 16-bit pools."""
+    lens, new = [60, 5, 33], [20, 0, 33]
+    c = Cache(34, "int8", 16, 2, 64, lens, "fp16")
+    T, kw = 64, {}
+    rows = [list(range(20)), [], list(range(20, 53))]
+    if grid:
+        T, rows = 3 * 40, [list(range(3, 23)), [], list(range(80, 113))]
+        kw = dict(q_rows=i32(sum(rows, [])), grid_width=40)
+    q = torch.randn(T, 8, 64, device=DEV).half()
+    out = torch.full_like(q, 7.0)
+    K().paged_prefill_q8(q, i32([0, 20, 20, 53]), 53, 33, *c.layer, *c.table, out=out, **kw)
+    for b in (0, 2):
+        check(c, out[rows[b]], q[rows[b]], b)
+    assert (out[sorted(set(range(T)) - set(sum(rows, [])))] == (0 if grid else 7)).all()

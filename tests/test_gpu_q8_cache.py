@@ -200,12 +200,13 @@ def test_rope_forward_is_the_eager_rotation(backend, ps, dtype):
         assert torch.equal(x.view(torch.int8) if x.element_size() == 1 else x, y.view(torch.int8) if y.element_size() == 1 else y)
 
 
+@pytest.mark.parametrize("ps", [16, 20])
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
-def test_graph_steps_match_eager_ones(code):
+def test_graph_steps_match_eager_ones(code, ps):
     """Steps replayed from the captured graphs, between eager work of another cache: the same bits."""
     from nanoslg_amd import kv_cache as KC
     g = torch.Generator().manual_seed(5)
-    ms = [make(code, "fp16", 16, pages=120, prefix=False) for _ in range(2)]
+    ms = [make(code, "fp16", ps, pages=120, prefix=False) for _ in range(2)]
     ids, lens = ["a", "b", "c"], [15, 16, 70]
     q0, k0 = torch.randn(3, 70, HQ, D, generator=g).half().to(DEV), torch.randn(3, 70, HKV, D, generator=g).half().to(DEV)
     for m in ms:
@@ -283,3 +284,28 @@ def test_refusals():
             K.paged_prefill_q8(**{**pre, **bad})
     with pytest.raises(TypeError):
         K.gather_kv_q8(x, x, s, s, i, i, i, 16, torch.float64)
+
+
+def test_decode_launch_refusals():
+    from nanoslg_amd import kernels as K
+    x = torch.zeros(L, 4, 16, HKV, D, dtype=torch.int8, device=DEV)
+    s = torch.zeros(L, 4, 1, HKV, device=DEV)
+    indptr, one = torch.tensor([0, 1], dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    ok = (x, x.clone(), s, s.clone(), one, indptr, one, one, 1, HQ)
+    for at, bad, err in ((0, x[0], ValueError), (1, x[:1], ValueError), (2, s[:, :, :, :1], ValueError), (3, s.half(), TypeError),
+                         (0, x.half(), ValueError), (0, x.cpu(), ValueError), (5, indptr.long(), ValueError), (9, HQ + 1, ValueError)):
+        with pytest.raises(err):
+            K.DecodeLaunchQ8(*ok[:at], bad, *ok[at + 1:])
+    launch = K.DecodeLaunchQ8(*ok)
+    q, r = torch.zeros(1, HQ, D, dtype=torch.float16, device=DEV), torch.zeros(1, HKV, D, dtype=torch.float16, device=DEV)
+    rope = torch.zeros(64, D, device=DEV)
+    for args, kw, err in (((L, q, r, r), {}, IndexError), ((-1, q, r, r), {}, IndexError), ((0, q.float(), r, r), {}, TypeError),
+                          ((0, q, r.bfloat16(), r), {}, TypeError), ((0, q[:, :3], r, r), {}, ValueError),
+                          ((0, q, r[:, :1], r), {}, ValueError), ((0, q, r, torch.cat([r, r])), {}, ValueError),
+                          ((0, q.cpu(), r, r), {}, ValueError), ((0, q, r, r), dict(rope=(rope, rope, one.long())), ValueError),
+                          ((0, q, r, r), dict(rope=(rope, rope, indptr)), ValueError)):
+        with pytest.raises(err):
+            launch(*args, **kw)
+    assert not x.any() and launch(0, q, r, r).shape == (1, HQ, D)
+    with pytest.raises(ValueError):
+        launch.rebind(one, torch.zeros(3, dtype=torch.int32, device=DEV), one, one, 1)
