@@ -150,7 +150,7 @@ __device__ inline u16x4 codes_to16(uint32_t w, float scale) {
   return __builtin_bit_cast(u16x4, r);
 }
 
-// Eight codes, any power of two as the scale.
+// Eight codes, any power of two as the scale; or, with kWide given, what four take.
 template <typename T, typename F>
 __device__ inline u16x8 codes_to16(u32x2 w, float scale) {
   u16x4 a, b;
@@ -159,6 +159,11 @@ __device__ inline u16x8 codes_to16(u32x2 w, float scale) {
   } else {
     a = codes_to16<T, F>(w[0], scale), b = codes_to16<T, F>(w[1], scale);
   }
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <typename T, typename F, bool kWide>
+__device__ inline u16x8 codes_to16(u32x2 w, float scale) {
+  const u16x4 a = codes_to16<T, F, kWide>(w[0], scale), b = codes_to16<T, F, kWide>(w[1], scale);
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 

@@ -1141,5 +1141,6 @@ _Q8_CALLS = ("append_kv_q8", "gather_kv_q8", "paged_decode_q8", "paged_decode_ap
 def __getattr__(name: str):
     if name in _Q8_CALLS:
         from . import kernels_q8
-        return getattr(kernels_q8, name)
+        globals().update((n, getattr(kernels_q8, n)) for n in _Q8_CALLS)
+        return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
