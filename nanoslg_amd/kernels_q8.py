@@ -216,7 +216,7 @@ def rotate_rows(q, k_new, v_new, positions, cos, sin):
     n = positions.numel()
     k_rot = torch.empty((n, 1, Hkv, D), dtype=k_new.dtype, device=k_new.device)
     slots = torch.arange(n, dtype=torch.int32, device=k_new.device)
-    q_rot = rope_append(q, k_new, v_new, positions, slots, cos, sin, k_rot, torch.empty_like(k_rot))
+    q_rot = _call(q.get_device(), rope_append, q, k_new, v_new, positions, slots, cos, sin, k_rot, torch.empty_like(k_rot))
     return q_rot, k_rot.view(n, Hkv, D)
 
 
@@ -401,6 +401,7 @@ class DecodeLaunchQ8(DecodeLaunch):
         if groups is not None and need == 0:
             raise ValueError("DecodeLaunchQ8: unsupported grouped decode shape")
         self.ws = self.workspace.get(need)
+        self.ws_args = (self.ws.data_ptr(), self.ws.numel())
         self._ws_pages = bound
         return self
 
@@ -414,12 +415,14 @@ class DecodeLaunchQ8(DecodeLaunch):
         if q.get_device() != di or k_new.get_device() != di or v_new.get_device() != di:
             raise ValueError(f"DecodeLaunchQ8: tensors must be on {self.device}")
         dt = _row_type("DecodeLaunchQ8", q, k_new, v_new)
-        out_shape = (B, Hq, D)
-        if q.dim() == 4 and q.shape[1] == 1:
-            q, out_shape = q[:, 0], (B, 1, Hq * D)
-        if q.shape != (B, Hq, D) or q.stride(2) != 1 or q.stride(1) != D:
+        qs, qst, out_shape = q.shape, q.stride(), (B, Hq, D)
+        if len(qs) == 4 and qs[1] == 1:
+            out_shape, ok = (B, 1, Hq * D), qs == (B, 1, Hq, D)
+        else:
+            ok = qs == out_shape
+        if not ok or qst[-1] != 1 or qst[-2] != D:
             raise ValueError(f"DecodeLaunchQ8: q must be [{B}, {Hq}, {D}] with a contiguous [Hq, D] block")
-        if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(0) < Hq * D:
+        if q.data_ptr() % 16 or qst[0] % 8 or qst[0] < Hq * D:
             q = q.clone(memory_format=torch.contiguous_format)
         tables = (None, None, None, 0, 0)
         if rope is not None:
@@ -432,7 +435,7 @@ class DecodeLaunchQ8(DecodeLaunch):
         rows = (None, 0, None, 0)
         if self.ps % BLOCK_TOKENS:
             if rope is not None:
-                q, k_new = rotate_rows(q, k_new, v_new, pos, cos, sin)
+                q, k_new = rotate_rows(q.reshape(B, Hq, D), k_new, v_new, pos, cos, sin)
             append_kv_q8(k_new, v_new, torch.arange(B + 1, dtype=torch.int32, device=self.device), B,
                          *(t[layer] for t in self.pools), *self.table)
         else:
@@ -451,7 +454,6 @@ class DecodeLaunchQ8(DecodeLaunch):
         off, soff = layer * self.layer_bytes, layer * self.scale_bytes
         rc = _call(di, self._f_decode8, q.data_ptr(), q.stride(0), *rows, *tables, self.kp0 + off, self.vp0 + off,
                    self.ksp0 + soff, self.vsp0 + soff, self.P, self.ps, *self.table_ptrs, self.total_pages, B, Hq, Hkv, D,
-                   self.scale, dt, self.q8, *self.grp, out.data_ptr(), Hq * D, self.ws.data_ptr(), self.ws.numel(), lay,
-                   _stream(q))
+                   self.scale, dt, self.q8, *self.grp, out.data_ptr(), Hq * D, *self.ws_args, lay, _stream(q))
         _lib.check(rc, "nslg_q8_paged_decode")
         return out
