@@ -656,11 +656,17 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
       // prefix: 25.0 -> 22.4 us per call; t_all / 48 the same as / 64).
       // 8-bit pools, half the bytes a token: t_all / 128, at most 192 tokens (with / 96 and 256: 32
       // sequences of 1k-3k tokens 35.1 -> 38.8 us, 16 of 700-6000 at D = 256 29.9 -> 32.0, 4 of 1k-4k 15.2 ->
-      // 16.1, 16 of 256-8191 28.2 -> 27.8; at most 160: 35.4, 34.7, 15.3, 30.1).
-      constexpr int64_t kLoDiv = kGrouped ? 64 : F::kQ8 ? 128 : 96;
-      constexpr int64_t kLoMax = F::kQ8 && !kGrouped ? 192 : 256;
-      int64_t lo = ((t_all / kLoDiv + 15) / 16) * 16;
-      lo = lo < 64 ? 64 : (lo > kLoMax ? kLoMax : lo);
+      // 16.1, 16 of 256-8191 28.2 -> 27.8; at most 160: 35.4, 34.7, 15.3, 30.1). Where one workgroup has all KV
+      // heads of a chunk, t_all / 192 (4 of 1k-4k tokens, 4 KV heads 12.0 -> 11.5 us, 2 at D = 256 14.9 -> 13.8), and
+      // with one or two waves in it at most 96 (16 of 700-6000, one KV head 15.5 -> 14.2, two 16.8 -> 16.0; four
+      // 18.1 -> 19.4).
+      int64_t lo_div = kGrouped ? 64 : 96, lo_max = 256;
+      if constexpr (F::kQ8 && !kGrouped) {
+        lo_div = p.head_groups == 1 ? 192 : 128;
+        lo_max = p.num_kv_heads <= 2 ? 96 : 192;
+      }
+      int64_t lo = ((t_all / lo_div + 15) / 16) * 16;
+      lo = lo < 64 ? 64 : (lo > lo_max ? lo_max : lo);
       hi = hi < lo ? lo : (hi > ((int64_t)1 << 30) ? ((int64_t)1 << 30) : hi);
       ct = fit_chunk_tokens<kGrouped>(p, ga, lens, (int)lo, (int)hi, p.chunk_budget);
     }
