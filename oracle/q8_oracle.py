@@ -93,8 +93,8 @@ class Layer:
 
 
 #: Weights (relative to the row's largest) under `below` are rounded by up to `by`, absolutely: half's subnormals; fp32's
-#: range, under which exp2 and the low half of a bf16 pair may be 0.
-LOW = {"fp16": (2.0 ** -14, 2.0 ** -25), "bf16": (2.0 ** -118, 2.0 ** -125)}
+#: range, under which exp2 and the low half of a bf16 pair may be 0. "bf16half": bf16 rows with half weights.
+LOW = {"fp16": (2.0 ** -14, 2.0 ** -25), "bf16": (2.0 ** -118, 2.0 ** -125), "bf16half": (2.0 ** -14, 2.0 ** -25)}
 
 
 def attend(q, k, v, scale=None, dtype="fp16"):
@@ -130,8 +130,10 @@ def attention_bound(out, mag, big, low, keys, dtype):
     2^-125 where a part leaves fp32's normal range; and once more where the kernel sums the rounded ones. P.V adds `keys` terms in fp32 and the merge of runs a few more:
     (keys + 64) * 2^-24. All of these are relative to sum p |v|.
     The output is rounded once, 2^-11 (half) or 2^-8 (bf16) of its value; half's subnormals count 2^-25 for it
-    and 2^-24 for V at half its scale."""
-    u_p, u_o, tiny = {"fp16": (2.0 ** -11, 2.0 ** -11, 2.0 ** -24 + 2.0 ** -25), "bf16": (2.0 ** -16, 2.0 ** -8, 1e-37)}[dtype]
+    and 2^-24 for V at half its scale. "bf16half": a bf16 prefill, whose weights are half's (V exact in half: its
+    scales are brought to 2^-15 .. 2^5, or the weights stay in bf16 pairs, which are closer)."""
+    u_p, u_o, tiny = {"fp16": (2.0 ** -11, 2.0 ** -11, 2.0 ** -24 + 2.0 ** -25), "bf16": (2.0 ** -16, 2.0 ** -8, 1e-37),
+                      "bf16half": (2.0 ** -11, 2.0 ** -8, 1e-37)}[dtype]
     delta = (260 * big + 4) * 2.0 ** -24
     err = mag * (2 * delta + 2 * u_p + (keys + 64) * 2.0 ** -24)
     err = err + 2 * low + keys * LOW[dtype][1] * mag  # (in the sum of P.V, and in the sum of the weights)

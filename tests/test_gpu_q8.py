@@ -247,10 +247,11 @@ def test_gather(code, out, page, d):
             assert not got[b, n:].any()
 
 
-def check(c, out, q, b, new=1, scale=None):
+def check(c, out, q, b, new=1, scale=None, prefill=False):
     """Sequence b's output rows against the oracle's."""
-    want, mag, big, low = Q.attend(q.cpu().double().numpy(), c.values("k", b), c.values("v", b), scale, c.dtype)
-    bound = Q.attention_bound(want, mag, big, low, c.lens[b], c.dtype)
+    dtype = "bf16half" if prefill and c.dtype == "bf16" else c.dtype
+    want, mag, big, low = Q.attend(q.cpu().double().numpy(), c.values("k", b), c.values("v", b), scale, dtype)
+    bound = Q.attention_bound(want, mag, big, low, c.lens[b], dtype)
     off = np.abs(out.cpu().double().numpy() - want)
     assert (off <= bound).all(), (b, float((off / bound).max()))
 
@@ -388,8 +389,8 @@ def test_prefill(code, dtype, page, d, hkv, group, lens, new):
     assert torch.equal(padded[rows], out)
     for b in range(len(lens)):
         if new[b]:
-            check(c, out[qo[b]:qo[b + 1]], q[qo[b]:qo[b + 1]], b)
-            check(c, whole[qo[b]:qo[b + 1]], q[qo[b]:qo[b + 1]], b)
+            check(c, out[qo[b]:qo[b + 1]], q[qo[b]:qo[b + 1]], b, prefill=True)
+            check(c, whole[qo[b]:qo[b + 1]], q[qo[b]:qo[b + 1]], b, prefill=True)
 
 
 def test_write_then_attend_as_a_forward_does():
@@ -419,7 +420,7 @@ def test_write_then_attend_as_a_forward_does():
             Q.write_kv(c.side["k"][0], c.side["v"][0], c.tables[b], done[b], kn[b][done[b]:now[b]].double().numpy(), vn[b][done[b]:now[b]].double().numpy())
         c.same()
         for b in range(2):
-            check(c, out[qo[b]:qo[b + 1]], q[qo[b]:qo[b + 1]], b)
+            check(c, out[qo[b]:qo[b + 1]], q[qo[b]:qo[b + 1]], b, prefill=step != [1, 1])
         done = now
 
 
@@ -478,7 +479,7 @@ def test_attention_at_the_ends_of_the_scales(code, dtype, page):
     pre = K().paged_prefill_q8(q, i32(range(B + 1)), B, 1, *c.layer, *c.table)
     for b in range(B):
         for o in (out, pre):
-            check(c, o[b:b + 1], q[b:b + 1], b)
+            check(c, o[b:b + 1], q[b:b + 1], b, prefill=o is pre)
 
 
 def test_offsets_past_32_bits():
@@ -564,3 +565,29 @@ def test_prefill_rows_of_no_token(grid):
     for b in (0, 2):
         check(c, out[rows[b]], q[rows[b]], b)
     assert (out[sorted(set(range(T)) - set(sum(rows, [])))] == (0 if grid else 7)).all()
+
+
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 20), (128, 16), (256, 16)])
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("at,apart", [(0, 0), (-118, 0), (100, 0), (0, 17), (0, 18), (0, 21), (-30, 60), (40, 100)])
+def test_bf16_prefill_over_scales(code, d, page, at, apart):
+    """V's scales anywhere in bf16's range, near each other (P.V in half) or with blocks far below the others (in bf16);
+    keys in one run and in several, whose ranges differ."""
+    lens, new = [700, 33], [70, 33]
+    c = Cache(35, code, page, 2, d, lens, "bf16", stale_nan=True)
+    lay, codes, scale = c.side["v"]
+    rng = np.random.default_rng(36)
+    lay.scale *= np.where(rng.random(lay.scale.shape) < 0.3, 2.0 ** (at - apart), 2.0 ** at)
+    keep = np.ones(lay.scale.shape, bool)
+    keep[c.tables[1]] = rng.random(lay.scale[c.tables[1]].shape) < 0.7  # some blocks of zeros, as written: codes too
+    lay.scale[~keep] = 0
+    slots = np.repeat(keep, 16, 1)[:, :page, :, None]
+    lay.values = np.where(slots, lay.values, 0)
+    scale.copy_(torch.from_numpy(lay.scale).float())
+    codes.copy_(torch.where(torch.from_numpy(slots).to(DEV), codes.float(), 0).to(codes.dtype))
+    qo = [0, 70, 103]
+    q = torch.randn(103, 8, d, device=DEV).bfloat16()
+    for max_kv in (None, 0, 20000):
+        out = K().paged_prefill_q8(q, i32(qo), 103, 70, *c.layer, *c.table, max_kv=max_kv)
+        for b in range(2):
+            check(c, out[qo[b]:qo[b + 1]], q[qo[b]:qo[b + 1]], b, prefill=True)

@@ -63,9 +63,10 @@ def forward(mgr, twins, ids, new, g, dtype, offs=None, rope=None, spread=1.0, ch
             assert not o[b, pad].any()
             if new[b] and check:
                 n = t.len + new[b]
+                by = "bf16half" if S > 1 and dtype == "bf16" else dtype  # a prefill's weights
                 want, mag, big, low = Q.attend(q[b, r].double().numpy(), t.side[layer][0].read(t.table, n),
-                                               t.side[layer][1].read(t.table, n), None, dtype)
-                bound = Q.attention_bound(want, mag, big, low, n, dtype)
+                                               t.side[layer][1].read(t.table, n), None, by)
+                bound = Q.attention_bound(want, mag, big, low, n, by)
                 off = np.abs(o[b, r] - want)
                 assert (off <= bound).all(), (layer, sid, float((off / bound).max()))
     mgr.end_forward(ctx)
