@@ -627,8 +627,7 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
   if constexpr (F::kQ8 && kSplitP) {
     // P.V in half where V's scales allow it: 2^20 from the smallest to the largest of the keys' blocks, the largest
     // taken to 2^5. V's values are then exact in half, P has 11 bits in one piece instead of two bf16's, and a
-    // third of the products go: 8 x 512 tokens over 3584, e4m3, 342 -> 262 us. Other scales: in bf16, P in two. The range is
-    // read ahead of the loop, one load a block of keys: about 1 us in 40.
+    // third of the products go: 8 x 512 tokens over 3584, e4m3, 342 -> 262 us. Other scales: in bf16, P in two.
     __shared__ uint32_t v_range[2];  // the largest scale's bits, and 2^31 - 1 less the smallest's (0: all zero)
     uint32_t big = 0, small = 0;
     if (n_kt > kt_first) {
