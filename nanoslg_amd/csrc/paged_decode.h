@@ -660,13 +660,16 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
       // heads of a chunk, t_all / 192 (4 of 1k-4k tokens, 4 KV heads 12.0 -> 11.5 us, 2 at D = 256 14.9 -> 13.8), and
       // with one or two waves in it at most 96 (16 of 700-6000, one KV head 15.5 -> 14.2, two 16.8 -> 16.0; four
       // 18.1 -> 19.4).
-      int64_t lo_div = kGrouped ? 64 : 96, lo_max = 256;
+      int64_t lo;
       if constexpr (F::kQ8 && !kGrouped) {
-        lo_div = p.head_groups == 1 ? 192 : 128;
-        lo_max = p.num_kv_heads <= 2 ? 96 : 192;
+        const int64_t lo_max = p.num_kv_heads <= 2 ? 96 : 192;
+        lo = ((t_all / (p.head_groups == 1 ? 192 : 128) + 15) / 16) * 16;
+        lo = lo < 64 ? 64 : (lo > lo_max ? lo_max : lo);
+      } else {
+        constexpr int64_t kLoDiv = kGrouped ? 64 : 96;
+        lo = ((t_all / kLoDiv + 15) / 16) * 16;
+        lo = lo < 64 ? 64 : (lo > 256 ? 256 : lo);
       }
-      int64_t lo = ((t_all / lo_div + 15) / 16) * 16;
-      lo = lo < 64 ? 64 : (lo > lo_max ? lo_max : lo);
       hi = hi < lo ? lo : (hi > ((int64_t)1 << 30) ? ((int64_t)1 << 30) : hi);
       ct = fit_chunk_tokens<kGrouped>(p, ga, lens, (int)lo, (int)hi, p.chunk_budget);
     }
@@ -1521,8 +1524,11 @@ int launch_decode(const DecodeParams& p, const MergeParams& mp, const GroupArgs<
     paged_decode_kernel<T, D, false, kTileDepth<F, false>, kGrouped, F><<<grid, 64 * waves, 0, s>>>(p, ga);
   int rc = check_launch("paged_decode");
   if (rc) return rc;
-  // sequences of many chunks (small batches) split their partials over 4 waves
-  if (p.max_chunks > kSplitMergeChunks * p.batch)
+  // sequences of many chunks (small batches) split their partials over 4 waves; over 8-bit pools where a wave would take
+  // more than two rounds of its 2048 / D rows (16 sequences of 700-6000 tokens, D = 256 29.2 -> 27.4 us; 8 of
+  // 500-4000, D = 64, no longer split, 15.0 -> 14.6)
+  constexpr int kSplitChunks = F::kQ8 ? 4096 / D : kSplitMergeChunks;
+  if (p.max_chunks > kSplitChunks * p.batch)
     decode_merge_kernel<T, D, kGrouped, true><<<dim3(p.batch, p.num_qo_heads), 256, 0, s>>>(mp, ga);
   else
     decode_merge_kernel<T, D, kGrouped, false><<<dim3(p.batch, (p.num_qo_heads + 3) / 4), 256, 0, s>>>(mp, ga);
