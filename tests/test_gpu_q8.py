@@ -190,24 +190,26 @@ def test_append_values_that_are_not_finite(code, bad):
 @pytest.mark.parametrize("in_v", [False, True])
 @pytest.mark.parametrize("page", [16, 20])
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
-def test_only_queries_that_see_it_get_what_is_not_finite(code, page, in_v):
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_only_queries_that_see_it_get_what_is_not_finite(dtype, code, page, in_v):
     """A token that is not finite, in K or V: NaN for its own and later queries of that KV head, nothing for those before it
     (int8: before its block)."""
     n, at = 70, 50
-    c = Cache(18, code, page, 2, 128, [n, 40], "fp16")
+    c = Cache(18, code, page, 2, 128, [n, 40], dtype)
     kn, vn = c.rows(n), c.rows(n)
     (vn if in_v else kn)[at, 1, 77] = math.inf
     append(c, [n, 0], kn.to(DEV), vn.to(DEV))
     c.same()
-    q = torch.randn(n, 8, 128, device=DEV).half()
+    q = torch.randn(n, 8, 128, device=DEV).to(DT[dtype])
     out = K().paged_prefill_q8(q, i32([0, n, n]), n, n, *c.layer, *c.table)
     first = at if code == "e4m3" else at - at % page % 16
     assert torch.isnan(out[at:, 4:]).all()
     assert torch.isfinite(out[:first, 4:]).all() and torch.isfinite(out[:, :4]).all()
     c.side["k"][0].values[np.isnan(c.side["k"][0].values)] = 0
     c.side["k"][0].scale[np.isnan(c.side["k"][0].scale)] = 0
-    want = Q.attend(q.cpu().double().numpy(), c.values("k", 0), c.values("v", 0), None, "fp16")
-    bound = Q.attention_bound(*want, n, "fp16")
+    by = "bf16half" if dtype == "bf16" else dtype
+    want = Q.attend(q.cpu().double().numpy(), c.values("k", 0), c.values("v", 0), None, by)
+    bound = Q.attention_bound(*want, n, by)
     off = np.abs(out.cpu().double().numpy() - want[0])
     assert (off <= bound)[:first].all() and (off <= bound)[:, :4].all()
 
