@@ -225,13 +225,14 @@ def _decode8(what, q, k_new, v_new, rope, k_layer, v_layer, k_scale, v_scale, kv
     dev = _one_device(q, k_layer, v_layer, k_scale, v_scale, kv_indptr, kv_indices, kv_last_page_len)
     P, ps, Hkv, D, code = _layer(what, k_layer, v_layer, k_scale, v_scale)
     B = _table(what, kv_indptr, kv_indices, kv_last_page_len)
-    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != D or q.stride(2) != 1 or q.stride(1) != D:
+    qs, qst = q.shape, q.stride()
+    if len(qs) != 3 or qs[0] != B or qs[2] != D or qst[2] != 1 or qst[1] != D:
         raise ValueError(f"{what}: q must be [{B}, Hq, {D}] with a contiguous [Hq, D] block")
-    Hq = q.shape[1]
+    Hq = qs[1]
     if Hq % Hkv:
         raise ValueError(f"{what}: Hq={Hq} is not a multiple of Hkv={Hkv}")
     if out is None:
-        out = q.new_empty((B, Hq, D))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif (out.shape != (B, Hq, D) or out.stride(2) != 1 or out.stride(1) != D or out.dtype != q.dtype
           or out.get_device() != q.get_device()):
         raise ValueError(f"{what}: bad out tensor")
@@ -314,7 +315,7 @@ def paged_prefill_q8(q: torch.Tensor, qo_indptr: torch.Tensor, total_q: int, max
         if q_rows.numel() < total_q or grid_width < 1 or T != B * grid_width:
             raise ValueError("paged_prefill_q8: a grid of B x grid_width rows of q and one q_rows entry per token")
     if out is None:
-        out = q.new_empty((T, Hq, D))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif (out.shape != (T, Hq, D) or out.stride(2) != 1 or out.stride(1) != D or out.dtype != q.dtype
           or out.get_device() != q.get_device()):
         raise ValueError("paged_prefill_q8: out must be shaped like q")
