@@ -581,16 +581,28 @@ __device__ inline void write_new_row8(const DecodeParams& p, int b, int h, int p
 template <int D, typename F>
 constexpr int kMinWaves = !F::kQ8 ? 1 : D == 64 ? 4 : D == 128 ? 3 : 2;
 
-template <typename T, int D, bool kTileInPage, int kDepth, bool kGrouped, typename F>
-__global__ void __launch_bounds__(64 * kMaxWaves, (kMinWaves<D, F>))
+// kOne (8-bit pools, batches of few tokens): a workgroup has one sequence and KV head, its waves a run of tiles each,
+// joined through LDS: no search for a chunk length, no partials in memory, no merge launch. Taken where the bound
+// on the call's tokens, and so its longest sequence, is at most kOneTokens, and one round of workgroups fills no more than
+// the chip. With 32 query heads on 8 KV heads, in chunks and so: 1 x 300 tokens 12.6 -> 8.8 us, 1 x 1000 12.9 -> 11.5, 1 x 1500
+// 13.0 -> 13.9, 4 x 250 13.0 -> 8.1, 16 x 60 11.1 -> 7.1, 64 x 30 10.6 -> 12.2, one KV head 1 x 900 12.2 -> 12.7; D = 256 (4 waves: registers) 1 x 300 15.9 -> 12.0, 1 x 1000
+// 16.1 -> 18.7; D = 64 1 x 1000 13.0 -> 10.3.
+template <int D>
+constexpr int kOneWaves = D == 256 ? 4 : 8;
+template <int D>
+constexpr int64_t kOneTokens = D == 64 ? 1536 : D == 128 ? 1024 : 512;
+
+template <typename T, int D, bool kTileInPage, int kDepth, bool kGrouped, typename F, bool kOne = false>
+__global__ void __launch_bounds__(64 * (kOne ? kOneWaves<D> : kMaxWaves), (kMinWaves<D, F>))
 paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
+  constexpr int kWgWaves = kOne ? kOneWaves<D> : kMaxWaves;
   constexpr int kSteps = D / 32;
   constexpr int NT = D / 16;
   constexpr bool kSplitP = T::kDtype == NSLG_BF16;  // P = hi + lo for bf16's 8-bit mantissa
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int chunk = blockIdx.x;
-  const int h = blockIdx.y * (blockDim.x >> 6) + wave;
+  const int h = kOne ? blockIdx.y : blockIdx.y * (blockDim.x >> 6) + wave;
   if (h >= p.num_kv_heads) return;
 
   // The chunk's work: unit u (sequence b's own tokens, or group g's prefix read
@@ -602,7 +614,25 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
   int u = 0, cstart = 0, nchunks = 0, b = 0, g = -1, t_begin = 0, t_end = 0, idx_off = 0, np_seq = 0;
   bool merged = false;
   bool mapped = false;
-  if (p.layout_mode < 0 && *p.layout_tag_ptr == p.layout_tag) {
+  if constexpr (kOne) {
+    u = b = blockIdx.x;
+    const int len = seq_len_of(p.indptr, p.last_len, b, p.page_size);
+    idx_off = p.indptr[b];
+    np_seq = p.indptr[b + 1] - idx_off;
+    if (len == 0) {
+      for (int i = 8 * threadIdx.x; i < p.group * D; i += 8 * blockDim.x)
+        *reinterpret_cast<u16x8*>(p.out + (int64_t)b * p.out_stride + (int64_t)h * p.group * D + i) = u16x8(0);
+      return;
+    }
+    const int ntiles = (len + 15) >> 4;
+    nchunks = min((ntiles + 1) >> 1, kWgWaves);
+    cstart = chunk - wave;  // (so that c_local is the wave)
+    if (wave < nchunks) {
+      t_begin = 16 * (wave * ntiles / nchunks);
+      t_end = min(16 * ((wave + 1) * ntiles / nchunks), len);
+    }
+  }
+  if (!kOne && p.layout_mode < 0 && *p.layout_tag_ptr == p.layout_tag) {
     const int4 e0 = p.layout_map[2 * chunk];
     const int4 e1 = p.layout_map[2 * chunk + 1];
     u = __builtin_amdgcn_readfirstlane(e0.x);
@@ -625,8 +655,8 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
              chunk < cstart + nchunks && idx_off >= 0 && (int64_t)idx_off + np_seq <= p.total_pages &&
              t_begin >= 0 && t_begin < t_end && (int64_t)t_end <= (int64_t)np_seq * p.page_size;
   }
-  const bool record = p.layout_mode > 0 && blockIdx.y == 0 && threadIdx.x == 0;
-  if (!mapped) {
+  const bool record = !kOne && p.layout_mode > 0 && blockIdx.y == 0 && threadIdx.x == 0;
+  if (!kOne && !mapped) {
     g = -1;
     merged = false;
     if (chunk == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.layout_tag_ptr = p.layout_mode > 0 ? p.layout_tag : 0;
@@ -716,7 +746,7 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
   }
   // the chunk ranges of the merge (written by every call: a call between two calls
   // of one forward may have used the workspace)
-  if (chunk == cstart && blockIdx.y == 0 && threadIdx.x == 0) {
+  if (!kOne && chunk == cstart && blockIdx.y == 0 && threadIdx.x == 0) {
     if constexpr (kGrouped) {
       if (g >= 0)
         ga.group_meta[g] = make_int2(cstart, nchunks);
@@ -912,13 +942,13 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
   // (D = 256: the Q operand, 32 registers, is read back from LDS step by step; held, the loop spilled: 36 us a call of
   // 16 conversations of 700 to 6000 tokens, 42 with spills)
   constexpr bool kQInLds = F::kQ8 && kTileInPage && D == 256;
-  __shared__ u16x8 q_stage[kQInLds ? kMaxWaves : 1][kQInLds ? kSteps : 1][kQInLds ? 64 : 1];
+  __shared__ u16x8 q_stage[kQInLds ? kWgWaves : 1][kQInLds ? kSteps : 1][kQInLds ? 64 : 1];
   if constexpr (kQInLds) {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) q_stage[wave][s][lane] = qb[s];  // (each lane reads its own)
   }
   // Two tiles of one block each, tokens t0 .. t0 + 31: lane l has tokens 4(l/16) + j of both.
-  __shared__ __attribute__((aligned(16))) KStage8<D> k_stage8[kTileInPage && F::kQ8 && D > 64 ? kMaxWaves : 1];
+  __shared__ __attribute__((aligned(16))) KStage8<D> k_stage8[kTileInPage && F::kQ8 && D > 64 ? kWgWaves : 1];
   auto process8 = [&](auto& cur, int t0) {  // (Tile8[2])
     KStage8<D>& st = k_stage8[D > 64 ? wave : 0];
     k8_stage<D>(st, cur);
@@ -1180,12 +1210,47 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
   };
   bool stream = p.stream != 0;
   if constexpr (kGrouped) stream = stream && g < 0;  // a group's prefix: read by every group sharing it
-  if (stream)
+  if (kOne) {
+    if (wave < nchunks) pipeline(std::false_type{});
+  } else if (stream) {
     pipeline(std::true_type{});
-  else
+  } else {
     pipeline(std::false_type{});
+  }
 
   const float l_tot = rows_sum(l_run);
+  if constexpr (kOne) {
+    // the waves' (m, l, O) through LDS; wave w then joins columns w, w + kWgWaves, ..
+    constexpr int kPer = D / 64;  // elements of a row per lane
+    __shared__ __attribute__((aligned(16))) float one_o[kWgWaves][kGroupCols][D];
+    __shared__ float2 one_ml[kWgWaves][kGroupCols];
+    if (head_ok && wave < nchunks) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int n4 = 0; n4 < NT; n4 += 4)
+          *reinterpret_cast<f32x4*>(&one_o[wave][r][NT * (4 * gq + i) + n4]) =
+              f32x4{o[n4][i], o[n4 + 1][i], o[n4 + 2][i], o[n4 + 3][i]};
+      if (gq == 0) one_ml[wave][r] = make_float2(m_run, l_tot);
+    }
+    __syncthreads();
+    for (int c = wave; c < p.group; c += kWgWaves) {
+      float mx = -INFINITY, l = 0.f, acc[kPer] = {};
+      for (int w = 0; w < nchunks; ++w) mx = fmaxf(mx, one_ml[w][c].x);
+      for (int w = 0; w < nchunks; ++w) {
+        const float2 ml = one_ml[w][c];
+        const float f = fast_exp2(ml.x - mx);
+        l += f * ml.y;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) acc[e] += f * one_o[w][c][kPer * lane + e];
+      }
+      const float inv = 2.f / l;  // V went in at half its scale
+      uint16_t* orow = p.out + (int64_t)b * p.out_stride + (int64_t)(h * p.group + c) * D + kPer * lane;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) orow[e] = T::from_f32(acc[e] * inv);
+    }
+    return;
+  }
   if (!head_ok) return;
   if constexpr (F::kQ8) {  // V went in at half its scale
 #pragma unroll
@@ -1517,6 +1582,13 @@ DecodeShape shape_of(int32_t dtype, int32_t head_dim, int32_t units, int32_t num
 template <typename T, int D, bool kGrouped, typename F>
 int launch_decode(const DecodeParams& p, const MergeParams& mp, const GroupArgs<kGrouped>& ga, int waves,
                   hipStream_t s) {
+  if constexpr (F::kQ8 && !kGrouped) {
+    if (p.total_pages * p.page_size <= kOneTokens<D> && p.page_size % 16 == 0 && (int64_t)p.batch * p.num_kv_heads <= 256) {
+      paged_decode_kernel<T, D, true, kTileDepth<F, true>, false, F, true>
+          <<<dim3(p.batch, p.num_kv_heads), 64 * kOneWaves<D>, 0, s>>>(p, ga);
+      return check_launch("paged_decode");
+    }
+  }
   const dim3 grid((unsigned)p.max_chunks, (unsigned)p.head_groups);
   if (p.page_size % 16 == 0)
     paged_decode_kernel<T, D, true, kTileDepth<F, true>, kGrouped, F><<<grid, 64 * waves, 0, s>>>(p, ga);

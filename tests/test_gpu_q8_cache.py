@@ -201,15 +201,17 @@ def test_rope_forward_is_the_eager_rotation(backend, ps, dtype):
         assert torch.equal(x.view(torch.int8) if x.element_size() == 1 else x, y.view(torch.int8) if y.element_size() == 1 else y)
 
 
+@pytest.mark.parametrize("longest", [1070, 70])
 @pytest.mark.parametrize("ps", [16, 20])
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
-def test_graph_steps_match_eager_ones(code, ps):
-    """Steps replayed from the captured graphs, between eager work of another cache: the same bits."""
+def test_graph_steps_match_eager_ones(code, ps, longest):
+    """Steps replayed from the captured graphs, between eager work of another cache: the same bits. Few tokens: eager
+    steps go out in one launch where 16 divides the page, so their sums are in another order."""
     from nanoslg_amd import kv_cache as KC
     g = torch.Generator().manual_seed(5)
     ms = [make(code, "fp16", ps, pages=120, prefix=False) for _ in range(2)]
-    ids, lens = ["a", "b", "c"], [15, 16, 70]
-    q0, k0 = torch.randn(3, 70, HQ, D, generator=g).half().to(DEV), torch.randn(3, 70, HKV, D, generator=g).half().to(DEV)
+    ids, lens = ["a", "b", "c"], [15, 16, longest]
+    q0, k0 = (torch.randn(3, longest, h, D, generator=g).half().to(DEV) for h in (HQ, HKV))
     for m in ms:
         for s, n in zip(ids, lens):
             m.allocate_sequence(s, num_tokens=n)
@@ -228,7 +230,13 @@ def test_graph_steps_match_eager_ones(code, ps):
         ms[1].end_forward(c)
         torch.cuda.synchronize()
         for x, y in zip(outs, ref):
-            assert torch.equal(x, y.reshape(x.shape))
+            if longest < 1000 and ps == 16:
+                # each is within 2^-11 |out| + (1 + 2^-11) (2 * 2^-11 + 2^-14) sum p |v| of the exact output (half weights,
+                # rounded for P.V and for their sum; the scores' part for |q k| / sqrt(D) < 100; half's subnormals far
+                # less), and sum p |v| <= max |v| < 6 here
+                torch.testing.assert_close(x, y.reshape(x.shape), rtol=2 ** -10, atol=2 * 6 * (2 ** -10 + 2 ** -13))
+            else:
+                assert torch.equal(x, y.reshape(x.shape))
     for s in ids:
         a, b = (m.seqs[s].block_table for m in ms)
         assert torch.equal(ms[0].pool.k.view(torch.int8)[:, a], ms[1].pool.k.view(torch.int8)[:, b])
