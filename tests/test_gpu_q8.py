@@ -268,6 +268,12 @@ DECODE = [  # page, d, hkv, group, lens
     (20, 128, 4, 4, [1, 39, 40, 41, 777]),
     (8, 256, 2, 2, [9, 250]),
     (1, 64, 2, 3, [1, 50]),
+    (16, 128, 8, 4, [1, 16, 0, 1700]),  # (past what one launch takes; of the above the first, third and sixth are not)
+    (32, 256, 4, 4, [1, 33, 300]),
+    (16, 128, 1, 16, [300, 5]),
+    (64, 128, 3, 7, [129, 500]),
+    (16, 64, 16, 2, [1, 15, 16, 17, 31, 32, 33, 0, 64, 255, 257]),
+    (16, 128, 64, 1, [20, 100, 3, 4, 5]),
 ]
 
 
@@ -306,15 +312,16 @@ def test_decode_append(code, dtype, page, d, hkv, group, lens):
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("d,page", [(64, 16), (128, 32), (256, 16), (128, 20)])
-def test_decode_rope_append(dtype, d, page):
+@pytest.mark.parametrize("longest", [257, 1800])
+def test_decode_rope_append(dtype, d, page, longest):
     """Bit for bit rope_append into rows of its own, then the decode of the rotated rows."""
-    lens, hkv, G = [5, 40, 257], 2, 4
+    lens, hkv, G = [5, 40, longest], 2, 4
     c = Cache(11, "e4m3", page, hkv, d, lens, dtype)
     twin = [t.clone() for t in c.layer]
     B = len(lens)
     q = torch.randn(B, hkv * G, d, device=DEV).to(DT[dtype])
     kn, vn = c.rows(B, 5).to(DEV), c.rows(B, 5).to(DEV)
-    a = torch.outer(torch.arange(300, dtype=torch.float64), 1e4 ** (-torch.arange(0, d, 2) / d))
+    a = torch.outer(torch.arange(2000, dtype=torch.float64), 1e4 ** (-torch.arange(0, d, 2) / d))
     a = torch.cat([a, a], 1)
     cos, sin = a.cos().float().to(DEV), a.sin().float().to(DEV)
     pos = i32([n - 1 for n in lens])
@@ -345,10 +352,11 @@ def test_decode_groups(code):
         check(c, out[b:b + 1], q[b:b + 1], b)
 
 
+@pytest.mark.parametrize("n", [40, 1000])
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
-def test_decode_of_a_block_that_is_not_finite(code):
+def test_decode_of_a_block_that_is_not_finite(code, n):
     """What reads such a block is NaN; other heads and sequences are not touched."""
-    c = Cache(13, code, 16, 2, 64, [40, 40], "fp16")
+    c = Cache(13, code, 16, 2, 64, [n, n], "fp16")
     x = c.rows(2)
     x[0, 0, 7] = math.nan
     q = torch.randn(2, 4, 64, device=DEV).half()
@@ -426,9 +434,10 @@ def test_write_then_attend_as_a_forward_does():
         done = now
 
 
-def test_side_stream_and_graph_replays():
+@pytest.mark.parametrize("lens", [[300, 77, 1000], [300, 77, 100]])
+def test_side_stream_and_graph_replays(lens):
     """The step captured into a graph and replayed between eager work: every replay gives the eager bits."""
-    c = Cache(16, "e4m3", 16, 4, 128, [300, 77, 1000], "fp16")
+    c = Cache(16, "e4m3", 16, 4, 128, lens, "fp16")
     q = torch.randn(3, 16, 128, device=DEV).half()
     kn, vn = c.rows(3).to(DEV), c.rows(3).to(DEV)
     ws, ws2 = K().Workspace(torch.device(DEV)), K().Workspace(torch.device(DEV))
@@ -451,13 +460,14 @@ def test_side_stream_and_graph_replays():
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("longest", [200, 1500])
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("page", [16, 20])
-def test_attention_at_the_ends_of_the_scales(code, dtype, page):
+def test_attention_at_the_ends_of_the_scales(code, dtype, page, longest):
     """Blocks with scales from under half's range to its largest values (a code may stand for 65536), next to each
     other; and bf16's."""
-    c = Cache(17, code, page, 2, 128, [70, 33, 200], dtype)
+    c = Cache(17, code, page, 2, 128, [70, 33, longest], dtype)
     top = 65504.0 if dtype == "fp16" else 1e30
     for name in "kv":
         lay, codes, scale = c.side[name]
