@@ -48,6 +48,7 @@
 #include "nslg_common.h"
 #include "q8_common.h"
 
+#include <float.h>
 #include <math.h>
 
 #include <atomic>
@@ -847,7 +848,10 @@ paged_decode_kernel(DecodeParams p, GroupArgs<kGrouped> ga) {
     for (int s = 0; s < kSteps; ++s) qb[s] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
   }
 
-  float m_run = -INFINITY;
+  // The running maximum starts at the lowest finite value, not at -inf: keys at -inf then have weight 0 (not
+  // exp2(-inf + inf)) also in a chunk of nothing else, and a chunk whose scores are all NaN leaves a maximum that the
+  // merge tells from that of a wave or lane without chunks, and so its NaN.
+  float m_run = -FLT_MAX;
   float l_run = 0.f;
   f32x4 o[NT];
 #pragma unroll
@@ -1446,7 +1450,7 @@ __global__ void __launch_bounds__(256) decode_merge_kernel(MergeParams p, GroupA
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < kParts; ++w) {
-      if (s_m[w] == -INFINITY) continue;
+      if (s_m[w] == -INFINITY) continue;  // a wave without chunks
       const float f = fast_exp2(s_m[w] - M);
       L += f * s_l[w];
       o += f * *reinterpret_cast<const f32x4*>(&s_o[w][d0]);
