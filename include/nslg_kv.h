@@ -132,7 +132,8 @@ int nslg_gather_kv(const void* k_pool, const void* v_pool, int64_t num_pages,
  *   total_pages       host copy of kv_indptr[batch] (sizes the launch)
  *   sm_scale          softmax scale (1/sqrt(D) for the reference)
  *   workspace         caller-owned device scratch of at least
- *                     nslg_paged_decode_workspace_size(...) bytes, 256-byte aligned;
+ *                     nslg_paged_decode_workspace_size(...) bytes, 256-byte aligned
+ *                     (the size for total_pages serves every call of fewer pages too);
  *                     one call at a time per workspace (calls of any kind may take
  *                     it in turn)
  *   layout            0: the call cuts its sequences into chunks from their lengths
@@ -214,7 +215,7 @@ int nslg_paged_decode_append(const void* q, int64_t q_stride,
  * Arguments and results as nslg_paged_decode (same kernels, bit-identical output),
  * without workspace / workspace_bytes. The call's device is the current device
  * (hipSetDevice), which must be the stream's. A call that would need more scratch
- * than the static array (nslg_paged_decode_workspace_size(...) >
+ * than the static array (at most nslg_paged_decode_workspace_size(...), against
  * NSLG_NOALLOC_SCRATCH_BYTES: e.g. batches of several hundred long sequences)
  * returns NSLG_EWORKSPACE without launching. All calls on one GPU share the one
  * array: calls that overlap on a GPU (different streams, or host threads, without

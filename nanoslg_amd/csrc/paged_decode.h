@@ -1528,6 +1528,7 @@ struct DecodeShape {
   int chunk_tokens;  // upper bound passed to the kernel
   int chunk_budget;  // 0: no device-side search
   int64_t max_chunks;
+  int64_t most_chunks;  // the largest max_chunks of any call of as many tokens or fewer
 };
 
 // Chunk length for `total_tokens` (an upper bound of the units' tokens) over
@@ -1561,7 +1562,12 @@ DecodeShape decode_shape(int32_t units, int32_t num_kv_heads, int64_t total_toke
   if (c > ((int64_t)1 << 30)) c = (int64_t)1 << 30;
   sh.chunk_tokens = (int)c;
   sh.chunk_budget = fit ? (int)capacity : 0;
-  sh.max_chunks = fit ? capacity : (total_tokens + c - 1) / c + units;
+  const int64_t chunks = (total_tokens + c - 1) / c;
+  sh.max_chunks = fit ? capacity : chunks + units;
+  // (the length goes up in steps of 16, so a call of fewer tokens may have more chunks: of 64 tokens at
+  // least, and no more than fill `usable`)
+  const int64_t most = (total_tokens + 63) / 64 < usable ? (total_tokens + 63) / 64 : usable;
+  sh.most_chunks = fit ? capacity : (most > chunks ? most : chunks) + units;
   return sh;
 }
 
@@ -1616,12 +1622,14 @@ inline size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 // Workspace: the recorded chunk layout (a 16-byte tag, then two int4 per chunk), partials
 // [max_chunks, slot_members, Hq, D] and [..., 2] fp32, then each sequence's chunk range,
 // then each group prefix's chunk range (int32 pairs), each region rounded up to 256 bytes.
-inline size_t layout_bytes(const DecodeShape& sh) { return round256(16 + (size_t)sh.max_chunks * 32); }
+inline size_t layout_bytes(int64_t chunks) { return round256(16 + (size_t)chunks * 32); }
 
-size_t workspace_bytes_for(const DecodeShape& sh, int32_t batch, int32_t num_qo_heads, int32_t head_dim,
-                           int32_t slot_members, int32_t num_groups) {
-  return layout_bytes(sh) +
-         (size_t)(sh.max_chunks * slot_members * num_qo_heads * (head_dim + 2) * (int64_t)sizeof(float)) +
+// chunks: a shape's max_chunks for what its call needs; its most_chunks for the size queries, whose answer
+// serves every call of as many pages or fewer.
+size_t workspace_bytes_for(int64_t chunks, int32_t batch, int32_t num_qo_heads, int32_t head_dim, int32_t slot_members,
+                           int32_t num_groups) {
+  return layout_bytes(chunks) +
+         (size_t)(chunks * slot_members * num_qo_heads * (head_dim + 2) * (int64_t)sizeof(float)) +
          round256((size_t)batch * 8) + (num_groups > 0 ? round256((size_t)num_groups * 8) : 0);
 }
 
@@ -1765,7 +1773,7 @@ int decode_impl(const void* q, int64_t q_stride, const void* k_pool, const void*
                 "stream capture; make one call, or a workspace-size query, outside the capture first",
                 dtype, head_dim, page_size);
   const int64_t mc = sh.max_chunks;
-  const size_t need = workspace_bytes_for(sh, batch, num_qo_heads, head_dim, slot_members, num_groups);
+  const size_t need = workspace_bytes_for(mc, batch, num_qo_heads, head_dim, slot_members, num_groups);
   if (!workspace || workspace_bytes < need)
     return fail(NSLG_EWORKSPACE, "paged_decode: workspace %zu < %zu bytes", workspace_bytes, need);
   if (((uintptr_t)workspace) & 255) return fail(NSLG_EINVAL, "paged_decode: workspace must be 256-byte aligned");
@@ -1824,7 +1832,7 @@ int decode_impl(const void* q, int64_t q_stride, const void* k_pool, const void*
   p.layout_tag = (uint64_t)(layout > 0 ? layout : -layout);
   p.layout_tag_ptr = reinterpret_cast<uint64_t*>(ws);
   p.layout_map = reinterpret_cast<int4*>(ws + 16);
-  p.part_o = (float*)(ws + layout_bytes(sh));
+  p.part_o = (float*)(ws + layout_bytes(mc));
   p.part_ml = p.part_o + mc * slot_members * num_qo_heads * head_dim;
   char* meta = reinterpret_cast<char*>(p.part_ml + mc * slot_members * num_qo_heads * 2);
   p.meta = reinterpret_cast<int2*>(meta);

@@ -3,17 +3,27 @@
 
 using namespace nslg;
 
-extern "C" size_t nslg_paged_decode_workspace_size(int32_t batch, int32_t num_qo_heads,
-                                                   int32_t num_kv_heads, int32_t head_dim,
-                                                   int64_t total_pages, int32_t page_size,
-                                                   int32_t dtype) {
+namespace {
+
+// Workspace bytes of an ungrouped call: for this call, or for it and every call of fewer pages.
+size_t plain_bytes(int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim, int64_t total_pages,
+                   int32_t page_size, int32_t dtype, bool smaller_too) {
   if (!shape_ok(batch, num_qo_heads, num_kv_heads, head_dim, total_pages, page_size)) return 0;
-  if (dtype == NSLG_F32)  // partials of the key splits of the fp32 path
+  if (dtype == NSLG_F32)  // partials of the key splits of the fp32 path (their number grows with the pages)
     return attention_f32_workspace(batch, num_qo_heads, head_dim,
                                    attention_f32_decode_splits(batch, num_kv_heads,
                                                                total_pages * (int64_t)page_size));
   const DecodeShape sh = shape_of<false>(dtype, head_dim, batch, num_kv_heads, total_pages * page_size, page_size);
-  return workspace_bytes_for(sh, batch, num_qo_heads, head_dim, 1, 0);
+  return workspace_bytes_for(smaller_too ? sh.most_chunks : sh.max_chunks, batch, num_qo_heads, head_dim, 1, 0);
+}
+
+}  // namespace
+
+extern "C" size_t nslg_paged_decode_workspace_size(int32_t batch, int32_t num_qo_heads,
+                                                   int32_t num_kv_heads, int32_t head_dim,
+                                                   int64_t total_pages, int32_t page_size,
+                                                   int32_t dtype) {
+  return plain_bytes(batch, num_qo_heads, num_kv_heads, head_dim, total_pages, page_size, dtype, true);
 }
 
 extern "C" size_t nslg_paged_decode_grouped_workspace_size(int32_t batch, int32_t num_qo_heads,
@@ -27,7 +37,7 @@ extern "C" size_t nslg_paged_decode_grouped_workspace_size(int32_t batch, int32_
   if (group > kGroupCols) return 0;
   const DecodeShape sh =
       shape_of<true>(dtype, head_dim, batch + num_groups, num_kv_heads, total_pages * page_size, page_size);
-  return workspace_bytes_for(sh, batch, num_qo_heads, head_dim, kGroupCols / group, num_groups);
+  return workspace_bytes_for(sh.most_chunks, batch, num_qo_heads, head_dim, kGroupCols / group, num_groups);
 }
 
 extern "C" int nslg_paged_decode(const void* q, int64_t q_stride, const void* k_pool,
@@ -90,10 +100,9 @@ extern "C" int nslg_paged_decode_noalloc(const void* q, int64_t q_stride, const 
                                          int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
                                          int32_t head_dim, float sm_scale, int32_t dtype, void* out,
                                          int64_t out_stride, nslg_stream_t stream) {
-  // Same scratch layout and size as nslg_paged_decode's workspace; nothing in it has
+  // Same scratch layout as nslg_paged_decode's workspace, of what this call needs; nothing in it has
   // to start at zero (every chunk range and partial is written before it is read).
-  const size_t need = nslg_paged_decode_workspace_size(batch, num_qo_heads, num_kv_heads, head_dim, total_pages,
-                                                       page_size, dtype);
+  const size_t need = plain_bytes(batch, num_qo_heads, num_kv_heads, head_dim, total_pages, page_size, dtype, false);
   if (need > (size_t)NSLG_NOALLOC_SCRATCH_BYTES)
     return fail(NSLG_EWORKSPACE,
                 "paged_decode_noalloc: this call needs %zu bytes of scratch, more than the %zu-byte static "

@@ -25,10 +25,11 @@ extern "C" size_t nslg_q8_paged_decode_workspace_size(int32_t batch, int32_t num
   if (group > kGroupCols) return 0;
   const int64_t tokens = total_pages * page_size;
   if (num_groups == 0)
-    return workspace_bytes_for(shape8<false>(code, dtype, head_dim, batch, num_kv_heads, tokens, page_size), batch,
-                               num_qo_heads, head_dim, 1, 0);
-  return workspace_bytes_for(shape8<true>(code, dtype, head_dim, batch + num_groups, num_kv_heads, tokens, page_size), batch,
-                             num_qo_heads, head_dim, kGroupCols / group, num_groups);
+    return workspace_bytes_for(shape8<false>(code, dtype, head_dim, batch, num_kv_heads, tokens, page_size).most_chunks,
+                               batch, num_qo_heads, head_dim, 1, 0);
+  return workspace_bytes_for(
+      shape8<true>(code, dtype, head_dim, batch + num_groups, num_kv_heads, tokens, page_size).most_chunks, batch,
+      num_qo_heads, head_dim, kGroupCols / group, num_groups);
 }
 
 extern "C" int nslg_q8_paged_decode(

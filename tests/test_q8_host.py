@@ -206,3 +206,25 @@ def test_fast_binding_of_the_8_bit_entry_points():
     assert len(found) == 4
     for fn, sig in found:
         assert sig == "".join(code[t] for t in L.SIGNATURES["nslg_" + fn][1]), fn
+
+
+@pytest.mark.parametrize("groups", [0, 3])
+@pytest.mark.parametrize("batch,hq,hkv,d,page", [(192, 64, 8, 128, 16), (288, 48, 8, 128, 128), (300, 32, 8, 64, 20), (400, 16, 2, 256, 32),
+                                                 (1500, 8, 1, 128, 16), (5, 32, 8, 128, 16)])
+def test_workspace_size_serves_every_smaller_call(batch, hq, hkv, d, page, groups):
+    """A workspace sized for a number of pages is enough for a call of fewer (as DecodeLaunch and DecodeLaunchQ8 rely on):
+    the size asked for does not fall as pages come, though a call's own chunks may become fewer."""
+    from nanoslg_amd import _lib as L
+    lib = L.load()
+    pages = sorted({batch, *range(batch, batch + 40), *(batch + round(1.03 ** i) for i in range(330))})
+    for dt in (L.NSLG_F16, L.NSLG_BF16, L.NSLG_F32):
+        sizes = []
+        if dt != L.NSLG_F32:
+            sizes = [[lib.nslg_q8_paged_decode_workspace_size(batch, hq, hkv, d, p, page, dt, code, groups) for p in pages]
+                     for code in (L.NSLG_E4M3, L.NSLG_INT8)]
+        if not groups:
+            sizes.append([lib.nslg_paged_decode_workspace_size(batch, hq, hkv, d, p, page, dt) for p in pages])
+        elif dt != L.NSLG_F32:
+            sizes.append([lib.nslg_paged_decode_grouped_workspace_size(batch, hq, hkv, d, p, page, dt, groups) for p in pages])
+        for s in sizes:
+            assert min(s) > 0 and s == sorted(s)
