@@ -140,8 +140,8 @@ int nslg_gather_kv(const void* k_pool, const void* v_pool, int64_t num_pages,
  *                     (every wave reads the lengths and searches the chunk length);
  *                     t > 0: the same, and the chunks' work is recorded in the
  *                     workspace under tag t; -t: a later call of the same forward
- *                     (another layer: same batch, block table, lengths, sizes and
- *                     workspace) reads the record instead, when the workspace still
+ *                     (another layer: same batch, block table, lengths, sizes, types
+ *                     and workspace) reads the record instead, when the workspace still
  *                     holds tag t (its first word, which every call that puts partials
  *                     into a workspace sets; else it cuts the chunks itself). Results are
  *                     bit-identical in all three modes; a tag must not be reused for

@@ -337,7 +337,7 @@ class DecodeLaunchQ8(DecodeLaunch):
     ``kernels.DecodeLaunch`` does over 16-bit pools, with its interface. The step's rows go in
     in the decode launch (nslg_q8_paged_decode with new rows; on pages that 16 does not divide
     nslg_q8_append_kv goes ahead), with RoPE rotated there too. The forward's first call
-    records its chunk layout for the other layers'."""
+    of a row type records its chunk layout for the other layers'."""
 
     def __init__(self, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                  slot_mapping: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
@@ -375,7 +375,7 @@ class DecodeLaunchQ8(DecodeLaunch):
         """Point the launcher at another forward's plan of the same batch size (slot_mapping is not used: the
         slots come from the block table)."""
         B = self.B
-        self._layout = 0
+        self._layouts = [0, 0]  # by row type, whose kernels may cut the plan into other chunks
         if check:
             _require_gpu(self.pools[0], kv_indptr, kv_indices, kv_last_page_len)
             if _table("DecodeLaunchQ8", kv_indptr, kv_indices, kv_last_page_len) != B:
@@ -448,10 +448,10 @@ class DecodeLaunchQ8(DecodeLaunch):
                     cos, sin = (t[:, :D].clone(memory_format=torch.contiguous_format) for t in (cos, sin))
                 tables = (pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0])
         out = q.new_empty(out_shape)
-        lay = self._layout  # < 0: read the layout recorded under tag -lay
-        if lay == 0:  # the first call on this plan records its chunk layout
+        lay = self._layouts[dt]  # < 0: read the layout recorded under tag -lay
+        if lay == 0:  # the first call of this type on this plan records its chunk layout
             lay = next(_LAYOUT_TAGS)
-            self._layout = -lay
+            self._layouts[dt] = -lay
         off, soff = layer * self.layer_bytes, layer * self.scale_bytes
         rc = _call(di, self._f_decode8, q.data_ptr(), q.stride(0), *rows, *tables, self.kp0 + off, self.vp0 + off,
                    self.ksp0 + soff, self.vsp0 + soff, self.P, self.ps, *self.table_ptrs, self.total_pages, B, Hq, Hkv, D,
