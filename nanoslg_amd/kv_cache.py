@@ -1079,6 +1079,8 @@ class PagedCacheContext(CacheContext):
                 if cow_src:
                     pool.copy(cow_src, cow_dst)
                 raise RuntimeError("KV OOM during CoW")
+            if pool.k_scale is not None:  # (of the copy's tokens only this sequence's count: see release_sequence)
+                pool.tokens_used[new] = max(st.num_tokens - p * ps, 0)
             cow_src.append(pid)
             cow_dst.append(new)
             st.set_page(p, new)
@@ -1817,6 +1819,13 @@ class PagedKVCache(KVCacheManager):
         if self.tree and st.token_ids:
             if self.tree.share_partial:  # the full pages and the last, partial one
                 n = min(st.num_tokens, len(st.token_ids), st.n_pages * ps)
+                if n and self.pool.k_scale is not None:
+                    # a block of 8-bit codes has one scale: where the page also holds later tokens (ids never
+                    # given, or rows of a forward that did not end), the tail block's has grown with them, and
+                    # int8's K may be NaN through them; that block is not shared
+                    tail = n - (n - 1) // ps * ps
+                    if tail % _SCALE_BLOCK and tail < ps and self.pool.tokens_used[st.bt[(n - 1) // ps]] > tail:
+                        n -= tail % _SCALE_BLOCK
                 if n:
                     self.tree.insert(st.token_ids[:n], st.block_table[:-(-n // ps)])
             else:

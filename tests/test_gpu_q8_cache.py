@@ -318,3 +318,27 @@ def test_decode_launch_refusals():
     assert not x.any() and launch(0, q, r, r).shape == (1, HQ, D)
     with pytest.raises(ValueError):
         launch.rebind(one, torch.zeros(3, dtype=torch.int32, device=DEV), one, one, 1)
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("bad", [float("inf"), 6e4])
+def test_a_request_does_not_change_the_prompt_that_others_share(code, bad):
+    """A sequence writes a prompt and then a token that is not finite, or far larger than the prompt's, and is released
+    with the prompt's ids alone. The next request on that prompt reads it as it was written."""
+    g = torch.Generator().manual_seed(6)
+    prompt = list(range(500, 521))
+    m = make(code)
+    twins = {"a": Twin(code, 16)}
+    m.allocate_sequence("a", token_ids=prompt)
+    forward(m, twins, ["a"], [21], g, "fp16")
+    c = m.begin_forward(["a"], [1])
+    for layer in range(L):
+        x = torch.ones(1, 1, HQ, D, dtype=torch.float16, device=DEV)
+        c.attend(layer, x, x[:, :, :HKV] * bad, x[:, :, :HKV] * bad, HQ, HKV)
+    m.end_forward(c)
+    m.release_sequence("a")
+    got = m.allocate_sequence("b", token_ids=prompt + [9])
+    twins = {"b": twins["a"].prefix(got)}
+    o = forward(m, twins, ["b"], [22 - got], g, "fp16")
+    assert all(torch.isfinite(x).all() for x in o)
+    stored(m, twins)

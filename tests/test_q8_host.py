@@ -228,3 +228,43 @@ def test_workspace_size_serves_every_smaller_call(batch, hq, hkv, d, page, group
             sizes.append([lib.nslg_paged_decode_grouped_workspace_size(batch, hq, hkv, d, p, page, dt, groups) for p in pages])
         for s in sizes:
             assert min(s) > 0 and s == sorted(s)
+
+
+@pytest.mark.parametrize("code", [None, "int8", "fp8"])
+@pytest.mark.parametrize("page,prompt,later,want", [
+    (16, 21, 2, 16),  # the tail block (tokens 16 .. 20) holds tokens 21 and 22 too
+    (16, 21, 0, 21), (16, 32, 3, 32), (16, 9, 1, 0), (16, 9, 0, 9),
+    (64, 16 * 6 + 5, 1, 16 * 6), (64, 16 * 6 + 5, 0, 16 * 6 + 5), (64, 16 * 6, 9, 16 * 6), (64, 70, 59, 64),
+    (20, 39, 1, 36), (20, 20, 7, 20), (20, 33, 2, 20), (20, 37, 2, 36),
+])
+def test_a_cached_tail_holds_no_later_tokens(code, page, prompt, later, want):
+    """A released sequence's last page is cached for the ids that were given. Where it holds later tokens (generated, ids
+    never given), their values are in an 8-bit block's scale: what is shared ends with the last block without them."""
+    import fake_kernels
+    from nanoslg_amd import KVCacheConfig, PagedKVCache
+    m = PagedKVCache(KVCacheConfig(num_layers=1, num_kv_heads=2, num_qo_heads=4, head_dim=64, page_size=page, max_pages=40,
+                                   cache_dtype=code), kernels=fake_kernels)
+    ids = list(range(100, 100 + prompt))
+    assert m.allocate_sequence("a", token_ids=ids) == 0
+    for n in [prompt] + [1] * later:
+        m.end_forward(m.begin_forward(["a"], [n]))
+    m.release_sequence("a")
+    want = prompt if code is None else want
+    assert m.allocate_sequence("b", token_ids=ids + [7, 8]) == want
+    m.end_forward(m.begin_forward(["b"], [prompt + 2 - want]))  # (its ids are all given: its whole tail is cached)
+    m.release_sequence("b")
+    assert m.allocate_sequence("c", token_ids=ids + [7, 8, 9]) == prompt + 2
+
+
+def test_a_failed_forward_leaves_no_tail_to_share():
+    """Rows of a forward that did not end are in the tail block's scale too."""
+    import fake_kernels
+    from nanoslg_amd import KVCacheConfig, PagedKVCache
+    m = PagedKVCache(KVCacheConfig(num_layers=1, num_kv_heads=2, num_qo_heads=4, head_dim=64, page_size=16, max_pages=40,
+                                   cache_dtype="int8"), kernels=fake_kernels)
+    ids = list(range(100, 121))
+    m.allocate_sequence("a", token_ids=ids)
+    m.end_forward(m.begin_forward(["a"], [21]))
+    m.begin_forward(["a"], [1])  # written, perhaps, and given up
+    m.release_sequence("a")
+    assert m.allocate_sequence("b", token_ids=ids) == 16
