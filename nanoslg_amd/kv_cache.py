@@ -536,27 +536,41 @@ class _Pools:
     scale has a meaning once its first slot is written; zero-on-alloc leaves it).
 
     k_words / v_words: the pools as the page-moving kernels and the planners take them, in
-    16-bit words where they hold 8-bit codes."""
+    16-bit words where they hold 8-bit codes. All of it goes by the tensors that k, v, k_scale and v_scale
+    are now: a caller may have replaced them."""
 
     def __init__(self, cfg: KVCacheConfig, pages: int, page_size: int, device: torch.device):
         shape = (cfg.num_layers, pages, page_size, cfg.num_kv_heads, cfg.head_dim)
         dtype = cfg.cache_dtype or cfg.dtype
         self.k = torch.zeros(shape, dtype=dtype, device=device)
         self.v = torch.zeros(shape, dtype=dtype, device=device)
-        self.k_words, self.v_words = self.k, self.v
         self.k_scale = self.v_scale = None
         if cfg.cache_dtype is not None:
-            self.k_words, self.v_words = self.k.view(torch.float16), self.v.view(torch.float16)
             shape = (cfg.num_layers, pages, cfg.scale_blocks(page_size), cfg.num_kv_heads)
             self.k_scale = torch.zeros(shape, dtype=torch.float32, device=device)
             self.v_scale = torch.zeros(shape, dtype=torch.float32, device=device)
-        self._layers8: List[Tuple[torch.Tensor, ...]] = []
+        self._layers8: Tuple[Tuple[int, ...], List[Tuple[torch.Tensor, ...]]] = ((), [])
+
+    @property
+    def k_words(self) -> torch.Tensor:
+        return self.k if self.k_scale is None else self.k.view(torch.float16)
+
+    @property
+    def v_words(self) -> torch.Tensor:
+        return self.v if self.k_scale is None else self.v.view(torch.float16)
+
+    def addresses(self) -> Tuple[int, ...]:
+        """Where the pools (and scales) are."""
+        if self.k_scale is None:
+            return self.k.data_ptr(), self.v.data_ptr()
+        return self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
 
     def layer8(self, i: int) -> Tuple[torch.Tensor, ...]:
-        """Layer i of an 8-bit cache: codes of K and V, scales of K and V."""
-        if not self._layers8:
-            self._layers8 = list(zip(*(t.unbind(0) for t in (self.k, self.v, self.k_scale, self.v_scale))))
-        return self._layers8[i]
+        """Layer i of an 8-bit cache: codes of K and V, scales of K and V (views made once)."""
+        at = self.addresses()
+        if self._layers8[0] != at:
+            self._layers8 = at, list(zip(*(t.unbind(0) for t in (self.k, self.v, self.k_scale, self.v_scale))))
+        return self._layers8[1][i]
 
     def decode_launch(self, kern, *args, **kw):
         """The decode launcher over these pools (kernels.DecodeLaunch, or its 8-bit form)."""
@@ -1999,18 +2013,19 @@ class ContiguousCacheContext(CacheContext):
         call with other heads, or after the pools moved, gets a new one. None where q's
         heads are no multiple of the cache's."""
         cache, plan = self.cache, self._plan
-        of = (q.shape[2], cache.k.data_ptr(), cache.v.data_ptr())
+        of = (q.shape[2], *cache.pools.addresses())
         got = self._decode_launch
         if got is None or got[0] != of:
             if of[0] % cache.cfg.num_kv_heads:
                 return None
             prev, kern = cache._launcher, cache.kernels
             args = (plan.slot, plan.indptr, plan.indices, plan.lpl, plan.total_pages)
-            if (prev is not None and hasattr(prev, "bound_to") and prev.B == plan.batch
-                    and (prev.Hq, prev.kp0, prev.vp0) == of):
+            if getattr(prev, "of", None) == of and prev.B == plan.batch:
                 launch = prev.bound_to(*args)
             else:
                 launch = cache.pools.decode_launch(kern, *args, q.shape[2], workspace=cache.workspace)
+                if hasattr(launch, "bound_to"):
+                    launch.of = of
             cache._launcher = launch
             self._decode_launch = got = (of, launch)
         return got[1]
@@ -2044,11 +2059,26 @@ class ContiguousKVCache(KVCacheManager):
         _check_head_dim(cfg, self.kernels)
         self.device = torch.device(cfg.device) if cfg.device is not None else torch.device("cpu")
         self.pools = _Pools(cfg, cfg.max_batch_size, cfg.max_seq_len, self.device)  # a slot is a page of max_seq_len
-        self.k, self.v = self.pools.k, self.pools.v
         self.states: Dict[str, _ContigSeqState] = {}
         self._slot = 0
         self.workspace = self.kernels.Workspace(self.device, 16 << 20)
         self._launcher = None  # the last decode forward's kernels.DecodeLaunch: the next one's is made from it
+
+    @property
+    def k(self) -> torch.Tensor:
+        return self.pools.k
+
+    @k.setter
+    def k(self, t: torch.Tensor) -> None:
+        self.pools.k = t
+
+    @property
+    def v(self) -> torch.Tensor:
+        return self.pools.v
+
+    @v.setter
+    def v(self, t: torch.Tensor) -> None:
+        self.pools.v = t
 
     def paged_view(self, layer_idx):
         return self.k[layer_idx], self.v[layer_idx]
