@@ -351,7 +351,7 @@ def paged_decode_rope_append(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.
     [max_positions, >= D] tables. Same result, bit for bit, as rope_append of q, k_new
     and v_new at those positions into the sequences' new slots followed by
     paged_decode of the rotated q. f16/bf16 pools."""
-    _require_gpu(positions, cos, sin)
+    _require_gpu(q, positions, cos, sin)
     _i32(positions, "positions")
     if positions.numel() != q.shape[0] or not positions.is_contiguous():
         raise ValueError("paged_decode_rope_append: one position per sequence, contiguous")

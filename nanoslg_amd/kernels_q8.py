@@ -200,7 +200,7 @@ def paged_decode_rope_append_q8(q: torch.Tensor, k_new: torch.Tensor, v_new: tor
                                 layout: int = 0) -> torch.Tensor:
     """paged_decode_append_q8 of q and k_new rotated at each sequence's `positions` entry (int32 [B]) with
     the model's [max_positions, >= D] cos / sin tables, as in ``kernels.paged_decode_rope_append``."""
-    _require_gpu(positions, cos, sin)
+    _require_gpu(q, positions, cos, sin)
     _i32(positions, "positions")
     if positions.numel() != q.shape[0]:
         raise ValueError("paged_decode_rope_append_q8: one position per sequence")

@@ -268,3 +268,26 @@ def test_a_failed_forward_leaves_no_tail_to_share():
     m.begin_forward(["a"], [1])  # written, perhaps, and given up
     m.release_sequence("a")
     assert m.allocate_sequence("b", token_ids=ids) == 16
+
+
+@pytest.mark.parametrize("call", ["paged_decode_rope_append", "paged_decode_rope_append_q8"])
+def test_rope_tables_on_another_device_are_refused(call):
+    """Positions and tables that agree with each other, but are not where q is (stand-ins: only what the check looks at)."""
+    from types import SimpleNamespace
+    from nanoslg_amd import kernels as K
+
+    def on(device, *shape, dtype=torch.float32):
+        n = int(np.prod(shape))
+        return SimpleNamespace(is_cuda=True, device=torch.device(device), get_device=lambda: int(device[-1]), dtype=dtype, shape=shape,
+                               numel=lambda: n, is_contiguous=lambda: True, dim=lambda: len(shape), stride=lambda i: (shape[-1], 1)[i])
+
+    q = on("cuda:0", 2, 4, 64, dtype=torch.float16)
+    for other in range(3):
+        pos, cos, sin = (on("cuda:1" if other != i else "cuda:0", *s, dtype=t) for i, (s, t) in
+                         enumerate((((2,), torch.int32), ((9, 64), torch.float32), ((9, 64), torch.float32))))
+        rest = [q] * (8 if call.endswith("q8") else 6)
+        with pytest.raises(ValueError, match="different devices"):
+            getattr(K, call)(q, q, q, pos, cos, sin, *rest[:-1], 1)
+    pos, cos, sin = on("cuda:1", 2, dtype=torch.int32), on("cuda:1", 9, 64), on("cuda:1", 9, 64)
+    with pytest.raises(ValueError, match="different devices"):
+        getattr(K, call)(q, q, q, pos, cos, sin, *rest[:-1], 1)
