@@ -288,10 +288,12 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
   const unsigned short one16 = T::from_f32(1.f);
   const u16x8 ones_t = u16x8{one16, one16, one16, one16, one16, one16, one16, one16};
   // per column block: raw-score threshold above which the running max must be raised,
-  // and the exponent offset -m (0 while m = -inf); both change only with m, which is not
+  // and the exponent offset -m + p_up (0 while m = -inf); both change only with m, which is not
   // held itself (two registers that the block loop has not got)
   float thr[kCB];
   float neg_m[kCB];
+  constexpr bool kMayHalfPV = F::kQ8 && kSplitP;
+  float p_up = 0.f;  // (kMayHalfPV) log2 of a factor on the probabilities, and so on o and lsum
   const float inv_scale_log2 = 1.f / p.scale_log2;
   f32x4 o[kCB][NT];
 #pragma unroll
@@ -512,7 +514,10 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
       va[n] = __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   };
-  auto run_max = [&](int cb) { return thr[cb] == -INFINITY ? -INFINITY : -neg_m[cb]; };
+  auto run_max = [&](int cb) {
+    if constexpr (kMayHalfPV) return thr[cb] == -INFINITY ? -INFINITY : p_up - neg_m[cb];
+    return thr[cb] == -INFINITY ? -INFINITY : -neg_m[cb];
+  };
   // masking (blocks touching the causal diagonal or the end of the keys) and the lazy
   // rescale: the row's running max m is raised only when some score of the block
   // exceeds it by more than the slack, which each lane checks on its own 8 scores;
@@ -539,7 +544,10 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[cb][n] *= alpha;
         thr[cb] = (m_new + kRescaleSlack) * inv_scale_log2;
-        neg_m[cb] = m_new == -INFINITY ? 0.f : -m_new;
+        if constexpr (kMayHalfPV)
+          neg_m[cb] = m_new == -INFINITY ? 0.f : p_up - m_new;
+        else
+          neg_m[cb] = m_new == -INFINITY ? 0.f : -m_new;
       }
     }
   };
@@ -624,10 +632,14 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
     }
   };
 
-  if constexpr (F::kQ8 && kSplitP) {
-    // P.V in half where V's scales allow it: 2^20 from the smallest to the largest of the keys' blocks, the largest
-    // taken to 2^5. V's values are then exact in half, P has 11 bits in one piece instead of two bf16's, and a
-    // third of the products go: 8 x 512 tokens over 3584, e4m3, 342 -> 262 us. Other scales: in bf16, P in two.
+  if constexpr (kMayHalfPV) {
+    // P.V in half where V's scales allow it: 2^8 from the smallest to the largest of the keys' blocks, the largest
+    // taken to 2^5. V's values are then exact in half, P has 11 bits in one piece instead of two bf16's (the output
+    // has 8), and a third of the products go: 8 x 512 tokens over 3584, e4m3, 342 -> 262 us.
+    // P goes in times 2^7, at most 2^15 (the maximum may lag by 2^8): 11 bits down to 2^-21 of the row's largest, below
+    // within 2^-32, which 2^15 keys of a V 2^8 times as large make a bf16 rounding of the others'. Beside an
+    // attention sink whole rows live on such weights; without the factor those of 2^-21 were 6 % off.
+    // Scales further apart: in bf16, P in two.
     __shared__ uint32_t v_range[2];  // the largest scale's bits, and 2^31 - 1 less the smallest's (0: all zero)
     uint32_t big = 0, small = 0;
     if (n_kt > kt_first) {
@@ -651,11 +663,12 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
     __syncthreads();
     const uint32_t top = __builtin_amdgcn_readfirstlane(v_range[0]);
     const uint32_t low = 0x7fffffffu - __builtin_amdgcn_readfirstlane(v_range[1]);
-    if (top < 0x7f800000u && (top == 0 || (top >> 23) - (low >> 23) <= 20u)) {
+    if (top < 0x7f800000u && (top == 0 || (top >> 23) - (low >> 23) <= 8u)) {
       // exponent fields: the largest scale to 2^5, at least the 127 - 120 of a factor that is a normal number
       const uint32_t ex = top == 0 ? 127u : max(top >> 23, 12u) - 5u;
       v_in = __uint_as_float((254u - ex) << 23);
       v_out = __uint_as_float(ex << 23);
+      p_up = 7.f;
       constexpr std::true_type half_pv;
 #include "paged_prefill_loop.inc"
     } else {
@@ -686,7 +699,8 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
       if (q0 + t >= p.total_q) continue;  // past the partials: not a row of this call
       if (merged) {
         const int64_t slot = (int64_t)(run / p.num_kv_heads) * p.total_q * p.num_qo_heads + pr;
-        if (gq == 0) p.part_ml[slot] = float2{run_max(cb), l_tot};
+        // (m for the factor on P too: l and o are relative to 2^-neg_m)
+        if (gq == 0) p.part_ml[slot] = float2{thr[cb] == -INFINITY ? -INFINITY : -neg_m[cb], l_tot};
         float* po = p.part_o + slot * D + 4 * gq;
 #pragma unroll
         for (int n = 0; n < NT; ++n) *reinterpret_cast<f32x4*>(po + 16 * n) = o[cb][n];

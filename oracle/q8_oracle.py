@@ -95,6 +95,9 @@ class Layer:
 #: Weights (relative to the row's largest) under `below` are rounded by up to `by`, absolutely: half's subnormals; fp32's
 #: range, under which exp2 and the low half of a bf16 pair may be 0. "bf16half": bf16 rows with half weights.
 LOW = {"fp16": (2.0 ** -14, 2.0 ** -25), "bf16": (2.0 ** -118, 2.0 ** -125), "bf16half": (2.0 ** -14, 2.0 ** -25)}
+#: "bf16up": such weights times 2^7, where V's scales lie within 2^8 of each other (else a bf16 pair's: "bf16"); "bf16runs":
+#: either of them by the run of keys, each run with a weight near its largest on every key that counts.
+LOW["bf16up"], LOW["bf16runs"] = (2.0 ** -21, 2.0 ** -32), LOW["bf16"]
 
 
 def attend(q, k, v, scale=None, dtype="fp16"):
@@ -133,7 +136,8 @@ def attention_bound(out, mag, big, low, keys, dtype):
     and 2^-24 for V at half its scale. "bf16half": a bf16 prefill, whose weights are half's (V exact in half: its
     scales are brought to 2^-15 .. 2^5, or the weights stay in bf16 pairs, which are closer)."""
     u_p, u_o, tiny = {"fp16": (2.0 ** -11, 2.0 ** -11, 2.0 ** -24 + 2.0 ** -25), "bf16": (2.0 ** -16, 2.0 ** -8, 1e-37),
-                      "bf16half": (2.0 ** -11, 2.0 ** -8, 1e-37)}[dtype]
+                      "bf16half": (2.0 ** -11, 2.0 ** -8, 1e-37), "bf16up": (2.0 ** -11, 2.0 ** -8, 1e-37),
+                      "bf16runs": (2.0 ** -11, 2.0 ** -8, 1e-37)}[dtype]
     delta = (260 * big + 4) * 2.0 ** -24
     err = mag * (2 * delta + 2 * u_p + (keys + 64) * 2.0 ** -24)
     err = err + 2 * low + keys * LOW[dtype][1] * mag  # (in the sum of P.V, and in the sum of the weights)
