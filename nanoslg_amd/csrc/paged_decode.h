@@ -584,14 +584,29 @@ constexpr int kMinWaves = !F::kQ8 ? 1 : D == 64 ? 4 : D == 128 ? 3 : 2;
 
 // kOne (8-bit pools, batches of few tokens): a workgroup has one sequence and KV head, its waves a run of tiles each,
 // joined through LDS: no search for a chunk length, no partials in memory, no merge launch. Taken where the bound
-// on the call's tokens, and so its longest sequence, is at most kOneTokens, and one round of workgroups fills no more than
-// the chip. With 32 query heads on 8 KV heads, in chunks and so: 1 x 300 tokens 12.6 -> 8.8 us, 1 x 1000 12.9 -> 11.5, 1 x 1500
-// 13.0 -> 13.9, 4 x 250 13.0 -> 8.1, 16 x 60 11.1 -> 7.1, 64 x 30 10.6 -> 12.2, one KV head 1 x 900 12.2 -> 12.7; D = 256 (4 waves: registers) 1 x 300 15.9 -> 12.0, 1 x 1000
-// 16.1 -> 18.7; D = 64 1 x 1000 13.0 -> 10.3.
+// on the call's tokens, and so its longest sequence, is at most one_launch_tokens, and one round of workgroups fills no
+// more than the chip (64 sequences of 30 tokens on 8 KV heads 10.6 us in chunks, 12.2 so).
 template <int D>
-constexpr int kOneWaves = D == 256 ? 4 : 8;
+constexpr int kOneWaves = D == 256 ? 4 : 8;  // (registers)
 template <int D>
 constexpr int64_t kOneTokens = D == 64 ? 1536 : D == 128 ? 1024 : 512;
+
+// Microseconds in chunks -> in one launch, steps of fp16 rows (bf16 rows: up to 0.8 more in one launch), D = 128. e4m3: 1 x 1024
+// tokens, one KV head of 8 query heads, 11.6 -> 10.7; 1 x 512 11.6 -> 8.3; 8 KV heads of 4, 1 x 1024 12.1 -> 10.9, 4 x 256 12.4
+// -> 7.5, 16 x 64 10.5 -> 6.3. At D = 64 1 x 1536 10.2 -> 9.8, at 256 1 x 512 14.4 -> 12.9. A call of few KV heads takes
+// fewer workgroups in chunks, and int8's conversions and more query heads' joins cost one launch more:
+//   int8, one KV head of 8: 1 x 768 11.9 -> 10.8, 1 x 1024 12.0 -> 12.2 (8 KV heads of 8: 13.0 -> 12.9; D = 256, 1 x 512: 14.5
+//   -> 14.5)
+//   one KV head of 16: e4m3 1 x 768 11.6 -> 10.5, 1 x 1024 11.8 -> 11.9; int8 1 x 512 12.2 -> 10.2, 1 x 768 12.1 -> 12.3 (8 KV
+//   heads of 16: e4m3 1 x 1024 13.1 -> 12.4; int8 1 x 768 13.7 -> 12.7, 1 x 896 13.7 -> 14.1; D = 256, 1 x 512 22.3 -> 16.3)
+template <int D, typename F>
+int64_t one_launch_tokens(const DecodeParams& p) {
+  const bool few_heads = p.head_groups == 1, many_cols = p.group > 8;
+  int64_t most = kOneTokens<D>;
+  if (F::kNanScale && D < 256 && (few_heads || many_cols)) most = most * 3 / 4;
+  if (few_heads && many_cols) most = most * 3 / 4;
+  return most;
+}
 
 template <typename T, int D, bool kTileInPage, int kDepth, bool kGrouped, typename F, bool kOne = false>
 __global__ void __launch_bounds__(64 * (kOne ? kOneWaves<D> : kMaxWaves), (kMinWaves<D, F>))
@@ -1593,7 +1608,8 @@ template <typename T, int D, bool kGrouped, typename F>
 int launch_decode(const DecodeParams& p, const MergeParams& mp, const GroupArgs<kGrouped>& ga, int waves,
                   hipStream_t s) {
   if constexpr (F::kQ8 && !kGrouped) {
-    if (p.total_pages * p.page_size <= kOneTokens<D> && p.page_size % 16 == 0 && (int64_t)p.batch * p.num_kv_heads <= 256) {
+    if (p.total_pages * p.page_size <= one_launch_tokens<D, F>(p) && p.page_size % 16 == 0 &&
+        (int64_t)p.batch * p.num_kv_heads <= 256) {
       paged_decode_kernel<T, D, true, kTileDepth<F, true>, false, F, true>
           <<<dim3(p.batch, p.num_kv_heads), 64 * kOneWaves<D>, 0, s>>>(p, ga);
       return check_launch("paged_decode");
