@@ -1504,14 +1504,13 @@ inline bool stream_capturing(hipStream_t s) {
 // loads; smaller ones are left in the caches (MI355X: 256 MB of memory-side cache).
 constexpr int64_t kStreamBytes = (int64_t)128 << 20;
 
+// Buffers of tiles: one computed, the others in flight. (16-bit tiles of 16 tokens and pairs of 8-bit ones
+// are 8 KB of K and V at D = 128.)
+constexpr int kTileDepth = 2;
+
 // The first call of a variant on a device queries the device (attribute and
 // occupancy); a call whose stream is being captured into a graph must not make
 // those queries, so it returns 0 (refused) when the figure is not cached yet.
-// Buffers of tiles: one computed, the others in flight. (16-bit tiles of 16 tokens and pairs of 8-bit ones
-// are 8 KB of K and V at D = 128.)
-template <typename F, bool kTileInPage>
-constexpr int kTileDepth = 2;
-
 template <typename T, int D, bool kTileInPage, bool kGrouped, typename F>
 int decode_wg_slots(int waves, const CaptureCheck& cc) {
   static std::atomic<int> cache[kMaxDevices][kMaxWaves + 1];
@@ -1525,8 +1524,8 @@ int decode_wg_slots(int waves, const CaptureCheck& cc) {
   if (cc.check && stream_capturing(cc.stream)) return 0;
   int cus = 0, per_cu = 0;
   if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-      hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, paged_decode_kernel<T, D, kTileInPage, kTileDepth<F, kTileInPage>, kGrouped, F>,
-                                                   64 * waves, 0) != hipSuccess ||
+      hipOccupancyMaxActiveBlocksPerMultiprocessor(
+          &per_cu, paged_decode_kernel<T, D, kTileInPage, kTileDepth, kGrouped, F>, 64 * waves, 0) != hipSuccess ||
       cus <= 0 || per_cu <= 0) {
     (void)hipGetLastError();
     return kDefaultSlots;
@@ -1610,16 +1609,16 @@ int launch_decode(const DecodeParams& p, const MergeParams& mp, const GroupArgs<
   if constexpr (F::kQ8 && !kGrouped) {
     if (p.total_pages * p.page_size <= one_launch_tokens<D, F>(p) && p.page_size % 16 == 0 &&
         (int64_t)p.batch * p.num_kv_heads <= 256) {
-      paged_decode_kernel<T, D, true, kTileDepth<F, true>, false, F, true>
+      paged_decode_kernel<T, D, true, kTileDepth, false, F, true>
           <<<dim3(p.batch, p.num_kv_heads), 64 * kOneWaves<D>, 0, s>>>(p, ga);
       return check_launch("paged_decode");
     }
   }
   const dim3 grid((unsigned)p.max_chunks, (unsigned)p.head_groups);
   if (p.page_size % 16 == 0)
-    paged_decode_kernel<T, D, true, kTileDepth<F, true>, kGrouped, F><<<grid, 64 * waves, 0, s>>>(p, ga);
+    paged_decode_kernel<T, D, true, kTileDepth, kGrouped, F><<<grid, 64 * waves, 0, s>>>(p, ga);
   else
-    paged_decode_kernel<T, D, false, kTileDepth<F, false>, kGrouped, F><<<grid, 64 * waves, 0, s>>>(p, ga);
+    paged_decode_kernel<T, D, false, kTileDepth, kGrouped, F><<<grid, 64 * waves, 0, s>>>(p, ga);
   int rc = check_launch("paged_decode");
   if (rc) return rc;
   // sequences of many chunks (small batches) split their partials over 4 waves; over 8-bit pools where a wave would take

@@ -177,7 +177,7 @@ __device__ inline void transpose4x4(const uint32_t (&r)[4], uint32_t (&c)[4]) {
   c[3] = __builtin_amdgcn_perm(t3, t1, 0x07060302u);
 }
 
-// Largest of the lanes' values (bit patterns of non-negative floats), and whether any lane's flag is set.
+// Largest of the lanes' values (bit patterns of non-negative floats).
 __device__ inline uint32_t wave_max_bits(uint32_t x) { return (uint32_t)wave_max_i32((int)x); }
 
 // A wave's new rows of one block of one KV head: each lane holds 8 elements of one row, 512 / D rows a
