@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
   float thr[kCB];
   float neg_m[kCB];
   constexpr bool kMayHalfPV = F::kQ8 && kSplitP;
-  float p_up = 0.f;  // (kMayHalfPV) log2 of a factor on the probabilities, and so on o and lsum
+  float p_up = 0.f;  // (kMayHalfPV) log2 of a factor on the probabilities, taken out of o and lsum after the loop
   const float inv_scale_log2 = 1.f / p.scale_log2;
   f32x4 o[kCB][NT];
 #pragma unroll
@@ -667,7 +667,7 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
       // exponent fields: the largest scale to 2^5, at least the 127 - 120 of a factor that is a normal number
       const uint32_t ex = top == 0 ? 127u : max(top >> 23, 12u) - 5u;
       v_in = __uint_as_float((254u - ex) << 23);
-      v_out = __uint_as_float(ex << 23);
+      v_out = __uint_as_float(ex << 23) * 0x1p-7f;
       p_up = 7.f;
       constexpr std::true_type half_pv;
 #include "paged_prefill_loop.inc"
@@ -686,11 +686,12 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
   asm volatile("" : "+v"(er));
 #pragma unroll
   for (int cb = 0; cb < kCB; ++cb) {
-    if constexpr (F::kQ8) {  // V went in at another scale
+    if constexpr (F::kQ8) {  // V went in at another scale (and P)
 #pragma unroll
       for (int n = 0; n < NT; ++n) o[cb][n] *= v_out;
     }
-    const float l_tot = lsum[cb][0];
+    float l_tot = lsum[cb][0];
+    if constexpr (kMayHalfPV) l_tot *= p_up != 0.f ? 0x1p-7f : 1.f;
     const int row = row0_wg + wave * kRowsPerWave + cb * 16 + er;
     if (row >= nrows) continue;
     const int t = row / G;
@@ -699,8 +700,7 @@ __global__ void __launch_bounds__(64 * PrefillTile<D>::kWaves) paged_prefill_ker
       if (q0 + t >= p.total_q) continue;  // past the partials: not a row of this call
       if (merged) {
         const int64_t slot = (int64_t)(run / p.num_kv_heads) * p.total_q * p.num_qo_heads + pr;
-        // (m for the factor on P too: l and o are relative to 2^-neg_m)
-        if (gq == 0) p.part_ml[slot] = float2{thr[cb] == -INFINITY ? -INFINITY : -neg_m[cb], l_tot};
+        if (gq == 0) p.part_ml[slot] = float2{run_max(cb), l_tot};
         float* po = p.part_o + slot * D + 4 * gq;
 #pragma unroll
         for (int n = 0; n < NT; ++n) *reinterpret_cast<f32x4*>(po + 16 * n) = o[cb][n];

@@ -82,3 +82,14 @@ def test_small_weights_on_large_values(code, d, max_kv, apart):
     # (in several runs, those behind the sink's have one scale and equal weights)
     by = "bf16up" if apart <= 8 else "bf16runs" if max_kv else "bf16"
     prefill(twins, pools, n, rows, np.arange(2, 41) + 0.5, max_kv, by)
+
+
+@pytest.mark.parametrize("max_kv", [0, 20000])
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_equal_weights_on_values_near_bf16s_end(code, max_kv):
+    """1500 keys of V up to 2^110.8: their sum, 2^121.4, is in fp32's range with room for the maximum's lag only."""
+    n, rows = 1500, 40
+    g = np.random.default_rng(3)
+    v = g.integers(1, 8, (1, HKV, 128)) * 8.0 + np.zeros((n, 1, 1))
+    twins, pools = layer(code, 128, n, v, np.full(-(-n // PAGE), 2.0 ** 105))
+    prefill(twins, pools, n, rows, np.zeros(1), max_kv, "bf16up")
