@@ -681,6 +681,99 @@ int nslg_rope_append(const void* q, int64_t q_stride, void* q_out, int64_t q_out
                      int32_t head_dim, void* k_pool, void* v_pool, int64_t pool_slots,
                      int32_t dtype, nslg_stream_t stream);
 
+/*
+ * ---- trees of drafted tokens (speculative decoding) ----
+ *
+ * A tree has n_b nodes, each one token: node 0, its root, is the sequence's last sampled token; the
+ * others are drafted. parents[j] < j is node j's parent, -1 a root's; children of a node are in the order of
+ * their indices. The trees of a batch are ragged: nodes of sequence b are rows qo_indptr[b] ..
+ * qo_indptr[b + 1] - 1 of total_q; a tree has at most max_q nodes, max_q <= 1024. While a tree is verified its
+ * nodes are the last n_b of the sequence's L_b tokens, in the order of their indices, start_b = L_b - n_b.
+ * With q_rows (int32[total_q]), rows of the model's tensors are those of a padded grid of batch * grid_width
+ * rows, as in nslg_paged_prefill_grid. Tables of plan and trees are device arrays.
+ */
+
+/*
+ * Masks and positions of a batch of trees.
+ *   parents         int32[total_q]; an entry that is not below its node's index counts as -1
+ *   start           int32[batch]: tokens before each tree
+ *   mask            uint32[total_q][mask_words], mask_words >= ceil(max_q / 32): bit j % 32 of word j / 32 of
+ *                   node t's row is set when t sees node j of its tree: an ancestor or t itself
+ *   positions       int32[total_q], or with q_rows [batch * grid_width] (0 on rows without a node):
+ *                   start + the number of ancestors
+ */
+int nslg_tree_plan(const int32_t* parents, const int32_t* qo_indptr, const int32_t* start, const int32_t* q_rows,
+                   int32_t grid_width, int64_t total_q, int32_t max_q, int32_t batch, uint32_t* mask,
+                   int32_t mask_words, int32_t* positions, nslg_stream_t stream);
+
+/*
+ * Attention of a batch of trees over one layer of a paged cache: node t of sequence b sees the start_b tokens before its
+ * tree and the nodes whose bits its mask row has (nslg_tree_plan's, or any other). A row that sees no token is zero.
+ * What an unseen token holds (infinities and NaN too) does not reach a row.
+ *   k_new, v_new    null: the nodes' K/V rows are in the pool; else rows of Hkv*D elements at element
+ *                   strides, 16-byte aligned, laid out as q's rows: they are written to the nodes' slots and read from
+ *                   there, in the same launch. No other sequence of the call may read a page written.
+ *   total_pages     host copy of kv_indptr[batch] (sizes the launch; another value only costs time)
+ *   workspace       of nslg_paged_tree_workspace_size bytes: keys are then cut into chunks and merged (a second
+ *                   launch). Null or smaller: fewer chunks, or one. One call at a time may use it; calls of other
+ *                   kinds may take it in turn.
+ *   other arguments as nslg_paged_prefill_grid. f16, bf16 and f32, D in {64, 128, 256}, 1 <= Hq/Hkv <= 16.
+ */
+size_t nslg_paged_tree_workspace_size(int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
+                                      int64_t total_pages, int32_t page_size, int32_t max_q, int32_t dtype);
+int nslg_paged_tree_attention(const void* q, int64_t q_stride, const uint32_t* mask, int32_t mask_words,
+                              const int32_t* qo_indptr, const int32_t* q_rows, int32_t grid_width, int64_t total_q,
+                              int32_t max_q, const void* k_new, int64_t k_new_stride, const void* v_new,
+                              int64_t v_new_stride, void* k_pool, void* v_pool, int64_t num_pages,
+                              int32_t page_size, const int32_t* kv_indptr, const int32_t* kv_indices,
+                              const int32_t* kv_last_page_len, int64_t total_pages, int32_t batch,
+                              int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim, float sm_scale,
+                              int32_t dtype, void* out, int64_t out_stride, void* workspace, size_t workspace_bytes,
+                              nslg_stream_t stream);
+
+/*
+ * Verify drafted tokens against the target's probabilities, from given uniform numbers in [0, 1). At a node (the root
+ * first) with target row p, its children are tried in the order of their indices, child j with token x:
+ *   draft_probs null (drafted tokens are given, not drawn):
+ *       accepted if u_accept[j] W < r(x), r = p and W = 1 at first; once rejected, W loses r(x) and r(x) is 0;
+ *   draft_probs given (children drawn, independently, from the node's draft row q):
+ *       accepted if u_accept[j] q(x) W < r(x); once rejected, r becomes max(r / W - q, 0) and W its sum.
+ * The accepted child is the next node. Where none is, the next token is drawn from r: the first one at which the
+ * running sum of r exceeds u_next[b] times its sum. Tokens so accepted and drawn have the target's distribution.
+ * Tests and sums are in 64 bits. Negative weights and those that are not finite count as 0; where nothing is left
+ * of r the token is drawn from p, and next_token is -1 where p holds nothing either (or the sequence has no nodes).
+ * A drafted token outside the vocabulary is rejected. Probabilities of exactly one token (p(x) = 1) make
+ * this greedy verification.
+ *   target_probs, draft_probs   num_rows rows of vocab values (f16, bf16 or f32) at element strides: the row of node
+ *                   t is t, or q_rows[t]
+ *   u_accept        float[total_q] (a root's is not read); u_next float[batch]
+ *   path            int32[batch][max_q]: the accepted nodes, node 0 first, -1 after them
+ *   count, next_token   int32[batch]
+ *   workspace       may be null
+ * vocab <= 2^20.
+ */
+int nslg_verify_tree(const int32_t* tokens, const int32_t* parents, const int32_t* qo_indptr, const int32_t* q_rows,
+                     int64_t total_q, int32_t max_q, int32_t batch, const void* target_probs, int64_t target_stride,
+                     const void* draft_probs, int64_t draft_stride, int64_t num_rows, int32_t vocab, int32_t dtype,
+                     const float* u_accept, const float* u_next, int32_t* path, int32_t* count, int32_t* next_token,
+                     void* workspace, size_t workspace_bytes, nslg_stream_t stream);
+
+/*
+ * Move the accepted nodes' K/V rows to the slots behind their sequence's tokens, in every layer: the row of node
+ * path[b][i] to position start_b + i, for i < count[b].
+ *   k_pool, v_pool  the [L, P, page_size, Hkv, D] pools
+ *   path            int32[batch][path_stride], rising node indices (a sequence whose first count[b] entries are
+ *                   not rising nodes of its tree is left as it is)
+ *   qo_indptr, kv_indptr, kv_indices, kv_last_page_len   the trees and the block table that the tree's
+ *                   attention ran with
+ * Rows whose page id is outside the pool are skipped. Bit-exact copy. batch <= 65535.
+ */
+int nslg_move_accepted(void* k_pool, void* v_pool, int32_t num_layers, int64_t num_pages, int32_t page_size,
+                       int32_t num_kv_heads, int32_t head_dim, int32_t dtype, const int32_t* path,
+                       int32_t path_stride, const int32_t* count, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                       const int32_t* kv_indices, const int32_t* kv_last_page_len, int32_t batch,
+                       nslg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

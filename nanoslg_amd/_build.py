@@ -24,6 +24,8 @@ FAST_SRC = CSRC / "fastcall.c"
 FAST_PATH = PKG_DIR / ("_nslg_fast" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 FAST_Q8_SRC = CSRC / "fastcall_q8.c"  # the same of the 8-bit cache's entry points
 FAST_Q8_PATH = PKG_DIR / ("_nslg_fast_q8" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+FAST_TREE_SRC = CSRC / "fastcall_tree.c"  # and of those for trees of drafted tokens
+FAST_TREE_PATH = PKG_DIR / ("_nslg_fast_tree" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 # the host-side forward planner (plain C over the CPython API, no GPU code)
 HOST_SRC = CSRC / "host_plan.c"
 HOST_PATH = PKG_DIR / ("_nslg_host" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
@@ -92,7 +94,7 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
     _build_host()
     if verbose:
         print(f"[nanoslg_amd] built {LIB_PATH} from {len(srcs)} sources, {FAST_PATH.name}, "
-              f"{FAST_Q8_PATH.name} and {HOST_PATH.name}",
+              f"{FAST_Q8_PATH.name}, {FAST_TREE_PATH.name} and {HOST_PATH.name}",
               file=sys.stderr)
     return LIB_PATH
 
@@ -117,7 +119,7 @@ def _build_ext(src: Path, out: Path, link: list[str]) -> None:
 def _build_fast() -> None:
     """Compile the fast-call bindings (host C, the system compiler) against the
     library just linked; they find the library next to themselves at run time."""
-    for src, out in ((FAST_SRC, FAST_PATH), (FAST_Q8_SRC, FAST_Q8_PATH)):
+    for src, out in ((FAST_SRC, FAST_PATH), (FAST_Q8_SRC, FAST_Q8_PATH), (FAST_TREE_SRC, FAST_TREE_PATH)):
         _build_ext(src, out, [f"-L{PKG_DIR}", "-lnslg_kv", "-Wl,-rpath,$ORIGIN"])
 
 

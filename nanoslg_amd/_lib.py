@@ -122,6 +122,21 @@ SIGNATURES = {
                                         c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p,
                                         c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_int32, c_void_p,
                                         c_int64, c_void_p, c_size_t, c_void_p]),
+    "nslg_tree_plan": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int32, c_void_p,
+                                 c_int32, c_void_p, c_void_p]),
+    "nslg_paged_tree_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int64, c_int32, c_int32,
+                                                  c_int32]),
+    "nslg_paged_tree_attention": (c_int32, [c_void_p, c_int64, c_void_p, c_int32, c_void_p, c_void_p, c_int32,
+                                            c_int64, c_int32, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                            c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_int64,
+                                            c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_void_p, c_int64,
+                                            c_void_p, c_size_t, c_void_p]),
+    "nslg_verify_tree": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_void_p,
+                                   c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, c_void_p, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "nslg_move_accepted": (c_int32, [c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int32, c_int32, c_int32,
+                                     c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32,
+                                     c_void_p]),
 }
 
 _lib = None
@@ -190,6 +205,24 @@ def fast_q8():
                                  "run `python -m nanoslg_amd._build` (or __graft_entry__.build()) first") from e
     _fast_q8 = _nslg_fast_q8
     return _fast_q8
+
+
+_fast_tree = None
+
+
+def fast_tree():
+    """The fast-call binding of the entry points for trees of drafted tokens, as fast() is of the others."""
+    global _fast_tree
+    if _fast_tree is not None:
+        return _fast_tree
+    load()
+    try:
+        from . import _nslg_fast_tree
+    except ImportError as e:
+        raise KernelLibraryError(f"the fast-call binding of {LIB_PATH} is not built or does not load ({e}); "
+                                 "run `python -m nanoslg_amd._build` (or __graft_entry__.build()) first") from e
+    _fast_tree = _nslg_fast_tree
+    return _fast_tree
 
 
 _host = None

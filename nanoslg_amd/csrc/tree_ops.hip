@@ -1,0 +1,484 @@
+// What a step of speculative decoding needs besides its attention, for gfx950: the trees' ancestor masks and positions, the
+// verification of the drafted tokens, and the move of the accepted nodes' K/V.
+#include "nslg_common.h"
+
+namespace nslg {
+namespace {
+
+constexpr int kTreeMaxNodes = 1024;
+
+// ---- masks and positions ---------------------------------------------------------------
+// One workgroup per tree: the parents in LDS, a thread a node. A node's ancestors have falling indices, so its
+// words are built from the last to the first in one register.
+struct TreePlanParams {
+  const int32_t* parents;
+  const int32_t* qo_indptr;
+  const int32_t* start;
+  const int32_t* q_rows;
+  int32_t grid_width;
+  int64_t total_q;
+  int32_t max_q;
+  int32_t batch;
+  uint32_t* mask;
+  int32_t mask_words;
+  int32_t* positions;
+};
+
+__global__ void __launch_bounds__(256) tree_plan_kernel(TreePlanParams p) {
+  __shared__ int parent[kTreeMaxNodes];
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const int q0 = p.qo_indptr[b];
+  const int n = (int)min((int64_t)min(max(p.qo_indptr[b + 1] - q0, 0), p.max_q), p.total_q - q0);
+  for (int j = tid; j < n; j += 256) parent[j] = p.parents[q0 + j];
+  const int64_t row0 = (int64_t)b * p.grid_width;
+  int64_t at0 = 0;  // the grid row of node 0
+  if (p.q_rows) {
+    at0 = n > 0 ? (int64_t)p.q_rows[q0] : row0;
+    for (int c = tid; c < p.grid_width; c += 256)
+      if (row0 + c < at0 || row0 + c >= at0 + n) p.positions[row0 + c] = 0;
+  }
+  __syncthreads();
+  const int start = p.start[b];
+  for (int j = tid; j < n; j += 256) {
+    uint32_t* row = p.mask + (int64_t)(q0 + j) * p.mask_words;
+    int a = j, depth = 0;
+    for (int w = p.mask_words - 1; w >= 0; --w) {
+      uint32_t bits = 0;
+      while (a >= 0 && a >> 5 == w) {
+        bits |= 1u << (a & 31);
+        const int up = parent[a];
+        a = up < a ? up : -1;  // (an ancestor that does not lie before its child: a root)
+        depth += a >= 0;
+      }
+      row[w] = bits;
+    }
+    const int64_t at = p.q_rows ? p.q_rows[q0 + j] : q0 + j;
+    if (!p.q_rows || (at >= 0 && at < (int64_t)p.batch * p.grid_width)) p.positions[at] = start + depth;
+  }
+}
+
+// ---- verification ----------------------------------------------------------------------
+// One workgroup per sequence. Its first wave walks down from the root, 64 nodes at a time with the probabilities
+// that their tests take already loaded. At a node with target row p and draft row q, what is left of p once drawn
+// children were rejected is, up to a factor, max(p - c q, 0): taking max(r / W - q, 0), W the sum of r, from r =
+// max(p - c q, 0) leaves max(p - (c + W) q, 0) / W. So a rejection needs the sum of that at the new c and nothing else,
+// which all waves find together. Then the row that the next token is drawn from is summed in pieces of
+// kVerPiece tokens, the piece that holds it found from their running sum, and the token inside it.
+//
+// Sums and tests are in 64 bits: the order of adding decides no token.
+struct VerifyParams {
+  const int32_t* tokens;
+  const int32_t* parents;
+  const int32_t* qo_indptr;
+  const int32_t* q_rows;
+  int64_t total_q;
+  int32_t max_q;
+  int32_t batch;
+  int64_t rows;  // rows of the probabilities
+  const char* target;
+  int64_t target_stride;  // bytes
+  const char* draft;
+  int64_t draft_stride;
+  int32_t vocab;
+  const float* u_accept;
+  const float* u_next;
+  int32_t* path;
+  int32_t* count;
+  int32_t* next;
+};
+
+constexpr int kVerThreads = 1024;
+constexpr int kVerWaves = kVerThreads / 64;
+constexpr int kVerPiece = 256;       // tokens of a piece: a wave, four each
+constexpr int kVerMaxPieces = 4096;  // (32 KB of LDS)
+
+template <typename T>
+__device__ inline float prob_of(const char* row, int i) {
+  if constexpr (T::kDtype == NSLG_F32)
+    return reinterpret_cast<const float*>(row)[i];
+  else
+    return T::to_f32(reinterpret_cast<const uint16_t*>(row)[i]);
+}
+
+struct VF32 {
+  static constexpr int kDtype = NSLG_F32;
+};
+
+// The weight that token i has left: p - c q, not below 0; what is no number counts nothing.
+template <typename T, bool kDraft>
+__device__ inline double weight_of(const char* prow, const char* qrow, double c, int i) {
+  double x = (double)prob_of<T>(prow, i);
+  if constexpr (kDraft)
+    if (c != 0.0) x -= c * (double)prob_of<T>(qrow, i);
+  return x > 0.0 && x < INFINITY ? x : 0.0;
+}
+
+__device__ inline double wave_sum_f64(double x) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
+
+template <typename T, bool kDraft>
+__global__ void __launch_bounds__(kVerThreads) tree_verify_kernel(VerifyParams p) {
+  __shared__ double piece[kVerMaxPieces];
+  __shared__ double wave_part[kVerWaves];
+  __shared__ int rejected[kDraft ? 1 : kTreeMaxNodes];  // tokens rejected at the present node
+  __shared__ int s_cmd, s_row, s_rejects, s_at;
+  __shared__ double s_c, s_sum;
+
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int q0 = p.qo_indptr[b];
+  const int n = (int)min((int64_t)min(max(p.qo_indptr[b + 1] - q0, 0), p.max_q), p.total_q - q0);
+  int32_t* path = p.path + (int64_t)b * p.max_q;
+  if (n <= 0) {  // no tree: nothing accepted, no token
+    for (int i = tid; i < p.max_q; i += kVerThreads) path[i] = -1;
+    if (tid == 0) p.count[b] = 0, p.next[b] = -1;
+    return;
+  }
+  auto row_of = [&](int node) -> int64_t {
+    const int64_t at = p.q_rows ? p.q_rows[q0 + node] : q0 + node;
+    return at < 0 ? 0 : (at >= p.rows ? p.rows - 1 : at);
+  };
+  // state of the walk (wave 0, uniform)
+  int cur = 0, from = 1, count = 1, rejects = 0;
+  double c = 0.0, W = 1.0;
+  if (tid == 0) path[0] = 0;
+  while (true) {
+    if (wave == 0) {
+      int cmd = 0;  // 1: the sum at c is wanted, 0: done
+      while (from < n && cmd == 0) {
+        const int base = from & ~63;
+        const int j = base + lane;
+        const int up = j < n ? p.parents[q0 + j] : -2;
+        const int x = j < n ? p.tokens[q0 + j] : -1;
+        const float u = j < n ? p.u_accept[q0 + j] : 0.f;
+        const bool tried = up >= 0 && up < j && x >= 0 && x < p.vocab;
+        double pj = 0.0, qj = 1.0;
+        if (tried) {
+          const int64_t at = row_of(up);
+          pj = (double)prob_of<T>(p.target + at * p.target_stride, x);
+          if constexpr (kDraft) qj = (double)prob_of<T>(p.draft + at * p.draft_stride, x);
+        }
+        while (cmd == 0) {
+          const unsigned long long m = __ballot(j >= from && j < n && up == cur);
+          if (m == 0) {
+            from = base + 64;
+            break;
+          }
+          const int src = __ffsll((long long)m) - 1;
+          from = base + src + 1;
+          const bool ok_token = __shfl((int)tried, src, 64);
+          const int xs = __shfl(x, src, 64);
+          double left = __shfl(pj, src, 64);
+          const double q = __shfl(qj, src, 64);
+          const double us = (double)__shfl(u, src, 64);
+          if constexpr (kDraft) {
+            if (c != 0.0) left -= c * q;
+          } else {
+            bool again = false;
+            for (int i = lane; i < rejects; i += 64) again |= rejected[i] == xs;
+            if (__ballot(again)) left = 0.0;
+          }
+          left = ok_token && left > 0.0 && left < INFINITY ? left : 0.0;
+          if (us * W * q < left) {  // accepted
+            cur = base + src;
+            if (lane == 0 && count < p.max_q) path[count] = cur;
+            ++count;
+            c = 0.0, W = 1.0, rejects = 0;
+            continue;
+          }
+          if constexpr (kDraft) {
+            if (W > 0.0) c += W, cmd = 1;
+          } else {
+            W -= left;
+            if (left > 0.0) {
+              if (lane == 0) rejected[rejects] = xs;
+              ++rejects;
+              // (one wave's LDS operations complete in order; the fence is for the compiler)
+              __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            }
+          }
+        }
+      }
+      if (lane == 0) s_cmd = cmd, s_row = cur, s_c = c, s_rejects = rejects;
+    }
+    __syncthreads();
+    if (s_cmd == 0) break;
+    // the sum of what is left at c
+    const int64_t at = row_of(s_row);
+    const char* prow = p.target + at * p.target_stride;
+    const char* qrow = p.draft + at * p.draft_stride;
+    double x = 0.0;
+    for (int i = tid; i < p.vocab; i += kVerThreads) x += weight_of<T, kDraft>(prow, qrow, s_c, i);
+    x = wave_sum_f64(x);
+    if (lane == 0) wave_part[wave] = x;
+    __syncthreads();
+    if (wave == 0) {
+      double sum = 0.0;
+      for (int i = 0; i < kVerWaves; ++i) sum += wave_part[i];
+      W = sum;
+    }
+    __syncthreads();
+  }
+  if (wave == 0) {
+    for (int i = count + lane; i < p.max_q; i += 64) path[i] = -1;
+    if (lane == 0) p.count[b] = count;
+  }
+
+  // ---- the next token
+  const int64_t at = row_of(s_row);
+  const char* prow = p.target + at * p.target_stride;
+  const char* qrow = kDraft ? p.draft + at * p.draft_stride : nullptr;
+  const int pieces = (p.vocab + kVerPiece - 1) / kVerPiece;
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    // (a second time with the row as it is, where rejections left nothing of it)
+    const double cc = attempt ? 0.0 : s_c;
+    const int gone = attempt || kDraft ? 0 : s_rejects;
+    auto left_of = [&](int i) -> double {
+      if (i >= p.vocab) return 0.0;
+      if constexpr (!kDraft)
+        for (int k = 0; k < gone; ++k)
+          if (rejected[k] == i) return 0.0;
+      return weight_of<T, kDraft>(prow, qrow, cc, i);
+    };
+    for (int g = wave; g < pieces; g += kVerWaves) {
+      double x = 0.0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x += left_of(g * kVerPiece + 64 * e + lane);
+      x = wave_sum_f64(x);
+      if (lane == 0) piece[g] = x;
+    }
+    __syncthreads();
+    if (wave == 0) {
+      double total = 0.0;
+      for (int g = lane; g < pieces; g += 64) total += piece[g];
+      total = wave_sum_f64(total);
+      int found = -1;
+      if (total > 0.0) {
+        const double goal = (double)p.u_next[b] * total;
+        double run = 0.0;
+        int last = -1;  // the last piece with any weight: where rounding leaves the goal unreached
+        double last_run = 0.0;
+        int g_at = -1;
+        for (int g0 = 0; g0 < pieces && g_at < 0; g0 += 64) {
+          const double mine = g0 + lane < pieces ? piece[g0 + lane] : 0.0;
+          double incl = mine;
+#pragma unroll
+          for (int off = 1; off < 64; off <<= 1) {
+            const double y = __shfl_up(incl, off, 64);
+            if (lane >= off) incl += y;
+          }
+          const unsigned long long hit = __ballot(run + incl > goal && mine > 0.0);
+          const unsigned long long some = __ballot(mine > 0.0);
+          if (hit) {
+            const int src = __ffsll((long long)hit) - 1;
+            g_at = g0 + src;
+            run += __shfl(incl - mine, src, 64);
+          } else {
+            if (some) {
+              const int src = 63 - __clzll((long long)some);
+              last = g0 + src;
+              last_run = run + __shfl(incl - mine, src, 64);
+            }
+            run += __shfl(incl, 63, 64);
+          }
+        }
+        if (g_at < 0) g_at = last, run = last_run;
+        for (int e = 0; e < 4 && found < 0; ++e) {
+          const int i = g_at * kVerPiece + 64 * e + lane;
+          const double mine = left_of(i);
+          double incl = mine;
+#pragma unroll
+          for (int off = 1; off < 64; off <<= 1) {
+            const double y = __shfl_up(incl, off, 64);
+            if (lane >= off) incl += y;
+          }
+          const unsigned long long hit = __ballot(run + incl > goal && mine > 0.0);
+          if (hit) found = g_at * kVerPiece + 64 * e + __ffsll((long long)hit) - 1;
+          run += __shfl(incl, 63, 64);
+        }
+        for (int e = 3; e >= 0 && found < 0; --e) {  // (not reached by a rounding: the last token with any weight)
+          const unsigned long long some = __ballot(left_of(g_at * kVerPiece + 64 * e + lane) > 0.0);
+          if (some) found = g_at * kVerPiece + 64 * e + 63 - __clzll((long long)some);
+        }
+      }
+      if (lane == 0) s_at = found;
+    }
+    __syncthreads();
+    if (s_at >= 0) break;
+    __syncthreads();  // (s_at is read before the second attempt writes it)
+  }
+  if (tid == 0) p.next[b] = s_at;
+}
+
+// ---- the accepted nodes' K/V -------------------------------------------------------------
+// A path's nodes have rising indices, so node path[i] >= i: reading eight of them ahead of the eight writes and
+// going up overwrites nothing that is still to be read. Workgroup: (layer and K | V, sequence); a thread keeps its
+// 16-byte word of the rows.
+struct MoveParams {
+  char* k_pool;
+  char* v_pool;
+  int64_t num_pages;
+  int32_t page_size;
+  int64_t row_bytes;
+  const int32_t* path;
+  int32_t path_stride;
+  const int32_t* count;
+  const int32_t* qo_indptr;
+  const int32_t* indptr;
+  const int32_t* indices;
+  const int32_t* last_len;
+};
+
+template <typename V>
+__global__ void __launch_bounds__(256) tree_move_kernel(MoveParams p) {
+  __shared__ int64_t src_lds[8], dst_lds[8];
+  const int b = blockIdx.y, tid = threadIdx.x;
+  const int layer = blockIdx.x >> 1;
+  const int n = max(p.qo_indptr[b + 1] - p.qo_indptr[b], 0);
+  const int count = min(p.count[b], min(n, p.path_stride));
+  const int32_t* path = p.path + (int64_t)b * p.path_stride;
+  // a path: rising nodes of the tree
+  bool ok = true;
+  for (int i = tid; i < count; i += 256) {
+    const int a = path[i];
+    ok &= a >= 0 && a < n && (i == 0 || a > path[i - 1]);
+  }
+  if (__syncthreads_or(!ok)) return;
+  const int np = p.indptr[b + 1] - p.indptr[b];
+  int lpl = p.last_len[b];
+  lpl = lpl < 1 ? 1 : (lpl > p.page_size ? p.page_size : lpl);
+  const int len = np > 0 ? (np - 1) * p.page_size + lpl : 0;
+  const int start = len - n;
+  if (start < 0) return;
+  const int32_t* idx = p.indices + p.indptr[b];
+  char* pool = (blockIdx.x & 1 ? p.v_pool : p.k_pool) + (int64_t)layer * p.num_pages * p.page_size * p.row_bytes;
+  auto slot = [&](int node) -> int64_t {
+    const int pos = start + node;
+    const int pid = idx[pos / p.page_size];
+    return pid < 0 || (int64_t)pid >= p.num_pages ? -1 : (int64_t)pid * p.page_size + pos % p.page_size;
+  };
+  const int vecs = (int)(p.row_bytes / (int64_t)sizeof(V));
+  for (int i0 = 0; i0 < count; i0 += 8) {
+    if (tid < 8) {
+      const int i = i0 + tid;
+      int64_t s = -1, d = -1;
+      if (i < count && path[i] != i) s = slot(path[i]), d = slot(i);
+      src_lds[tid] = s < 0 || d < 0 ? -1 : s;
+      dst_lds[tid] = d;
+    }
+    __syncthreads();
+    for (int w = tid; w < vecs; w += 256) {
+      V x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (src_lds[u] >= 0) x[u] = reinterpret_cast<const V*>(pool + src_lds[u] * p.row_bytes)[w];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (src_lds[u] >= 0) reinterpret_cast<V*>(pool + dst_lds[u] * p.row_bytes)[w] = x[u];
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace
+}  // namespace nslg
+
+using namespace nslg;
+
+extern "C" int nslg_tree_plan(const int32_t* parents, const int32_t* qo_indptr, const int32_t* start,
+                              const int32_t* q_rows, int32_t grid_width, int64_t total_q, int32_t max_q, int32_t batch,
+                              uint32_t* mask, int32_t mask_words, int32_t* positions, nslg_stream_t stream) {
+  if (batch < 0 || total_q < 0 || max_q < 0 || (int64_t)max_q * batch < total_q)
+    return fail(NSLG_EINVAL, "tree_plan: %lld nodes in %d trees of at most %d", (long long)total_q, batch, max_q);
+  if (max_q > kTreeMaxNodes) return fail(NSLG_EUNSUPPORTED, "tree_plan: trees of up to %d nodes (%d)", kTreeMaxNodes, max_q);
+  if (q_rows && (grid_width < 1 || (int64_t)batch * grid_width > 0x7fffffff || total_q > (int64_t)batch * grid_width))
+    return fail(NSLG_EINVAL, "tree_plan: grid of %d x %d rows for %lld nodes", batch, grid_width, (long long)total_q);
+  if (batch == 0 || (total_q == 0 && !q_rows)) return NSLG_OK;
+  if (mask_words < (max_q + 31) / 32) return fail(NSLG_EINVAL, "tree_plan: masks of %d words for %d nodes", mask_words, max_q);
+  if (!qo_indptr || !start || !positions || (total_q > 0 && (!parents || !mask)))
+    return fail(NSLG_EINVAL, "tree_plan: null pointer");
+  TreePlanParams p = {parents, qo_indptr, start, q_rows, grid_width, total_q, max_q, batch, mask, mask_words, positions};
+  tree_plan_kernel<<<dim3((unsigned)batch), 256, 0, as_stream(stream)>>>(p);
+  return check_launch("tree_plan");
+}
+
+extern "C" int nslg_verify_tree(const int32_t* tokens, const int32_t* parents, const int32_t* qo_indptr,
+                                const int32_t* q_rows, int64_t total_q, int32_t max_q, int32_t batch,
+                                const void* target_probs, int64_t target_stride, const void* draft_probs,
+                                int64_t draft_stride, int64_t num_rows, int32_t vocab, int32_t dtype,
+                                const float* u_accept, const float* u_next, int32_t* path, int32_t* count,
+                                int32_t* next_token, void* workspace, size_t workspace_bytes, nslg_stream_t stream) {
+  (void)workspace;
+  (void)workspace_bytes;
+  const int eb = elem_bytes(dtype);
+  if (!eb) return fail(NSLG_EINVAL, "verify_tree: bad dtype %d", dtype);
+  if (batch < 0 || total_q < 0 || max_q < 0 || (int64_t)max_q * batch < total_q)
+    return fail(NSLG_EINVAL, "verify_tree: %lld nodes in %d trees of at most %d", (long long)total_q, batch, max_q);
+  if (max_q > kTreeMaxNodes)
+    return fail(NSLG_EUNSUPPORTED, "verify_tree: trees of up to %d nodes (%d)", kTreeMaxNodes, max_q);
+  if (vocab < 1 || num_rows < 0 || (num_rows < 1 && total_q > 0) || (!q_rows && num_rows < total_q))
+    return fail(NSLG_EINVAL, "verify_tree: %lld rows of %d probabilities for %lld nodes", (long long)num_rows, vocab,
+                (long long)total_q);
+  if (batch == 0) return NSLG_OK;
+  if (vocab > kVerMaxPieces * kVerPiece)
+    return fail(NSLG_EUNSUPPORTED, "verify_tree: vocabularies of up to %d tokens (%d)", kVerMaxPieces * kVerPiece, vocab);
+  if (!qo_indptr || !count || !next_token || !u_next || (max_q > 0 && !path) ||
+      (total_q > 0 && (!tokens || !parents || !target_probs || !u_accept)))
+    return fail(NSLG_EINVAL, "verify_tree: null pointer");
+  if (target_stride < vocab || (draft_probs && draft_stride < vocab))
+    return fail(NSLG_EINVAL, "verify_tree: row stride smaller than the vocabulary");
+  if (((uintptr_t)target_probs | (uintptr_t)draft_probs) % eb) return fail(NSLG_EINVAL, "verify_tree: unaligned rows");
+  VerifyParams p = {tokens, parents, qo_indptr, q_rows, total_q, max_q, batch, num_rows,
+                    (const char*)target_probs, target_stride * eb, (const char*)draft_probs, draft_stride * eb, vocab,
+                    u_accept, u_next, path, count, next_token};
+  hipStream_t s = as_stream(stream);
+  const dim3 grid((unsigned)batch);
+  auto launch = [&](auto type) {
+    using T = decltype(type);
+    if (draft_probs)
+      tree_verify_kernel<T, true><<<grid, kVerThreads, 0, s>>>(p);
+    else
+      tree_verify_kernel<T, false><<<grid, kVerThreads, 0, s>>>(p);
+  };
+  if (dtype == NSLG_F16)
+    launch(F16());
+  else if (dtype == NSLG_BF16)
+    launch(BF16());
+  else
+    launch(VF32());
+  return check_launch("verify_tree");
+}
+
+extern "C" int nslg_move_accepted(void* k_pool, void* v_pool, int32_t num_layers, int64_t num_pages, int32_t page_size,
+                                  int32_t num_kv_heads, int32_t head_dim, int32_t dtype, const int32_t* path,
+                                  int32_t path_stride, const int32_t* count, const int32_t* qo_indptr,
+                                  const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                                  int32_t batch, nslg_stream_t stream) {
+  const int eb = elem_bytes(dtype);
+  if (!eb) return fail(NSLG_EINVAL, "move_accepted: bad dtype %d", dtype);
+  if (num_layers <= 0 || num_pages <= 0 || page_size <= 0 || num_kv_heads <= 0 || head_dim <= 0 || batch < 0 || path_stride < 0)
+    return fail(NSLG_EINVAL, "move_accepted: bad sizes");
+  if (batch == 0 || path_stride == 0) return NSLG_OK;
+  if (!k_pool || !v_pool || !path || !count || !qo_indptr || !kv_indptr || !kv_indices || !kv_last_page_len)
+    return fail(NSLG_EINVAL, "move_accepted: null pointer");
+  if (batch > 65535) return fail(NSLG_EUNSUPPORTED, "move_accepted: batches of up to 65535 (%d)", batch);
+  if (num_layers > (1 << 24)) return fail(NSLG_EUNSUPPORTED, "move_accepted: too many layers");
+  if (num_pages * (int64_t)page_size >= ((int64_t)1 << 31))
+    return fail(NSLG_EUNSUPPORTED, "move_accepted: pool has >= 2^31 token slots");
+  const int64_t row_bytes = (int64_t)num_kv_heads * head_dim * eb;
+  MoveParams p = {(char*)k_pool, (char*)v_pool, num_pages, page_size, row_bytes, path, path_stride, count,
+                  qo_indptr, kv_indptr, kv_indices, kv_last_page_len};
+  const dim3 grid((unsigned)(2 * num_layers), (unsigned)batch);
+  hipStream_t s = as_stream(stream);
+  const uintptr_t all = (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)row_bytes;
+  if (all % 16 == 0)
+    tree_move_kernel<u32x4><<<grid, 256, 0, s>>>(p);
+  else if (all % 4 == 0)
+    tree_move_kernel<uint32_t><<<grid, 256, 0, s>>>(p);
+  else
+    tree_move_kernel<uint16_t><<<grid, 256, 0, s>>>(p);
+  return check_launch("move_accepted");
+}

@@ -1133,14 +1133,20 @@ def paged_prefill(q: torch.Tensor, qo_indptr: torch.Tensor, total_q: int, max_q:
     return out
 
 
-# the 8-bit cache's calls (nanoslg_amd.kernels_q8, which uses the above) under this module's name too
+# the 8-bit cache's calls (nanoslg_amd.kernels_q8, which uses the above) and those for trees of drafted tokens
+# (nanoslg_amd.kernels_tree) under this module's name too
 _Q8_CALLS = ("append_kv_q8", "gather_kv_q8", "paged_decode_q8", "paged_decode_append_q8", "paged_decode_rope_append_q8",
              "paged_prefill_q8", "rotate_rows", "DecodeLaunchQ8")
+_TREE_CALLS = ("tree_plan", "paged_tree_attention", "verify_tree", "move_accepted")
 
 
 def __getattr__(name: str):
     if name in _Q8_CALLS:
         from . import kernels_q8
         globals().update((n, getattr(kernels_q8, n)) for n in _Q8_CALLS)
+        return globals()[name]
+    if name in _TREE_CALLS:
+        from . import kernels_tree
+        globals().update((n, getattr(kernels_tree, n)) for n in _TREE_CALLS)
         return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
