@@ -20,14 +20,33 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace nslg {
 namespace {
 
-constexpr int kTreeWaves = 4;
-constexpr int kTreeThreads = 64 * kTreeWaves;
 constexpr int kTreeCUs = 256;
 constexpr int kTreeMaxNodes = 1024;
+constexpr int kTreeWin = 1024;    // page ids in LDS
+constexpr int kTreeRowWaves = 8;                  // waves that share a row tile's rows, 16 each
+constexpr int kTreeRows = 16 * kTreeRowWaves;     // rows of a tile
+constexpr int kTreeBlockBytes = 16384;            // K, or V, of a block of keys
+constexpr int kTreeSlots = 4;                     // blocks in LDS
 constexpr float kTreeSlack = 8.0f;  // how far (log2) scores may rise above the running maximum that P is taken at
+
+// Division of 0 .. 2^31 - 1 by a number that the host knows: with 2^l >= d, m = floor(2^(31 + l) / d) + 1 exceeds
+// 2^(31 + l) / d by at most 2^l / d of what a quotient's floor allows.
+struct Divisor {
+  uint32_t m;
+  int32_t l;
+  int32_t d;
+  __host__ static Divisor of(int32_t d) {
+    int l = 0;
+    while (((int64_t)1 << l) < d) ++l;
+    return Divisor{(uint32_t)((((uint64_t)1 << (31 + l)) / (uint64_t)d) + 1), l, d};
+  }
+  __device__ inline int quotient(int n) const { return (int)(__umulhi(2u * (uint32_t)n, m) >> l); }
+};
 
 struct TreeParams {
   const char* q;
@@ -56,14 +75,17 @@ struct TreeParams {
   const char* v_new;
   int64_t k_new_stride;
   int64_t v_new_stride;
+  Divisor page_div;    // by page_size
+  Divisor group_div;   // by group
   int32_t max_nodes;   // a tree's nodes, at most (more are cut off)
-  int32_t max_chunks;  // chunks of the batch, at most; 0: one a sequence, no partials
-  int32_t num_work;    // workgroups that attend; the others write the new rows
-  int64_t part_rows;   // rows of the partials
+  int32_t spans;       // workgroups per KV head
+  int32_t whole;       // no partials: a workgroup takes a whole row tile
+  int32_t stream;      // the call's K/V exceed the caches and are read once: loaded past them
+  int32_t num_work;    // workgroups that attend (spans a KV head); the others write the new rows
   uint64_t* ws_tag;    // the workspace's first word: a decode call's record in the same memory is void
-  int4* meta;          // per sequence: first row of its partials, chunks, rows
-  float2* part_ml;     // [part_rows]: running maximum (log2 units), sum
-  float* part_o;       // [part_rows, D]
+  int4* meta;          // per sequence: its first unit of work, its blocks, units a workgroup
+  float2* part_ml;     // [num_work, 2, kTreeRows]: running maximum (log2 units), sum
+  f32x4* part_o;       // [num_work, 2, kTreeRowWaves, D / 16, 64]: a wave's output tiles, as its lanes hold them
 };
 
 // Element types: fp32 takes its products on the fp32 matrix instructions.
@@ -75,25 +97,30 @@ template <typename T, int D>
 struct TreeTile {
   static constexpr bool kF32 = T::kDtype == NSLG_F32;
   static constexpr int kBytes = kF32 ? 4 : 2;
-  static constexpr int kSub = kF32 && D == 256 ? 1 : 2;        // 16-key pieces of a block
-  static constexpr int kBlocks = kF32 || D == 256 ? 1 : 2;     // blocks of a tile
-  static constexpr int kKeys = 16 * kSub * kBlocks;            // keys of a tile: two workgroups fit a CU
-  static constexpr int kPitch = D * kBytes + (kF32 ? 16 : 32); // bytes of a tile's row in LDS (no bank conflicts)
+  static constexpr int kRowBytes = D * kBytes;
+  static constexpr int kWaves = D == 256 ? 8 : 16;       // (the registers of 256-wide rows leave two waves a SIMD)
+  static constexpr int kThreads = 64 * kWaves;
+  static constexpr int kGroups = kWaves / kTreeRowWaves; // groups of waves that share a block's keys
+  static constexpr int kKeys = kTreeBlockBytes / kRowBytes;  // keys of a block
+  static constexpr int kGroupKeys = kKeys / kGroups;     // a group's
+  static constexpr int kStep = kGroupKeys < 32 ? 16 : 32;    // keys taken at a time
+  static constexpr int kSub = kStep / 16;                // in pieces of 16
 };
 
 struct SeqOf {
-  int nodes, len;
+  int nodes, len, q0, page0;  // its nodes and tokens (nodes among them), first ragged row, first entry of its table
 };
 
-// Sequence s's nodes and tokens (nodes among them).
 __device__ inline SeqOf tree_seq(const TreeParams& p, int s) {
-  SeqOf x = {0, 0};
+  SeqOf x = {0, 0, 0, 0};
   if (s < p.batch) {
-    const int np = p.indptr[s + 1] - p.indptr[s];
+    x.page0 = p.indptr[s];
+    x.q0 = p.qo_indptr[s];
+    const int np = p.indptr[s + 1] - x.page0;
     int lpl = p.last_len[s];
     lpl = lpl < 1 ? 1 : (lpl > p.page_size ? p.page_size : lpl);
     x.len = np > 0 ? (np - 1) * p.page_size + lpl : 0;
-    x.nodes = min(max(p.qo_indptr[s + 1] - p.qo_indptr[s], 0), p.max_nodes);
+    x.nodes = min(max(p.qo_indptr[s + 1] - x.q0, 0), p.max_nodes);
     if (x.nodes == 0) x.len = 0;
   }
   return x;
@@ -105,28 +132,14 @@ __device__ inline int64_t tree_row(const TreeParams& p, int t) {
   return r >= 0 && r < (int64_t)p.batch * p.grid_width ? r : -1;
 }
 
-// Keys per chunk: ceil(all keys / (budget - batch)) rounded up to whole tiles; a sequence of L keys then
-// has at most L / chunk + 1, all of them at most `budget`.
-__device__ inline int tree_chunk(const TreeParams& p, int64_t keys, int tile) {
-  const int64_t room = p.max_chunks - p.batch;
-  if (room <= 0) return 0x7fffffff / tile * tile;
-  const int64_t c = (keys + room - 1) / room;
-  const int64_t up = (c + tile - 1) / tile * tile;
-  return (int)(up < tile ? tile : up);
-}
-
-__device__ inline int64_t wave_sum_i64(int64_t x) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off, 64);
-  return x;
-}
-__device__ inline int wave_scan_i32(int x) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(x, off, 64);
-    if (lane >= off) x += y;
-  }
+// Sum over the lanes up to one's own.
+__device__ inline int wave_scan_i32(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);  // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);  // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);  // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
   return x;
 }
 
@@ -136,9 +149,8 @@ __device__ inline void write_row(char* dst, const char* src, int vecs) {
     stream_store(reinterpret_cast<u32x4*>(dst) + i, reinterpret_cast<const u32x4*>(src)[i]);
 }
 
-__device__ inline void tree_write_new(const TreeParams& p, int wg, int row_bytes) {
+__device__ inline void tree_write_new(const TreeParams& p, int64_t t, int row_bytes) {
   const int lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)wg * kTreeWaves + (threadIdx.x >> 6);
   if (t >= p.total_q) return;
   // the row's sequence: the last one that starts at or before it
   int b = -1;
@@ -176,570 +188,671 @@ __device__ inline u32x4 drop_not_finite(u32x4 x, bool& bad) {
   return x;
 }
 
-template <typename T, int D, int kCB>
-__global__ void __launch_bounds__(kTreeThreads, 2) tree_attention_kernel(TreeParams p) {
+// Where piece `c` (16 bytes) of key `key`'s row lies in its block: permuted so that the operand reads of 16 (V: 8) keys
+// fall on distinct banks without padding, which the direct loads into LDS could not write.
+template <int kVecs>
+__device__ inline int swizzle_k(int key) {
+  return kVecs >= 16 ? key & 15 : (key >> 1) & 7;
+}
+template <typename T, int kVecs>
+__device__ inline int swizzle_v(int key) {
+  if constexpr (T::kDtype == NSLG_F32) return 0;  // (read as whole rows)
+  return kVecs >= 16 ? (key & 7) << 1 : ((key >> 1) & 3) << 1;
+}
+
+// A lane's 16 bytes into LDS at dst + 16 * lane (dst uniform).
+template <bool kStream>
+__device__ inline void load_lds16(const char* src, char* dst) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                   (__attribute__((address_space(3))) void*)dst, 16, 0, kStream ? 2 : 0);
+}
+
+// The wave's direct loads but the last `kLeft`, and its LDS reads, are over; then all waves meet.
+template <int kLeft>
+__device__ inline void wait_and_meet() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLeft) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// A lane's share of a row: o[n][i] is d = 16 n + 4 gq + i (fp32: d = 64 (n / 4) + 16 gq + 4 i + n % 4).
+template <typename T, int NT>
+__device__ inline void store_row(char* dst, int gq, const f32x4 (&o)[NT]) {
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if constexpr (T::kDtype == NSLG_F32) {
+      const int c = n >> 2, i = n & 3;
+      *reinterpret_cast<f32x4*>(dst + 4 * (64 * c + 16 * gq + 4 * i)) = f32x4{o[4 * c][i], o[4 * c + 1][i], o[4 * c + 2][i], o[4 * c + 3][i]};
+    } else {
+      u16x4 x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = T::from_f32(o[n][i]);
+      *reinterpret_cast<u16x4*>(dst + 2 * (16 * n + 4 * gq)) = x;
+    }
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__((TreeTile<T, D>::kThreads), (TreeTile<T, D>::kWaves / 4)) tree_attention_kernel(TreeParams p) {
   using Tile = TreeTile<T, D>;
   constexpr bool kF32 = Tile::kF32;
-  constexpr int kBytes = Tile::kBytes;
-  constexpr int kSub = Tile::kSub, kBlocks = Tile::kBlocks, kKeys = Tile::kKeys, kBlockKeys = 16 * kSub;
-  constexpr int kPitch = Tile::kPitch;
-  constexpr int kRows = 16 * kCB * kTreeWaves;
+  constexpr int kBytes = Tile::kBytes, kWaves = Tile::kWaves, kThreads = Tile::kThreads, kGroups = Tile::kGroups;
+  constexpr int kSub = Tile::kSub, kStep = Tile::kStep, kGroupKeys = Tile::kGroupKeys, kKeys = Tile::kKeys;
+  constexpr int kRowBytes = Tile::kRowBytes, kRows = kTreeRows, kBlockBytes = kTreeBlockBytes, kSlots = kTreeSlots;
   constexpr int NT = D / 16;
-  constexpr int kSteps = kF32 ? D / 16 : D / 32;            // 16-byte operands of a key or row
-  constexpr int kVecs = D * kBytes / 16;                    // 16-byte pieces of a row
-  constexpr int kPer = kKeys * kVecs / kTreeThreads;        // pieces of K (and of V) a thread and tile
-  constexpr int kStep = kTreeThreads / kVecs;               // keys between a thread's pieces
+  constexpr int kOps = kRowBytes / 64;                      // 16-byte operands of a key or row, a lane
+  constexpr int kVecs = kRowBytes / 16;                     // 16-byte pieces of a row
+  constexpr int kPer = kBlockBytes / (16 * kThreads);       // pieces of K (and of V) a thread and block
+  constexpr int kSteps = kGroupKeys / kStep;                // steps of a group's keys of a block
   constexpr bool kSplitP = T::kDtype == NSLG_BF16;
 
-  __shared__ __attribute__((aligned(16))) char k_lds[2][kKeys * kPitch];
-  __shared__ __attribute__((aligned(16))) char v_lds[2][kKeys * kPitch];
-  // keys of a tile with a value of V that is not finite (three tiles' words in turn: one is cleared a barrier
-  // before the tile that writes it)
-  __shared__ uint32_t bad_lds[3][kBlocks];
+  __shared__ __attribute__((aligned(1024))) char kv_lds[2 * kSlots * kBlockBytes];
+  __shared__ float2 ml_lds[kGroups == 2 ? kRows : 1];
+  __shared__ int32_t page_lds[kTreeWin];
+  __shared__ SeqOf seq_lds[64];   // 64 sequences, and the units before each and up to its end
+  __shared__ int2 unit_lds[64];
+  __shared__ uint32_t bad_lds[2][kKeys / kStep];  // keys of a step with a value of V that is not finite (blocks in turn)
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = lane & 15, gq = lane >> 4;
+  const int row_wave = wave % kTreeRowWaves, group = wave / kTreeRowWaves;
+  char* k_lds = kv_lds;
+  char* v_lds = kv_lds + kSlots * kBlockBytes;
+  // The lane's number, anew: what is derived from it is then not kept in registers from block to block. (Spilled, a
+  // register's reload would wait for all of the wave's direct loads.)
+  auto fresh_lane = [&]() {
+    int x = lane;
+    asm volatile("" : "+v"(x));
+    return x;
+  };
   const int G = p.group, ps = p.page_size;
-  const int row_bytes = p.num_kv_heads * D * kBytes;
+  const int row_bytes = p.num_kv_heads * kRowBytes;
   const int w = (int)blockIdx.x;
   if (p.q_rows)
-    zero_pad_rows(p.qo_indptr, p.q_rows, p.grid_width, p.batch, p.out, p.out_stride, p.num_qo_heads * D * kBytes,
-                  w * kTreeWaves + wave, (int)gridDim.x * kTreeWaves);
+    zero_pad_rows(p.qo_indptr, p.q_rows, p.grid_width, p.batch, p.out, p.out_stride, p.num_qo_heads * kRowBytes,
+                  w * kWaves + wave, (int)gridDim.x * kWaves);
   if (w >= p.num_work) {
-    tree_write_new(p, w - p.num_work, row_bytes);
+    tree_write_new(p, (int64_t)(w - p.num_work) * kWaves + wave, row_bytes);
     return;
   }
   if (w == 0 && tid == 0 && p.ws_tag) *p.ws_tag = 0;
-  if (tid < 3 * kBlocks) bad_lds[tid / kBlocks][tid % kBlocks] = 0;
 
-  // ---- the workgroup's item: KV head (in turn: neighbours of a head share an XCD's L2), then sequence, chunk, row tile
+  // ---- the workgroup's span of work. A KV head's work is one line of units: sequence after sequence, row tile after
+  // row tile, block of keys after block; workgroup j of the head takes `span` of them from j * span on (KV heads in turn:
+  // a head's neighbours share an XCD's L2). What begins or ends inside a row tile's keys leaves a partial. Without
+  // partials a unit is a row tile with all its keys.
   const int h = w % p.num_kv_heads;
-  int k = w / p.num_kv_heads;
-  int64_t keys = 0;
-  for (int s0 = 0; s0 < p.batch; s0 += 64) keys += tree_seq(p, s0 + lane).len;
-  const int chunk = tree_chunk(p, wave_sum_i64(keys), kKeys);
-  int b = -1, n_nodes = 0, L = 0, n_chunks = 0, n_tiles = 0;
-  int64_t part0 = 0;  // the sequence's first row of the partials (of one KV head)
-  for (int s0 = 0; s0 < p.batch; s0 += 64) {
-    const SeqOf sq = tree_seq(p, s0 + lane);
-    const int rows = sq.nodes * G;
-    const int tiles = (rows + kRows - 1) / kRows;
-    const int chunks = sq.len > 0 ? (sq.len - 1) / chunk + 1 : 0;
-    const int items = tiles * chunks;
-    const int incl = wave_scan_i32(items);
-    const int parts = chunks > 1 ? chunks * rows : 0;
-    const int pincl = wave_scan_i32(parts);
-    const int total = __builtin_amdgcn_readlane(incl, 63);
-    if (k >= total) {
-      k -= total;
-      part0 += __builtin_amdgcn_readlane(pincl, 63);
-      continue;
-    }
-    const int src = __ffsll((long long)__ballot(k < incl)) - 1;
-    k -= __builtin_amdgcn_readlane(incl - items, src);
-    part0 += __builtin_amdgcn_readlane(pincl - parts, src);
-    b = s0 + src;
-    n_nodes = __builtin_amdgcn_readlane(sq.nodes, src);
-    L = __builtin_amdgcn_readlane(sq.len, src);
-    n_chunks = __builtin_amdgcn_readlane(chunks, src);
-    n_tiles = __builtin_amdgcn_readlane(tiles, src);
-    break;
+  const int j = w / p.num_kv_heads;
+  auto units_of = [&](const SeqOf& x, int& tiles, int& blocks) {
+    tiles = (x.nodes * G + kRows - 1) / kRows;
+    blocks = (x.len + kKeys - 1) / kKeys;
+    return p.whole ? (blocks > 0 ? tiles : 0) : tiles * blocks;
+  };
+  int group0 = 0, before = 0;  // the first of the sequences in seq_lds, the units before it
+  int total;
+  {
+    int x, y;
+    const SeqOf s = tree_seq(p, lane);
+    const int u = units_of(s, x, y);
+    const int incl = wave_scan_i32(u);
+    if (wave == 0) seq_lds[lane] = s, unit_lds[lane] = int2{incl - u, incl};
+    total = __builtin_amdgcn_readlane(incl, 63);
   }
-  if (b < 0) return;  // uniform over the workgroup
-  const int c_no = k / n_tiles, tile = k - c_no * n_tiles;  // (the row tiles of a chunk next to each other)
+  for (int s0 = 64; s0 < p.batch; s0 += 64) {
+    int x, y;
+    total += wave_sum_i32(units_of(tree_seq(p, s0 + lane), x, y));
+  }
+  const int span = p.whole ? 1 : max(__builtin_amdgcn_readfirstlane((total + p.spans - 1) / p.spans), 1);
+  int pos = __builtin_amdgcn_readfirstlane((int)min((int64_t)j * span, (int64_t)total));
+  const int pos_end = __builtin_amdgcn_readfirstlane(min(total - pos, span) + pos);
+  if (w == 0 && wave == 0 && p.meta) {
+    int at = 0;
+    for (int s0 = 0; s0 < p.batch; s0 += 64) {
+      int x, y;
+      const int u = units_of(tree_seq(p, s0 + lane), x, y);
+      const int sum = wave_scan_i32(u);
+      if (s0 + lane < p.batch) p.meta[s0 + lane] = int4{at + sum - u, y, span, 0};
+      at += __builtin_amdgcn_readlane(sum, 63);
+    }
+  }
+  __syncthreads();
+  while (pos < pos_end) {
+  while (pos - before >= unit_lds[63].y) {  // uniform: beyond these sequences
+    before = __builtin_amdgcn_readfirstlane(before + unit_lds[63].y);
+    group0 += 64;
+    int x, y;
+    const SeqOf s = tree_seq(p, group0 + lane);
+    const int u = units_of(s, x, y);
+    const int incl = wave_scan_i32(u);
+    __syncthreads();
+    if (wave == 0) seq_lds[lane] = s, unit_lds[lane] = int2{incl - u, incl};
+    __syncthreads();
+  }
+  const int src = __ffsll((long long)__ballot(pos - before < unit_lds[lane].y)) - 1;
+  const SeqOf seq = seq_lds[src];
+
+  const int first_unit = __builtin_amdgcn_readfirstlane(before + unit_lds[src].x);
+  const int n_nodes = __builtin_amdgcn_readfirstlane(seq.nodes), L = __builtin_amdgcn_readfirstlane(seq.len);
+  const int q0 = __builtin_amdgcn_readfirstlane(seq.q0);
+  const int32_t* idx = p.indices + __builtin_amdgcn_readfirstlane(seq.page0);
+  const int all_blk = (L + kKeys - 1) / kKeys;
+  int tile = 0, blk0 = pos - first_unit;
+  if (p.whole) {
+    tile = blk0;
+    blk0 = 0;
+  } else if (blk0 >= all_blk) {
+    tile = blk0 / all_blk;
+    blk0 -= tile * all_blk;
+  }
+  const int n_blk = p.whole ? all_blk : min(pos_end - pos, all_blk - blk0);
+  const bool to_end = blk0 + n_blk == all_blk;
+  const bool partial = blk0 > 0 || !to_end;
+  pos += p.whole ? 1 : n_blk;
   const int nrows = n_nodes * G;
   const int start = max(L - n_nodes, 0);
-  const int q0 = p.qo_indptr[b];
-  const int kv_begin = c_no * chunk;
-  const int kv_end = min(L - kv_begin, chunk) + kv_begin;
-  if (p.meta && h == 0 && k == 0 && tid == 0) p.meta[b] = int4{(int)part0, n_chunks, nrows, 0};
-  const int32_t* idx = p.indices + p.indptr[b];
+  const int kv_begin = blk0 * kKeys;
+  const int kv_end = to_end ? L : kv_begin + n_blk * kKeys;
 
-  // ---- the wave's rows
-  const int wave_row0 = tile * kRows + 16 * kCB * wave;
-  const bool wave_on = wave_row0 < nrows;  // (a wave without rows only helps to stage the tiles)
-  u32x4 qb[kCB][kSteps];
-  const uint32_t* mrow[kCB];
-  bool row_ok[kCB];
-#pragma unroll
-  for (int cb = 0; cb < kCB; ++cb) {
-    const int row = wave_row0 + 16 * cb + r;
-    const int t = row / G;
-    row_ok[cb] = row < nrows && q0 + t < p.total_q;
-    const int64_t at = row_ok[cb] ? tree_row(p, q0 + t) : -1;
-    mrow[cb] = p.mask + (int64_t)(row_ok[cb] ? q0 + t : 0) * p.mask_words;
-    const char* src = p.q + (at >= 0 ? at : 0) * p.q_stride + ((int64_t)(h * G + row % G) * D) * kBytes + 16 * gq;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) qb[cb][s] = at >= 0 ? *reinterpret_cast<const u32x4*>(src + 64 * s) : u32x4{0, 0, 0, 0};
-  }
-  float thr[kCB], neg_m[kCB];  // the raw score above which the maximum is raised; -maximum (log2 units; 0: none yet)
-  f32x4 lsum[kCB], o[kCB][NT];
-#pragma unroll
-  for (int cb = 0; cb < kCB; ++cb) {
-    thr[cb] = -INFINITY;
-    neg_m[cb] = 0.f;
-    lsum[cb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int n = 0; n < NT; ++n) o[cb][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  const float inv_scale = 1.f / p.scale_log2;
-
-  // ---- tiles: thread tid moves piece tid % kVecs of keys tid / kVecs + kStep i
-  const int f_c = 16 * (tid % kVecs), f_key = tid / kVecs;
-  const int head_off = h * D * kBytes;
-  const bool pow2 = (ps & (ps - 1)) == 0;
-  const int ps_shift = __builtin_ctz((unsigned)ps);
-  u32x4 kreg[kPer], vreg[kPer];
-  int pid[kPer];
-  auto page_of = [&](int key) { return pow2 ? key >> ps_shift : key / ps; };
-  // where key's K and V rows of this head are: a page slot, or the forward's new row
-  auto pool_at = [&](int key, int page) {
-    page = page < 0 || (int64_t)page >= p.num_pages ? 0 : page;
-    return ((int64_t)page * ps + (key - page_of(key) * ps)) * row_bytes + head_off;
+  // ---- the wave's rows: lane's row r of them, its row of q and out (-1: none), its node and its bytes' offset there
+  const int wave_row0 = tile * kRows + 16 * row_wave;
+  const bool wave_on = wave_row0 < nrows;  // (a wave without rows only helps to load)
+  struct Row {
+    int64_t at;
+    int node, off;
+    bool ok;
   };
-  int64_t new_row0 = q0;  // row of k_new / v_new of node 0 (a tree's rows are contiguous)
-  if (p.k_new && p.q_rows) {
-    const int64_t at = tree_row(p, q0);
-    const int64_t rows = (int64_t)p.batch * p.grid_width;
-    new_row0 = at < 0 || at + n_nodes > rows ? 0 : at;
+  auto row_of = [&](int r) {
+    const int row = wave_row0 + r;
+    Row x;
+    x.node = p.group_div.quotient(row);
+    x.ok = row < nrows && q0 + x.node < p.total_q;
+    x.at = x.ok ? tree_row(p, q0 + x.node) : -1;
+    x.off = (h * G + row - x.node * G) * kRowBytes;
+    return x;
+  };
+  u32x4 qb[kOps];
+  {
+    const Row x = row_of(lane & 15);
+    const char* src = p.q + (x.at >= 0 ? x.at * p.q_stride + x.off : 0) + 16 * (lane >> 4);
+#pragma unroll
+    for (int s = 0; s < kOps; ++s) qb[s] = x.at >= 0 ? *reinterpret_cast<const u32x4*>(src + 64 * s) : u32x4{0, 0, 0, 0};
   }
+
+  // ---- blocks of keys: wave-wide loads of 1 KB straight into LDS. Load u of a block fills bytes 1024 u .. + 1023, lane l
+  // the 16 at 16 l: piece l % kVecs of key u * (64 / kVecs) + l / kVecs, where the swizzle has put piece (l % kVecs) ^
+  // swizzle(key) of the row.
+  const int head_off = h * kRowBytes;
+  auto page_of = [&](int key) { return p.page_div.quotient(key); };
+  auto checked = [&](int page) { return page < 0 || (int64_t)page >= p.num_pages ? 0 : page; };
   const bool fresh = p.k_new != nullptr;
+  int64_t new_row0 = q0;  // row of k_new / v_new of node 0 (a tree's rows are contiguous)
+  if (fresh && p.q_rows) {
+    const int64_t at = tree_row(p, q0);
+    new_row0 = at < 0 ? 0 : at;
+  }
   const int64_t new_last = (p.q_rows ? (int64_t)p.batch * p.grid_width : p.total_q) - 1;
   auto new_at = [&](int key) { return min(new_row0 + (key - start), new_last); };
-  auto fetch_pages = [&](int key0) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) pid[i] = idx[page_of(min(key0 + f_key + kStep * i, kv_end - 1))];
+  // page_lds[i]: what is added to a key of page win + i to make its slot
+  int win = 0, win_blk = 0;  // the window's first page; the first block that reaches past it
+  auto load_pages = [&](int key) {
+    win = page_of(key);
+    const int last = page_of(kv_end - 1);
+    for (int i = tid; i < kTreeWin && win + i <= last; i += kThreads) page_lds[i] = (checked(idx[win + i]) - (win + i)) * ps;
+    win_blk = last < win + kTreeWin ? 0x7fffffff : ((win + kTreeWin) * ps - kv_begin) / kKeys;
   };
-  auto fetch = [&](int key0) {
+  auto key_of = [&](int ln) { return wave * (64 / kVecs) + ln / kVecs; };  // of a lane's first piece
+  constexpr int kKeyStep = kWaves * (64 / kVecs);  // keys between a lane's pieces
+  constexpr int kTurn = kPer == 1 ? 0 : kKeyStep % 16;  // (the swizzles repeat after 16 keys)
+  static_assert(kTurn == 0 || (kTurn == 8 && kPer == 2 && kF32), "a lane's second piece is swizzled as key + 8, fp32 V not at all");
+  auto issue = [&](int blk) {
+    char* ks = k_lds + (blk & (kSlots - 1)) * kBlockBytes + 1024 * wave;
+    char* vs = v_lds + (blk & (kSlots - 1)) * kBlockBytes + 1024 * wave;
+    const int key0 = kv_begin + blk * kKeys;
+    const bool nodes = fresh && key0 + kKeys > start;  // uniform: some of the block's rows are not in the pool
+    const int ln = fresh_lane();
+    const int l_key = key_of(ln), l_piece = ln % kVecs;
+    const int v_piece = head_off + 16 * (l_piece ^ swizzle_v<T, kVecs>(l_key));
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int key = min(key0 + f_key + kStep * i, kv_end - 1);
-      const char *ks, *vs;
-      if (fresh && key >= start) {
-        const int64_t at = new_at(key);
-        ks = p.k_new + at * p.k_new_stride + head_off;
-        vs = p.v_new + at * p.v_new_stride + head_off;
+      const int k_piece = head_off + 16 * (l_piece ^ swizzle_k<kVecs>(l_key + kTurn * i));
+      const int kabs = min(key0 + l_key + kKeyStep * i, kv_end - 1);
+      const uint32_t slot = (uint32_t)(kabs + page_lds[page_of(kabs) - win]);
+      const char* kp = p.k_pool + k_piece + (uint64_t)slot * (uint32_t)row_bytes;
+      const char* vp = p.v_pool + v_piece + (uint64_t)slot * (uint32_t)row_bytes;
+      if (nodes && kabs >= start) {
+        const int64_t at = new_at(kabs);
+        kp = p.k_new + at * p.k_new_stride + k_piece;
+        vp = p.v_new + at * p.v_new_stride + v_piece;
+      }
+      if (p.stream) {  // uniform
+        load_lds16<true>(kp, ks + 1024 * kWaves * i);
+        load_lds16<true>(vp, vs + 1024 * kWaves * i);
       } else {
-        const int64_t at = pool_at(key, pid[i]);
-        ks = p.k_pool + at;
-        vs = p.v_pool + at;
-      }
-      kreg[i] = *reinterpret_cast<const u32x4*>(ks + f_c);
-      vreg[i] = *reinterpret_cast<const u32x4*>(vs + f_c);
-    }
-  };
-  auto stash = [&](int key0, int stage, int rot) {
-    if (key0 + kKeys > start) {  // uniform: a tile with nodes, or the end of the keys
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int key = f_key + kStep * i;
-        bool bad = false;
-        if (key0 + key >= kv_end) {
-          vreg[i] = u32x4{0, 0, 0, 0};
-        } else if (key0 + key >= start) {
-          vreg[i] = drop_not_finite<T>(vreg[i], bad);
-        }
-        if (bad) atomicOr(&bad_lds[rot][key / kBlockKeys], 1u << (key % kBlockKeys));
+        load_lds16<false>(kp, ks + 1024 * kWaves * i);
+        load_lds16<false>(vp, vs + 1024 * kWaves * i);
       }
     }
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int key = f_key + kStep * i;
-      *reinterpret_cast<u32x4*>(&k_lds[stage][key * kPitch + f_c]) = kreg[i];
-      *reinterpret_cast<u32x4*>(&v_lds[stage][key * kPitch + f_c]) = vreg[i];
-    }
   };
-  // the bits of the block's keys that row cb of the lane sees
-  auto visible = [&](int kbase, int cb) -> uint32_t {
+  load_pages(kv_begin);
+  if (tid < 2 * (kKeys / kStep)) bad_lds[tid / (kKeys / kStep)][tid % (kKeys / kStep)] = 0;
+  __syncthreads();
+  static_assert(kSlots * kKeys <= kTreeWin);  // the blocks on the way, even of single-token pages
+#pragma unroll 1
+  for (int i = 0; i < min(n_blk, kSlots - 1); ++i) issue(i);
+
+  float thr = -INFINITY, neg_m = 0.f;  // the raw score above which the maximum is raised; -maximum (log2 units; 0: none yet)
+  f32x4 lsum = {0.f, 0.f, 0.f, 0.f}, o[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float inv_scale = 1.f / p.scale_log2;
+
+  // the bits of a step's keys (kbase on) that row r sees
+  auto visible = [&](int kbase, int r) -> uint32_t {
+    const Row x = row_of(r);
+    const uint32_t* mrow = p.mask + (int64_t)(x.ok ? q0 + x.node : 0) * p.mask_words;
     const int rel = kbase - start;
     const int words = p.mask_words;
     uint32_t v;
     if (rel >= 0) {
       const int wi = rel >> 5, sh = rel & 31;
-      const uint32_t lo = wi < words ? mrow[cb][wi] : 0u;
-      const uint32_t hi = wi + 1 < words ? mrow[cb][wi + 1] : 0u;
+      const uint32_t lo = wi < words ? mrow[wi] : 0u;
+      const uint32_t hi = wi + 1 < words ? mrow[wi + 1] : 0u;
       v = sh ? (lo >> sh) | (hi << (32 - sh)) : lo;
+    } else if (rel > -32) {
+      v = (1u << -rel) - 1u;
+      v |= mrow[0] << -rel;
     } else {
-      v = (1u << -rel) - 1u;  // (rel > -kBlockKeys >= -32: not all of the block lies before the tree)
-      v |= mrow[cb][0] << -rel;
+      v = ~0u;
     }
     const int left = kv_end - kbase;
-    if (left < 32) v &= (1u << left) - 1u;
-    return row_ok[cb] ? v : 0u;
+    if (left < 32) v &= left > 0 ? (1u << left) - 1u : 0u;
+    return x.ok ? v : 0u;
   };
 
-  auto compute = [&](int key0, int stage, int rot) {
+  const int share = group * (kGroupKeys * kRowBytes);  // the group's share of a block
+  // One step of a block: scores, mask (`tail`: a block with nodes, or past the end), probabilities, product with V.
+  auto step = [&](int blk, int u, auto tail) {
+    constexpr bool kTail = decltype(tail)::value;
+    const int kbase = kv_begin + blk * kKeys + group * kGroupKeys + u * kStep;
+    const char* ksrc = k_lds + (blk & (kSlots - 1)) * kBlockBytes + u * kStep * kRowBytes;
+    const char* vsrc = v_lds + (blk & (kSlots - 1)) * kBlockBytes + u * kStep * kRowBytes;
+    const int ln = fresh_lane(), r = ln & 15, gq = ln >> 4;
+    // LDS offsets of the lane's operands: K at operand i is k_at ^ 64 i, V of output tile n (16 bits) v_at ^ 32 n
+    const int k_at = share + r * kRowBytes + 16 * (gq ^ swizzle_k<kVecs>(r));
+    const int v_key = kF32 ? 4 * gq : 4 * gq + (r >> 2);
+    const int v_at = share + v_key * kRowBytes + (kF32 ? 16 * r : 16 * swizzle_v<T, kVecs>(v_key) + 8 * (r & 3));
+    f32x4 s[kSub];
+    u32x4 ka[kSub][kOps];
 #pragma unroll
-    for (int blk = 0; blk < kBlocks; ++blk) {
-      const int kbase = key0 + blk * kBlockKeys;
-      if (kbase >= kv_end) break;
-      // scores
-      f32x4 s[kCB][kSub];
+    for (int t = 0; t < kSub; ++t)
 #pragma unroll
-      for (int t = 0; t < kSub; ++t) {
-        u32x4 ka[kSteps];
-        const char* krow = &k_lds[stage][(blk * kBlockKeys + 16 * t + r) * kPitch + 16 * gq];
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) ka[i] = *reinterpret_cast<const u32x4*>(krow + 64 * i);
-#pragma unroll
-        for (int cb = 0; cb < kCB; ++cb) {
-          if constexpr (kF32) {
-            f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-              const f32x4 a = __builtin_bit_cast(f32x4, ka[i]), q = __builtin_bit_cast(f32x4, qb[cb][i]);
-              x = __builtin_amdgcn_mfma_f32_16x16x4f32(a[0], q[0], x, 0, 0, 0);
-              y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[1], q[1], y, 0, 0, 0);
-              x = __builtin_amdgcn_mfma_f32_16x16x4f32(a[2], q[2], x, 0, 0, 0);
-              y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[3], q[3], y, 0, 0, 0);
-            }
-            s[cb][t] = x + y;
-          } else {
-            s[cb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i)
-              s[cb][t] = T::mma_k32(__builtin_bit_cast(u16x8, ka[i]), __builtin_bit_cast(u16x8, qb[cb][i]), s[cb][t]);
-          }
-        }
-      }
-      // mask, maximum, probabilities (in place of the scores)
-      const bool tail = kbase + kBlockKeys > start;  // uniform; the keys past the end are behind the nodes
-      uint32_t vis[kCB];
-      u16x8 pb[kCB], pb_lo[kCB];
-#pragma unroll
-      for (int cb = 0; cb < kCB; ++cb) {
-        if (tail) {
-          vis[cb] = visible(kbase, cb);
-#pragma unroll
-          for (int j = 0; j < 4 * kSub; ++j)
-            if (!(vis[cb] >> (16 * (j >> 2) + 4 * gq + (j & 3)) & 1)) s[cb][j >> 2][j & 3] = -INFINITY;
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 4 * kSub; ++j) top = fmaxf(top, s[cb][j >> 2][j & 3]);
-        if (__ballot(top > thr[cb])) {
-          const float m_run = thr[cb] == -INFINITY ? -INFINITY : -neg_m[cb];
-          const float m_new = fmaxf(m_run, rows_max(top * p.scale_log2));
-          const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
-          lsum[cb] *= alpha;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) o[cb][n] *= alpha;
-          thr[cb] = (m_new + kTreeSlack) * inv_scale;
-          neg_m[cb] = m_new == -INFINITY ? 0.f : -m_new;
-        }
-#pragma unroll
-        for (int j = 0; j < 4 * kSub; ++j) {
-          const float x = fast_exp2(fmaf(s[cb][j >> 2][j & 3], p.scale_log2, neg_m[cb]));
-          s[cb][j >> 2][j & 3] = x;
-          if constexpr (kF32) {
-            lsum[cb][j & 3] += x;
-          } else {
-            // half keeps 11 bits of a probability; bfloat16's 8 are too few for the 2e-3 of the 16-bit caches'
-            // attention: the rest goes in as a second term
-            pb[cb][j] = T::from_f32(x);
-            if constexpr (kSplitP) pb_lo[cb][j] = T::from_f32(x - T::to_f32(pb[cb][j]));
-          }
-        }
-      }
-      // O^T += V^T P^T
-      if constexpr (kF32) {
-#pragma unroll
-        for (int t = 0; t < kSub; ++t)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const char* vrow = &v_lds[stage][(blk * kBlockKeys + 16 * t + 4 * gq + j) * kPitch + 16 * r];
-#pragma unroll
-            for (int c = 0; c < D / 64; ++c) {
-              const f32x4 v = *reinterpret_cast<const f32x4*>(vrow + 256 * c);
-#pragma unroll
-              for (int cb = 0; cb < kCB; ++cb)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  o[cb][4 * c + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e], s[cb][t][j], o[cb][4 * c + e], 0, 0, 0);
-            }
-          }
-      } else {
-        typedef short i16x4_t __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) i16x4_t* lds_i16x4;
-        // lane r of a 16-lane group addresses keys 4 gq + r / 4 (then + 16), columns 16 n + 4 (r % 4) .. + 3, and
-        // receives keys 4 gq + 0..3 (+ 16) at d = 16 n + r
-        const char* vsrc = &v_lds[stage][(blk * kBlockKeys + 4 * gq + (r >> 2)) * kPitch + 8 * (r & 3)];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vsrc + 32 * n));
-          const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(vsrc + 32 * n + 16 * kPitch));
-          const u16x8 va = __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-          for (int cb = 0; cb < kCB; ++cb) {
-            o[cb][n] = T::mma_k32(va, pb[cb], o[cb][n]);
-            if constexpr (kSplitP) o[cb][n] = T::mma_k32(va, pb_lo[cb], o[cb][n]);
-          }
-        }
-        // the rows' sums by an all-ones operand: of the probabilities as they were multiplied
-        const u16x8 ones = u16x8(T::from_f32(1.f));
-#pragma unroll
-        for (int cb = 0; cb < kCB; ++cb) {
-          lsum[cb] = T::mma_k32(ones, pb[cb], lsum[cb]);
-          if constexpr (kSplitP) lsum[cb] = T::mma_k32(ones, pb_lo[cb], lsum[cb]);
-        }
-      }
-      // nodes whose V is not finite: those elements, for the rows that see the node
-      uint32_t bad = tail ? __builtin_amdgcn_readfirstlane(bad_lds[rot][blk]) : 0u;
-      while (bad) {
-        const int kk = __ffs(bad) - 1;
-        bad &= bad - 1;
-        const int key = kbase + kk;
-        const char* vsrc = fresh ? p.v_new + new_at(key) * p.v_new_stride + head_off
-                                 : p.v_pool + pool_at(key, idx[page_of(key)]);
-#pragma unroll
-        for (int cb = 0; cb < kCB; ++cb) {
-          float pr = 0.f;
-#pragma unroll
-          for (int j = 0; j < 4 * kSub; ++j)
-            if (16 * (j >> 2) + (j & 3) == (kk & ~12)) pr = s[cb][j >> 2][j & 3];
-          pr = __shfl(pr, 16 * ((kk >> 2) & 3) + r, 64);
-          if (!(vis[cb] >> kk & 1)) continue;
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if constexpr (kF32) {
-                const float v = reinterpret_cast<const float*>(vsrc)[64 * (n >> 2) + 16 * gq + 4 * i + (n & 3)];
-                if (!(fabsf(v) < INFINITY)) o[cb][n][i] += pr * v;
-              } else {
-                const float v = T::to_f32(reinterpret_cast<const uint16_t*>(vsrc)[16 * n + 4 * gq + i]);
-                if (!(fabsf(v) < INFINITY)) o[cb][n][i] += pr * v;
-              }
-            }
-        }
-      }
-    }
-  };
-
-  __syncthreads();  // bad_lds is clear
-  fetch_pages(kv_begin);
-  fetch(kv_begin);
-  fetch_pages(kv_begin + kKeys);
-  stash(kv_begin, 0, 0);
-  int stage = 0, rot = 0;
-  for (int key0 = kv_begin; key0 < kv_end; key0 += kKeys) {
-    __syncthreads();  // this tile is staged, the one before is read
-    const int next = rot == 2 ? 0 : rot + 1, after = next == 2 ? 0 : next + 1;
-    if (tid < kBlocks) bad_lds[after][tid] = 0;
-    const bool more = key0 + kKeys < kv_end;
-    if (more) {
-      fetch(key0 + kKeys);
-      fetch_pages(key0 + 2 * kKeys);
-    }
-    if (wave_on) compute(key0, stage, rot);
-    if (more) stash(key0 + kKeys, stage ^ 1, next);
-    stage ^= 1;
-    rot = next;
-  }
-  if (!wave_on) return;
-
-  // ---- the rows: normalised into `out`, or the chunk's share as a partial
-#pragma unroll
-  for (int cb = 0; cb < kCB; ++cb) {
-    float l;
-    if constexpr (kF32)
-      l = rows_sum((lsum[cb][0] + lsum[cb][1]) + (lsum[cb][2] + lsum[cb][3]));
-    else
-      l = lsum[cb][0];
-    if (!row_ok[cb]) continue;
-    const int row = wave_row0 + 16 * cb + r;
-    float f = 1.f;
-    char* dst;
-    bool wide = true;  // fp32 elements
-    if (n_chunks > 1) {
-      const int64_t slot = (part0 + (int64_t)c_no * nrows + row) * p.num_kv_heads + h;
-      if (slot >= p.part_rows) continue;
-      if (gq == 0) p.part_ml[slot] = float2{thr[cb] == -INFINITY ? -INFINITY : -neg_m[cb], l};
-      dst = reinterpret_cast<char*>(p.part_o + slot * D);
-    } else {
-      const int64_t at = tree_row(p, q0 + row / G);
-      if (at < 0) continue;
-      f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (a sum that is NaN makes the row NaN)
-      dst = p.out + at * p.out_stride + (int64_t)(h * G + row % G) * D * kBytes;
-      wide = kF32;
-    }
+      for (int i = 0; i < kOps; ++i) ka[t][i] = *reinterpret_cast<const u32x4*>(ksrc + 16 * t * kRowBytes + (k_at ^ (64 * i)));
     if constexpr (kF32) {
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c)
+      for (int t = 0; t < kSub; ++t) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kOps; ++i) {
+          const f32x4 a = __builtin_bit_cast(f32x4, ka[t][i]), q = __builtin_bit_cast(f32x4, qb[i]);
+          x = __builtin_amdgcn_mfma_f32_16x16x4f32(a[0], q[0], x, 0, 0, 0);
+          y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[1], q[1], y, 0, 0, 0);
+          x = __builtin_amdgcn_mfma_f32_16x16x4f32(a[2], q[2], x, 0, 0, 0);
+          y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[3], q[3], y, 0, 0, 0);
+        }
+        s[t] = x + y;
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < kSub; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kOps; ++i)
+#pragma unroll
+        for (int t = 0; t < kSub; ++t) s[t] = T::mma_k32(__builtin_bit_cast(u16x8, ka[t][i]), __builtin_bit_cast(u16x8, qb[i]), s[t]);
+    }
+    // V's operand of output tile n (16 bits): lane r of a 16-lane group addresses keys 4 gq + r / 4 (then + 16), columns 16 n
+    // + 4 (r % 4) .. + 3, and receives keys 4 gq + 0..3 (+ 16) at d = 16 n + r. Read ahead of the softmax, which covers
+    // their way (read one by one as they are used, the reads took most of the time).
+    typedef short i16x4_t __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) i16x4_t* lds_i16x4;
+    u16x8 va[kF32 ? 1 : NT];
+    if constexpr (!kF32) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const char* at = vsrc + (v_at ^ (32 * n));
+        const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)at);
+        const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at + 16 * kRowBytes));
+        va[n] = __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // A later block's loads go out here: at the block's start the waves waited to get rid of theirs, all at once, before any
+    // product (265 us with 32 trees of 32 nodes over 2k-16k tokens, 308 from there).
+    if (u == 0 && blk + kSlots - 1 < n_blk) issue(blk + kSlots - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    uint32_t vis = 0;
+    if constexpr (kTail) {
+      vis = visible(kbase, r);
+#pragma unroll
+      for (int j = 0; j < 4 * kSub; ++j)
+        if (!(vis >> (16 * (j >> 2) + 4 * gq + (j & 3)) & 1)) s[j >> 2][j & 3] = -INFINITY;
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4 * kSub; ++j) top = fmaxf(top, s[j >> 2][j & 3]);
+    if (__ballot(top > thr)) {
+      const float m_run = thr == -INFINITY ? -INFINITY : -neg_m;
+      const float m_new = fmaxf(m_run, rows_max(top * p.scale_log2));
+      const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+      lsum *= alpha;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) o[n] *= alpha;
+      thr = (m_new + kTreeSlack) * inv_scale;
+      neg_m = m_new == -INFINITY ? 0.f : -m_new;
+    }
+    u16x8 pb, pb_lo;
+#pragma unroll
+    for (int j = 0; j < 4 * kSub; ++j) {
+      const float x = fast_exp2(fmaf(s[j >> 2][j & 3], p.scale_log2, neg_m));
+      s[j >> 2][j & 3] = x;
+      if constexpr (kF32) {
+        lsum[j & 3] += x;
+      } else {
+        // half keeps 11 bits of a probability; bfloat16's 8 are too few for the 2e-3 of the 16-bit caches'
+        // attention: the rest goes in as a second term
+        pb[j] = T::from_f32(x);
+        if constexpr (kSplitP) pb_lo[j] = T::from_f32(x - T::to_f32(pb[j]));
+      }
+    }
+    // O^T += V^T P^T
+    if constexpr (kF32) {
+#pragma unroll
+      for (int t = 0; t < kSub; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<f32x4*>(dst + 4 * (64 * c + 16 * gq + 4 * j)) =
-              f32x4{o[cb][4 * c][j], o[cb][4 * c + 1][j], o[cb][4 * c + 2][j], o[cb][4 * c + 3][j]} * f;
-    } else if (wide) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) *reinterpret_cast<f32x4*>(dst + 4 * (16 * n + 4 * gq)) = o[cb][n];
+          for (int c = 0; c < D / 64; ++c) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(vsrc + (16 * t + j) * kRowBytes + v_at + 256 * c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[4 * c + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e], s[t][j], o[4 * c + e], 0, 0, 0);
+          }
     } else {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        u16x4 x;
+        o[n] = T::mma_k32(va[n], pb, o[n]);
+        if constexpr (kSplitP) o[n] = T::mma_k32(va[n], pb_lo, o[n]);
+      }
+      // the rows' sums by an all-ones operand: of the probabilities as they were multiplied
+      const u16x8 ones = u16x8(T::from_f32(1.f));
+      lsum = T::mma_k32(ones, pb, lsum);
+      if constexpr (kSplitP) lsum = T::mma_k32(ones, pb_lo, lsum);
+    }
+    // nodes whose V is not finite: those elements, for the rows that see the node
+    if constexpr (kTail) {
+      uint32_t bad = __builtin_amdgcn_readfirstlane(bad_lds[blk & 1][group * kSteps + u]);
+      while (__builtin_expect(bad != 0, 0)) {
+        const int kk = __ffs(bad) - 1;
+        bad &= bad - 1;
+        const int key = kbase + kk;
+        const char* vrow = (fresh ? p.v_new + new_at(key) * p.v_new_stride
+                                  : p.v_pool + ((int64_t)checked(idx[page_of(key)]) * ps + (key - page_of(key) * ps)) * row_bytes) +
+                           head_off;
+        float pr = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = T::from_f32(o[cb][n][i] * f);
-        *reinterpret_cast<u16x4*>(dst + 2 * (16 * n + 4 * gq)) = x;
+        for (int j = 0; j < 4 * kSub; ++j)
+          if (16 * (j >> 2) + (j & 3) == (kk & ~12)) pr = s[j >> 2][j & 3];
+        pr = __shfl(pr, 16 * ((kk >> 2) & 3) + r, 64);
+        if (!(vis >> kk & 1)) continue;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float v;
+            if constexpr (kF32)
+              v = reinterpret_cast<const float*>(vrow)[64 * (n >> 2) + 16 * gq + 4 * i + (n & 3)];
+            else
+              v = T::to_f32(reinterpret_cast<const uint16_t*>(vrow)[16 * n + 4 * gq + i]);
+            if (!(fabsf(v) < INFINITY)) o[n][i] += pr * v;
+          }
       }
     }
+  };
+  // Values of a block's V that are not finite, and those past the end, become 0 in LDS.
+  auto tidy = [&](int blk) {
+    char* vs = v_lds + (blk & (kSlots - 1)) * kBlockBytes;
+    const int ln = fresh_lane();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int key = key_of(ln) + kKeyStep * i;
+      const int kabs = kv_begin + blk * kKeys + key;
+      u32x4* at = reinterpret_cast<u32x4*>(vs + 1024 * (wave + kWaves * i) + 16 * ln);
+      if (kabs >= kv_end) {
+        *at = u32x4{0, 0, 0, 0};
+      } else if (kabs >= start) {
+        bool bad = false;
+        const u32x4 x = drop_not_finite<T>(*at, bad);
+        if (bad) {
+          *at = x;
+          atomicOr(&bad_lds[blk & 1][key / kStep], 1u << (key % kStep));
+        }
+      }
+    }
+  };
+
+  // A block has landed for all waves once each has waited for its loads and all have met; then the block before it has
+  // been read, and the loads of block i + kSlots - 1 take its slot.
+  auto block = [&](int blk, auto tail) {
+    if (blk + kSlots - 2 < n_blk)
+      wait_and_meet<2 * kPer * (kSlots - 2)>();
+    else
+      wait_and_meet<0>();
+    if (blk + kSlots - 1 < n_blk) {
+      if (blk + kSlots - 1 >= win_blk) {  // uniform
+        load_pages(kv_begin + (blk + kSlots - 1) * kKeys);
+        __syncthreads();
+      }
+      if (!wave_on) issue(blk + kSlots - 1);  // (the others in the course of their step)
+    }
+    if constexpr (decltype(tail)::value) {
+      tidy(blk);
+      __syncthreads();
+      if (tid < kKeys / kStep) bad_lds[(blk + 1) & 1][tid] = 0;
+    }
+    if (wave_on) {
+#pragma unroll
+      for (int u = 0; u < kSteps; ++u) step(blk, u, tail);
+    }
+  };
+  const int n_plain = min(max(start - kv_begin, 0) / kKeys, n_blk);  // blocks that lie before the tree
+  int blk = 0;
+  for (; blk < n_plain; ++blk) block(blk, std::false_type());
+  for (; blk < n_blk; ++blk) block(blk, std::true_type());
+
+  // ---- the second group's rows to the first's, lane by lane, through the blocks' LDS
+  const int r = lane & 15, gq = lane >> 4;
+  float l = lsum[0];
+  if constexpr (kF32) l = rows_sum((lsum[0] + lsum[1]) + (lsum[2] + lsum[3]));
+  float m = thr == -INFINITY ? -INFINITY : -neg_m;
+  if constexpr (kGroups == 2) {
+    wait_and_meet<0>();
+    f32x4* buf = reinterpret_cast<f32x4*>(kv_lds) + row_wave * (64 * NT) + lane;
+    static_assert(kTreeRowWaves * 64 * NT * 16 <= 2 * kSlots * kBlockBytes);
+    if (group && wave_on) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) buf[64 * n] = o[n];
+      if (gq == 0) ml_lds[16 * row_wave + r] = float2{m, l};
+    }
+    wait_and_meet<0>();
+    if (!group && wave_on) {
+      const float2 other = ml_lds[16 * row_wave + r];
+      const float top = fmaxf(m, other.x);
+      const float f0 = l == 0.f ? 0.f : fast_exp2(m - top);  // 0: no key of the group seen
+      const float f1 = other.y == 0.f ? 0.f : fast_exp2(other.x - top);
+      l = fmaf(f0, l, f1 * other.y);
+      m = top;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const f32x4 x = buf[64 * n];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] = fmaf(f0, o[n][e], f1 * x[e]);
+      }
+    }
+  }
+
+  // ---- the rows: normalised into `out`, or the span's share as a partial
+  if (partial && wave_on && group == 0) {
+    // (a workgroup has at most one that began before its span and one that goes on behind it)
+    const int64_t slot = ((int64_t)2 * w + (blk0 == 0)) * kTreeRowWaves + row_wave;
+    if (gq == 0) p.part_ml[16 * slot + r] = float2{m, l};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) p.part_o[(slot * NT + n) * 64 + lane] = o[n];
+  } else if (!partial && wave_on && group == 0) {
+    const Row x = row_of(r);
+    const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (a sum that is NaN makes the row NaN)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[n] *= f;
+    if (x.at >= 0) store_row<T, NT>(p.out + x.at * p.out_stride + x.off, gq, o);
+  }
+  if (pos < pos_end) __syncthreads();  // the next row tile's loads overwrite what the other waves may still read
   }
 }
 
-// Log-sum-exp merge of the chunks of each (node, query head): D / 4 lanes take a chunk's row, kParts such groups the
-// row's chunks in turn.
-template <typename T, int D, int kParts>
-__global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
-  constexpr int kLanes = D / 4;
-  constexpr int kRows = 256 / (kLanes * kParts);  // rows a workgroup
-  __shared__ f32x4 o_lds[kParts > 1 ? kRows * kParts * kLanes : 1];
-  __shared__ float2 ml_lds[kParts > 1 ? kRows * kParts : 1];
-  const int part = threadIdx.x / kLanes % kParts, wg_row = threadIdx.x / (kLanes * kParts);
-  const int col = threadIdx.x % kLanes;
-  const int64_t rows = p.total_q * p.num_qo_heads;
-  const int64_t row = (int64_t)blockIdx.x * kRows + wg_row;
-  const int t = (int)min(row / p.num_qo_heads, p.total_q - 1);
-  const int head = (int)(row - (int64_t)t * p.num_qo_heads);
-  // the row's sequence: the last one that starts at or before it (binary search)
-  int lo = 0, hi = p.batch;  // qo_indptr[lo] <= t < qo_indptr[hi], if in any
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.qo_indptr[mid] <= t)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  const int node = t - p.qo_indptr[lo];
-  int4 meta = int4{0, 0, 0, 0};
-  const bool in = row < rows && node >= 0 && t < p.qo_indptr[lo + 1] && node < p.max_nodes;
-  if (in && p.indptr[lo + 1] > p.indptr[lo]) meta = p.meta[lo];  // (a sequence without tokens has no entry)
-  const int chunks = meta.y;
-  const int h = head / p.group, g = head - h * p.group;
-  const int64_t slot0 = ((int64_t)meta.x + node * p.group + g) * p.num_kv_heads + h;
-  const int64_t step = (int64_t)meta.z * p.num_kv_heads;
-  const bool on = chunks > 1 && slot0 + (chunks - 1) * step < p.part_rows;
+// Log-sum-exp merge of the parts of 16 rows (a row wave's) of one KV head. Waves 0 .. kTileWaves - 1 of a workgroup share
+// the output tiles, kSplit such sets the parts, four at a time each; the sets' sums go through LDS.
+template <typename T, int D, int kSplit>
+__global__ void __launch_bounds__(256 * kSplit) tree_merge_kernel(TreeParams p, int row_waves) {
+  constexpr int NT = D / 16, kN = T::kDtype == NSLG_F32 ? 4 : NT / 4;  // (fp32 rows are stored four tiles at a time)
+  constexpr int kTileWaves = NT / kN;
+  __shared__ f32x4 o_lds[kSplit > 1 ? kSplit - 1 : 1][kSplit > 1 ? NT * 64 : 1];
+  __shared__ float2 ml_lds[kSplit][16];
+  const int lane = threadIdx.x & 63, r = lane & 15, gq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int tw = wave % kTileWaves, set = wave / kTileWaves;
+  const int h = blockIdx.x % p.num_kv_heads;
+  const int k = blockIdx.x / p.num_kv_heads;
+  const int b = k / row_waves, rw = k - b * row_waves;
+  const int G = p.group;
+  const int4 meta = p.meta[b];
+  const int q0 = p.qo_indptr[b];
+  const int nodes = min(max(p.qo_indptr[b + 1] - q0, 0), p.max_nodes);
+  if (16 * rw >= nodes * G || meta.y <= 0) return;
+  const int tile = rw / kTreeRowWaves;
+  const int first = meta.x + tile * meta.y;
+  const int j0 = first / meta.z;
+  const int parts = (first + meta.y - 1) / meta.z - j0 + 1;
+  if (parts < 2 || j0 + parts > p.spans) return;  // uniform over the workgroup
+  // the partial of the rows' part i: the first part goes on behind its workgroup's span, the others began before theirs
+  auto slot_of = [&](int i) {
+    return ((int64_t)2 * ((j0 + i) * p.num_kv_heads + h) + (i == 0)) * kTreeRowWaves + rw - tile * kTreeRowWaves;
+  };
   float m = -INFINITY, l = 0.f;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  if (on) {
-    for (int c0 = part; c0 < chunks; c0 += 4 * kParts) {
+  f32x4 o[kN];
+#pragma unroll
+  for (int n = 0; n < kN; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto join = [&](float m1, float l1, const f32x4 (&x)[kN]) {
+    if (l1 == 0.f) return;  // no key of the part seen
+    const float top = fmaxf(m, m1);
+    const float f0 = l == 0.f ? 0.f : fast_exp2(m - top), f1 = fast_exp2(m1 - top);
+    l = fmaf(f0, l, f1 * l1);
+    m = top;
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][e] = fmaf(f0, o[n][e], f1 * x[n][e]);
+  };
+  const int each = (parts + kSplit - 1) / kSplit;
+  const int end = min(parts, (set + 1) * each);
+  if (set < kSplit) {
+    for (int i0 = set * each; i0 < end; i0 += 4) {
       float2 ml[4];
-      f32x4 o[4];
+      f32x4 x[4][kN];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int64_t slot = slot0 + min(c0 + u * kParts, chunks - 1) * step;
-        ml[u] = p.part_ml[slot];
-        o[u] = *reinterpret_cast<const f32x4*>(p.part_o + slot * D + 4 * col);
+        const int64_t slot = slot_of(min(i0 + u, end - 1));
+        ml[u] = p.part_ml[16 * slot + r];
+#pragma unroll
+        for (int n = 0; n < kN; ++n) x[u][n] = p.part_o[(slot * NT + tw * kN + n) * 64 + lane];
       }
-      float top = m;
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (c0 + u * kParts < chunks) top = fmaxf(top, ml[u].x);
-      const float f0 = l == 0.f ? 0.f : fast_exp2(m - top);
-      l *= f0;
-      acc *= f0;
-      m = top;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (c0 + u * kParts >= chunks || ml[u].y == 0.f) continue;  // 0: no key of the chunk seen
-        const float f = fast_exp2(ml[u].x - m);
-        l = fmaf(f, ml[u].y, l);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, o[u][e], acc[e]);
-      }
+        if (i0 + u < end) join(ml[u].x, ml[u].y, x[u]);
     }
   }
-  if constexpr (kParts > 1) {
-    const int at = wg_row * kParts + part;
-    o_lds[at * kLanes + col] = acc;
-    if (col == 0) ml_lds[at] = float2{m, l};
+  if constexpr (kSplit > 1) {
+    if (set > 0 && set < kSplit) {
+#pragma unroll
+      for (int n = 0; n < kN; ++n) o_lds[set - 1][(tw * kN + n) * 64 + lane] = o[n];
+      if (tw == 0 && gq == 0) ml_lds[set][r] = float2{m, l};
+    }
     __syncthreads();
-    if (part) return;
-    float2 ml[kParts];
+    if (set) return;
 #pragma unroll
-    for (int i = 0; i < kParts; ++i) ml[i] = ml_lds[wg_row * kParts + i], m = fmaxf(m, ml[i].x);
-    l = 0.f;
-    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 1; i < kSplit; ++i) {
+      f32x4 x[kN];
 #pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-      const float f = ml[i].y == 0.f ? 0.f : fast_exp2(ml[i].x - m);
-      if (ml[i].y == 0.f) continue;
-      l = fmaf(f, ml[i].y, l);
-      const f32x4 x = o_lds[(wg_row * kParts + i) * kLanes + col];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, x[e], acc[e]);
+      for (int n = 0; n < kN; ++n) x[n] = o_lds[i - 1][(tw * kN + n) * 64 + lane];
+      join(ml_lds[i][r].x, ml_lds[i][r].y, x);
     }
-  }
-  if (!on) return;
-  const int64_t at = tree_row(p, t);
-  if (at < 0) return;
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  acc *= inv;
-  char* dst = p.out + at * p.out_stride;
-  if constexpr (T::kDtype == NSLG_F32) {
-    *reinterpret_cast<f32x4*>(dst + 4 * ((int64_t)head * D + 4 * col)) = acc;
   } else {
-    u16x4 x;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = T::from_f32(acc[e]);
-    *reinterpret_cast<u16x4*>(dst + 2 * ((int64_t)head * D + 4 * col)) = x;
+    if (set) return;
   }
+  const int row = 16 * rw + r;
+  const int node = p.group_div.quotient(row);
+  if (row >= nodes * G || q0 + node >= p.total_q) return;
+  const int64_t at = tree_row(p, q0 + node);
+  if (at < 0) return;
+  const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+  for (int n = 0; n < kN; ++n) o[n] *= f;
+  constexpr int kBytes = T::kDtype == NSLG_F32 ? 4 : 2;
+  char* dst = p.out + at * p.out_stride + (int64_t)(h * G + row - node * G) * D * kBytes;
+  store_row<T, kN>(dst + tw * 16 * kN * kBytes, gq, o);
 }
 
 // ---- host ------------------------------------------------------------------------------
 
-// Rows of a workgroup: two column blocks a wave where the trees' rows fill them (registers: not at D = 256, nor fp32).
-inline int tree_row_blocks(int64_t rows, int head_dim, int dtype) {
-  return dtype != NSLG_F32 && head_dim != 256 && rows > 64 ? 2 : 1;
-}
-inline int tree_tile_keys(int head_dim, int dtype) {
-  if (dtype == NSLG_F32) return head_dim == 256 ? 16 : 32;
-  return head_dim == 256 ? 32 : 64;
+inline int64_t tree_tiles(int64_t rows) { return (rows + kTreeRows - 1) / kTreeRows; }
+
+// Workgroups per KV head: one a CU, which its blocks in LDS fill.
+int64_t tree_spans(int64_t batch, int64_t total_keys, int64_t rows, int num_kv_heads, int head_dim, int dtype) {
+  int64_t n = kTreeCUs / num_kv_heads;
+  const int64_t most = (total_keys * head_dim * elem_bytes(dtype) / kTreeBlockBytes + batch) * tree_tiles(rows);
+  n = n > most ? most : n;
+  return n < 1 ? 1 : n;
 }
 
-// Chunks of a call's sequences, at most: enough for about four workgroups a CU.
-int64_t tree_chunks(int64_t batch, int64_t total_keys, int64_t rows, int num_kv_heads, int head_dim, int dtype) {
-  const int64_t rows_wg = 64 * tree_row_blocks(rows, head_dim, dtype);
-  const int64_t tiles = (rows + rows_wg - 1) / rows_wg;
-  int64_t n = 4 * kTreeCUs / (tiles * num_kv_heads);
-  const int64_t most = total_keys / tree_tile_keys(head_dim, dtype) + 1;  // (a tile each)
-  n = n < 1 ? 1 : (n > most ? most : n);
-  return n + batch;
-}
-
-size_t tree_bytes(int64_t batch, int64_t part_rows, int head_dim) {
-  const size_t meta = ((size_t)batch * 16 + 255) / 256 * 256;
-  const size_t ml = ((size_t)part_rows * 8 + 255) / 256 * 256;
-  return 512 + meta + ml + (size_t)part_rows * head_dim * 4;
+// The workspace of n such workgroups: the first word, the sequences' entries, two partials of a row tile each.
+size_t tree_bytes(int64_t batch, int64_t n, int num_kv_heads, int head_dim) {
+  const size_t rows = (size_t)n * num_kv_heads * 2 * kTreeRows;
+  return 512 + ((size_t)batch * 16 + 255) / 256 * 256 + (rows * 8 + 255) / 256 * 256 + rows * head_dim * 4;
 }
 
 template <typename T, int D>
-int launch_tree(const TreeParams& p, int64_t rows, int64_t wgs, hipStream_t s) {
-  if (tree_row_blocks(rows, D, T::kDtype) == 2) {
-    if constexpr (T::kDtype != NSLG_F32 && D != 256)
-      tree_attention_kernel<T, D, 2><<<dim3((unsigned)wgs), kTreeThreads, 0, s>>>(p);
-  } else {
-    tree_attention_kernel<T, D, 1><<<dim3((unsigned)wgs), kTreeThreads, 0, s>>>(p);
-  }
+int launch_tree(TreeParams p, hipStream_t s) {
+  constexpr int kWaves = TreeTile<T, D>::kWaves;
+  int64_t wgs = p.num_work + (p.k_new ? (p.total_q + kWaves - 1) / kWaves : 0);
+  if (wgs == 0) wgs = p.batch;  // pad rows only
+  if (wgs > 0x7fffffff / 16) return fail(NSLG_EUNSUPPORTED, "paged_tree_attention: too many rows");
+  tree_attention_kernel<T, D><<<dim3((unsigned)wgs), 64 * kWaves, 0, s>>>(p);
   const int rc = check_launch("paged_tree_attention");
-  if (rc || p.max_chunks == 0) return rc;
-  const int64_t out_rows = p.total_q * p.num_qo_heads;
-  const int64_t each = p.max_chunks / p.batch;  // chunks of a sequence, on average
-  auto grid = [&](int parts) { return dim3((unsigned)((out_rows + 1024 / (D * parts) - 1) / (1024 / (D * parts)))); };
-  if (each >= 8 && D <= 128)
-    tree_merge_kernel<T, D, D <= 128 ? 8 : 4><<<grid(D <= 128 ? 8 : 4), 256, 0, s>>>(p);
-  else if (each >= 8)
-    tree_merge_kernel<T, D, 4><<<grid(4), 256, 0, s>>>(p);
+  if (rc || p.whole) return rc;
+  const int row_waves = (p.max_nodes * p.group + 15) / 16;
+  const int64_t merges = (int64_t)p.batch * row_waves * p.num_kv_heads;
+  if (merges > 0x7fffffff) return fail(NSLG_EUNSUPPORTED, "paged_tree_attention: too many rows");
+  // Several sets of waves where a sequence has many parts on average (one sequence, 16 nodes over 2k tokens, 17 parts:
+  // 12 -> 5 us; 32 trees of 2 to 3 parts: 12 and 15).
+  if (p.spans >= 8 * p.batch)
+    tree_merge_kernel<T, D, 4><<<dim3((unsigned)merges), 1024, 0, s>>>(p, row_waves);
   else
-    tree_merge_kernel<T, D, 1><<<grid(1), 256, 0, s>>>(p);
+    tree_merge_kernel<T, D, 1><<<dim3((unsigned)merges), 256, 0, s>>>(p, row_waves);
   return check_launch("paged_tree_attention merge");
 }
 
 template <typename T>
-int launch_tree_dim(const TreeParams& p, int head_dim, int64_t rows, int64_t wgs, hipStream_t s) {
+int launch_tree_dim(const TreeParams& p, int head_dim, hipStream_t s) {
   switch (head_dim) {
-    case 64: return launch_tree<T, 64>(p, rows, wgs, s);
-    case 128: return launch_tree<T, 128>(p, rows, wgs, s);
-    default: return launch_tree<T, 256>(p, rows, wgs, s);
+    case 64: return launch_tree<T, 64>(p, s);
+    case 128: return launch_tree<T, 128>(p, s);
+    default: return launch_tree<T, 256>(p, s);
   }
 }
 
@@ -756,8 +869,8 @@ extern "C" size_t nslg_paged_tree_workspace_size(int32_t batch, int32_t num_qo_h
       (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return 0;
   const int64_t rows = (int64_t)max_q * (num_qo_heads / num_kv_heads);
-  const int64_t n = tree_chunks(batch, total_pages * page_size, rows, num_kv_heads, head_dim, dtype);
-  return tree_bytes(batch, n * rows * num_kv_heads, head_dim);
+  const int64_t n = tree_spans(batch, total_pages * page_size, rows, num_kv_heads, head_dim, dtype);
+  return tree_bytes(batch, n, num_kv_heads, head_dim);
 }
 
 extern "C" int nslg_paged_tree_attention(const void* q, int64_t q_stride, const uint32_t* mask, int32_t mask_words,
@@ -837,6 +950,8 @@ extern "C" int nslg_paged_tree_attention(const void* q, int64_t q_stride, const 
   p.num_qo_heads = num_qo_heads;
   p.num_kv_heads = num_kv_heads;
   p.group = group;
+  p.page_div = Divisor::of(page_size);
+  p.group_div = Divisor::of(group);
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.out = (char*)out;
   p.out_stride = out_stride * eb;
@@ -845,33 +960,32 @@ extern "C" int nslg_paged_tree_attention(const void* q, int64_t q_stride, const 
   p.k_new_stride = k_new_stride * eb;
   p.v_new_stride = v_new_stride * eb;
   p.max_nodes = max_q;
-  int64_t chunks = batch;
+  int64_t spans = batch * tree_tiles(rows);
+  p.whole = 1;
   if (workspace && total_q > 0) {
-    int64_t n = tree_chunks(batch, total_pages * page_size, rows, num_kv_heads, head_dim, dtype);
-    const int64_t each = rows * num_kv_heads;
-    while (n > batch && tree_bytes(batch, n * each, head_dim) > workspace_bytes) --n;
-    if (n > batch && n < 0x7fffffff && n * each < 0x7fffffff) {
+    int64_t n = tree_spans(batch, total_pages * page_size, rows, num_kv_heads, head_dim, dtype);
+    while (n > 0 && tree_bytes(batch, n, num_kv_heads, head_dim) > workspace_bytes) --n;
+    if (n > 0) {
       char* ws = (char*)(((uintptr_t)workspace + 255) / 256 * 256);  // (tree_bytes has room for this)
-      p.max_chunks = (int32_t)n;
-      p.part_rows = n * each;
+      const size_t part_rows = (size_t)n * num_kv_heads * 2 * kTreeRows;
+      p.whole = 0;
       p.ws_tag = (uint64_t*)ws;
       ws += 256;
       p.meta = (int4*)ws;
       ws += ((size_t)batch * 16 + 255) / 256 * 256;
       p.part_ml = (float2*)ws;
-      ws += ((size_t)p.part_rows * 8 + 255) / 256 * 256;
-      p.part_o = (float*)ws;
-      chunks = n;
+      ws += (part_rows * 8 + 255) / 256 * 256;
+      p.part_o = (f32x4*)ws;
+      spans = n;
     }
   }
-  const int64_t rows_wg = 64 * tree_row_blocks(rows, head_dim, dtype);
-  const int64_t work = total_q > 0 ? chunks * ((rows + rows_wg - 1) / rows_wg) * num_kv_heads : 0;
-  int64_t wgs = work + (k_new ? (total_q + kTreeWaves - 1) / kTreeWaves : 0);
-  if (wgs == 0) wgs = batch;  // pad rows only
-  if (wgs > 0x7fffffff / 8) return fail(NSLG_EUNSUPPORTED, "paged_tree_attention: too many rows");
+  if (spans * num_kv_heads > 0x7fffffff / 8) return fail(NSLG_EUNSUPPORTED, "paged_tree_attention: too many rows");
+  p.spans = (int32_t)spans;
+  const int64_t work = total_q > 0 ? spans * num_kv_heads : 0;
   p.num_work = (int32_t)work;
+  p.stream = tree_tiles(rows) == 1 && total_pages * page_size * num_kv_heads * head_dim * 2 * eb > ((int64_t)256 << 20);
   hipStream_t s = as_stream(stream);
-  if (dtype == NSLG_F16) return launch_tree_dim<F16>(p, head_dim, rows, wgs, s);
-  if (dtype == NSLG_BF16) return launch_tree_dim<BF16>(p, head_dim, rows, wgs, s);
-  return launch_tree_dim<F32>(p, head_dim, rows, wgs, s);
+  if (dtype == NSLG_F16) return launch_tree_dim<F16>(p, head_dim, s);
+  if (dtype == NSLG_BF16) return launch_tree_dim<BF16>(p, head_dim, s);
+  return launch_tree_dim<F32>(p, head_dim, s);
 }
