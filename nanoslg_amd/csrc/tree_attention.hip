@@ -28,8 +28,6 @@ namespace {
 constexpr int kTreeCUs = 256;
 constexpr int kTreeMaxNodes = 1024;
 constexpr int kTreeWin = 1024;    // page ids in LDS
-constexpr int kTreeRowWaves = 8;                  // waves that share a row tile's rows, 16 each
-constexpr int kTreeRows = 16 * kTreeRowWaves;     // rows of a tile
 constexpr int kTreeBlockBytes = 16384;            // K, or V, of a block of keys
 constexpr int kTreeSlots = 4;                     // blocks in LDS
 constexpr float kTreeSlack = 8.0f;  // how far (log2) scores may rise above the running maximum that P is taken at
@@ -79,13 +77,14 @@ struct TreeParams {
   Divisor group_div;   // by group
   int32_t max_nodes;   // a tree's nodes, at most (more are cut off)
   int32_t spans;       // workgroups per KV head
+  int32_t tile_waves;  // waves of 16 rows of a row tile
   int32_t whole;       // no partials: a workgroup takes a whole row tile
   int32_t stream;      // the call's K/V exceed the caches and are read once: loaded past them
   int32_t num_work;    // workgroups that attend (spans a KV head); the others write the new rows
   uint64_t* ws_tag;    // the workspace's first word: a decode call's record in the same memory is void
   int4* meta;          // per sequence: its first unit of work, its blocks, units a workgroup
-  float2* part_ml;     // [num_work, 2, kTreeRows]: running maximum (log2 units), sum
-  f32x4* part_o;       // [num_work, 2, kTreeRowWaves, D / 16, 64]: a wave's output tiles, as its lanes hold them
+  float2* part_ml;     // [num_work, 2, 16 * tile_waves]: running maximum (log2 units), sum
+  f32x4* part_o;       // [num_work, 2, tile_waves, D / 16, 64]: a wave's output tiles, as its lanes hold them
 };
 
 // Element types: fp32 takes its products on the fp32 matrix instructions.
@@ -93,14 +92,19 @@ struct F32 {
   static constexpr int kDtype = NSLG_F32;
 };
 
-template <typename T, int D>
+// A row tile is kRW waves of 16 rows; the workgroup's other waves, a second group, take half of every block's keys. 128
+// rows a tile; 256 for trees of more, whose keys are then loaded once (8 trees of 24 to 60 nodes 66 us, in two tiles 77),
+// but not with rows of 512 bytes and more, whose registers leave two waves a SIMD.
+template <typename T, int D, int kRW>
 struct TreeTile {
   static constexpr bool kF32 = T::kDtype == NSLG_F32;
   static constexpr int kBytes = kF32 ? 4 : 2;
   static constexpr int kRowBytes = D * kBytes;
-  static constexpr int kWaves = D == 256 ? 8 : 16;       // (the registers of 256-wide rows leave two waves a SIMD)
+  static constexpr int kWaves = kRowBytes >= 512 ? 8 : 16;
+  static constexpr int kRowWaves = kRW;
+  static constexpr int kRows = 16 * kRowWaves;
   static constexpr int kThreads = 64 * kWaves;
-  static constexpr int kGroups = kWaves / kTreeRowWaves; // groups of waves that share a block's keys
+  static constexpr int kGroups = kWaves / kRowWaves;     // groups of waves that share a block's keys
   static constexpr int kKeys = kTreeBlockBytes / kRowBytes;  // keys of a block
   static constexpr int kGroupKeys = kKeys / kGroups;     // a group's
   static constexpr int kStep = kGroupKeys < 32 ? 16 : 32;    // keys taken at a time
@@ -232,13 +236,14 @@ __device__ inline void store_row(char* dst, int gq, const f32x4 (&o)[NT]) {
   }
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__((TreeTile<T, D>::kThreads), (TreeTile<T, D>::kWaves / 4)) tree_attention_kernel(TreeParams p) {
-  using Tile = TreeTile<T, D>;
+template <typename T, int D, int kRW>
+__global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, D, kRW>::kWaves / 4)) tree_attention_kernel(TreeParams p) {
+  using Tile = TreeTile<T, D, kRW>;
+  static_assert(Tile::kGroups <= 2 && (Tile::kF32 ? Tile::kGroupKeys % 16 : Tile::kGroupKeys % 32) == 0);
   constexpr bool kF32 = Tile::kF32;
   constexpr int kBytes = Tile::kBytes, kWaves = Tile::kWaves, kThreads = Tile::kThreads, kGroups = Tile::kGroups;
   constexpr int kSub = Tile::kSub, kStep = Tile::kStep, kGroupKeys = Tile::kGroupKeys, kKeys = Tile::kKeys;
-  constexpr int kRowBytes = Tile::kRowBytes, kRows = kTreeRows, kBlockBytes = kTreeBlockBytes, kSlots = kTreeSlots;
+  constexpr int kRowBytes = Tile::kRowBytes, kRowWaves = Tile::kRowWaves, kRows = Tile::kRows, kBlockBytes = kTreeBlockBytes, kSlots = kTreeSlots;
   constexpr int NT = D / 16;
   constexpr int kOps = kRowBytes / 64;                      // 16-byte operands of a key or row, a lane
   constexpr int kVecs = kRowBytes / 16;                     // 16-byte pieces of a row
@@ -255,7 +260,7 @@ __global__ void __launch_bounds__((TreeTile<T, D>::kThreads), (TreeTile<T, D>::k
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int row_wave = wave % kTreeRowWaves, group = wave / kTreeRowWaves;
+  const int row_wave = wave % kRowWaves, group = wave / kRowWaves;
   char* k_lds = kv_lds;
   char* v_lds = kv_lds + kSlots * kBlockBytes;
   // The lane's number, anew: what is derived from it is then not kept in registers from block to block. (Spilled, a
@@ -675,7 +680,7 @@ __global__ void __launch_bounds__((TreeTile<T, D>::kThreads), (TreeTile<T, D>::k
   if constexpr (kGroups == 2) {
     wait_and_meet<0>();
     f32x4* buf = reinterpret_cast<f32x4*>(kv_lds) + row_wave * (64 * NT) + lane;
-    static_assert(kTreeRowWaves * 64 * NT * 16 <= 2 * kSlots * kBlockBytes);
+    static_assert(kRowWaves * 64 * NT * 16 <= 2 * kSlots * kBlockBytes);
     if (group && wave_on) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) buf[64 * n] = o[n];
@@ -701,7 +706,7 @@ __global__ void __launch_bounds__((TreeTile<T, D>::kThreads), (TreeTile<T, D>::k
   // ---- the rows: normalised into `out`, or the span's share as a partial
   if (partial && wave_on && group == 0) {
     // (a workgroup has at most one that began before its span and one that goes on behind it)
-    const int64_t slot = ((int64_t)2 * w + (blk0 == 0)) * kTreeRowWaves + row_wave;
+    const int64_t slot = ((int64_t)2 * w + (blk0 == 0)) * kRowWaves + row_wave;
     if (gq == 0) p.part_ml[16 * slot + r] = float2{m, l};
 #pragma unroll
     for (int n = 0; n < NT; ++n) p.part_o[(slot * NT + n) * 64 + lane] = o[n];
@@ -735,14 +740,14 @@ __global__ void __launch_bounds__(256 * kSplit) tree_merge_kernel(TreeParams p, 
   const int q0 = p.qo_indptr[b];
   const int nodes = min(max(p.qo_indptr[b + 1] - q0, 0), p.max_nodes);
   if (16 * rw >= nodes * G || meta.y <= 0) return;
-  const int tile = rw / kTreeRowWaves;
+  const int tile = rw / p.tile_waves;
   const int first = meta.x + tile * meta.y;
   const int j0 = first / meta.z;
   const int parts = (first + meta.y - 1) / meta.z - j0 + 1;
   if (parts < 2 || j0 + parts > p.spans) return;  // uniform over the workgroup
   // the partial of the rows' part i: the first part goes on behind its workgroup's span, the others began before theirs
   auto slot_of = [&](int i) {
-    return ((int64_t)2 * ((j0 + i) * p.num_kv_heads + h) + (i == 0)) * kTreeRowWaves + rw - tile * kTreeRowWaves;
+    return ((int64_t)2 * ((j0 + i) * p.num_kv_heads + h) + (i == 0)) * p.tile_waves + rw - tile * p.tile_waves;
   };
   float m = -INFINITY, l = 0.f;
   f32x4 o[kN];
@@ -810,29 +815,40 @@ __global__ void __launch_bounds__(256 * kSplit) tree_merge_kernel(TreeParams p, 
 
 // ---- host ------------------------------------------------------------------------------
 
-inline int64_t tree_tiles(int64_t rows) { return (rows + kTreeRows - 1) / kTreeRows; }
+inline int64_t tree_rows(int64_t rows, int head_dim, int dtype) {
+  return rows > 128 && head_dim * elem_bytes(dtype) < 512 ? 256 : 128;
+}
+inline int64_t tree_tiles(int64_t rows, int head_dim, int dtype) {
+  const int64_t n = tree_rows(rows, head_dim, dtype);
+  return (rows + n - 1) / n;
+}
 
 // Workgroups per KV head: one a CU, which its blocks in LDS fill.
 int64_t tree_spans(int64_t batch, int64_t total_keys, int64_t rows, int num_kv_heads, int head_dim, int dtype) {
   int64_t n = kTreeCUs / num_kv_heads;
-  const int64_t most = (total_keys * head_dim * elem_bytes(dtype) / kTreeBlockBytes + batch) * tree_tiles(rows);
+  const int64_t most = (total_keys * head_dim * elem_bytes(dtype) / kTreeBlockBytes + batch) * tree_tiles(rows, head_dim, dtype);
   n = n > most ? most : n;
   return n < 1 ? 1 : n;
 }
 
 // The workspace of n such workgroups: the first word, the sequences' entries, two partials of a row tile each.
-size_t tree_bytes(int64_t batch, int64_t n, int num_kv_heads, int head_dim) {
-  const size_t rows = (size_t)n * num_kv_heads * 2 * kTreeRows;
+size_t tree_bytes(int64_t batch, int64_t n, int num_kv_heads, int64_t tile_rows, int head_dim) {
+  const size_t rows = (size_t)n * num_kv_heads * 2 * tile_rows;
   return 512 + ((size_t)batch * 16 + 255) / 256 * 256 + (rows * 8 + 255) / 256 * 256 + rows * head_dim * 4;
 }
 
 template <typename T, int D>
 int launch_tree(TreeParams p, hipStream_t s) {
-  constexpr int kWaves = TreeTile<T, D>::kWaves;
+  constexpr int kWaves = TreeTile<T, D, 8>::kWaves;
   int64_t wgs = p.num_work + (p.k_new ? (p.total_q + kWaves - 1) / kWaves : 0);
   if (wgs == 0) wgs = p.batch;  // pad rows only
   if (wgs > 0x7fffffff / 16) return fail(NSLG_EUNSUPPORTED, "paged_tree_attention: too many rows");
-  tree_attention_kernel<T, D><<<dim3((unsigned)wgs), 64 * kWaves, 0, s>>>(p);
+  const dim3 grid((unsigned)wgs);
+  if (p.tile_waves == 8) {
+    tree_attention_kernel<T, D, 8><<<grid, 64 * kWaves, 0, s>>>(p);
+  } else if constexpr (kWaves == 16) {
+    tree_attention_kernel<T, D, 16><<<grid, 64 * kWaves, 0, s>>>(p);
+  }
   const int rc = check_launch("paged_tree_attention");
   if (rc || p.whole) return rc;
   const int row_waves = (p.max_nodes * p.group + 15) / 16;
@@ -870,7 +886,7 @@ extern "C" size_t nslg_paged_tree_workspace_size(int32_t batch, int32_t num_qo_h
     return 0;
   const int64_t rows = (int64_t)max_q * (num_qo_heads / num_kv_heads);
   const int64_t n = tree_spans(batch, total_pages * page_size, rows, num_kv_heads, head_dim, dtype);
-  return tree_bytes(batch, n, num_kv_heads, head_dim);
+  return tree_bytes(batch, n, num_kv_heads, tree_rows(rows, head_dim, dtype), head_dim);
 }
 
 extern "C" int nslg_paged_tree_attention(const void* q, int64_t q_stride, const uint32_t* mask, int32_t mask_words,
@@ -960,14 +976,16 @@ extern "C" int nslg_paged_tree_attention(const void* q, int64_t q_stride, const 
   p.k_new_stride = k_new_stride * eb;
   p.v_new_stride = v_new_stride * eb;
   p.max_nodes = max_q;
-  int64_t spans = batch * tree_tiles(rows);
+  const int64_t tile_rows = tree_rows(rows, head_dim, dtype);
+  p.tile_waves = (int32_t)(tile_rows / 16);
+  int64_t spans = batch * tree_tiles(rows, head_dim, dtype);
   p.whole = 1;
   if (workspace && total_q > 0) {
     int64_t n = tree_spans(batch, total_pages * page_size, rows, num_kv_heads, head_dim, dtype);
-    while (n > 0 && tree_bytes(batch, n, num_kv_heads, head_dim) > workspace_bytes) --n;
+    while (n > 0 && tree_bytes(batch, n, num_kv_heads, tile_rows, head_dim) > workspace_bytes) --n;
     if (n > 0) {
       char* ws = (char*)(((uintptr_t)workspace + 255) / 256 * 256);  // (tree_bytes has room for this)
-      const size_t part_rows = (size_t)n * num_kv_heads * 2 * kTreeRows;
+      const size_t part_rows = (size_t)n * num_kv_heads * 2 * tile_rows;
       p.whole = 0;
       p.ws_tag = (uint64_t*)ws;
       ws += 256;
@@ -983,7 +1001,7 @@ extern "C" int nslg_paged_tree_attention(const void* q, int64_t q_stride, const 
   p.spans = (int32_t)spans;
   const int64_t work = total_q > 0 ? spans * num_kv_heads : 0;
   p.num_work = (int32_t)work;
-  p.stream = tree_tiles(rows) == 1 && total_pages * page_size * num_kv_heads * head_dim * 2 * eb > ((int64_t)256 << 20);
+  p.stream = tree_tiles(rows, head_dim, dtype) == 1 && total_pages * page_size * num_kv_heads * head_dim * 2 * eb > ((int64_t)256 << 20);
   hipStream_t s = as_stream(stream);
   if (dtype == NSLG_F16) return launch_tree_dim<F16>(p, head_dim, s);
   if (dtype == NSLG_BF16) return launch_tree_dim<BF16>(p, head_dim, s);
