@@ -749,9 +749,11 @@ int nslg_paged_tree_attention(const void* q, int64_t q_stride, const uint32_t* m
  *   u_accept        float[total_q] (a root's is not read); u_next float[batch]
  *   path            int32[batch][max_q]: the accepted nodes, node 0 first, -1 after them
  *   count, next_token   int32[batch]
- *   workspace       may be null
- * vocab <= 2^20.
+ *   workspace       of nslg_verify_tree_workspace_size bytes (0: none), 8-byte aligned, zeroed once before its first use
+ *                   and used for nothing else; one call at a time. Several workgroups then take a sequence. Null: one.
+ * vocab <= 2^20, batch <= 65535.
  */
+size_t nslg_verify_tree_workspace_size(int32_t batch, int32_t vocab);
 int nslg_verify_tree(const int32_t* tokens, const int32_t* parents, const int32_t* qo_indptr, const int32_t* q_rows,
                      int64_t total_q, int32_t max_q, int32_t batch, const void* target_probs, int64_t target_stride,
                      const void* draft_probs, int64_t draft_stride, int64_t num_rows, int32_t vocab, int32_t dtype,

@@ -131,6 +131,7 @@ SIGNATURES = {
                                             c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_int64,
                                             c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_void_p, c_int64,
                                             c_void_p, c_size_t, c_void_p]),
+    "nslg_verify_tree_workspace_size": (c_size_t, [c_int32, c_int32]),
     "nslg_verify_tree": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_void_p,
                                    c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, c_void_p, c_void_p,
                                    c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),

@@ -58,14 +58,16 @@ __global__ void __launch_bounds__(256) tree_plan_kernel(TreePlanParams p) {
 }
 
 // ---- verification ----------------------------------------------------------------------
-// One workgroup per sequence. Its first wave walks down from the root, 64 nodes at a time with the probabilities
-// that their tests take already loaded. At a node with target row p and draft row q, what is left of p once drawn
-// children were rejected is, up to a factor, max(p - c q, 0): taking max(r / W - q, 0), W the sum of r, from r =
-// max(p - c q, 0) leaves max(p - (c + W) q, 0) / W. So a rejection needs the sum of that at the new c and nothing else,
-// which all waves find together. Then the row that the next token is drawn from is summed in pieces of
-// kVerPiece tokens, the piece that holds it found from their running sum, and the token inside it.
+// At a node with target row p and draft row q, what is left of p once drawn children were rejected is, up to a factor,
+// max(p - c q, 0): taking max(r / W - q, 0), W the sum of r, from r = max(p - c q, 0) leaves max(p - (c + W) q, 0) / W. So a
+// rejection needs the sum of that at the new c and nothing else, and those sums, kept by pieces of kVerPiece tokens, are also
+// what the next token is found from: its piece from their running sum, then the token inside it.
 //
-// Sums and tests are in 64 bits: the order of adding decides no token.
+// Bound by latency, then by how fast a workgroup reads a row (0.5 MB at 128k tokens in fp32; one alone took 25 us of it). So
+// `slices` workgroups take a sequence: each walks down from the root (64 nodes at a time, with the probabilities that
+// their tests take already loaded) to the first sum that is wanted, and sums its slice of the row. The last one to be done goes
+// on alone: in most trees it only has the next token to find. Sums and tests are in 64 bits: the order of adding
+// decides no token.
 struct VerifyParams {
   const int32_t* tokens;
   const int32_t* parents;
@@ -85,12 +87,16 @@ struct VerifyParams {
   int32_t* path;
   int32_t* count;
   int32_t* next;
+  int32_t slices;    // workgroups a sequence
+  int32_t* arrived;  // [batch]: those done, 0 between calls (slices > 1)
+  double* sums;      // [batch, pieces]
 };
 
 constexpr int kVerThreads = 1024;
 constexpr int kVerWaves = kVerThreads / 64;
 constexpr int kVerPiece = 256;       // tokens of a piece: a wave, four each
 constexpr int kVerMaxPieces = 4096;  // (32 KB of LDS)
+constexpr int kVerBatch = 8;         // pieces that a wave loads at a time
 
 template <typename T>
 __device__ inline float prob_of(const char* row, int i) {
@@ -104,213 +110,298 @@ struct VF32 {
   static constexpr int kDtype = NSLG_F32;
 };
 
-// The weight that token i has left: p - c q, not below 0; what is no number counts nothing.
-template <typename T, bool kDraft>
-__device__ inline double weight_of(const char* prow, const char* qrow, double c, int i) {
-  double x = (double)prob_of<T>(prow, i);
+// Tokens i .. i + 3 of a row, 4 elements aligned.
+template <typename T>
+__device__ inline void load4(const char* row, int i, float (&x)[4]) {
+  if constexpr (T::kDtype == NSLG_F32) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(row + 4 * (int64_t)i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = v[e];
+  } else {
+    const u16x4 v = *reinterpret_cast<const u16x4*>(row + 2 * (int64_t)i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = T::to_f32(v[e]);
+  }
+}
+
+// The weight that is left of p at c: p - c q, not below 0; what is no number counts nothing.
+template <bool kDraft>
+__device__ inline double weight(float p, float q, double c) {
+  double x = (double)p;
   if constexpr (kDraft)
-    if (c != 0.0) x -= c * (double)prob_of<T>(qrow, i);
+    if (c != 0.0) x -= c * (double)q;
   return x > 0.0 && x < INFINITY ? x : 0.0;
 }
 
+// Sum over the wave's lanes: rotations within 16 lanes, then the row swaps.
 __device__ inline double wave_sum_f64(double x) {
+  auto halves = [](unsigned lo, unsigned hi) { return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo); };
+  auto lo = [](double v) { return (unsigned)__builtin_bit_cast(uint64_t, v); };
+  auto hi = [](double v) { return (unsigned)(__builtin_bit_cast(uint64_t, v) >> 32); };
+#define NSLG_TURN(ctrl) \
+  x += halves(__builtin_amdgcn_mov_dpp(lo(x), ctrl, 0xf, 0xf, false), __builtin_amdgcn_mov_dpp(hi(x), ctrl, 0xf, 0xf, false))
+  NSLG_TURN(0x128);  // row_ror:8
+  NSLG_TURN(0x124);  // row_ror:4
+  NSLG_TURN(0x122);  // row_ror:2
+  NSLG_TURN(0x121);  // row_ror:1
+#undef NSLG_TURN
+  {
+    const auto a = __builtin_amdgcn_permlane16_swap(lo(x), lo(x), false, false), c = __builtin_amdgcn_permlane16_swap(hi(x), hi(x), false, false);
+    x = halves(a[0], c[0]) + halves(a[1], c[1]);
+  }
+  const auto a = __builtin_amdgcn_permlane32_swap(lo(x), lo(x), false, false), c = __builtin_amdgcn_permlane32_swap(hi(x), hi(x), false, false);
+  return halves(a[0], c[0]) + halves(a[1], c[1]);
+}
+__device__ inline double wave_scan_f64(double x) {  // sum over the lanes up to one's own
+  const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off, 64);
+  for (int off = 1; off < 64; off <<= 1) {
+    const double y = __shfl_up(x, off, 64);
+    if (lane >= off) x += y;
+  }
   return x;
 }
 
 template <typename T, bool kDraft>
 __global__ void __launch_bounds__(kVerThreads) tree_verify_kernel(VerifyParams p) {
   __shared__ double piece[kVerMaxPieces];
-  __shared__ double wave_part[kVerWaves];
   __shared__ int rejected[kDraft ? 1 : kTreeMaxNodes];  // tokens rejected at the present node
-  __shared__ int s_cmd, s_row, s_rejects, s_at;
-  __shared__ double s_c, s_sum;
+  __shared__ int path_lds[kTreeMaxNodes];
+  __shared__ int s_done, s_row, s_rejects, s_next;
+  __shared__ double s_c;
 
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int b = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q0 = p.qo_indptr[b];
   const int n = (int)min((int64_t)min(max(p.qo_indptr[b + 1] - q0, 0), p.max_q), p.total_q - q0);
   int32_t* path = p.path + (int64_t)b * p.max_q;
   if (n <= 0) {  // no tree: nothing accepted, no token
-    for (int i = tid; i < p.max_q; i += kVerThreads) path[i] = -1;
-    if (tid == 0) p.count[b] = 0, p.next[b] = -1;
+    if (slice == 0) {
+      for (int i = tid; i < p.max_q; i += kVerThreads) path[i] = -1;
+      if (tid == 0) p.count[b] = 0, p.next[b] = -1;
+    }
     return;
   }
   auto row_of = [&](int node) -> int64_t {
     const int64_t at = p.q_rows ? p.q_rows[q0 + node] : q0 + node;
     return at < 0 ? 0 : (at >= p.rows ? p.rows - 1 : at);
   };
-  // state of the walk (wave 0, uniform)
+  // The state of the walk (wave 0, uniform): node, next child to look at, accepted nodes, rejections at the node (tokens
+  // given), c and the sum W of what is left (tokens drawn).
   int cur = 0, from = 1, count = 1, rejects = 0;
   double c = 0.0, W = 1.0;
-  if (tid == 0) path[0] = 0;
-  while (true) {
-    if (wave == 0) {
-      int cmd = 0;  // 1: the sum at c is wanted, 0: done
-      while (from < n && cmd == 0) {
-        const int base = from & ~63;
-        const int j = base + lane;
-        const int up = j < n ? p.parents[q0 + j] : -2;
-        const int x = j < n ? p.tokens[q0 + j] : -1;
-        const float u = j < n ? p.u_accept[q0 + j] : 0.f;
-        const bool tried = up >= 0 && up < j && x >= 0 && x < p.vocab;
-        double pj = 0.0, qj = 1.0;
+  // the lane's node of the 64 from `loaded` on: parent, token, number, the probabilities of its test
+  int loaded = -1, up = -2, x = -1;
+  float u = 0.f;
+  bool tried = false;
+  double pj = 0.0, qj = 1.0;
+  // Down to the first sum that is wanted, or to the end.
+  auto walk = [&]() {
+    bool wanted = false;
+    while (from < n && !wanted) {
+      const int base = from & ~63;
+      const int j = base + lane;
+      if (base != loaded) {
+        loaded = base;
+        up = j < n ? p.parents[q0 + j] : -2;
+        x = j < n ? p.tokens[q0 + j] : -1;
+        u = j < n ? p.u_accept[q0 + j] : 0.f;
+        tried = up >= 0 && up < j && x >= 0 && x < p.vocab;
         if (tried) {
           const int64_t at = row_of(up);
           pj = (double)prob_of<T>(p.target + at * p.target_stride, x);
           if constexpr (kDraft) qj = (double)prob_of<T>(p.draft + at * p.draft_stride, x);
         }
-        while (cmd == 0) {
-          const unsigned long long m = __ballot(j >= from && j < n && up == cur);
-          if (m == 0) {
-            from = base + 64;
-            break;
-          }
-          const int src = __ffsll((long long)m) - 1;
-          from = base + src + 1;
-          const bool ok_token = __shfl((int)tried, src, 64);
-          const int xs = __shfl(x, src, 64);
-          double left = __shfl(pj, src, 64);
-          const double q = __shfl(qj, src, 64);
-          const double us = (double)__shfl(u, src, 64);
-          if constexpr (kDraft) {
-            if (c != 0.0) left -= c * q;
-          } else {
-            bool again = false;
-            for (int i = lane; i < rejects; i += 64) again |= rejected[i] == xs;
-            if (__ballot(again)) left = 0.0;
-          }
-          left = ok_token && left > 0.0 && left < INFINITY ? left : 0.0;
-          if (us * W * q < left) {  // accepted
-            cur = base + src;
-            if (lane == 0 && count < p.max_q) path[count] = cur;
-            ++count;
-            c = 0.0, W = 1.0, rejects = 0;
-            continue;
-          }
-          if constexpr (kDraft) {
-            if (W > 0.0) c += W, cmd = 1;
-          } else {
-            W -= left;
-            if (left > 0.0) {
-              if (lane == 0) rejected[rejects] = xs;
-              ++rejects;
-              // (one wave's LDS operations complete in order; the fence is for the compiler)
-              __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            }
+      }
+      while (!wanted) {
+        const unsigned long long m = __ballot(j >= from && j < n && up == cur);
+        if (m == 0) {
+          from = base + 64;
+          break;
+        }
+        const int src = __ffsll((long long)m) - 1;
+        from = base + src + 1;
+        const bool ok_token = __shfl((int)tried, src, 64);
+        const int xs = __shfl(x, src, 64);
+        double left = __shfl(pj, src, 64);
+        const double q = __shfl(qj, src, 64);
+        const double us = (double)__shfl(u, src, 64);
+        if constexpr (kDraft) {
+          if (c != 0.0) left -= c * q;
+        } else {
+          bool again = false;
+          for (int i = lane; i < rejects; i += 64) again |= rejected[i] == xs;
+          if (__ballot(again)) left = 0.0;
+        }
+        left = ok_token && left > 0.0 && left < INFINITY ? left : 0.0;
+        if (us * W * q < left) {  // accepted
+          cur = base + src;
+          if (lane == 0) path_lds[count] = cur;
+          ++count;
+          c = 0.0, W = 1.0, rejects = 0;
+          continue;
+        }
+        if constexpr (kDraft) {
+          if (W > 0.0) c += W, wanted = true;
+        } else {
+          W -= left;
+          if (left > 0.0) {
+            if (lane == 0) rejected[rejects] = xs;
+            ++rejects;
+            // (one wave's LDS operations complete in order; the fence is for the compiler)
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           }
         }
       }
-      if (lane == 0) s_cmd = cmd, s_row = cur, s_c = c, s_rejects = rejects;
     }
-    __syncthreads();
-    if (s_cmd == 0) break;
-    // the sum of what is left at c
-    const int64_t at = row_of(s_row);
+    if (lane == 0) s_done = !wanted, s_row = cur, s_c = c, s_rejects = rejects;
+  };
+  // The sums of pieces g0 .. g1 - 1 of what is left of a row, the workgroup's waves kVerBatch pieces at a time.
+  auto sum_pieces = [&](int row, double cc, int gone, int g0, int g1) {
+    const int64_t at = row_of(row);
     const char* prow = p.target + at * p.target_stride;
-    const char* qrow = p.draft + at * p.draft_stride;
-    double x = 0.0;
-    for (int i = tid; i < p.vocab; i += kVerThreads) x += weight_of<T, kDraft>(prow, qrow, s_c, i);
-    x = wave_sum_f64(x);
-    if (lane == 0) wave_part[wave] = x;
-    __syncthreads();
-    if (wave == 0) {
-      double sum = 0.0;
-      for (int i = 0; i < kVerWaves; ++i) sum += wave_part[i];
-      W = sum;
+    const char* qrow = kDraft ? p.draft + at * p.draft_stride : nullptr;
+    const bool need_q = kDraft && cc != 0.0;
+    const bool wide = ((uintptr_t)prow | (uintptr_t)(need_q ? qrow : prow)) % (T::kDtype == NSLG_F32 ? 16 : 8) == 0;
+    for (int g = g0 + wave * kVerBatch; g < g1; g += kVerWaves * kVerBatch) {
+      // (a lane takes four tokens in a row of each piece: one load where the rows allow it)
+      float pv[kVerBatch][4], qv[kVerBatch][4];
+#pragma unroll
+      for (int k = 0; k < kVerBatch; ++k) {
+        const int i = (g + k) * kVerPiece + 4 * lane;
+        if (wide && i + 4 <= p.vocab) {
+          load4<T>(prow, i, pv[k]);
+          if (need_q) load4<T>(qrow, i, qv[k]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            pv[k][e] = prob_of<T>(prow, min(i + e, p.vocab - 1));
+            if (need_q) qv[k][e] = prob_of<T>(qrow, min(i + e, p.vocab - 1));
+          }
+        }
+      }
+      double x[kVerBatch];
+#pragma unroll
+      for (int k = 0; k < kVerBatch; ++k) {
+        x[k] = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = (g + k) * kVerPiece + 4 * lane + e;
+          double v = i < p.vocab ? weight<kDraft>(pv[k][e], need_q ? qv[k][e] : 0.f, cc) : 0.0;
+          if constexpr (!kDraft)
+            for (int z = 0; z < gone; ++z) v = rejected[z] == i ? 0.0 : v;
+          x[k] += v;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kVerBatch; ++k) x[k] = wave_sum_f64(x[k]);
+      if (lane == 0) {
+#pragma unroll
+        for (int k = 0; k < kVerBatch; ++k)
+          if (g + k < g1) piece[g + k] = x[k];
+      }
     }
+  };
+  const int pieces = (p.vocab + kVerPiece - 1) / kVerPiece;
+
+  if (tid == 0) path_lds[0] = 0;
+  if (wave == 0) walk();
+  __syncthreads();
+  const int each = ((pieces + p.slices - 1) / p.slices + kVerBatch - 1) / kVerBatch * kVerBatch;
+  const int g0 = min(slice * each, pieces), g1 = min(g0 + each, pieces);
+  sum_pieces(s_row, s_c, s_rejects, g0, g1);
+  __syncthreads();
+  if (p.slices > 1) {
+    // The sums go past the caches of the workgroup's XCD (stores and loads at the device's scope), and each wave's are there
+    // before the workgroup counts itself in: the last one sees them all. (A fence at that scope in each workgroup, which
+    // writes the XCD's cache back, took 64 sequences from 27 to 144 us.)
+    double* sums = p.sums + (int64_t)b * pieces;
+    for (int g = g0 + tid; g < g1; g += kVerThreads) __hip_atomic_store(&sums[g], piece[g], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) s_next = __hip_atomic_fetch_add(&p.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (s_next != p.slices - 1) return;
+    if (tid == 0) __hip_atomic_store(&p.arrived[b], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int g = tid; g < pieces; g += kVerThreads)
+      piece[g] = __hip_atomic_load(&sums[g], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+  }
+  // The sequence's last workgroup. The pieces are those of row s_row at s_c; a lane takes `run` of them in turn.
+  const int run = (pieces + 63) / 64;
+  while (true) {
+    const int done = s_done, row = s_row, gone = s_rejects;
+    const double at_c = s_c;
+    double mine = 0.0;
+    if (wave == 0) {
+      for (int g = lane * run; g < min((lane + 1) * run, pieces); ++g) mine += piece[g];
+      W = wave_sum_f64(mine);
+    }
+    __syncthreads();  // the state is read
+    if (!done) {
+      if (wave == 0) walk();
+      __syncthreads();
+      if (s_row != row || s_c != at_c) {
+        sum_pieces(s_row, s_c, s_rejects, 0, pieces);
+        __syncthreads();
+      }
+      continue;
+    }
+    // the next token
+    int found = -1;
+    if (wave == 0) {
+      if (W > 0.0) {
+        const double goal = (double)p.u_next[b] * W;
+        const int64_t at = row_of(row);
+        const char* prow = p.target + at * p.target_stride;
+        const char* qrow = kDraft ? p.draft + at * p.draft_stride : nullptr;
+        const double incl = wave_scan_f64(mine);
+        // the lane whose pieces the goal lies in (the last one with any weight where a rounding leaves it unreached)
+        const unsigned long long hit = __ballot(incl > goal && mine > 0.0), some = __ballot(mine > 0.0);
+        const int src = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)some);
+        double base = __shfl(incl - mine, src, 64);
+        int g = -1;
+        double g_base = 0.0;
+        for (int k = src * run; k < min((src + 1) * run, pieces); ++k) {
+          const double x = piece[k];
+          if (x > 0.0) g = k, g_base = base;
+          base += x;
+          if (x > 0.0 && base > goal) break;
+        }
+        auto left_of = [&](int i) -> double {
+          if (i >= p.vocab) return 0.0;
+          if constexpr (!kDraft)
+            for (int z = 0; z < gone; ++z)
+              if (rejected[z] == i) return 0.0;
+          return weight<kDraft>(prob_of<T>(prow, i), kDraft && at_c != 0.0 ? prob_of<T>(qrow, i) : 0.f, at_c);
+        };
+        double v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = left_of(g * kVerPiece + 64 * e + lane);
+        int last = -1;
+        for (int e = 0; e < 4 && found < 0; ++e) {
+          const double sum = wave_scan_f64(v[e]);
+          const unsigned long long at_goal = __ballot(g_base + sum > goal && v[e] > 0.0), any = __ballot(v[e] > 0.0);
+          if (any) last = g * kVerPiece + 64 * e + 63 - __clzll((long long)any);
+          if (at_goal) found = g * kVerPiece + 64 * e + __ffsll((long long)at_goal) - 1;
+          g_base += __shfl(sum, 63, 64);
+        }
+        if (found < 0) found = last;
+      }
+      if (lane == 0) s_next = found;
+    }
+    __syncthreads();
+    if (s_next >= 0 || (at_c == 0.0 && gone == 0)) break;
+    // rejections have left nothing of the row: from the row as it is
+    if (tid == 0) s_c = 0.0, s_rejects = 0;
+    __syncthreads();
+    sum_pieces(row, 0.0, 0, 0, pieces);
     __syncthreads();
   }
   if (wave == 0) {
-    for (int i = count + lane; i < p.max_q; i += 64) path[i] = -1;
-    if (lane == 0) p.count[b] = count;
+    for (int i = lane; i < p.max_q; i += 64) path[i] = i < count ? path_lds[i] : -1;
+    if (lane == 0) p.count[b] = count, p.next[b] = s_next;
   }
-
-  // ---- the next token
-  const int64_t at = row_of(s_row);
-  const char* prow = p.target + at * p.target_stride;
-  const char* qrow = kDraft ? p.draft + at * p.draft_stride : nullptr;
-  const int pieces = (p.vocab + kVerPiece - 1) / kVerPiece;
-  for (int attempt = 0; attempt < 2; ++attempt) {
-    // (a second time with the row as it is, where rejections left nothing of it)
-    const double cc = attempt ? 0.0 : s_c;
-    const int gone = attempt || kDraft ? 0 : s_rejects;
-    auto left_of = [&](int i) -> double {
-      if (i >= p.vocab) return 0.0;
-      if constexpr (!kDraft)
-        for (int k = 0; k < gone; ++k)
-          if (rejected[k] == i) return 0.0;
-      return weight_of<T, kDraft>(prow, qrow, cc, i);
-    };
-    for (int g = wave; g < pieces; g += kVerWaves) {
-      double x = 0.0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x += left_of(g * kVerPiece + 64 * e + lane);
-      x = wave_sum_f64(x);
-      if (lane == 0) piece[g] = x;
-    }
-    __syncthreads();
-    if (wave == 0) {
-      double total = 0.0;
-      for (int g = lane; g < pieces; g += 64) total += piece[g];
-      total = wave_sum_f64(total);
-      int found = -1;
-      if (total > 0.0) {
-        const double goal = (double)p.u_next[b] * total;
-        double run = 0.0;
-        int last = -1;  // the last piece with any weight: where rounding leaves the goal unreached
-        double last_run = 0.0;
-        int g_at = -1;
-        for (int g0 = 0; g0 < pieces && g_at < 0; g0 += 64) {
-          const double mine = g0 + lane < pieces ? piece[g0 + lane] : 0.0;
-          double incl = mine;
-#pragma unroll
-          for (int off = 1; off < 64; off <<= 1) {
-            const double y = __shfl_up(incl, off, 64);
-            if (lane >= off) incl += y;
-          }
-          const unsigned long long hit = __ballot(run + incl > goal && mine > 0.0);
-          const unsigned long long some = __ballot(mine > 0.0);
-          if (hit) {
-            const int src = __ffsll((long long)hit) - 1;
-            g_at = g0 + src;
-            run += __shfl(incl - mine, src, 64);
-          } else {
-            if (some) {
-              const int src = 63 - __clzll((long long)some);
-              last = g0 + src;
-              last_run = run + __shfl(incl - mine, src, 64);
-            }
-            run += __shfl(incl, 63, 64);
-          }
-        }
-        if (g_at < 0) g_at = last, run = last_run;
-        for (int e = 0; e < 4 && found < 0; ++e) {
-          const int i = g_at * kVerPiece + 64 * e + lane;
-          const double mine = left_of(i);
-          double incl = mine;
-#pragma unroll
-          for (int off = 1; off < 64; off <<= 1) {
-            const double y = __shfl_up(incl, off, 64);
-            if (lane >= off) incl += y;
-          }
-          const unsigned long long hit = __ballot(run + incl > goal && mine > 0.0);
-          if (hit) found = g_at * kVerPiece + 64 * e + __ffsll((long long)hit) - 1;
-          run += __shfl(incl, 63, 64);
-        }
-        for (int e = 3; e >= 0 && found < 0; --e) {  // (not reached by a rounding: the last token with any weight)
-          const unsigned long long some = __ballot(left_of(g_at * kVerPiece + 64 * e + lane) > 0.0);
-          if (some) found = g_at * kVerPiece + 64 * e + 63 - __clzll((long long)some);
-        }
-      }
-      if (lane == 0) s_at = found;
-    }
-    __syncthreads();
-    if (s_at >= 0) break;
-    __syncthreads();  // (s_at is read before the second attempt writes it)
-  }
-  if (tid == 0) p.next[b] = s_at;
 }
 
 // ---- the accepted nodes' K/V -------------------------------------------------------------
@@ -405,14 +496,28 @@ extern "C" int nslg_tree_plan(const int32_t* parents, const int32_t* qo_indptr, 
   return check_launch("tree_plan");
 }
 
+// Workgroups a sequence: of 16 pieces (4096 tokens) each at least, about two a CU in all.
+static int verify_slices(int32_t batch, int32_t vocab) {
+  const int by_row = (vocab + 16 * kVerPiece - 1) / (16 * kVerPiece);
+  const int by_cus = 512 / batch;
+  const int n = by_row < by_cus ? by_row : by_cus;
+  return n < 1 ? 1 : n;
+}
+static size_t verify_bytes(int32_t batch, int32_t vocab) {
+  return ((size_t)batch * 4 + 255) / 256 * 256 + (size_t)batch * ((vocab + kVerPiece - 1) / kVerPiece) * 8;
+}
+
+extern "C" size_t nslg_verify_tree_workspace_size(int32_t batch, int32_t vocab) {
+  if (batch <= 0 || vocab <= 0 || vocab > kVerMaxPieces * kVerPiece || verify_slices(batch, vocab) == 1) return 0;
+  return verify_bytes(batch, vocab);
+}
+
 extern "C" int nslg_verify_tree(const int32_t* tokens, const int32_t* parents, const int32_t* qo_indptr,
                                 const int32_t* q_rows, int64_t total_q, int32_t max_q, int32_t batch,
                                 const void* target_probs, int64_t target_stride, const void* draft_probs,
                                 int64_t draft_stride, int64_t num_rows, int32_t vocab, int32_t dtype,
                                 const float* u_accept, const float* u_next, int32_t* path, int32_t* count,
                                 int32_t* next_token, void* workspace, size_t workspace_bytes, nslg_stream_t stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   const int eb = elem_bytes(dtype);
   if (!eb) return fail(NSLG_EINVAL, "verify_tree: bad dtype %d", dtype);
   if (batch < 0 || total_q < 0 || max_q < 0 || (int64_t)max_q * batch < total_q)
@@ -431,11 +536,18 @@ extern "C" int nslg_verify_tree(const int32_t* tokens, const int32_t* parents, c
   if (target_stride < vocab || (draft_probs && draft_stride < vocab))
     return fail(NSLG_EINVAL, "verify_tree: row stride smaller than the vocabulary");
   if (((uintptr_t)target_probs | (uintptr_t)draft_probs) % eb) return fail(NSLG_EINVAL, "verify_tree: unaligned rows");
+  if (batch > 65535) return fail(NSLG_EUNSUPPORTED, "verify_tree: batches of up to 65535 (%d)", batch);
+  if ((uintptr_t)workspace & 7) return fail(NSLG_EINVAL, "verify_tree: the workspace must be 8-byte aligned");
   VerifyParams p = {tokens, parents, qo_indptr, q_rows, total_q, max_q, batch, num_rows,
                     (const char*)target_probs, target_stride * eb, (const char*)draft_probs, draft_stride * eb, vocab,
-                    u_accept, u_next, path, count, next_token};
+                    u_accept, u_next, path, count, next_token, 1, nullptr, nullptr};
+  if (workspace && workspace_bytes >= verify_bytes(batch, vocab)) {
+    p.slices = verify_slices(batch, vocab);
+    p.arrived = (int32_t*)workspace;
+    p.sums = (double*)((char*)workspace + ((size_t)batch * 4 + 255) / 256 * 256);
+  }
   hipStream_t s = as_stream(stream);
-  const dim3 grid((unsigned)batch);
+  const dim3 grid((unsigned)p.slices, (unsigned)batch);
   auto launch = [&](auto type) {
     using T = decltype(type);
     if (draft_probs)

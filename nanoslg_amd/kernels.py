@@ -257,6 +257,7 @@ class Workspace:
         self.buf = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=self.device)
 
         self.prefill_buf: Optional[torch.Tensor] = None
+        self.verify_buf: Optional[torch.Tensor] = None
 
     def get(self, nbytes: int) -> torch.Tensor:
         if self.buf.numel() < nbytes:
@@ -269,6 +270,12 @@ class Workspace:
         if self.prefill_buf is None or self.prefill_buf.numel() < nbytes:
             self.prefill_buf = torch.empty(int(nbytes * 1.25) + 256, dtype=torch.uint8, device=self.device)
         return self.prefill_buf
+
+    def get_verify(self, nbytes: int) -> torch.Tensor:
+        """Scratch of verify_tree calls: memory of its own, since they expect the zeros that they leave."""
+        if self.verify_buf is None or self.verify_buf.numel() < nbytes:
+            self.verify_buf = torch.zeros(int(nbytes * 1.25) + 256, dtype=torch.uint8, device=self.device)
+        return self.verify_buf
 
 
 class DecodeGroups:

@@ -148,6 +148,9 @@ def paged_tree_attention(q: torch.Tensor, mask: torch.Tensor, qo_indptr: torch.T
     return out
 
 
+_VERIFY_BYTES: Dict[Tuple[int, int], int] = {}  # nslg_verify_tree_workspace_size by batch and vocabulary
+
+
 def verify_tree(tokens: torch.Tensor, parents: torch.Tensor, qo_indptr: torch.Tensor, total_q: int, max_q: int,
                 target_probs: torch.Tensor, u_accept: torch.Tensor, u_next: torch.Tensor,
                 draft_probs: Optional[torch.Tensor] = None, q_rows: Optional[torch.Tensor] = None,
@@ -159,7 +162,8 @@ def verify_tree(tokens: torch.Tensor, parents: torch.Tensor, qo_indptr: torch.Te
     distribution that its children were drawn from, independently; without it the drafted tokens are taken as given.
     Returns (path, count, next): int32 [B, max_q] accepted nodes, the root first, -1 behind them; their number
     [B]; the token that follows [B]. Accepted and next tokens have the target's distribution. Rows with the
-    probability of one token 1 make this greedy verification."""
+    probability of one token 1 make this greedy verification. `workspace`: with it, kept from call to call and used by one call
+    at a time, several workgroups take a sequence."""
     dev = _one_device(tokens, parents, qo_indptr, target_probs, u_accept, u_next)
     B, total_q, max_q = _trees("verify_tree", qo_indptr, total_q, max_q, q_rows)
     _i32(tokens, "tokens")
@@ -185,12 +189,21 @@ def verify_tree(tokens: torch.Tensor, parents: torch.Tensor, qo_indptr: torch.Te
         if draft_probs.shape != target_probs.shape or draft_probs.stride(1) != 1:
             raise ValueError("verify_tree: draft_probs must be shaped like target_probs")
         ds = draft_probs.stride(0) if rows > 1 else vocab
+    ws, need = None, 0
+    if workspace is not None:
+        key = (B, vocab)
+        need = _VERIFY_BYTES.get(key)
+        if need is None:  # a pure function of the call shape
+            need = _VERIFY_BYTES[key] = int(_lib.load().nslg_verify_tree_workspace_size(B, vocab))
+        if need:
+            ws = workspace.get_verify(need)
     buf = torch.empty(B * (max_q + 2), dtype=torch.int32, device=tokens.device)
     at = buf.data_ptr()
     rc = _call(dev, _lib.fast_tree().verify_tree, tokens.data_ptr(), parents.data_ptr(), qo_indptr.data_ptr(),
                None if q_rows is None else q_rows.data_ptr(), total_q, max_q, B, target_probs.data_ptr(), ts,
                None if draft_probs is None else draft_probs.data_ptr(), ds, rows, vocab, code, u_accept.data_ptr(),
-               u_next.data_ptr(), at, at + 4 * B * max_q, at + 4 * B * (max_q + 1), None, 0, _stream(tokens))
+               u_next.data_ptr(), at, at + 4 * B * max_q, at + 4 * B * (max_q + 1), None if ws is None else ws.data_ptr(), need,
+               _stream(tokens))
     _lib.check(rc, "nslg_verify_tree")
     path, count, token = buf.split([B * max_q, B, B])
     return path.view(B, max_q), count, token

@@ -333,14 +333,25 @@ def _rows_like_a_model(g, n, V, dtype, noise=0.7, empty=0.0):
     return p.to(dtype), q.to(dtype)
 
 
-def _verify(trees, tokens, p, q, ua, un, rows=None, strides=None):
+def _verify(trees, tokens, p, q, ua, un, rows=None):
+    """The kernel with one workgroup a sequence and with several, against the oracle."""
+    from nanoslg_amd import kernels
+    for ws in (None, kernels.Workspace(torch.device(DEV))):
+        for _ in range(2 if ws else 1):
+            got = _verify1(trees, tokens, p, q, ua, un, rows, ws)
+        if ws and ws.verify_buf is not None:
+            assert not ws.verify_buf[:4 * len(trees)].any()  # the counters, for the next call
+    return got
+
+
+def _verify1(trees, tokens, p, q, ua, un, rows, workspace):
     from nanoslg_amd import kernels
     lens = [len(t) for t in trees]
     B, T, S = len(trees), sum(lens), max(lens)
     dp, dq = p.to(DEV), None if q is None else q.to(DEV)
     path, count, token = kernels.verify_tree(_i32(tokens), _i32([x for t in trees for x in t]),
                                              _i32([sum(lens[:b]) for b in range(B + 1)]), T, S, dp, ua.to(DEV), un.to(DEV),
-                                             draft_probs=dq, q_rows=None if rows is None else _i32(rows))
+                                             draft_probs=dq, q_rows=None if rows is None else _i32(rows), workspace=workspace)
     path, count, token = path.tolist(), count.tolist(), token.tolist()
     first = 0
     for b, t in enumerate(trees):

@@ -114,7 +114,8 @@ def test_attention_refusals():
 def test_workspace_sizes():
     from nanoslg_amd import _lib
     size = _lib.load().nslg_paged_tree_workspace_size
-    assert 0 < size(1, 32, 8, 128, 128, 16, 16, 0) < size(1, 32, 8, 128, 4096, 16, 16, 0)
+    assert 0 < size(1, 32, 8, 128, 12, 16, 16, 0) < size(1, 32, 8, 128, 4096, 16, 16, 0)
+    assert _lib.load().nslg_verify_tree_workspace_size(1, 4000) == 0 < _lib.load().nslg_verify_tree_workspace_size(1, 5000)
     assert size(64, 32, 8, 128, 100_000, 16, 64, 0) < 1 << 29
     for bad in ((0, 32, 8, 128, 9, 16, 16, 0), (1, 32, 8, 96, 9, 16, 16, 0), (1, 32, 8, 128, 9, 16, 2000, 0), (1, 30, 8, 128, 9, 16, 9, 0),
                 (1, 32, 8, 128, 9, 16, 9, 5)):
