@@ -503,8 +503,11 @@ static int verify_slices(int32_t batch, int32_t vocab) {
   const int n = by_row < by_cus ? by_row : by_cus;
   return n < 1 ? 1 : n;
 }
+// The counters (slices > 1: at most 256 sequences) before the sums, at an offset that does not depend on the call: a
+// later one of another batch finds its counters zero.
+constexpr int kVerHead = 1024;
 static size_t verify_bytes(int32_t batch, int32_t vocab) {
-  return ((size_t)batch * 4 + 255) / 256 * 256 + (size_t)batch * ((vocab + kVerPiece - 1) / kVerPiece) * 8;
+  return kVerHead + (size_t)batch * ((vocab + kVerPiece - 1) / kVerPiece) * 8;
 }
 
 extern "C" size_t nslg_verify_tree_workspace_size(int32_t batch, int32_t vocab) {
@@ -544,7 +547,7 @@ extern "C" int nslg_verify_tree(const int32_t* tokens, const int32_t* parents, c
   if (workspace && workspace_bytes >= verify_bytes(batch, vocab)) {
     p.slices = verify_slices(batch, vocab);
     p.arrived = (int32_t*)workspace;
-    p.sums = (double*)((char*)workspace + ((size_t)batch * 4 + 255) / 256 * 256);
+    p.sums = (double*)((char*)workspace + kVerHead);
   }
   hipStream_t s = as_stream(stream);
   const dim3 grid((unsigned)p.slices, (unsigned)batch);

@@ -435,6 +435,18 @@ def test_verify_odd_rows(drawn):
         _verify(trees, tokens, p, q if drawn else None, torch.rand(len(rows), generator=g), torch.rand(4, generator=g), rows)
 
 
+def test_verify_with_one_workspace_for_other_batches():
+    """A workspace that a call left is another batch's: its counters are where the sums were not."""
+    from nanoslg_amd import kernels
+    rng, g = random.Random(0), torch.Generator().manual_seed(0)
+    ws = kernels.Workspace(torch.device(DEV))
+    for B, V in ((1, 40000), (200, 9000), (256, 12000), (2, 1 << 20), (100, 5000), (1, 9000), (300, 9000)):
+        trees = [random_tree(rng, 3) for _ in range(B)]
+        p = torch.softmax(2 * torch.randn(3 * B, V, generator=g), -1)
+        tokens = [int(p[i].argmax()) for i in range(3 * B)]
+        _verify1(trees, tokens, p, None, torch.rand(3 * B, generator=g) * 0.01, torch.rand(B, generator=g), None, ws)
+
+
 @pytest.mark.parametrize("drawn", [True, False])
 def test_verified_tokens_have_the_targets_distribution(drawn):
     """The first token behind the root over 40000 trees of four children: its frequencies are the target's within five
