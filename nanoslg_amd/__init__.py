@@ -19,3 +19,5 @@ from .kv_cache import (  # noqa: F401
     attention_forward,
     create_cache_manager,
 )
+from .tree_cache import TreeCacheContext, TreeResult  # noqa: F401
+

@@ -1144,7 +1144,7 @@ def paged_prefill(q: torch.Tensor, qo_indptr: torch.Tensor, total_q: int, max_q:
 # (nanoslg_amd.kernels_tree) under this module's name too
 _Q8_CALLS = ("append_kv_q8", "gather_kv_q8", "paged_decode_q8", "paged_decode_append_q8", "paged_decode_rope_append_q8",
              "paged_prefill_q8", "rotate_rows", "DecodeLaunchQ8")
-_TREE_CALLS = ("tree_plan", "paged_tree_attention", "verify_tree", "move_accepted")
+_TREE_CALLS = ("tree_plan", "paged_tree_attention", "verify_tree", "move_accepted", "MAX_TREE_NODES")
 
 
 def __getattr__(name: str):

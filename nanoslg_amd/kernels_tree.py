@@ -21,7 +21,7 @@ from . import _lib
 from .kernels import _DTYPE_CODE, Workspace, _i32, _layer_geom, _pool_geom, _require_gpu, _stream
 from .kernels_q8 import _call, _new_rows, _one_device, _table
 
-MAX_NODES = 1024
+MAX_TREE_NODES = 1024
 
 
 def _trees(what: str, qo_indptr: torch.Tensor, total_q: int, max_q: int, q_rows: Optional[torch.Tensor],
@@ -31,8 +31,8 @@ def _trees(what: str, qo_indptr: torch.Tensor, total_q: int, max_q: int, q_rows:
     B, total_q, max_q = qo_indptr.numel() - 1, int(total_q), int(max_q)
     if B < 0 or total_q < 0 or max_q < 0 or max_q * B < total_q:
         raise ValueError(f"{what}: {total_q} nodes in {B} trees of at most {max_q}")
-    if max_q > MAX_NODES:
-        raise ValueError(f"{what}: trees of up to {MAX_NODES} nodes (max_q = {max_q})")
+    if max_q > MAX_TREE_NODES:
+        raise ValueError(f"{what}: trees of up to {MAX_TREE_NODES} nodes (max_q = {max_q})")
     if q_rows is not None:
         _i32(q_rows, "q_rows")
         if q_rows.numel() < total_q or grid_width < 1:

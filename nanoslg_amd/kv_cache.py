@@ -247,9 +247,37 @@ class KVCacheManager(ABC):
     @abstractmethod
     def reset(self): ...
 
+    # speculative decoding with trees of drafted tokens (tree_cache)
+
+    def begin_tree(self, seq_ids: List[str], parents):
+        """A forward over a tree of drafted tokens for each sequence (a tree_cache.TreeCacheContext). parents: for each
+        sequence its nodes' parents (node 0 the root: -1; each other one's lies before it), or an int32 tensor [B, nodes] on
+        the cache's device. Ended with accept_tree or end_tree, not with end_forward."""
+        from . import tree_cache
+        return tree_cache.TreeCacheContext(self, seq_ids, parents)
+
+    def accept_tree(self, ctx, tokens, target_probs, u_accept, u_next, draft_probs=None):
+        """Verify a tree forward's drafted tokens and end it with the accepted nodes. tokens and u_accept [B, S] on the
+        forward's grid (numbers in [0, 1); the roots' are not read), target_probs and draft_probs [B, S, vocabulary] (kernels.
+        verify_tree), u_next [B]. Returns a tree_cache.TreeResult; waits for the GPU."""
+        from . import tree_cache
+        return tree_cache.accept_tree(self, ctx, tokens, target_probs, u_accept, u_next, draft_probs)
+
+    def end_tree(self, ctx, path, count):
+        """End a tree forward with given paths: int32 [B, nodes] rising node indices and [B] their numbers, on the device.
+        Their K/V moves together behind the sequences' tokens, which they become; the other nodes are dropped. Returns the
+        numbers as a list; waits for the GPU."""
+        from . import tree_cache
+        return tree_cache.end_tree(self, ctx, path, count)
+
     @property
     @abstractmethod
     def stats(self) -> Dict: ...
+
+
+def _check_forward(ctx) -> None:
+    if getattr(ctx, "is_tree", False):
+        raise ValueError("a forward over trees ends with accept_tree or end_tree")
 
 
 # --------------------------------------------------------------------------------------
@@ -1820,8 +1848,31 @@ class PagedKVCache(KVCacheManager):
             raise
 
     def end_forward(self, ctx):
+        _check_forward(ctx)
         for b in range(ctx.batch_size):
             self.seqs[ctx.seq_ids[b]].num_tokens += ctx.new_token_counts[b]
+
+    # a tree forward's cache (tree_cache)
+
+    @property
+    def _kv_pools(self):
+        return self.pool
+
+    def _kv_layer(self, i):
+        return self.pool.layer(i)
+
+    @property
+    def _states(self):
+        return self.seqs
+
+    def _end_tree(self, st, accepted, nodes):
+        """End a forward of `nodes` tokens behind st's with the first `accepted` of them. The pages stay with the
+        sequence; what they hold behind its tokens is not used."""
+        self._dev_plan = None
+        ps, start = self.cfg.page_size, st.num_tokens
+        st.num_tokens += accepted
+        p = np.arange(start // ps, (start + nodes - 1) // ps + 1)
+        self.pool.tokens_used[st.bt[p]] = np.clip(st.num_tokens - p * ps, 0, ps)
 
     def release_sequence(self, seq_id):
         """kv_cache.py:739-751: cache full pages in the tree, unpin, release."""
@@ -2105,8 +2156,24 @@ class ContiguousKVCache(KVCacheManager):
         return ContiguousCacheContext(self, seq_ids, ntoks, offsets)
 
     def end_forward(self, ctx):
+        _check_forward(ctx)
         for b in range(ctx.batch_size):
             self.states[ctx.seq_ids[b]].num_tokens += ctx.new_token_counts[b]
+
+    # a tree forward's cache (tree_cache)
+
+    @property
+    def _kv_pools(self):
+        return self.pools
+
+    _kv_layer = paged_view
+
+    @property
+    def _states(self):
+        return self.states
+
+    def _end_tree(self, st, accepted, nodes):
+        st.num_tokens += accepted
 
     def release_sequence(self, seq_id):
         if seq_id in self.states:
