@@ -24,17 +24,27 @@ from .kernels_q8 import _call, _new_rows, _one_device, _table
 MAX_TREE_NODES = 1024
 
 
+def _ints(names: str, *ts: torch.Tensor) -> None:
+    """Contiguous int32 tensors."""
+    for t in ts:
+        if t.dtype is not torch.int32 or not t.is_contiguous():
+            break
+    else:
+        return
+    for t, name in zip(ts, names.split()):
+        _i32(t, name)  # raises its error
+
+
 def _trees(what: str, qo_indptr: torch.Tensor, total_q: int, max_q: int, q_rows: Optional[torch.Tensor],
            grid_width: int = 1) -> Tuple[int, int, int]:
     """(batch, total_q, max_q) of a batch of trees."""
-    _i32(qo_indptr, "qo_indptr")
     B, total_q, max_q = qo_indptr.numel() - 1, int(total_q), int(max_q)
     if B < 0 or total_q < 0 or max_q < 0 or max_q * B < total_q:
         raise ValueError(f"{what}: {total_q} nodes in {B} trees of at most {max_q}")
     if max_q > MAX_TREE_NODES:
         raise ValueError(f"{what}: trees of up to {MAX_TREE_NODES} nodes (max_q = {max_q})")
     if q_rows is not None:
-        _i32(q_rows, "q_rows")
+        _ints("q_rows", q_rows)
         if q_rows.numel() < total_q or grid_width < 1:
             raise ValueError(f"{what}: a grid of B x grid_width rows and one q_rows entry per node")
     return B, total_q, max_q
@@ -49,20 +59,19 @@ def tree_plan(parents: torch.Tensor, qo_indptr: torch.Tensor, start: torch.Tenso
     int32 [total_q] or, with q_rows, [B * grid_width] with 0 on rows without a node."""
     dev = _one_device(parents, qo_indptr, start) if q_rows is None else _one_device(parents, qo_indptr, start, q_rows)
     B, total_q, max_q = _trees("tree_plan", qo_indptr, total_q, max_q, q_rows, grid_width)
-    _i32(parents, "parents")
-    _i32(start, "start")
+    _ints("qo_indptr parents start", qo_indptr, parents, start)
     if parents.numel() < total_q or start.numel() < B:
         raise ValueError("tree_plan: one parent per node and one start per tree")
-    W = -(-max_q // 32)
+    W = (max_q + 31) // 32
     n_pos = total_q if q_rows is None else B * int(grid_width)
     buf = torch.empty(total_q * W + n_pos, dtype=torch.int32, device=parents.device)
     at = buf.data_ptr()
     rc = _call(dev, _lib.fast_tree().tree_plan, parents.data_ptr(), qo_indptr.data_ptr(), start.data_ptr(),
                None if q_rows is None else q_rows.data_ptr(), int(grid_width), total_q, max_q, B, at, W,
                at + 4 * total_q * W, _stream(parents))
-    _lib.check(rc, "nslg_tree_plan")
-    mask, positions = buf.split([total_q * W, n_pos])
-    return mask.view(total_q, W), positions
+    if rc:
+        _lib.check(rc, "nslg_tree_plan")
+    return buf.as_strided((total_q, W), (W, 1)), buf.as_strided((n_pos,), (1,), total_q * W)
 
 
 _WS_BYTES: Dict[Tuple[int, ...], int] = {}  # nslg_paged_tree_workspace_size by call shape
@@ -94,6 +103,7 @@ def paged_tree_attention(q: torch.Tensor, mask: torch.Tensor, qo_indptr: torch.T
     a call's scratch is allocated on the current stream."""
     dev = _one_device(q, mask, qo_indptr, k_layer, v_layer, kv_indptr, kv_indices, kv_last_page_len)
     B, total_q, max_q = _trees("paged_tree_attention", qo_indptr, total_q, max_q, q_rows, grid_width)
+    _ints("qo_indptr", qo_indptr)
     P, ps, Hkv, D = _layer_geom(k_layer, v_layer)
     dtype = q.dtype
     code = _DTYPE_CODE.get(dtype)
@@ -144,7 +154,8 @@ def paged_tree_attention(q: torch.Tensor, mask: torch.Tensor, qo_indptr: torch.T
                kv_last_page_len.data_ptr(), int(total_pages), B, Hq, Hkv, D,
                1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), code, out.data_ptr(), out_stride,
                None if ws is None else ws.data_ptr(), need, _stream(q))
-    _lib.check(rc, "nslg_paged_tree_attention")
+    if rc:
+        _lib.check(rc, "nslg_paged_tree_attention")
     return out
 
 
@@ -166,8 +177,7 @@ def verify_tree(tokens: torch.Tensor, parents: torch.Tensor, qo_indptr: torch.Te
     at a time, several workgroups take a sequence."""
     dev = _one_device(tokens, parents, qo_indptr, target_probs, u_accept, u_next)
     B, total_q, max_q = _trees("verify_tree", qo_indptr, total_q, max_q, q_rows)
-    _i32(tokens, "tokens")
-    _i32(parents, "parents")
+    _ints("qo_indptr tokens parents", qo_indptr, tokens, parents)
     if tokens.numel() < total_q or parents.numel() < total_q or u_accept.numel() < total_q or u_next.numel() < B:
         raise ValueError("verify_tree: a token, a parent and a number u_accept per node, and u_next per tree")
     if not (u_accept.dtype is u_next.dtype is torch.float32 and u_accept.is_contiguous() and u_next.is_contiguous()):
@@ -204,9 +214,10 @@ def verify_tree(tokens: torch.Tensor, parents: torch.Tensor, qo_indptr: torch.Te
                None if draft_probs is None else draft_probs.data_ptr(), ds, rows, vocab, code, u_accept.data_ptr(),
                u_next.data_ptr(), at, at + 4 * B * max_q, at + 4 * B * (max_q + 1), None if ws is None else ws.data_ptr(), need,
                _stream(tokens))
-    _lib.check(rc, "nslg_verify_tree")
-    path, count, token = buf.split([B * max_q, B, B])
-    return path.view(B, max_q), count, token
+    if rc:
+        _lib.check(rc, "nslg_verify_tree")
+    n = B * max_q
+    return buf.as_strided((B, max_q), (max_q, 1)), buf.as_strided((B,), (1,), n), buf.as_strided((B,), (1,), n + B)
 
 
 def move_accepted(k_pool: torch.Tensor, v_pool: torch.Tensor, path: torch.Tensor, count: torch.Tensor, qo_indptr: torch.Tensor,
@@ -221,12 +232,11 @@ def move_accepted(k_pool: torch.Tensor, v_pool: torch.Tensor, path: torch.Tensor
     if code is None:
         raise TypeError(f"move_accepted: float16, bfloat16 or float32 pools (got {k_pool.dtype})")
     B = _table("move_accepted", kv_indptr, kv_indices, kv_last_page_len)
-    _i32(path, "path")
-    _i32(count, "count")
-    _i32(qo_indptr, "qo_indptr")
+    _ints("path count qo_indptr", path, count, qo_indptr)
     if path.dim() != 2 or path.shape[0] != B or count.numel() != B or qo_indptr.numel() != B + 1:
         raise ValueError("move_accepted: path must be [B, width], count [B] and qo_indptr [B+1]")
     rc = _call(dev, _lib.fast_tree().move_accepted, k_pool.data_ptr(), v_pool.data_ptr(), L, P, ps, Hkv, D, code,
                path.data_ptr(), path.shape[1], count.data_ptr(), qo_indptr.data_ptr(), kv_indptr.data_ptr(),
                kv_indices.data_ptr(), kv_last_page_len.data_ptr(), B, _stream(k_pool))
-    _lib.check(rc, "nslg_move_accepted")
+    if rc:
+        _lib.check(rc, "nslg_move_accepted")
