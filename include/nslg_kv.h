@@ -714,8 +714,8 @@ int nslg_tree_plan(const int32_t* parents, const int32_t* qo_indptr, const int32
  *                   strides, 16-byte aligned, laid out as q's rows: they are written to the nodes' slots and read from
  *                   there, in the same launch. No other sequence of the call may read a page written.
  *   total_pages     host copy of kv_indptr[batch] (sizes the launch; another value only costs time)
- *   workspace       of nslg_paged_tree_workspace_size bytes: keys are then cut into chunks and merged (a second
- *                   launch). Null or smaller: fewer chunks, or one. One call at a time may use it; calls of other
+ *   workspace       of nslg_paged_tree_workspace_size bytes: the work is then cut into equal spans, and rows whose
+ *                   keys several spans take are merged (a second launch). Null: none are; smaller: fewer spans. One call at a time may use it; calls of other
  *                   kinds may take it in turn.
  *   other arguments as nslg_paged_prefill_grid. f16, bf16 and f32, D in {64, 128, 256}, 1 <= Hq/Hkv <= 16.
  */

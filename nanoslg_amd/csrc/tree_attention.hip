@@ -1,21 +1,35 @@
 // Attention of trees of drafted tokens over a paged cache, for gfx950 (CDNA4).
 //
-// Sequence b's last n_b tokens are the nodes of its tree; node t sees every token before
-// the tree and, of the nodes, those of its mask (its ancestors and itself). Query rows are
-// packed GQA-style, row = node * G + g, so one K/V load serves all G query heads of a KV head.
+// Sequence b's last n_b tokens are the nodes of its tree; node t sees every token before the tree and, of the nodes, those of
+// its mask (its ancestors and itself):
+//   out_t = sum_j exp(s_tj - m_t) v_j / sum_j exp(s_tj - m_t),  s_tj = scale q_t k_j, j over what t sees.
+// Query rows are packed GQA-style, row = node * G + g, so that one read of K and V serves the G query heads of a KV head.
 //
-// Work. The sequences' tokens are cut into chunks of one length, a multiple of the key tile, that every wave
-// finds from the lengths: the smallest one whose chunks fit the call's budget. A workgroup (4 waves)
-// takes one (chunk, KV head, tile of query rows): 64 rows, 16 a wave, or 128, 32 a wave. Key tiles go through
-// LDS, double buffered, the next tile's loads in flight during the present one's products. Per 32 keys:
-//   S^T[key x row] = K Q^T      (MFMA; lane (r, gq) then holds keys 16 t + 4 gq + j of row r)
+// Work. A KV head's work is one line of units, (sequence, tile of 128 or 256 rows, 16 KB block of keys), cut into equal spans, one
+// a workgroup and CU, so that lengths however uneven leave no CU idle (with chunks of one length, staged
+// through registers by 4 waves, 32 trees over 2k-16k tokens took 352 us). A workgroup finds its span from the lengths, walks its row tiles, and leaves an fp32 partial
+// (maximum, sum, rows as its lanes hold them) where a row tile's keys begin or end outside its span; tree_merge_kernel
+// joins those by their maxima. Without a workspace a workgroup takes a whole row tile.
+//
+// Within a workgroup, 16 waves (8 for rows of 512 bytes and more), 16 rows a wave; with 128 rows a second group of
+// waves takes the other half of every block's keys, joined through LDS at the row tile's end. Blocks of K and V come straight into
+// LDS, swizzled so that no read conflicts, three blocks ahead of the one in use. Per 32 keys a wave computes
+//   S^T[key x row] = K Q^T      (MFMA; lane (r, gq) then holds keys 16 t + 4 gq + j of row r: V's operand layout,
+//                                so that probabilities never leave their registers)
 //   online softmax in fp32, the running maximum raised lazily
-//   O^T[d x row] += V^T P^T     (MFMA; 16-bit V^T operands by transposing LDS reads)
-// The rows of a sequence of several chunks are left as fp32 partials for tree_merge_kernel.
+//   O^T[d x row] += V^T P^T     (MFMA; 16-bit V^T operands by transposing LDS reads), and the sums by a row of ones
+//
+// What bounds it (events, caches cold; fp16 and bf16, 32/8 heads of 128 but the fourth):
+//   32 trees of 32 over 2k-16k tokens   260 us: the keys' way from HBM, 1.13 GB at 4.3 TB/s (a 2 GiB copy: 4.96)
+//   8 trees of 24-60 over 256-8k         62 us: LDS reads, 32 KB a wave and block (128 B a cycle and CU), and a fixed
+//                                               8-10 us a row tile (tables, Q, first block, join, partial)
+//   1 tree of 16 over 2k                17.5 us: the chain of dependent reads (lengths, pages, keys, partials) and two launches
+//   4 trees of 128 over 1k-6k, D = 256   64 us: as the second; four row tiles read the keys anew (from L2)
+//   4 chains of 5-9 over 700-3k, fp32    30 us: fp32 MFMA, at 1/16 of bf16's rate, and the fixed part
 //
 // A key that a row does not see counts nothing, whatever it holds: its score is replaced, and since a
 // probability of 0 would not keep a value that is not finite out of a matrix product, such values of the nodes are
-// staged as 0 and added row by row to those that see them.
+// set to 0 in LDS and added row by row to those that see them.
 #include "nslg_common.h"
 
 #include <math.h>
@@ -27,9 +41,9 @@ namespace {
 
 constexpr int kTreeCUs = 256;
 constexpr int kTreeMaxNodes = 1024;
-constexpr int kTreeWin = 1024;    // page ids in LDS
-constexpr int kTreeBlockBytes = 16384;            // K, or V, of a block of keys
-constexpr int kTreeSlots = 4;                     // blocks in LDS
+constexpr int kTreeWin = 1024;          // pages whose place is in LDS
+constexpr int kTreeBlockBytes = 16384;  // K, or V, of a block of keys
+constexpr int kTreeSlots = 4;           // blocks in LDS: 128 KB, one workgroup a CU
 constexpr float kTreeSlack = 8.0f;  // how far (log2) scores may rise above the running maximum that P is taken at
 
 // Division of 0 .. 2^31 - 1 by a number that the host knows: with 2^l >= d, m = floor(2^(31 + l) / d) + 1 exceeds
@@ -322,402 +336,402 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
   }
   __syncthreads();
   while (pos < pos_end) {
-  while (pos - before >= unit_lds[63].y) {  // uniform: beyond these sequences
-    before = __builtin_amdgcn_readfirstlane(before + unit_lds[63].y);
-    group0 += 64;
-    int x, y;
-    const SeqOf s = tree_seq(p, group0 + lane);
-    const int u = units_of(s, x, y);
-    const int incl = wave_scan_i32(u);
-    __syncthreads();
-    if (wave == 0) seq_lds[lane] = s, unit_lds[lane] = int2{incl - u, incl};
-    __syncthreads();
-  }
-  const int src = __ffsll((long long)__ballot(pos - before < unit_lds[lane].y)) - 1;
-  const SeqOf seq = seq_lds[src];
-
-  const int first_unit = __builtin_amdgcn_readfirstlane(before + unit_lds[src].x);
-  const int n_nodes = __builtin_amdgcn_readfirstlane(seq.nodes), L = __builtin_amdgcn_readfirstlane(seq.len);
-  const int q0 = __builtin_amdgcn_readfirstlane(seq.q0);
-  const int32_t* idx = p.indices + __builtin_amdgcn_readfirstlane(seq.page0);
-  const int all_blk = (L + kKeys - 1) / kKeys;
-  int tile = 0, blk0 = pos - first_unit;
-  if (p.whole) {
-    tile = blk0;
-    blk0 = 0;
-  } else if (blk0 >= all_blk) {
-    tile = blk0 / all_blk;
-    blk0 -= tile * all_blk;
-  }
-  const int n_blk = p.whole ? all_blk : min(pos_end - pos, all_blk - blk0);
-  const bool to_end = blk0 + n_blk == all_blk;
-  const bool partial = blk0 > 0 || !to_end;
-  pos += p.whole ? 1 : n_blk;
-  const int nrows = n_nodes * G;
-  const int start = max(L - n_nodes, 0);
-  const int kv_begin = blk0 * kKeys;
-  const int kv_end = to_end ? L : kv_begin + n_blk * kKeys;
-
-  // ---- the wave's rows: lane's row r of them, its row of q and out (-1: none), its node and its bytes' offset there
-  const int wave_row0 = tile * kRows + 16 * row_wave;
-  const bool wave_on = wave_row0 < nrows;  // (a wave without rows only helps to load)
-  struct Row {
-    int64_t at;
-    int node, off;
-    bool ok;
-  };
-  auto row_of = [&](int r) {
-    const int row = wave_row0 + r;
-    Row x;
-    x.node = p.group_div.quotient(row);
-    x.ok = row < nrows && q0 + x.node < p.total_q;
-    x.at = x.ok ? tree_row(p, q0 + x.node) : -1;
-    x.off = (h * G + row - x.node * G) * kRowBytes;
-    return x;
-  };
-  u32x4 qb[kOps];
-  {
-    const Row x = row_of(lane & 15);
-    const char* src = p.q + (x.at >= 0 ? x.at * p.q_stride + x.off : 0) + 16 * (lane >> 4);
-#pragma unroll
-    for (int s = 0; s < kOps; ++s) qb[s] = x.at >= 0 ? *reinterpret_cast<const u32x4*>(src + 64 * s) : u32x4{0, 0, 0, 0};
-  }
-
-  // ---- blocks of keys: wave-wide loads of 1 KB straight into LDS. Load u of a block fills bytes 1024 u .. + 1023, lane l
-  // the 16 at 16 l: piece l % kVecs of key u * (64 / kVecs) + l / kVecs, where the swizzle has put piece (l % kVecs) ^
-  // swizzle(key) of the row.
-  const int head_off = h * kRowBytes;
-  auto page_of = [&](int key) { return p.page_div.quotient(key); };
-  auto checked = [&](int page) { return page < 0 || (int64_t)page >= p.num_pages ? 0 : page; };
-  const bool fresh = p.k_new != nullptr;
-  int64_t new_row0 = q0;  // row of k_new / v_new of node 0 (a tree's rows are contiguous)
-  if (fresh && p.q_rows) {
-    const int64_t at = tree_row(p, q0);
-    new_row0 = at < 0 ? 0 : at;
-  }
-  const int64_t new_last = (p.q_rows ? (int64_t)p.batch * p.grid_width : p.total_q) - 1;
-  auto new_at = [&](int key) { return min(new_row0 + (key - start), new_last); };
-  // page_lds[i]: what is added to a key of page win + i to make its slot
-  int win = 0, win_blk = 0;  // the window's first page; the first block that reaches past it
-  auto load_pages = [&](int key) {
-    win = page_of(key);
-    const int last = page_of(kv_end - 1);
-    for (int i = tid; i < kTreeWin && win + i <= last; i += kThreads) page_lds[i] = (checked(idx[win + i]) - (win + i)) * ps;
-    win_blk = last < win + kTreeWin ? 0x7fffffff : ((win + kTreeWin) * ps - kv_begin) / kKeys;
-  };
-  auto key_of = [&](int ln) { return wave * (64 / kVecs) + ln / kVecs; };  // of a lane's first piece
-  constexpr int kKeyStep = kWaves * (64 / kVecs);  // keys between a lane's pieces
-  constexpr int kTurn = kPer == 1 ? 0 : kKeyStep % 16;  // (the swizzles repeat after 16 keys)
-  static_assert(kTurn == 0 || (kTurn == 8 && kPer == 2 && kF32), "a lane's second piece is swizzled as key + 8, fp32 V not at all");
-  auto issue = [&](int blk) {
-    char* ks = k_lds + (blk & (kSlots - 1)) * kBlockBytes + 1024 * wave;
-    char* vs = v_lds + (blk & (kSlots - 1)) * kBlockBytes + 1024 * wave;
-    const int key0 = kv_begin + blk * kKeys;
-    const bool nodes = fresh && key0 + kKeys > start;  // uniform: some of the block's rows are not in the pool
-    const int ln = fresh_lane();
-    const int l_key = key_of(ln), l_piece = ln % kVecs;
-    const int v_piece = head_off + 16 * (l_piece ^ swizzle_v<T, kVecs>(l_key));
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int k_piece = head_off + 16 * (l_piece ^ swizzle_k<kVecs>(l_key + kTurn * i));
-      const int kabs = min(key0 + l_key + kKeyStep * i, kv_end - 1);
-      const uint32_t slot = (uint32_t)(kabs + page_lds[page_of(kabs) - win]);
-      const char* kp = p.k_pool + k_piece + (uint64_t)slot * (uint32_t)row_bytes;
-      const char* vp = p.v_pool + v_piece + (uint64_t)slot * (uint32_t)row_bytes;
-      if (nodes && kabs >= start) {
-        const int64_t at = new_at(kabs);
-        kp = p.k_new + at * p.k_new_stride + k_piece;
-        vp = p.v_new + at * p.v_new_stride + v_piece;
-      }
-      if (p.stream) {  // uniform
-        load_lds16<true>(kp, ks + 1024 * kWaves * i);
-        load_lds16<true>(vp, vs + 1024 * kWaves * i);
-      } else {
-        load_lds16<false>(kp, ks + 1024 * kWaves * i);
-        load_lds16<false>(vp, vs + 1024 * kWaves * i);
-      }
+    while (pos - before >= unit_lds[63].y) {  // uniform: beyond these sequences
+      before = __builtin_amdgcn_readfirstlane(before + unit_lds[63].y);
+      group0 += 64;
+      int x, y;
+      const SeqOf s = tree_seq(p, group0 + lane);
+      const int u = units_of(s, x, y);
+      const int incl = wave_scan_i32(u);
+      __syncthreads();
+      if (wave == 0) seq_lds[lane] = s, unit_lds[lane] = int2{incl - u, incl};
+      __syncthreads();
     }
-  };
-  load_pages(kv_begin);
-  if (tid < 2 * (kKeys / kStep)) bad_lds[tid / (kKeys / kStep)][tid % (kKeys / kStep)] = 0;
-  __syncthreads();
-  static_assert(kSlots * kKeys <= kTreeWin);  // the blocks on the way, even of single-token pages
-#pragma unroll 1
-  for (int i = 0; i < min(n_blk, kSlots - 1); ++i) issue(i);
+    const int src = __ffsll((long long)__ballot(pos - before < unit_lds[lane].y)) - 1;
+    const SeqOf seq = seq_lds[src];
 
-  float thr = -INFINITY, neg_m = 0.f;  // the raw score above which the maximum is raised; -maximum (log2 units; 0: none yet)
-  f32x4 lsum = {0.f, 0.f, 0.f, 0.f}, o[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const float inv_scale = 1.f / p.scale_log2;
-
-  // the bits of a step's keys (kbase on) that row r sees
-  auto visible = [&](int kbase, int r) -> uint32_t {
-    const Row x = row_of(r);
-    const uint32_t* mrow = p.mask + (int64_t)(x.ok ? q0 + x.node : 0) * p.mask_words;
-    const int rel = kbase - start;
-    const int words = p.mask_words;
-    uint32_t v;
-    if (rel >= 0) {
-      const int wi = rel >> 5, sh = rel & 31;
-      const uint32_t lo = wi < words ? mrow[wi] : 0u;
-      const uint32_t hi = wi + 1 < words ? mrow[wi + 1] : 0u;
-      v = sh ? (lo >> sh) | (hi << (32 - sh)) : lo;
-    } else if (rel > -32) {
-      v = (1u << -rel) - 1u;
-      v |= mrow[0] << -rel;
-    } else {
-      v = ~0u;
+    const int first_unit = __builtin_amdgcn_readfirstlane(before + unit_lds[src].x);
+    const int n_nodes = __builtin_amdgcn_readfirstlane(seq.nodes), L = __builtin_amdgcn_readfirstlane(seq.len);
+    const int q0 = __builtin_amdgcn_readfirstlane(seq.q0);
+    const int32_t* idx = p.indices + __builtin_amdgcn_readfirstlane(seq.page0);
+    const int all_blk = (L + kKeys - 1) / kKeys;
+    int tile = 0, blk0 = pos - first_unit;
+    if (p.whole) {
+      tile = blk0;
+      blk0 = 0;
+    } else if (blk0 >= all_blk) {
+      tile = blk0 / all_blk;
+      blk0 -= tile * all_blk;
     }
-    const int left = kv_end - kbase;
-    if (left < 32) v &= left > 0 ? (1u << left) - 1u : 0u;
-    return x.ok ? v : 0u;
-  };
+    const int n_blk = p.whole ? all_blk : min(pos_end - pos, all_blk - blk0);
+    const bool to_end = blk0 + n_blk == all_blk;
+    const bool partial = blk0 > 0 || !to_end;
+    pos += p.whole ? 1 : n_blk;
+    const int nrows = n_nodes * G;
+    const int start = max(L - n_nodes, 0);
+    const int kv_begin = blk0 * kKeys;
+    const int kv_end = to_end ? L : kv_begin + n_blk * kKeys;
 
-  const int share = group * (kGroupKeys * kRowBytes);  // the group's share of a block
-  // One step of a block: scores, mask (`tail`: a block with nodes, or past the end), probabilities, product with V.
-  auto step = [&](int blk, int u, auto tail) {
-    constexpr bool kTail = decltype(tail)::value;
-    const int kbase = kv_begin + blk * kKeys + group * kGroupKeys + u * kStep;
-    const char* ksrc = k_lds + (blk & (kSlots - 1)) * kBlockBytes + u * kStep * kRowBytes;
-    const char* vsrc = v_lds + (blk & (kSlots - 1)) * kBlockBytes + u * kStep * kRowBytes;
-    const int ln = fresh_lane(), r = ln & 15, gq = ln >> 4;
-    // LDS offsets of the lane's operands: K at operand i is k_at ^ 64 i, V of output tile n (16 bits) v_at ^ 32 n
-    const int k_at = share + r * kRowBytes + 16 * (gq ^ swizzle_k<kVecs>(r));
-    const int v_key = kF32 ? 4 * gq : 4 * gq + (r >> 2);
-    const int v_at = share + v_key * kRowBytes + (kF32 ? 16 * r : 16 * swizzle_v<T, kVecs>(v_key) + 8 * (r & 3));
-    f32x4 s[kSub];
-    u32x4 ka[kSub][kOps];
+    // ---- the wave's rows: lane's row r of them, its row of q and out (-1: none), its node and its bytes' offset there
+    const int wave_row0 = tile * kRows + 16 * row_wave;
+    const bool wave_on = wave_row0 < nrows;  // (a wave without rows only helps to load)
+    struct Row {
+      int64_t at;
+      int node, off;
+      bool ok;
+    };
+    auto row_of = [&](int r) {
+      const int row = wave_row0 + r;
+      Row x;
+      x.node = p.group_div.quotient(row);
+      x.ok = row < nrows && q0 + x.node < p.total_q;
+      x.at = x.ok ? tree_row(p, q0 + x.node) : -1;
+      x.off = (h * G + row - x.node * G) * kRowBytes;
+      return x;
+    };
+    u32x4 qb[kOps];
+    {
+      const Row x = row_of(lane & 15);
+      const char* src = p.q + (x.at >= 0 ? x.at * p.q_stride + x.off : 0) + 16 * (lane >> 4);
 #pragma unroll
-    for (int t = 0; t < kSub; ++t)
+      for (int s = 0; s < kOps; ++s) qb[s] = x.at >= 0 ? *reinterpret_cast<const u32x4*>(src + 64 * s) : u32x4{0, 0, 0, 0};
+    }
+
+    // ---- blocks of keys: wave-wide loads of 1 KB straight into LDS. Load u of a block fills bytes 1024 u .. + 1023, lane l
+    // the 16 at 16 l: piece l % kVecs of key u * (64 / kVecs) + l / kVecs, where the swizzle has put piece (l % kVecs) ^
+    // swizzle(key) of the row.
+    const int head_off = h * kRowBytes;
+    auto page_of = [&](int key) { return p.page_div.quotient(key); };
+    auto checked = [&](int page) { return page < 0 || (int64_t)page >= p.num_pages ? 0 : page; };
+    const bool fresh = p.k_new != nullptr;
+    int64_t new_row0 = q0;  // row of k_new / v_new of node 0 (a tree's rows are contiguous)
+    if (fresh && p.q_rows) {
+      const int64_t at = tree_row(p, q0);
+      new_row0 = at < 0 ? 0 : at;
+    }
+    const int64_t new_last = (p.q_rows ? (int64_t)p.batch * p.grid_width : p.total_q) - 1;
+    auto new_at = [&](int key) { return min(new_row0 + (key - start), new_last); };
+    // page_lds[i]: what is added to a key of page win + i to make its slot
+    int win = 0, win_blk = 0;  // the window's first page; the first block that reaches past it
+    auto load_pages = [&](int key) {
+      win = page_of(key);
+      const int last = page_of(kv_end - 1);
+      for (int i = tid; i < kTreeWin && win + i <= last; i += kThreads) page_lds[i] = (checked(idx[win + i]) - (win + i)) * ps;
+      win_blk = last < win + kTreeWin ? 0x7fffffff : ((win + kTreeWin) * ps - kv_begin) / kKeys;
+    };
+    auto key_of = [&](int ln) { return wave * (64 / kVecs) + ln / kVecs; };  // of a lane's first piece
+    constexpr int kKeyStep = kWaves * (64 / kVecs);  // keys between a lane's pieces
+    constexpr int kTurn = kPer == 1 ? 0 : kKeyStep % 16;  // (the swizzles repeat after 16 keys)
+    static_assert(kTurn == 0 || (kTurn == 8 && kPer == 2 && kF32), "a lane's second piece is swizzled as key + 8, fp32 V not at all");
+    auto issue = [&](int blk) {
+      char* ks = k_lds + (blk & (kSlots - 1)) * kBlockBytes + 1024 * wave;
+      char* vs = v_lds + (blk & (kSlots - 1)) * kBlockBytes + 1024 * wave;
+      const int key0 = kv_begin + blk * kKeys;
+      const bool nodes = fresh && key0 + kKeys > start;  // uniform: some of the block's rows are not in the pool
+      const int ln = fresh_lane();
+      const int l_key = key_of(ln), l_piece = ln % kVecs;
+      const int v_piece = head_off + 16 * (l_piece ^ swizzle_v<T, kVecs>(l_key));
 #pragma unroll
-      for (int i = 0; i < kOps; ++i) ka[t][i] = *reinterpret_cast<const u32x4*>(ksrc + 16 * t * kRowBytes + (k_at ^ (64 * i)));
-    if constexpr (kF32) {
-#pragma unroll
-      for (int t = 0; t < kSub; ++t) {
-        f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < kOps; ++i) {
-          const f32x4 a = __builtin_bit_cast(f32x4, ka[t][i]), q = __builtin_bit_cast(f32x4, qb[i]);
-          x = __builtin_amdgcn_mfma_f32_16x16x4f32(a[0], q[0], x, 0, 0, 0);
-          y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[1], q[1], y, 0, 0, 0);
-          x = __builtin_amdgcn_mfma_f32_16x16x4f32(a[2], q[2], x, 0, 0, 0);
-          y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[3], q[3], y, 0, 0, 0);
+      for (int i = 0; i < kPer; ++i) {
+        const int k_piece = head_off + 16 * (l_piece ^ swizzle_k<kVecs>(l_key + kTurn * i));
+        const int kabs = min(key0 + l_key + kKeyStep * i, kv_end - 1);
+        const uint32_t slot = (uint32_t)(kabs + page_lds[page_of(kabs) - win]);
+        const char* kp = p.k_pool + k_piece + (uint64_t)slot * (uint32_t)row_bytes;
+        const char* vp = p.v_pool + v_piece + (uint64_t)slot * (uint32_t)row_bytes;
+        if (nodes && kabs >= start) {
+          const int64_t at = new_at(kabs);
+          kp = p.k_new + at * p.k_new_stride + k_piece;
+          vp = p.v_new + at * p.v_new_stride + v_piece;
         }
-        s[t] = x + y;
+        if (p.stream) {  // uniform
+          load_lds16<true>(kp, ks + 1024 * kWaves * i);
+          load_lds16<true>(vp, vs + 1024 * kWaves * i);
+        } else {
+          load_lds16<false>(kp, ks + 1024 * kWaves * i);
+          load_lds16<false>(vp, vs + 1024 * kWaves * i);
+        }
       }
-    } else {
+    };
+    load_pages(kv_begin);
+    if (tid < 2 * (kKeys / kStep)) bad_lds[tid / (kKeys / kStep)][tid % (kKeys / kStep)] = 0;
+    __syncthreads();
+    static_assert(kSlots * kKeys <= kTreeWin);  // the blocks on the way, even of single-token pages
+#pragma unroll 1
+    for (int i = 0; i < min(n_blk, kSlots - 1); ++i) issue(i);
+
+    float thr = -INFINITY, neg_m = 0.f;  // the raw score above which the maximum is raised; -maximum (log2 units; 0: none yet)
+    f32x4 lsum = {0.f, 0.f, 0.f, 0.f}, o[NT];
 #pragma unroll
-      for (int t = 0; t < kSub; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < kOps; ++i)
-#pragma unroll
-        for (int t = 0; t < kSub; ++t) s[t] = T::mma_k32(__builtin_bit_cast(u16x8, ka[t][i]), __builtin_bit_cast(u16x8, qb[i]), s[t]);
-    }
-    // V's operand of output tile n (16 bits): lane r of a 16-lane group addresses keys 4 gq + r / 4 (then + 16), columns 16 n
-    // + 4 (r % 4) .. + 3, and receives keys 4 gq + 0..3 (+ 16) at d = 16 n + r. Read ahead of the softmax, which covers
-    // their way (read one by one as they are used, the reads took most of the time).
-    typedef short i16x4_t __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) i16x4_t* lds_i16x4;
-    u16x8 va[kF32 ? 1 : NT];
-    if constexpr (!kF32) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const char* at = vsrc + (v_at ^ (32 * n));
-        const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)at);
-        const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at + 16 * kRowBytes));
-        va[n] = __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    // A later block's loads go out here: at the block's start the waves waited to get rid of theirs, all at once, before any
-    // product (265 us with 32 trees of 32 nodes over 2k-16k tokens, 308 from there).
-    if (u == 0 && blk + kSlots - 1 < n_blk) issue(blk + kSlots - 1);
-    __builtin_amdgcn_sched_barrier(0);
-    uint32_t vis = 0;
-    if constexpr (kTail) {
-      vis = visible(kbase, r);
-#pragma unroll
-      for (int j = 0; j < 4 * kSub; ++j)
-        if (!(vis >> (16 * (j >> 2) + 4 * gq + (j & 3)) & 1)) s[j >> 2][j & 3] = -INFINITY;
-    }
-    float top = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 4 * kSub; ++j) top = fmaxf(top, s[j >> 2][j & 3]);
-    if (__ballot(top > thr)) {
-      const float m_run = thr == -INFINITY ? -INFINITY : -neg_m;
-      const float m_new = fmaxf(m_run, rows_max(top * p.scale_log2));
-      const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
-      lsum *= alpha;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) o[n] *= alpha;
-      thr = (m_new + kTreeSlack) * inv_scale;
-      neg_m = m_new == -INFINITY ? 0.f : -m_new;
-    }
-    u16x8 pb, pb_lo;
-#pragma unroll
-    for (int j = 0; j < 4 * kSub; ++j) {
-      const float x = fast_exp2(fmaf(s[j >> 2][j & 3], p.scale_log2, neg_m));
-      s[j >> 2][j & 3] = x;
-      if constexpr (kF32) {
-        lsum[j & 3] += x;
+    for (int n = 0; n < NT; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float inv_scale = 1.f / p.scale_log2;
+
+    // the bits of a step's keys (kbase on) that row r sees
+    auto visible = [&](int kbase, int r) -> uint32_t {
+      const Row x = row_of(r);
+      const uint32_t* mrow = p.mask + (int64_t)(x.ok ? q0 + x.node : 0) * p.mask_words;
+      const int rel = kbase - start;
+      const int words = p.mask_words;
+      uint32_t v;
+      if (rel >= 0) {
+        const int wi = rel >> 5, sh = rel & 31;
+        const uint32_t lo = wi < words ? mrow[wi] : 0u;
+        const uint32_t hi = wi + 1 < words ? mrow[wi + 1] : 0u;
+        v = sh ? (lo >> sh) | (hi << (32 - sh)) : lo;
+      } else if (rel > -32) {
+        v = (1u << -rel) - 1u;
+        v |= mrow[0] << -rel;
       } else {
-        // half keeps 11 bits of a probability; bfloat16's 8 are too few for the 2e-3 of the 16-bit caches'
-        // attention: the rest goes in as a second term
-        pb[j] = T::from_f32(x);
-        if constexpr (kSplitP) pb_lo[j] = T::from_f32(x - T::to_f32(pb[j]));
+        v = ~0u;
       }
-    }
-    // O^T += V^T P^T
-    if constexpr (kF32) {
+      const int left = kv_end - kbase;
+      if (left < 32) v &= left > 0 ? (1u << left) - 1u : 0u;
+      return x.ok ? v : 0u;
+    };
+
+    const int share = group * (kGroupKeys * kRowBytes);  // the group's share of a block
+    // One step of a block: scores, mask (`tail`: a block with nodes, or past the end), probabilities, product with V.
+    auto step = [&](int blk, int u, auto tail) {
+      constexpr bool kTail = decltype(tail)::value;
+      const int kbase = kv_begin + blk * kKeys + group * kGroupKeys + u * kStep;
+      const char* ksrc = k_lds + (blk & (kSlots - 1)) * kBlockBytes + u * kStep * kRowBytes;
+      const char* vsrc = v_lds + (blk & (kSlots - 1)) * kBlockBytes + u * kStep * kRowBytes;
+      const int ln = fresh_lane(), r = ln & 15, gq = ln >> 4;
+      // LDS offsets of the lane's operands: K at operand i is k_at ^ 64 i, V of output tile n (16 bits) v_at ^ 32 n
+      const int k_at = share + r * kRowBytes + 16 * (gq ^ swizzle_k<kVecs>(r));
+      const int v_key = kF32 ? 4 * gq : 4 * gq + (r >> 2);
+      const int v_at = share + v_key * kRowBytes + (kF32 ? 16 * r : 16 * swizzle_v<T, kVecs>(v_key) + 8 * (r & 3));
+      f32x4 s[kSub];
+      u32x4 ka[kSub][kOps];
 #pragma unroll
       for (int t = 0; t < kSub; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int i = 0; i < kOps; ++i) ka[t][i] = *reinterpret_cast<const u32x4*>(ksrc + 16 * t * kRowBytes + (k_at ^ (64 * i)));
+      if constexpr (kF32) {
 #pragma unroll
-          for (int c = 0; c < D / 64; ++c) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(vsrc + (16 * t + j) * kRowBytes + v_at + 256 * c);
+        for (int t = 0; t < kSub; ++t) {
+          f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[4 * c + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e], s[t][j], o[4 * c + e], 0, 0, 0);
+          for (int i = 0; i < kOps; ++i) {
+            const f32x4 a = __builtin_bit_cast(f32x4, ka[t][i]), q = __builtin_bit_cast(f32x4, qb[i]);
+            x = __builtin_amdgcn_mfma_f32_16x16x4f32(a[0], q[0], x, 0, 0, 0);
+            y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[1], q[1], y, 0, 0, 0);
+            x = __builtin_amdgcn_mfma_f32_16x16x4f32(a[2], q[2], x, 0, 0, 0);
+            y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[3], q[3], y, 0, 0, 0);
           }
-    } else {
+          s[t] = x + y;
+        }
+      } else {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        o[n] = T::mma_k32(va[n], pb, o[n]);
-        if constexpr (kSplitP) o[n] = T::mma_k32(va[n], pb_lo, o[n]);
+        for (int t = 0; t < kSub; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kOps; ++i)
+#pragma unroll
+          for (int t = 0; t < kSub; ++t) s[t] = T::mma_k32(__builtin_bit_cast(u16x8, ka[t][i]), __builtin_bit_cast(u16x8, qb[i]), s[t]);
       }
-      // the rows' sums by an all-ones operand: of the probabilities as they were multiplied
-      const u16x8 ones = u16x8(T::from_f32(1.f));
-      lsum = T::mma_k32(ones, pb, lsum);
-      if constexpr (kSplitP) lsum = T::mma_k32(ones, pb_lo, lsum);
-    }
-    // nodes whose V is not finite: those elements, for the rows that see the node
-    if constexpr (kTail) {
-      uint32_t bad = __builtin_amdgcn_readfirstlane(bad_lds[blk & 1][group * kSteps + u]);
-      while (__builtin_expect(bad != 0, 0)) {
-        const int kk = __ffs(bad) - 1;
-        bad &= bad - 1;
-        const int key = kbase + kk;
-        const char* vrow = (fresh ? p.v_new + new_at(key) * p.v_new_stride
-                                  : p.v_pool + ((int64_t)checked(idx[page_of(key)]) * ps + (key - page_of(key) * ps)) * row_bytes) +
-                           head_off;
-        float pr = 0.f;
+      // V's operand of output tile n (16 bits): lane r of a 16-lane group addresses keys 4 gq + r / 4 (then + 16), columns 16 n
+      // + 4 (r % 4) .. + 3, and receives keys 4 gq + 0..3 (+ 16) at d = 16 n + r. Read ahead of the softmax, which covers
+      // their way (read one by one as they are used, the reads took most of the time).
+      typedef short i16x4_t __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) i16x4_t* lds_i16x4;
+      u16x8 va[kF32 ? 1 : NT];
+      if constexpr (!kF32) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const char* at = vsrc + (v_at ^ (32 * n));
+          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)at);
+          const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at + 16 * kRowBytes));
+          va[n] = __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // A later block's loads go out here: at the block's start the waves waited to get rid of theirs, all at once, before any
+      // product (265 us with 32 trees of 32 nodes over 2k-16k tokens, 308 from there).
+      if (u == 0 && blk + kSlots - 1 < n_blk) issue(blk + kSlots - 1);
+      __builtin_amdgcn_sched_barrier(0);
+      uint32_t vis = 0;
+      if constexpr (kTail) {
+        vis = visible(kbase, r);
 #pragma unroll
         for (int j = 0; j < 4 * kSub; ++j)
-          if (16 * (j >> 2) + (j & 3) == (kk & ~12)) pr = s[j >> 2][j & 3];
-        pr = __shfl(pr, 16 * ((kk >> 2) & 3) + r, 64);
-        if (!(vis >> kk & 1)) continue;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float v;
-            if constexpr (kF32)
-              v = reinterpret_cast<const float*>(vrow)[64 * (n >> 2) + 16 * gq + 4 * i + (n & 3)];
-            else
-              v = T::to_f32(reinterpret_cast<const uint16_t*>(vrow)[16 * n + 4 * gq + i]);
-            if (!(fabsf(v) < INFINITY)) o[n][i] += pr * v;
-          }
+          if (!(vis >> (16 * (j >> 2) + 4 * gq + (j & 3)) & 1)) s[j >> 2][j & 3] = -INFINITY;
       }
-    }
-  };
-  // Values of a block's V that are not finite, and those past the end, become 0 in LDS.
-  auto tidy = [&](int blk) {
-    char* vs = v_lds + (blk & (kSlots - 1)) * kBlockBytes;
-    const int ln = fresh_lane();
+      float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int key = key_of(ln) + kKeyStep * i;
-      const int kabs = kv_begin + blk * kKeys + key;
-      u32x4* at = reinterpret_cast<u32x4*>(vs + 1024 * (wave + kWaves * i) + 16 * ln);
-      if (kabs >= kv_end) {
-        *at = u32x4{0, 0, 0, 0};
-      } else if (kabs >= start) {
-        bool bad = false;
-        const u32x4 x = drop_not_finite<T>(*at, bad);
-        if (bad) {
-          *at = x;
-          atomicOr(&bad_lds[blk & 1][key / kStep], 1u << (key % kStep));
+      for (int j = 0; j < 4 * kSub; ++j) top = fmaxf(top, s[j >> 2][j & 3]);
+      if (__ballot(top > thr)) {
+        const float m_run = thr == -INFINITY ? -INFINITY : -neg_m;
+        const float m_new = fmaxf(m_run, rows_max(top * p.scale_log2));
+        const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+        lsum *= alpha;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[n] *= alpha;
+        thr = (m_new + kTreeSlack) * inv_scale;
+        neg_m = m_new == -INFINITY ? 0.f : -m_new;
+      }
+      u16x8 pb, pb_lo;
+#pragma unroll
+      for (int j = 0; j < 4 * kSub; ++j) {
+        const float x = fast_exp2(fmaf(s[j >> 2][j & 3], p.scale_log2, neg_m));
+        s[j >> 2][j & 3] = x;
+        if constexpr (kF32) {
+          lsum[j & 3] += x;
+        } else {
+          // half keeps 11 bits of a probability; bfloat16's 8 are too few for the 2e-3 of the 16-bit caches'
+          // attention: the rest goes in as a second term
+          pb[j] = T::from_f32(x);
+          if constexpr (kSplitP) pb_lo[j] = T::from_f32(x - T::to_f32(pb[j]));
+        }
+      }
+      // O^T += V^T P^T
+      if constexpr (kF32) {
+#pragma unroll
+        for (int t = 0; t < kSub; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+              const f32x4 v = *reinterpret_cast<const f32x4*>(vsrc + (16 * t + j) * kRowBytes + v_at + 256 * c);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[4 * c + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e], s[t][j], o[4 * c + e], 0, 0, 0);
+            }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          o[n] = T::mma_k32(va[n], pb, o[n]);
+          if constexpr (kSplitP) o[n] = T::mma_k32(va[n], pb_lo, o[n]);
+        }
+        // the rows' sums by an all-ones operand: of the probabilities as they were multiplied
+        const u16x8 ones = u16x8(T::from_f32(1.f));
+        lsum = T::mma_k32(ones, pb, lsum);
+        if constexpr (kSplitP) lsum = T::mma_k32(ones, pb_lo, lsum);
+      }
+      // nodes whose V is not finite: those elements, for the rows that see the node
+      if constexpr (kTail) {
+        uint32_t bad = __builtin_amdgcn_readfirstlane(bad_lds[blk & 1][group * kSteps + u]);
+        while (__builtin_expect(bad != 0, 0)) {
+          const int kk = __ffs(bad) - 1;
+          bad &= bad - 1;
+          const int key = kbase + kk;
+          const char* vrow = (fresh ? p.v_new + new_at(key) * p.v_new_stride
+                                    : p.v_pool + ((int64_t)checked(idx[page_of(key)]) * ps + (key - page_of(key) * ps)) * row_bytes) +
+                             head_off;
+          float pr = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4 * kSub; ++j)
+            if (16 * (j >> 2) + (j & 3) == (kk & ~12)) pr = s[j >> 2][j & 3];
+          pr = __shfl(pr, 16 * ((kk >> 2) & 3) + r, 64);
+          if (!(vis >> kk & 1)) continue;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float v;
+              if constexpr (kF32)
+                v = reinterpret_cast<const float*>(vrow)[64 * (n >> 2) + 16 * gq + 4 * i + (n & 3)];
+              else
+                v = T::to_f32(reinterpret_cast<const uint16_t*>(vrow)[16 * n + 4 * gq + i]);
+              if (!(fabsf(v) < INFINITY)) o[n][i] += pr * v;
+            }
+        }
+      }
+    };
+    // Values of a block's V that are not finite, and those past the end, become 0 in LDS.
+    auto tidy = [&](int blk) {
+      char* vs = v_lds + (blk & (kSlots - 1)) * kBlockBytes;
+      const int ln = fresh_lane();
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int key = key_of(ln) + kKeyStep * i;
+        const int kabs = kv_begin + blk * kKeys + key;
+        u32x4* at = reinterpret_cast<u32x4*>(vs + 1024 * (wave + kWaves * i) + 16 * ln);
+        if (kabs >= kv_end) {
+          *at = u32x4{0, 0, 0, 0};
+        } else if (kabs >= start) {
+          bool bad = false;
+          const u32x4 x = drop_not_finite<T>(*at, bad);
+          if (bad) {
+            *at = x;
+            atomicOr(&bad_lds[blk & 1][key / kStep], 1u << (key % kStep));
+          }
+        }
+      }
+    };
+
+    // A block has landed for all waves once each has waited for its loads and all have met; then the block before it has
+    // been read, and the loads of block i + kSlots - 1 take its slot.
+    auto block = [&](int blk, auto tail) {
+      if (blk + kSlots - 2 < n_blk)
+        wait_and_meet<2 * kPer * (kSlots - 2)>();
+      else
+        wait_and_meet<0>();
+      if (blk + kSlots - 1 < n_blk) {
+        if (blk + kSlots - 1 >= win_blk) {  // uniform
+          load_pages(kv_begin + (blk + kSlots - 1) * kKeys);
+          __syncthreads();
+        }
+        if (!wave_on) issue(blk + kSlots - 1);  // (the others in the course of their step)
+      }
+      if constexpr (decltype(tail)::value) {
+        tidy(blk);
+        __syncthreads();
+        if (tid < kKeys / kStep) bad_lds[(blk + 1) & 1][tid] = 0;
+      }
+      if (wave_on) {
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u) step(blk, u, tail);
+      }
+    };
+    const int n_plain = min(max(start - kv_begin, 0) / kKeys, n_blk);  // blocks that lie before the tree
+    int blk = 0;
+    for (; blk < n_plain; ++blk) block(blk, std::false_type());
+    for (; blk < n_blk; ++blk) block(blk, std::true_type());
+
+    // ---- the second group's rows to the first's, lane by lane, through the blocks' LDS
+    const int r = lane & 15, gq = lane >> 4;
+    float l = lsum[0];
+    if constexpr (kF32) l = rows_sum((lsum[0] + lsum[1]) + (lsum[2] + lsum[3]));
+    float m = thr == -INFINITY ? -INFINITY : -neg_m;
+    if constexpr (kGroups == 2) {
+      wait_and_meet<0>();
+      f32x4* buf = reinterpret_cast<f32x4*>(kv_lds) + row_wave * (64 * NT) + lane;
+      static_assert(kRowWaves * 64 * NT * 16 <= 2 * kSlots * kBlockBytes);
+      if (group && wave_on) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) buf[64 * n] = o[n];
+        if (gq == 0) ml_lds[16 * row_wave + r] = float2{m, l};
+      }
+      wait_and_meet<0>();
+      if (!group && wave_on) {
+        const float2 other = ml_lds[16 * row_wave + r];
+        const float top = fmaxf(m, other.x);
+        const float f0 = l == 0.f ? 0.f : fast_exp2(m - top);  // 0: no key of the group seen
+        const float f1 = other.y == 0.f ? 0.f : fast_exp2(other.x - top);
+        l = fmaf(f0, l, f1 * other.y);
+        m = top;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const f32x4 x = buf[64 * n];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][e] = fmaf(f0, o[n][e], f1 * x[e]);
         }
       }
     }
-  };
 
-  // A block has landed for all waves once each has waited for its loads and all have met; then the block before it has
-  // been read, and the loads of block i + kSlots - 1 take its slot.
-  auto block = [&](int blk, auto tail) {
-    if (blk + kSlots - 2 < n_blk)
-      wait_and_meet<2 * kPer * (kSlots - 2)>();
-    else
-      wait_and_meet<0>();
-    if (blk + kSlots - 1 < n_blk) {
-      if (blk + kSlots - 1 >= win_blk) {  // uniform
-        load_pages(kv_begin + (blk + kSlots - 1) * kKeys);
-        __syncthreads();
-      }
-      if (!wave_on) issue(blk + kSlots - 1);  // (the others in the course of their step)
+    // ---- the rows: normalised into `out`, or the span's share as a partial
+    if (partial && wave_on && group == 0) {
+      // (a workgroup has at most one that began before its span and one that goes on behind it)
+      const int64_t slot = ((int64_t)2 * w + (blk0 == 0)) * kRowWaves + row_wave;
+      if (gq == 0) p.part_ml[16 * slot + r] = float2{m, l};
+#pragma unroll
+      for (int n = 0; n < NT; ++n) p.part_o[(slot * NT + n) * 64 + lane] = o[n];
+    } else if (!partial && wave_on && group == 0) {
+      const Row x = row_of(r);
+      const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (a sum that is NaN makes the row NaN)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) o[n] *= f;
+      if (x.at >= 0) store_row<T, NT>(p.out + x.at * p.out_stride + x.off, gq, o);
     }
-    if constexpr (decltype(tail)::value) {
-      tidy(blk);
-      __syncthreads();
-      if (tid < kKeys / kStep) bad_lds[(blk + 1) & 1][tid] = 0;
-    }
-    if (wave_on) {
-#pragma unroll
-      for (int u = 0; u < kSteps; ++u) step(blk, u, tail);
-    }
-  };
-  const int n_plain = min(max(start - kv_begin, 0) / kKeys, n_blk);  // blocks that lie before the tree
-  int blk = 0;
-  for (; blk < n_plain; ++blk) block(blk, std::false_type());
-  for (; blk < n_blk; ++blk) block(blk, std::true_type());
-
-  // ---- the second group's rows to the first's, lane by lane, through the blocks' LDS
-  const int r = lane & 15, gq = lane >> 4;
-  float l = lsum[0];
-  if constexpr (kF32) l = rows_sum((lsum[0] + lsum[1]) + (lsum[2] + lsum[3]));
-  float m = thr == -INFINITY ? -INFINITY : -neg_m;
-  if constexpr (kGroups == 2) {
-    wait_and_meet<0>();
-    f32x4* buf = reinterpret_cast<f32x4*>(kv_lds) + row_wave * (64 * NT) + lane;
-    static_assert(kRowWaves * 64 * NT * 16 <= 2 * kSlots * kBlockBytes);
-    if (group && wave_on) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) buf[64 * n] = o[n];
-      if (gq == 0) ml_lds[16 * row_wave + r] = float2{m, l};
-    }
-    wait_and_meet<0>();
-    if (!group && wave_on) {
-      const float2 other = ml_lds[16 * row_wave + r];
-      const float top = fmaxf(m, other.x);
-      const float f0 = l == 0.f ? 0.f : fast_exp2(m - top);  // 0: no key of the group seen
-      const float f1 = other.y == 0.f ? 0.f : fast_exp2(other.x - top);
-      l = fmaf(f0, l, f1 * other.y);
-      m = top;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const f32x4 x = buf[64 * n];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][e] = fmaf(f0, o[n][e], f1 * x[e]);
-      }
-    }
-  }
-
-  // ---- the rows: normalised into `out`, or the span's share as a partial
-  if (partial && wave_on && group == 0) {
-    // (a workgroup has at most one that began before its span and one that goes on behind it)
-    const int64_t slot = ((int64_t)2 * w + (blk0 == 0)) * kRowWaves + row_wave;
-    if (gq == 0) p.part_ml[16 * slot + r] = float2{m, l};
-#pragma unroll
-    for (int n = 0; n < NT; ++n) p.part_o[(slot * NT + n) * 64 + lane] = o[n];
-  } else if (!partial && wave_on && group == 0) {
-    const Row x = row_of(r);
-    const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (a sum that is NaN makes the row NaN)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) o[n] *= f;
-    if (x.at >= 0) store_row<T, NT>(p.out + x.at * p.out_stride + x.off, gq, o);
-  }
-  if (pos < pos_end) __syncthreads();  // the next row tile's loads overwrite what the other waves may still read
+    if (pos < pos_end) __syncthreads();  // the next row tile's loads overwrite what the other waves may still read
   }
 }
 
