@@ -389,14 +389,6 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
       x.off = (h * G + row - x.node * G) * kRowBytes;
       return x;
     };
-    u32x4 qb[kOps];
-    {
-      const Row x = row_of(lane & 15);
-      const char* src = p.q + (x.at >= 0 ? x.at * p.q_stride + x.off : 0) + 16 * (lane >> 4);
-#pragma unroll
-      for (int s = 0; s < kOps; ++s) qb[s] = x.at >= 0 ? *reinterpret_cast<const u32x4*>(src + 64 * s) : u32x4{0, 0, 0, 0};
-    }
-
     // ---- blocks of keys: wave-wide loads of 1 KB straight into LDS. Load u of a block fills bytes 1024 u .. + 1023, lane l
     // the 16 at 16 l: piece l % kVecs of key u * (64 / kVecs) + l / kVecs, where the swizzle has put piece (l % kVecs) ^
     // swizzle(key) of the row.
@@ -452,7 +444,26 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
         }
       }
     };
-    load_pages(kv_begin);
+    // The first pages and the row of q are under way together, then q's own rows while the first blocks are sent for.
+    constexpr int kWinPer = kTreeWin / kThreads;
+    int32_t first_pages[kWinPer];
+    const int last_page = page_of(kv_end - 1);
+    win = page_of(kv_begin);
+    win_blk = last_page < win + kTreeWin ? 0x7fffffff : ((win + kTreeWin) * ps - kv_begin) / kKeys;
+#pragma unroll
+    for (int i = 0; i < kWinPer; ++i) first_pages[i] = win + tid + kThreads * i <= last_page ? idx[win + tid + kThreads * i] : 0;
+    const Row q_row = row_of(lane & 15);
+#pragma unroll
+    for (int i = 0; i < kWinPer; ++i) {
+      const int at = tid + kThreads * i;
+      if (win + at <= last_page) page_lds[at] = (checked(first_pages[i]) - (win + at)) * ps;
+    }
+    u32x4 qb[kOps];
+    {
+      const char* src = p.q + (q_row.at >= 0 ? q_row.at * p.q_stride + q_row.off : 0) + 16 * (lane >> 4);
+#pragma unroll
+      for (int s = 0; s < kOps; ++s) qb[s] = q_row.at >= 0 ? *reinterpret_cast<const u32x4*>(src + 64 * s) : u32x4{0, 0, 0, 0};
+    }
     if (tid < 2 * (kKeys / kStep)) bad_lds[tid / (kKeys / kStep)][tid % (kKeys / kStep)] = 0;
     __syncthreads();
     static_assert(kSlots * kKeys <= kTreeWin);  // the blocks on the way, even of single-token pages
