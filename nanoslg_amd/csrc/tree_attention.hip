@@ -44,6 +44,7 @@ constexpr int kTreeMaxNodes = 1024;
 constexpr int kTreeWin = 1024;          // pages whose place is in LDS
 constexpr int kTreeBlockBytes = 16384;  // K, or V, of a block of keys
 constexpr int kTreeSlots = 4;           // blocks in LDS: 128 KB, one workgroup a CU
+constexpr int kTreeTurn = 3;            // blocks' time that a workgroup takes to begin a row tile
 constexpr float kTreeSlack = 8.0f;  // how far (log2) scores may rise above the running maximum that P is taken at
 
 // Division of 0 .. 2^31 - 1 by a number that the host knows: with 2^l >= d, m = floor(2^(31 + l) / d) + 1 exceeds
@@ -96,7 +97,7 @@ struct TreeParams {
   int32_t stream;      // the call's K/V exceed the caches and are read once: loaded past them
   int32_t num_work;    // workgroups that attend (spans a KV head); the others write the new rows
   uint64_t* ws_tag;    // the workspace's first word: a decode call's record in the same memory is void
-  int4* meta;          // per sequence: its first unit of work, its blocks, units a workgroup
+  int4* meta;          // per sequence: its first unit of work, its blocks, units a workgroup, units before a row tile's blocks
   float2* part_ml;     // [num_work, 2, 16 * tile_waves]: running maximum (log2 units), sum
   f32x4* part_o;       // [num_work, 2, tile_waves, D / 16, 64]: a wave's output tiles, as its lanes hold them
 };
@@ -298,28 +299,37 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
 
   // ---- the workgroup's span of work. A KV head's work is one line of units: sequence after sequence, row tile after
   // row tile, block of keys after block; workgroup j of the head takes `span` of them from j * span on (KV heads in turn:
-  // a head's neighbours share an XCD's L2). What begins or ends inside a row tile's keys leaves a partial. Without
-  // partials a unit is a row tile with all its keys.
+  // a head's neighbours share an XCD's L2). What begins or ends inside a row tile's keys leaves a partial. A row tile's blocks
+  // lie behind `turn` units without any, the time that it takes a workgroup to begin another row tile (8 trees of 24-60 nodes
+  // 66 -> 62 us, 4 fp32 chains 34.6 -> 31.8; 2 and 4 units do as well, 6 less); where spans are as short as that, every
+  // one lies in one or two row tiles, and a longer span only costs. Without partials a unit is a row tile with all its keys.
   const int h = w % p.num_kv_heads;
   const int j = w / p.num_kv_heads;
-  auto units_of = [&](const SeqOf& x, int& tiles, int& blocks) {
-    tiles = (x.nodes * G + kRows - 1) / kRows;
-    blocks = (x.len + kKeys - 1) / kKeys;
-    return p.whole ? (blocks > 0 ? tiles : 0) : tiles * blocks;
-  };
+  auto blocks_of = [&](const SeqOf& x) { return (x.len + kKeys - 1) / kKeys; };
+  auto tiles_of = [&](const SeqOf& x) { return x.len > 0 ? (x.nodes * G + kRows - 1) / kRows : 0; };
+  int turn = 0;
+  auto units_of = [&](const SeqOf& x) { return tiles_of(x) * (p.whole ? 1 : blocks_of(x) + turn); };
   int group0 = 0, before = 0;  // the first of the sequences in seq_lds, the units before it
   int total;
   {
-    int x, y;
     const SeqOf s = tree_seq(p, lane);
-    const int u = units_of(s, x, y);
-    const int incl = wave_scan_i32(u);
-    if (wave == 0) seq_lds[lane] = s, unit_lds[lane] = int2{incl - u, incl};
+    int u = units_of(s), tiles = tiles_of(s);
+    int incl = wave_scan_i32(u), incl_tiles = wave_scan_i32(tiles);
     total = __builtin_amdgcn_readlane(incl, 63);
-  }
-  for (int s0 = 64; s0 < p.batch; s0 += 64) {
-    int x, y;
-    total += wave_sum_i32(units_of(tree_seq(p, s0 + lane), x, y));
+    int all_tiles = __builtin_amdgcn_readlane(incl_tiles, 63);
+    for (int s0 = 64; s0 < p.batch; s0 += 64) {
+      const SeqOf x = tree_seq(p, s0 + lane);
+      total += wave_sum_i32(units_of(x));
+      all_tiles += wave_sum_i32(tiles_of(x));
+    }
+    total = __builtin_amdgcn_readfirstlane(total);
+    if (!p.whole && total >= kTreeTurn * p.spans) {  // uniform
+      turn = kTreeTurn;
+      total += turn * __builtin_amdgcn_readfirstlane(all_tiles);
+      u += turn * tiles;
+      incl += turn * incl_tiles;
+    }
+    if (wave == 0) seq_lds[lane] = s, unit_lds[lane] = int2{incl - u, incl};
   }
   const int span = p.whole ? 1 : max(__builtin_amdgcn_readfirstlane((total + p.spans - 1) / p.spans), 1);
   int pos = __builtin_amdgcn_readfirstlane((int)min((int64_t)j * span, (int64_t)total));
@@ -327,10 +337,10 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
   if (w == 0 && wave == 0 && p.meta) {
     int at = 0;
     for (int s0 = 0; s0 < p.batch; s0 += 64) {
-      int x, y;
-      const int u = units_of(tree_seq(p, s0 + lane), x, y);
+      const SeqOf x = tree_seq(p, s0 + lane);
+      const int u = units_of(x);
       const int sum = wave_scan_i32(u);
-      if (s0 + lane < p.batch) p.meta[s0 + lane] = int4{at + sum - u, y, span, 0};
+      if (s0 + lane < p.batch) p.meta[s0 + lane] = int4{at + sum - u, blocks_of(x), span, turn};
       at += __builtin_amdgcn_readlane(sum, 63);
     }
   }
@@ -339,9 +349,8 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
     while (pos - before >= unit_lds[63].y) {  // uniform: beyond these sequences
       before = __builtin_amdgcn_readfirstlane(before + unit_lds[63].y);
       group0 += 64;
-      int x, y;
       const SeqOf s = tree_seq(p, group0 + lane);
-      const int u = units_of(s, x, y);
+      const int u = units_of(s);
       const int incl = wave_scan_i32(u);
       __syncthreads();
       if (wave == 0) seq_lds[lane] = s, unit_lds[lane] = int2{incl - u, incl};
@@ -355,18 +364,26 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
     const int q0 = __builtin_amdgcn_readfirstlane(seq.q0);
     const int32_t* idx = p.indices + __builtin_amdgcn_readfirstlane(seq.page0);
     const int all_blk = (L + kKeys - 1) / kKeys;
-    int tile = 0, blk0 = pos - first_unit;
+    int tile = 0, blk0 = pos - first_unit, n_blk = all_blk;
     if (p.whole) {
       tile = blk0;
       blk0 = 0;
-    } else if (blk0 >= all_blk) {
-      tile = blk0 / all_blk;
-      blk0 -= tile * all_blk;
+      ++pos;
+    } else {
+      const int per = all_blk + turn;
+      if (blk0 >= per) {
+        tile = blk0 / per;
+        blk0 -= tile * per;
+      }
+      const int units = min(pos_end - pos, per - blk0);
+      pos += units;
+      n_blk = blk0 + units - turn;  // where the blocks end
+      blk0 = max(blk0 - turn, 0);
+      n_blk -= blk0;
+      if (n_blk <= 0) continue;  // uniform
     }
-    const int n_blk = p.whole ? all_blk : min(pos_end - pos, all_blk - blk0);
     const bool to_end = blk0 + n_blk == all_blk;
     const bool partial = blk0 > 0 || !to_end;
-    pos += p.whole ? 1 : n_blk;
     const int nrows = n_nodes * G;
     const int start = max(L - n_nodes, 0);
     const int kv_begin = blk0 * kKeys;
@@ -766,7 +783,7 @@ __global__ void __launch_bounds__(256 * kSplit) tree_merge_kernel(TreeParams p, 
   const int nodes = min(max(p.qo_indptr[b + 1] - q0, 0), p.max_nodes);
   if (16 * rw >= nodes * G || meta.y <= 0) return;
   const int tile = rw / p.tile_waves;
-  const int first = meta.x + tile * meta.y;
+  const int first = meta.x + tile * (meta.y + meta.w) + meta.w;  // the row tile's first block's unit
   const int j0 = first / meta.z;
   const int parts = (first + meta.y - 1) / meta.z - j0 + 1;
   if (parts < 2 || j0 + parts > p.spans) return;  // uniform over the workgroup
