@@ -17,7 +17,7 @@
 //   S^T[key x row] = K Q^T      (MFMA; lane (r, gq) then holds keys 16 t + 4 gq + j of row r: V's operand layout,
 //                                so that probabilities never leave their registers)
 //   online softmax in fp32, the running maximum raised lazily
-//   O^T[d x row] += V^T P^T     (MFMA; 16-bit V^T operands by transposing LDS reads), and the sums by a row of ones
+//   O^T[d x row] += V^T P^T     (MFMA; 16-bit V^T operands by transposing LDS reads; bf16's P in two terms)
 //
 // What bounds it (events, caches cold; fp16 and bf16, 32/8 heads of 128 but the fourth):
 //   32 trees of 32 over 2k-16k tokens   260 us: the keys' way from HBM, 1.13 GB at 4.3 TB/s (a 2 GiB copy: 4.96)
@@ -601,9 +601,10 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
       for (int j = 0; j < 4 * kSub; ++j) {
         const float x = fast_exp2(fmaf(s[j >> 2][j & 3], p.scale_log2, neg_m));
         s[j >> 2][j & 3] = x;
-        if constexpr (kF32) {
-          lsum[j & 3] += x;
-        } else {
+        // (the rows' sums take the probabilities before they are rounded, a lane's keys at a time; as a product with a row of ones
+        // they cost a matrix instruction in 13 to 17: 250 us with 32 trees over 2k-16k tokens, now 243)
+        lsum[j & 3] += x;
+        if constexpr (!kF32) {
           // half keeps 11 bits of a probability; bfloat16's 8 are too few for the 2e-3 of the 16-bit caches'
           // attention: the rest goes in as a second term
           pb[j] = T::from_f32(x);
@@ -628,10 +629,6 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
           o[n] = T::mma_k32(va[n], pb, o[n]);
           if constexpr (kSplitP) o[n] = T::mma_k32(va[n], pb_lo, o[n]);
         }
-        // the rows' sums by an all-ones operand: of the probabilities as they were multiplied
-        const u16x8 ones = u16x8(T::from_f32(1.f));
-        lsum = T::mma_k32(ones, pb, lsum);
-        if constexpr (kSplitP) lsum = T::mma_k32(ones, pb_lo, lsum);
       }
       // nodes whose V is not finite: those elements, for the rows that see the node
       if constexpr (kTail) {
@@ -716,8 +713,7 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
 
     // ---- the second group's rows to the first's, lane by lane, through the blocks' LDS
     const int r = lane & 15, gq = lane >> 4;
-    float l = lsum[0];
-    if constexpr (kF32) l = rows_sum((lsum[0] + lsum[1]) + (lsum[2] + lsum[3]));
+    float l = rows_sum((lsum[0] + lsum[1]) + (lsum[2] + lsum[3]));
     float m = thr == -INFINITY ? -INFINITY : -neg_m;
     if constexpr (kGroups == 2) {
       wait_and_meet<0>();
