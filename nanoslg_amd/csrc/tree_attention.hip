@@ -707,6 +707,9 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
       }
     };
     const int n_plain = min(max(start - kv_begin, 0) / kKeys, n_blk);  // blocks that lie before the tree
+    // q is waited for here: within the loop the wait for it would be one for every direct load on its way.
+#pragma unroll
+    for (int s = 0; s < kOps; ++s) asm volatile("" : "+v"(qb[s]));
     int blk = 0;
     for (; blk < n_plain; ++blk) block(blk, std::false_type());
     for (; blk < n_blk; ++blk) block(blk, std::true_type());
