@@ -742,7 +742,7 @@ int nslg_paged_tree_attention(const void* q, int64_t q_stride, const uint32_t* m
  * running sum of r exceeds u_next[b] times its sum. Tokens so accepted and drawn have the target's distribution.
  * Tests and sums are in 64 bits. Negative weights and those that are not finite count as 0; where nothing is left
  * of r the token is drawn from p, and next_token is -1 where p holds nothing either (or the sequence has no nodes).
- * A drafted token outside the vocabulary is rejected. Probabilities of exactly one token (p(x) = 1) make
+ * A drafted token without weight, or outside the vocabulary, is rejected whatever its number. Probabilities of exactly one token (p(x) = 1) make
  * this greedy verification.
  *   target_probs, draft_probs   num_rows rows of vocab values (f16, bf16 or f32) at element strides: the row of node
  *                   t is t, or q_rows[t]

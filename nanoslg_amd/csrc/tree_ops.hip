@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kVerThreads) tree_verify_kernel(VerifyParams p
           if (__ballot(again)) left = 0.0;
         }
         left = ok_token && left > 0.0 && left < INFINITY ? left : 0.0;
-        if (us * W * q < left) {  // accepted
+        if (left > 0.0 && us * W * q < left) {  // accepted
           cur = base + src;
           if (lane == 0) path_lds[count] = cur;
           ++count;

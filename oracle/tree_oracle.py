@@ -79,7 +79,7 @@ def verify(parents, tokens, target, u_accept, u_next, draft=None, rows=None):
             x = tokens[j]
             has = float(r[x]) if 0 <= x < r.numel() else 0.0
             qx = (float(q[x]) if 0 <= x < r.numel() else 1.0) if q is not None else 1.0
-            if u_accept[j] * qx * W < has:
+            if has > 0 and u_accept[j] * qx * W < has:
                 down = j
                 break
             if q is None:
