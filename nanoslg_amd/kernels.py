@@ -258,6 +258,7 @@ class Workspace:
 
         self.prefill_buf: Optional[torch.Tensor] = None
         self.verify_buf: Optional[torch.Tensor] = None
+        self._verify_kept: list = []
 
     def get(self, nbytes: int) -> torch.Tensor:
         if self.buf.numel() < nbytes:
@@ -272,8 +273,12 @@ class Workspace:
         return self.prefill_buf
 
     def get_verify(self, nbytes: int) -> torch.Tensor:
-        """Scratch of verify_tree calls: memory of its own, since they expect the zeros that they leave."""
+        """Scratch of verify_tree calls: memory of its own, since they expect the zeros that they leave. What a larger call
+        replaces is kept, for graphs that hold its address."""
         if self.verify_buf is None or self.verify_buf.numel() < nbytes:
+            if torch.cuda.is_current_stream_capturing():  # (the zeros would be written by replays only)
+                raise RuntimeError("verify_tree: use the workspace in a call of this size before it is captured")
+            self._verify_kept.append(self.verify_buf)
             self.verify_buf = torch.zeros(int(nbytes * 1.25) + 256, dtype=torch.uint8, device=self.device)
         return self.verify_buf
 

@@ -435,6 +435,42 @@ def test_verify_odd_rows(drawn):
         _verify(trees, tokens, p, q if drawn else None, torch.rand(len(rows), generator=g), torch.rand(4, generator=g), rows)
 
 
+def test_tokens_without_weight_are_rejected_whatever_their_number():
+    """Numbers outside [0, 1) (1 from a rounding, say) accept nothing that the target cannot give."""
+    p = torch.zeros(6, 5)
+    p[:, 0], p[:, 1] = 0.75, 0.25
+    for q in (None, torch.full((6, 5), 0.2)):
+        for u in (-1.0, 0.0, 1.0, 2.0, float("nan")):
+            path, count, token = _verify([[-1, 0, 0, 0, 0, 0]], [0, 2, 9, -1, 0, 1], p, q, torch.tensor([0.0] + [u] * 5), torch.tensor([0.5]))
+            assert path[0][:count[0]] in ([0], [0, 4], [0, 5]) and token[0] in (0, 1)
+
+
+def test_a_workspace_is_not_made_in_a_capture():
+    """Its zeros would be written by replays only."""
+    from nanoslg_amd import kernels
+    V, ws = 40000, kernels.Workspace(torch.device(DEV))
+    args = (_i32([0, 1]), _i32([-1, 0]), _i32([0, 2]), 2, 2, torch.full((2, V), 1 / V, device=DEV), torch.zeros(2, device=DEV), torch.zeros(1, device=DEV))
+    kernels.verify_tree(*args)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="before"):
+            kernels.verify_tree(*args, workspace=ws)
+        args[5].add_(0)
+    want = kernels.verify_tree(*args)
+    assert all(torch.equal(a, b) for a, b in zip(want, kernels.verify_tree(*args, workspace=ws)))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = kernels.verify_tree(*args, workspace=ws)
+    used = ws.verify_buf.data_ptr()
+    ws.get_verify(2 * ws.verify_buf.numel())  # the graph's memory stays its own
+    other = torch.zeros(ws.verify_buf.numel() // 4, device=DEV)
+    assert used not in (ws.verify_buf.data_ptr(), other.data_ptr())
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, held)) and not other.any()
+
+
 def test_verify_with_one_workspace_for_other_batches():
     """A workspace that a call left is another batch's: its counters are where the sums were not."""
     from nanoslg_amd import kernels
