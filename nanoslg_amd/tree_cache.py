@@ -73,7 +73,7 @@ class TreeCacheContext(CacheContext):
         start = np.asarray(self.start_positions, np.int32)
         if self._host_parents is None:
             (self._start,) = _upload_i32([start], device)
-            self._parents = parents.reshape(-1)
+            self._parents = parents.reshape(-1).clone()  # (the caller may write the next trees there)
         else:
             self._start, self._parents = _upload_i32([start, self._host_parents.astype(np.int32)], device)
         self._mask, pos = kern.tree_plan(self._parents, self._plan.qo_indptr, self._start, self._total, self._max_q,
@@ -82,6 +82,8 @@ class TreeCacheContext(CacheContext):
 
     def _rows(self, S: int):
         """The kernels' row arguments for [B, S] grids."""
+        if not self._open:
+            raise ValueError("the context's forward has ended")
         if S < self._max_q:
             raise ValueError(f"the input grid has {S} columns; this forward's trees need {self._max_q}")
         return {} if self._uniform and S == self._max_q else {"q_rows": self._plan.rows_for(S), "grid_width": S}

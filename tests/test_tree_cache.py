@@ -403,6 +403,23 @@ def test_refusals(backend):
 
 
 @pytest.mark.parametrize("backend", ["paged", "contiguous"])
+def test_an_ended_context_attends_nothing(backend):
+    cache, model = make(backend, "cpu", CPU), Model("cpu")
+    ids, _ = prefill(cache, model, [[1, 2, 3]], "cpu")
+    parents = torch.tensor([[-1, 0, 1]], dtype=torch.int32)
+    ctx = cache.begin_tree(ids, parents)
+    parents.fill_(-1)  # the context has its own
+    probs = torch.zeros(1, 3, V).scatter_(2, torch.tensor([[[5], [6], [7]]]), 1.0)
+    done = cache.accept_tree(ctx, torch.tensor([[4, 5, 6]]), probs, torch.zeros(1, 3), torch.zeros(1))
+    assert done.counts == [3] and done.next_tokens.tolist() == [7]
+    x = torch.zeros(1, 3, HQ, D)
+    for call in (lambda: ctx.attend(0, x, x[:, :, :HKV], x[:, :, :HKV], HQ, HKV),
+                 lambda: ctx.attend_rope(0, x, x[:, :, :HKV], x[:, :, :HKV], model.cos, model.sin, HQ, HKV)):
+        with pytest.raises(ValueError, match="has ended"):
+            call()
+
+
+@pytest.mark.parametrize("backend", ["paged", "contiguous"])
 def test_eight_bit_caches_are_refused(backend):
     cache = make(backend, "cpu", CPU, dtype=torch.float16, cache_dtype=torch.int8)
     cache.allocate_sequence("a")
