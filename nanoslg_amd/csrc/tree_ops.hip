@@ -137,24 +137,45 @@ __device__ inline double weight(float p, float q, double c) {
   return x > 0.0 && x < INFINITY ? x : 0.0;
 }
 
+__device__ inline double f64_of(unsigned lo, unsigned hi) { return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo); }
+__device__ inline unsigned lo_of(double v) { return (unsigned)__builtin_bit_cast(uint64_t, v); }
+__device__ inline unsigned hi_of(double v) { return (unsigned)(__builtin_bit_cast(uint64_t, v) >> 32); }
+template <int kCtrl>
+__device__ inline double dpp_f64(double x) {
+  return f64_of(__builtin_amdgcn_mov_dpp(lo_of(x), kCtrl, 0xf, 0xf, false), __builtin_amdgcn_mov_dpp(hi_of(x), kCtrl, 0xf, 0xf, false));
+}
+// Two sums a step on their way: of x in even rows of 16 lanes and of y in odd ones; of x in the lower half of the wave and
+// of y in the upper.
+__device__ inline double join16_f64(double x, double y) {
+  const auto a = __builtin_amdgcn_permlane16_swap(lo_of(x), lo_of(y), false, false), c = __builtin_amdgcn_permlane16_swap(hi_of(x), hi_of(y), false, false);
+  return f64_of(a[0], c[0]) + f64_of(a[1], c[1]);
+}
+__device__ inline double join32_f64(double x, double y) {
+  const auto a = __builtin_amdgcn_permlane32_swap(lo_of(x), lo_of(y), false, false), c = __builtin_amdgcn_permlane32_swap(hi_of(x), hi_of(y), false, false);
+  return f64_of(a[0], c[0]) + f64_of(a[1], c[1]);
+}
+
 // Sum over the wave's lanes: rotations within 16 lanes, then the row swaps.
 __device__ inline double wave_sum_f64(double x) {
-  auto halves = [](unsigned lo, unsigned hi) { return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo); };
-  auto lo = [](double v) { return (unsigned)__builtin_bit_cast(uint64_t, v); };
-  auto hi = [](double v) { return (unsigned)(__builtin_bit_cast(uint64_t, v) >> 32); };
-#define NSLG_TURN(ctrl) \
-  x += halves(__builtin_amdgcn_mov_dpp(lo(x), ctrl, 0xf, 0xf, false), __builtin_amdgcn_mov_dpp(hi(x), ctrl, 0xf, 0xf, false))
-  NSLG_TURN(0x128);  // row_ror:8
-  NSLG_TURN(0x124);  // row_ror:4
-  NSLG_TURN(0x122);  // row_ror:2
-  NSLG_TURN(0x121);  // row_ror:1
-#undef NSLG_TURN
-  {
-    const auto a = __builtin_amdgcn_permlane16_swap(lo(x), lo(x), false, false), c = __builtin_amdgcn_permlane16_swap(hi(x), hi(x), false, false);
-    x = halves(a[0], c[0]) + halves(a[1], c[1]);
-  }
-  const auto a = __builtin_amdgcn_permlane32_swap(lo(x), lo(x), false, false), c = __builtin_amdgcn_permlane32_swap(hi(x), hi(x), false, false);
-  return halves(a[0], c[0]) + halves(a[1], c[1]);
+  x += dpp_f64<0x128>(x);  // row_ror:8
+  x += dpp_f64<0x124>(x);  // row_ror:4
+  x += dpp_f64<0x122>(x);  // row_ror:2
+  x += dpp_f64<0x121>(x);  // row_ror:1
+  x = join16_f64(x, x);
+  return join32_f64(x, x);
+}
+
+// Eight sums over the wave's lanes, each step joining two of them (10 additions where eight sums by themselves take 48): the lanes
+// of each eight have the sum of x[sum8_of(lane)].
+__device__ inline int sum8_of(int lane) { return (lane >> 1 & 4) | (lane >> 3 & 2) | (lane >> 5 & 1); }
+__device__ inline double wave_sum8_f64(const double (&x)[8]) {
+  const double a = join16_f64(join32_f64(x[0], x[1]), join32_f64(x[2], x[3]));
+  const double b = join16_f64(join32_f64(x[4], x[5]), join32_f64(x[6], x[7]));
+  const bool upper = threadIdx.x & 8;
+  double s = (upper ? b : a) + dpp_f64<0x128>(upper ? a : b);  // row_ror:8
+  s += dpp_f64<0xb1>(s);                                       // quad_perm 1 0 3 2
+  s += dpp_f64<0x4e>(s);                                       // quad_perm 2 3 0 1
+  return s + dpp_f64<0x141>(s);                                // row_half_mirror
 }
 __device__ inline double wave_scan_f64(double x) {  // sum over the lanes up to one's own
   const int lane = threadIdx.x & 63;
@@ -297,13 +318,10 @@ __global__ void __launch_bounds__(kVerThreads) tree_verify_kernel(VerifyParams p
           x[k] += v;
         }
       }
-#pragma unroll
-      for (int k = 0; k < kVerBatch; ++k) x[k] = wave_sum_f64(x[k]);
-      if (lane == 0) {
-#pragma unroll
-        for (int k = 0; k < kVerBatch; ++k)
-          if (g + k < g1) piece[g + k] = x[k];
-      }
+      static_assert(kVerBatch == 8);
+      const double sum = wave_sum8_f64(x);
+      const int k = sum8_of(lane);
+      if (lane % 8 == 0 && g + k < g1) piece[g + k] = sum;
     }
   };
   const int pieces = (p.vocab + kVerPiece - 1) / kVerPiece;
