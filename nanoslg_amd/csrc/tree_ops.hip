@@ -70,8 +70,8 @@ __global__ void __launch_bounds__(256) tree_plan_kernel(TreePlanParams p) {
 // on alone: in most trees it only has the next token to find. Sums and tests are in 64 bits: the order of adding
 // decides no token.
 //
-// One tree of 26 nodes over 128k fp32 tokens 9.9 us, 64 drawn chains of 4 to 8 over them 26.6 (66 MB: 13 at a copy's
-// rate), 16 drawn trees of 32 over 32k bf16 tokens 32: what the last workgroup rejects one after the other.
+// One tree of 26 nodes over 128k fp32 tokens 9.6 us, 64 drawn chains of 4 to 8 over them 18.6 (66 MB: 13 at a copy's
+// rate), 16 drawn trees of 32 over 32k bf16 tokens 29.5: what the last workgroup rejects one after the other.
 struct VerifyParams {
   const int32_t* tokens;
   const int32_t* parents;
@@ -518,14 +518,15 @@ extern "C" int nslg_tree_plan(const int32_t* parents, const int32_t* qo_indptr, 
   return check_launch("tree_plan");
 }
 
-// Workgroups a sequence: of 16 pieces (4096 tokens) each at least, about two a CU in all.
+// Workgroups a sequence: of 16 pieces (4096 tokens) each at least, and as many as the CUs take at once, one each (twice as
+// many: 64 chains over 128k tokens 25.5 us, now 18.6).
 static int verify_slices(int32_t batch, int32_t vocab) {
   const int by_row = (vocab + 16 * kVerPiece - 1) / (16 * kVerPiece);
-  const int by_cus = 512 / batch;
+  const int by_cus = 256 / batch;
   const int n = by_row < by_cus ? by_row : by_cus;
   return n < 1 ? 1 : n;
 }
-// The counters (slices > 1: at most 256 sequences) before the sums, at an offset that does not depend on the call: a
+// The counters (slices > 1: at most 128 sequences) before the sums, at an offset that does not depend on the call: a
 // later one of another batch finds its counters zero.
 constexpr int kVerHead = 1024;
 static size_t verify_bytes(int32_t batch, int32_t vocab) {
