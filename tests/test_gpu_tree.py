@@ -166,6 +166,25 @@ def test_attention(name, fused):
         assert not out[pads].any()
 
 
+@pytest.mark.parametrize("dtype,Hq,Hkv,D,B,most,nodes", [
+    (torch.float16, 16, 8, 128, 70, 900, 20), (torch.bfloat16, 16, 8, 128, 130, 500, 9), (torch.float16, 32, 8, 128, 12, 2500, 90),
+    (torch.bfloat16, 8, 4, 256, 9, 1500, 150), (torch.float32, 16, 8, 128, 67, 400, 9), (torch.float16, 32, 32, 64, 66, 1200, 8),
+    (torch.float16, 16, 4, 64, 3, 6000, 700)])
+def test_long_spans(dtype, Hq, Hkv, D, B, most, nodes):
+    """Spans of many blocks over several sequences and row tiles, that end where a row tile begins, in its first blocks and in its
+    last; batches of more sequences than a wave has lanes."""
+    rng = random.Random(B)
+    ctx = [rng.choice([0, rng.randint(0, 60), rng.randint(0, most), most]) for _ in range(B)]
+    trees = [random_tree(rng, rng.choice([0, 1, rng.randint(1, nodes), nodes])) for _ in range(B)]
+    s = Setup(B, ctx, trees, dtype, Hq, Hkv, D)
+    k, v = s.written()
+    out = s.run()
+    s.check(out, k, v)
+    assert torch.equal(s.k, k) and torch.equal(s.v, v)
+    for pages in (1, 400):  # longer spans
+        s.check(s.run(False, total_pages=pages), k, v)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 def test_masks_of_any_form(dtype):
     """Rows that see nothing at all, later nodes, not themselves; masks wider than needed."""
