@@ -19,7 +19,7 @@
 //   S^T[key x row] = K Q^T      (MFMA; lane (r, gq) then holds keys 16 t + 4 gq + j of row r: V's operand layout,
 //                                so that probabilities never leave their registers)
 //   online softmax in fp32, the running maximum raised lazily
-//   O^T[d x row] += V^T P^T     (MFMA; 16-bit V^T operands by transposing LDS reads; bf16's P in two terms)
+//   O^T[d x row] += V^T P^T     (MFMA; 16-bit V^T operands by transposing LDS reads; P in two terms)
 //
 // What bounds it (a call among others; 32/8 heads, D = 128 but in the fourth):
 //   32 trees of 32 over 2k-16k, fp16      259 us: the keys' way from HBM into LDS, 1.13 GB at 4.65 TB/s in the kernel (a 2 GiB
@@ -51,6 +51,8 @@ constexpr int kTreeBlockBytes = 16384;  // K, or V, of a block of keys
 constexpr int kTreeSlots = 4;           // blocks in LDS: 128 KB, one workgroup a CU
 constexpr int kTreeTurn = 3;            // blocks' time that a workgroup takes to begin a row tile
 constexpr float kTreeSlack = 8.0f;  // how far (log2) scores may rise above the running maximum that P is taken at
+constexpr float kTreeHalfUp = 7.0f;  // log2 of what half's P are taken times: with the slack 2^15 at most, and half a step of half's smallest
+                                     // numbers is 2^-32 of a row's largest weight (2^-25 without; 128k weak keys beside a strong one then lost 4e-3)
 
 // Division of 0 .. 2^31 - 1 by a number that the host knows: with 2^l >= d, m = floor(2^(31 + l) / d) + 1 exceeds
 // 2^(31 + l) / d by at most 2^l / d of what a quotient's floor allows.
@@ -269,7 +271,7 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
   constexpr int kVecs = kRowBytes / 16;                     // 16-byte pieces of a row
   constexpr int kPer = kBlockBytes / (16 * kThreads);       // pieces of K (and of V) a thread and block
   constexpr int kSteps = kGroupKeys / kStep;                // steps of a group's keys of a block
-  constexpr bool kSplitP = T::kDtype == NSLG_BF16;
+  constexpr float kUp = T::kDtype == NSLG_F16 ? kTreeHalfUp : 0.f;
 
   __shared__ __attribute__((aligned(1024))) char kv_lds[2 * kSlots * kBlockBytes];
   __shared__ float2 ml_lds[kGroups == 2 ? kRows : 1];
@@ -492,7 +494,8 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
 #pragma unroll 1
     for (int i = 0; i < min(n_blk, kSlots - 1); ++i) issue(i);
 
-    float thr = -INFINITY, neg_m = 0.f;  // the raw score above which the maximum is raised; -maximum (log2 units; 0: none yet)
+    // the raw score above which the maximum is raised; kUp - maximum (log2 units; 0: none yet), the exponents' offset
+    float thr = -INFINITY, neg_m = 0.f;
     f32x4 lsum = {0.f, 0.f, 0.f, 0.f}, o[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -593,12 +596,12 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
       for (int j = 0; j < 4 * kSub; ++j) top = fmaxf(top, s[j >> 2][j & 3]);
       if (__ballot(top > thr)) {
         const float m_run = thr == -INFINITY ? -INFINITY : -neg_m;
-        const float m_new = fmaxf(m_run, rows_max(top * p.scale_log2));
+        const float m_new = fmaxf(m_run, rows_max(top * p.scale_log2) - kUp);
         const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
         lsum *= alpha;
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[n] *= alpha;
-        thr = (m_new + kTreeSlack) * inv_scale;
+        thr = (m_new + (kUp + kTreeSlack)) * inv_scale;
         neg_m = m_new == -INFINITY ? 0.f : -m_new;
       }
       u16x8 pb, pb_lo;
@@ -609,12 +612,28 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
         // (the rows' sums take the probabilities before they are rounded, a lane's keys at a time; as a product with a row of ones
         // they cost a matrix instruction in 13 to 17: 250 us with 32 trees over 2k-16k tokens, now 243)
         lsum[j & 3] += x;
-        if constexpr (!kF32) {
-          // half keeps 11 bits of a probability; bfloat16's 8 are too few for the 2e-3 of the 16-bit caches'
-          // attention: the rest goes in as a second term
+        // a probability goes into the product in two terms: 16 bits of bfloat16, 22 of half (one term, of 11, was seen in the outputs:
+        // 1.4 times the error of probabilities in fp32)
+        if constexpr (T::kDtype == NSLG_BF16) {
           pb[j] = T::from_f32(x);
-          if constexpr (kSplitP) pb_lo[j] = T::from_f32(x - T::to_f32(pb[j]));
+          pb_lo[j] = T::from_f32(x - T::to_f32(pb[j]));
         }
+      }
+      if constexpr (T::kDtype == NSLG_F16) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        u32x4 ph, pl;
+        float minus_one = -1.f;  // (known to the compiler, it would make three instructions of a rest)
+        asm("" : "+s"(minus_one));
+#pragma unroll
+        for (int j = 0; j < 4 * kSub; j += 2) {  // (an instruction for two first terms, one for each rest: a mixed fma)
+          const float x = s[j >> 2][j & 3], y = s[j >> 2][(j & 3) + 1];
+          uint32_t pair = __builtin_bit_cast(uint32_t, f16x2{(_Float16)x, (_Float16)y});
+          asm("" : "+v"(pair));  // (the rests take them from here, not from conversions of their own)
+          const f16x2 hi = __builtin_bit_cast(f16x2, pair);
+          ph[j >> 1] = pair;
+          pl[j >> 1] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)fmaf((float)hi[0], minus_one, x), (_Float16)fmaf((float)hi[1], minus_one, y)});
+        }
+        pb = __builtin_bit_cast(u16x8, ph), pb_lo = __builtin_bit_cast(u16x8, pl);
       }
       // O^T += V^T P^T
       if constexpr (kF32) {
@@ -632,7 +651,7 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           o[n] = T::mma_k32(va[n], pb, o[n]);
-          if constexpr (kSplitP) o[n] = T::mma_k32(va[n], pb_lo, o[n]);
+          o[n] = T::mma_k32(va[n], pb_lo, o[n]);
         }
       }
       // nodes whose V is not finite: those elements, for the rows that see the node
