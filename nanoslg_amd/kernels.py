@@ -257,6 +257,8 @@ class Workspace:
         self.buf = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=self.device)
 
         self.prefill_buf: Optional[torch.Tensor] = None
+        self._prefill_in_graph = False  # a capture was given prefill_buf
+        self._prefill_kept: list = []
         self.verify_buf: Optional[torch.Tensor] = None
         self._verify_kept: list = []
 
@@ -265,12 +267,25 @@ class Workspace:
             self.buf = torch.zeros(int(nbytes * 1.25) + 256, dtype=torch.uint8, device=self.device)
         return self.buf
 
+    def _capturing(self) -> bool:
+        return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
     def get_prefill(self, nbytes: int) -> torch.Tensor:
         """Scratch of prefill calls: memory of its own, since a chunk layout that a decode
-        call recorded in get()'s is read again after the calls in between."""
-        if self.prefill_buf is None or self.prefill_buf.numel() < nbytes:
-            self.prefill_buf = torch.empty(int(nbytes * 1.25) + 256, dtype=torch.uint8, device=self.device)
-        return self.prefill_buf
+        call recorded in get()'s is read again after the calls in between. What a larger call replaces is kept
+        where a graph holds its address; else it is free once the present stream, which the call before
+        it is over for, comes to this place."""
+        buf, capturing = self.prefill_buf, self._capturing()
+        if buf is None or buf.numel() < nbytes:
+            if buf is not None and (capturing or self._prefill_in_graph):
+                self._prefill_kept.append(buf)
+            elif buf is not None and buf.is_cuda:
+                buf.record_stream(torch.cuda.current_stream(buf.device))
+            self._prefill_in_graph = False
+            buf = self.prefill_buf = torch.empty(int(nbytes * 1.25) + 256, dtype=torch.uint8, device=self.device)
+        if capturing:
+            self._prefill_in_graph = True
+        return buf
 
     def get_verify(self, nbytes: int) -> torch.Tensor:
         """Scratch of verify_tree calls: memory of its own, since they expect the zeros that they leave. What a larger call
