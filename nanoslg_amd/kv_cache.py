@@ -249,6 +249,16 @@ class KVCacheManager(ABC):
 
     # speculative decoding with trees of drafted tokens (tree_cache)
 
+    _open_trees: Dict[str, list]  # sequence -> [True], shared with the context of the tree forward that is its last one begun
+
+    def _drop_trees(self, seq_ids) -> None:
+        """Other forwards of these sequences were begun, or the sequences were released: the contexts of trees that are
+        still open for them are dropped."""
+        for s in seq_ids:
+            live = self._open_trees.pop(s, None)
+            if live:
+                live[0] = False
+
     def begin_tree(self, seq_ids: List[str], parents):
         """A forward over a tree of drafted tokens for each sequence (a tree_cache.TreeCacheContext). parents: for each
         sequence its nodes' parents (node 0 the root: -1; each other one's lies before it), or an int32 tensor [B, nodes] on
@@ -1402,6 +1412,7 @@ class PagedKVCache(KVCacheManager):
         self.tree = (RadixTree(cfg.page_size, self.pool, share_partial=cfg.share_partial_pages)
                      if cfg.enable_prefix_caching else None)
         self.seqs: Dict[str, _PagedSeqState] = {}
+        self._open_trees = {}
         self.workspace = self.kernels.Workspace(self.pool.device, 128 << 20)
         self._pending_zero: List[int] = []
         self._dev_plan = None  # the last decode forward's plan: (ids, plan, lens), see below
@@ -1801,6 +1812,7 @@ class PagedKVCache(KVCacheManager):
         old = self.seqs.get(seq_id)
         if old is not None:  # a re-used id: its old table's device row is free again
             self._tables.release(old)
+            self._drop_trees([seq_id])
         self.seqs[seq_id] = st
         return plen
 
@@ -1814,6 +1826,8 @@ class PagedKVCache(KVCacheManager):
         if offsets is None and self._dev_plan is not None:
             ctx = self._begin_steady_decode(seq_ids, ntoks)
             if ctx is not None:
+                if self._open_trees:
+                    self._drop_trees(seq_ids)
                 return ctx
         ps = self.cfg.page_size
         if any(n != 1 for n in ntoks):
@@ -1839,13 +1853,16 @@ class PagedKVCache(KVCacheManager):
                 st.extend(self._alloc(k, defer_zero=True))
         zero, self._pending_zero = self._pending_zero, []
         try:
-            return PagedCacheContext(self, seq_ids, ntoks, offsets, zero_pages=zero)
+            ctx = PagedCacheContext(self, seq_ids, ntoks, offsets, zero_pages=zero)
         except RuntimeError:
             # the pages this call took stay with their sequences and are zeroed, as
             # allocation zeroes them (kv_cache.py:411), whatever stopped the forward
             if zero:
                 self.pool.zero(zero)
             raise
+        if self._open_trees:
+            self._drop_trees(seq_ids)
+        return ctx
 
     def end_forward(self, ctx):
         _check_forward(ctx)
@@ -1901,6 +1918,7 @@ class PagedKVCache(KVCacheManager):
                 self.tree.dec_refs(st.token_ids[:st.prefix_len])
         self.pool.release_many(st.bt[:st.n_pages])
         self._tables.release(st)
+        self._drop_trees([seq_id])
         del self.seqs[seq_id]
 
     def append_token_ids(self, seq_id, ids):
@@ -2111,6 +2129,7 @@ class ContiguousKVCache(KVCacheManager):
         self.device = torch.device(cfg.device) if cfg.device is not None else torch.device("cpu")
         self.pools = _Pools(cfg, cfg.max_batch_size, cfg.max_seq_len, self.device)  # a slot is a page of max_seq_len
         self.states: Dict[str, _ContigSeqState] = {}
+        self._open_trees = {}
         self._slot = 0
         self.workspace = self.kernels.Workspace(self.device, 16 << 20)
         self._launcher = None  # the last decode forward's kernels.DecodeLaunch: the next one's is made from it
@@ -2143,6 +2162,7 @@ class ContiguousKVCache(KVCacheManager):
         st = _ContigSeqState(seq_id, s)
         if token_ids:
             st.token_ids = list(token_ids)
+        self._drop_trees([seq_id])
         self.states[seq_id] = st
         return 0
 
@@ -2153,7 +2173,10 @@ class ContiguousKVCache(KVCacheManager):
     def begin_forward(self, seq_ids, ntoks, offsets=None):
         for sid, n in zip(seq_ids, ntoks):
             self.extend_sequence(sid, n)
-        return ContiguousCacheContext(self, seq_ids, ntoks, offsets)
+        ctx = ContiguousCacheContext(self, seq_ids, ntoks, offsets)
+        if self._open_trees:
+            self._drop_trees(seq_ids)
+        return ctx
 
     def end_forward(self, ctx):
         _check_forward(ctx)
@@ -2177,6 +2200,7 @@ class ContiguousKVCache(KVCacheManager):
 
     def release_sequence(self, seq_id):
         if seq_id in self.states:
+            self._drop_trees([seq_id])
             del self.states[seq_id]
             if not self.states:
                 self._slot = 0

@@ -11,7 +11,8 @@ parents[j] < j is node j's parent; a node's children are tried in the order of t
 behind the sequence's tokens; each node sees those tokens, its ancestors and itself, and has the position of a token behind its
 ancestors. accept_tree verifies the drafted tokens (``kernels.verify_tree``), moves the accepted nodes' K/V together in
 every layer and advances the sequences by them; the token that follows them is the next step's root. end_tree ends a
-forward with paths that the caller has found. A context that is dropped leaves its sequences as they were.
+forward with paths that the caller has found. A context that is dropped leaves its sequences as they were; it is dropped by
+the next forward of any of its sequences (begin_forward, begin_tree) and by a sequence's release, if not before.
 """
 from __future__ import annotations
 
@@ -69,7 +70,7 @@ class TreeCacheContext(CacheContext):
         self.max_kv_len = ctx.max_kv_len
         self._plan, self._max_q, self._total = ctx._plan, max(counts), sum(counts)
         self._uniform = min(counts) == self._max_q
-        self._open = True
+        self._open, self._live = True, [True]  # not ended; not dropped (kv_cache._drop_trees)
         start = np.asarray(self.start_positions, np.int32)
         if self._host_parents is None:
             (self._start,) = _upload_i32([start], device)
@@ -79,11 +80,12 @@ class TreeCacheContext(CacheContext):
         self._mask, pos = kern.tree_plan(self._parents, self._plan.qo_indptr, self._start, self._total, self._max_q,
                                          **self._rows(self._max_q))
         self._pos = {self._max_q: pos}  # by grid width
+        cache._open_trees.update(dict.fromkeys(seq_ids, self._live))
 
     def _rows(self, S: int):
         """The kernels' row arguments for [B, S] grids."""
-        if not self._open:
-            raise ValueError("the context's forward has ended")
+        if not self._open or not self._live[0]:
+            raise ValueError("the context's forward has ended" if not self._open else "the context's sequences have changed since begin_tree")
         if S < self._max_q:
             raise ValueError(f"the input grid has {S} columns; this forward's trees need {self._max_q}")
         return {} if self._uniform and S == self._max_q else {"q_rows": self._plan.rows_for(S), "grid_width": S}
@@ -154,8 +156,9 @@ class TreeResult:
 def _check_open(cache, ctx, what: str) -> None:
     if not isinstance(ctx, TreeCacheContext) or ctx.cache is not cache or not ctx._open:
         raise ValueError(f"{what}: needs an open context of this cache's begin_tree")
+    # (a forward begun since writes the same slots; a sequence released has given its pages away, whoever has its id)
     for sid, start in zip(ctx.seq_ids, ctx.start_positions):
-        if sid not in cache._states or cache._states[sid].num_tokens != start:
+        if not ctx._live[0] or cache._states[sid].num_tokens != start:
             raise ValueError(f"{what}: sequence {sid!r} has changed since begin_tree")
 
 
@@ -212,4 +215,5 @@ def _move(cache, ctx: TreeCacheContext, path: torch.Tensor, count: torch.Tensor)
 def _advance(cache, ctx: TreeCacheContext, counts: List[int]) -> None:
     for sid, c, n in zip(ctx.seq_ids, counts, ctx.new_token_counts):
         cache._end_tree(cache._states[sid], c, n)
+        del cache._open_trees[sid]
     ctx._open = False
