@@ -50,6 +50,12 @@ def _trees(what: str, qo_indptr: torch.Tensor, total_q: int, max_q: int, q_rows:
     return B, total_q, max_q
 
 
+def _rows_ptr(q_rows: Optional[torch.Tensor], total_q: int, qo_indptr: torch.Tensor) -> Optional[int]:
+    """q_rows as the entry points take it: null is no grid, so a grid without nodes, whose q_rows may be empty and is not read,
+    goes by another address."""
+    return None if q_rows is None else q_rows.data_ptr() if total_q else qo_indptr.data_ptr()
+
+
 def tree_plan(parents: torch.Tensor, qo_indptr: torch.Tensor, start: torch.Tensor, total_q: int, max_q: int,
               q_rows: Optional[torch.Tensor] = None, grid_width: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
     """Ancestor masks and positions of a batch of trees (nslg_tree_plan).
@@ -67,7 +73,7 @@ def tree_plan(parents: torch.Tensor, qo_indptr: torch.Tensor, start: torch.Tenso
     buf = torch.empty(total_q * W + n_pos, dtype=torch.int32, device=parents.device)
     at = buf.data_ptr()
     rc = _call(dev, _lib.fast_tree().tree_plan, parents.data_ptr(), qo_indptr.data_ptr(), start.data_ptr(),
-               None if q_rows is None else q_rows.data_ptr(), int(grid_width), total_q, max_q, B, at, W,
+               _rows_ptr(q_rows, total_q, qo_indptr), int(grid_width), total_q, max_q, B, at, W,
                at + 4 * total_q * W, _stream(parents))
     if rc:
         _lib.check(rc, "nslg_tree_plan")
@@ -149,7 +155,7 @@ def paged_tree_attention(q: torch.Tensor, mask: torch.Tensor, qo_indptr: torch.T
     if need:
         ws = workspace.get_prefill(need) if workspace is not None else torch.empty(need, dtype=torch.uint8, device=q.device)
     rc = _call(dev, _lib.fast_tree().paged_tree_attention, q.data_ptr(), q_stride, mask.data_ptr(), mask.shape[1],
-               qo_indptr.data_ptr(), None if q_rows is None else q_rows.data_ptr(), int(grid_width), total_q, max_q, *new,
+               qo_indptr.data_ptr(), _rows_ptr(q_rows, total_q, qo_indptr), int(grid_width), total_q, max_q, *new,
                k_layer.data_ptr(), v_layer.data_ptr(), P, ps, kv_indptr.data_ptr(), kv_indices.data_ptr(),
                kv_last_page_len.data_ptr(), int(total_pages), B, Hq, Hkv, D,
                1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), code, out.data_ptr(), out_stride,
