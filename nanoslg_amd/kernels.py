@@ -256,6 +256,7 @@ class Workspace:
         self.device = torch.device(device)
         self.buf = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=self.device)
 
+        self._index = self.buf.get_device()  # -1: not on a GPU
         self.prefill_buf: Optional[torch.Tensor] = None
         self._prefill_in_graph = False  # a capture was given prefill_buf
         self._prefill_kept: list = []
@@ -268,7 +269,9 @@ class Workspace:
         return self.buf
 
     def _capturing(self) -> bool:
-        return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+        # (the default stream, which no capture takes, is told by its address: 0.1 us where the question itself takes 0.3)
+        return self._index >= 0 and _stream(self.buf) != 0 and (
+            torch.cuda.current_device() != self._index or torch.cuda.is_current_stream_capturing())
 
     def get_prefill(self, nbytes: int) -> torch.Tensor:
         """Scratch of prefill calls: memory of its own, since a chunk layout that a decode
