@@ -33,8 +33,9 @@
 //   4 chains of 5-9 over 700-3k, fp32      27 us: the same, and products at a ninth of bf16's rate
 //
 // A key that a row does not see counts nothing, whatever it holds: its score is replaced, and since a
-// probability of 0 would not keep a value that is not finite out of a matrix product, such values of the nodes are
-// set to 0 in LDS and added row by row to those that see them.
+// probability of 0 would not keep a value that is not finite out of a matrix product, such values of the blocks with nodes are
+// set to 0 in LDS and added row by row to those that see them. In the blocks before, which every row sees, they go through the
+// product, and come out as they went in because no probability there has a term that is 0 or below.
 #include "nslg_common.h"
 
 #include <math.h>
@@ -605,6 +606,10 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
         neg_m = m_new == -INFINITY ? 0.f : -m_new;
       }
       u16x8 pb, pb_lo;
+      typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+      float minus_one = -1.f;  // (known to the compiler, it would make three instructions of a half's rest)
+      asm("" : "+s"(minus_one));
 #pragma unroll
       for (int j = 0; j < 4 * kSub; ++j) {
         const float x = fast_exp2(fmaf(s[j >> 2][j & 3], p.scale_log2, neg_m));
@@ -612,28 +617,36 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
         // (the rows' sums take the probabilities before they are rounded, a lane's keys at a time; as a product with a row of ones
         // they cost a matrix instruction in 13 to 17: 250 us with 32 trees over 2k-16k tokens, now 243)
         lsum[j & 3] += x;
-        // a probability goes into the product in two terms: 16 bits of bfloat16, 22 of half (one term, of 11, was seen in the outputs:
-        // 1.4 times the error of probabilities in fp32)
-        if constexpr (T::kDtype == NSLG_BF16) {
-          pb[j] = T::from_f32(x);
-          pb_lo[j] = T::from_f32(x - T::to_f32(pb[j]));
-        }
       }
-      if constexpr (T::kDtype == NSLG_F16) {
-        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-        u32x4 ph, pl;
-        float minus_one = -1.f;  // (known to the compiler, it would make three instructions of a rest)
-        asm("" : "+s"(minus_one));
+      // A probability goes into the product in two terms: 16 bits of bfloat16, 21 of half (one term, of 11, was seen in the outputs:
+      // 1.4 times the error of probabilities in fp32). The first is cut off, so that neither is negative, and
+      // over blocks that every row sees no term of a probability above 0 is 0: what is infinite in V stays that.
+      if constexpr (!kF32) {
+        u32x4 hi, lo;
 #pragma unroll
-        for (int j = 0; j < 4 * kSub; j += 2) {  // (an instruction for two first terms, one for each rest: a mixed fma)
+        for (int j = 0; j < 4 * kSub; j += 2) {
           const float x = s[j >> 2][j & 3], y = s[j >> 2][(j & 3) + 1];
-          uint32_t pair = __builtin_bit_cast(uint32_t, f16x2{(_Float16)x, (_Float16)y});
-          asm("" : "+v"(pair));  // (the rests take them from here, not from conversions of their own)
-          const f16x2 hi = __builtin_bit_cast(f16x2, pair);
-          ph[j >> 1] = pair;
-          pl[j >> 1] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)fmaf((float)hi[0], minus_one, x), (_Float16)fmaf((float)hi[1], minus_one, y)});
+          if constexpr (T::kDtype == NSLG_BF16) {
+            const uint32_t xh = __float_as_uint(x) & 0xffff0000u, yh = __float_as_uint(y) & 0xffff0000u;
+            hi[j >> 1] = xh >> 16 | yh;
+            // (2^-23 of the probability more than the rest)
+            lo[j >> 1] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)fmaf(x, 0x1.000002p+0f, -__uint_as_float(xh)),
+                                                             (__bf16)fmaf(y, 0x1.000002p+0f, -__uint_as_float(yh))});
+          } else {
+            // (half's smallest number, 2^-31 of the row's largest weight, or more)
+            constexpr _Float16 kLeast = kTail ? (_Float16)0.f : (_Float16)0x1p-24f;
+            const f16x2 least = {kLeast, kLeast};
+            uint32_t pair = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+            if constexpr (!kTail) pair = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(f16x2, pair), least));
+            asm("" : "+v"(pair));  // (the rests take them from here, not from conversions of their own)
+            const f16x2 h = __builtin_bit_cast(f16x2, pair);
+            f16x2 rest = {(_Float16)fmaf((float)h[0], minus_one, x), (_Float16)fmaf((float)h[1], minus_one, y)};
+            if constexpr (!kTail) rest = __builtin_elementwise_max(rest, least);
+            hi[j >> 1] = pair;
+            lo[j >> 1] = __builtin_bit_cast(uint32_t, rest);
+          }
         }
-        pb = __builtin_bit_cast(u16x8, ph), pb_lo = __builtin_bit_cast(u16x8, pl);
+        pb = __builtin_bit_cast(u16x8, hi), pb_lo = __builtin_bit_cast(u16x8, lo);
       }
       // O^T += V^T P^T
       if constexpr (kF32) {
@@ -661,7 +674,7 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
           const int kk = __ffs(bad) - 1;
           bad &= bad - 1;
           const int key = kbase + kk;
-          const char* vrow = (fresh ? p.v_new + new_at(key) * p.v_new_stride
+          const char* vrow = (fresh && key >= start ? p.v_new + new_at(key) * p.v_new_stride
                                     : p.v_pool + ((int64_t)checked(idx[page_of(key)]) * ps + (key - page_of(key) * ps)) * row_bytes) +
                              head_off;
           float pr = 0.f;
@@ -695,7 +708,7 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
         u32x4* at = reinterpret_cast<u32x4*>(vs + 1024 * (wave + kWaves * i) + 16 * ln);
         if (kabs >= kv_end) {
           *at = u32x4{0, 0, 0, 0};
-        } else if (kabs >= start) {
+        } else {
           bool bad = false;
           const u32x4 x = drop_not_finite<T>(*at, bad);
           if (bad) {

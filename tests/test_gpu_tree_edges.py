@@ -1,10 +1,11 @@
 """Calls for trees of drafted tokens at the edges of what the wrappers take."""
+import math
 import random
 
 import pytest
 import torch
 
-from test_gpu_tree import DEV, Setup, _i32, chain, random_tree
+from test_gpu_tree import DEV, U, Setup, _i32, chain, random_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +36,74 @@ def test_grids_without_nodes_are_zeroed(empty, max_q):
     path, count, token = kernels.verify_tree(none, none, zeros, 0, max_q, torch.rand(B * S, 9, device=DEV), torch.zeros(0, device=DEV),
                                              torch.rand(B, device=DEV), q_rows=q_rows)
     assert path.shape == (B, max_q) and (path == -1).all() and not count.any() and (token == -1).all()
+
+
+@pytest.mark.parametrize("workspace", [True, False])
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("dtype,D,nodes,ps", [(torch.float16, 128, 20, 16), (torch.bfloat16, 128, 20, 16), (torch.bfloat16, 64, 60, 1),
+                                              (torch.float16, 256, 9, 16), (torch.float32, 128, 20, 16), (torch.bfloat16, 128, 90, 16)])
+def test_infinite_values_of_cached_tokens(dtype, D, nodes, ps, fused, workspace):
+    """Every row sees the tokens before its tree: an infinite element of their values makes the output's element that
+    infinity (both signs, or NaN: NaN), at a token of a weight of 1, of ordinary and of small weights, and the others stay exact."""
+    from test_gpu_tree_exact import _whole
+    trees = [random_tree(random.Random(1), nodes), chain(3), random_tree(random.Random(2), nodes)]
+    s = Setup(5, [700, 0, 1301], trees, dtype, 8, 2, D, ps)
+    # sequence 2's token 9 outweighs all others of KV head 0: its weight is 1 to the last bit
+    at = s.slots(2)
+    s.k.view(-1, 2, D)[at[9], 0] = 0
+    s.k.view(-1, 2, D)[at[9], 0, 0] = 240
+    s.q[s.n[0] + 3:, :4, 0] = 8
+    k, v = s.written()
+    want = _formula(s, k, v)
+    inf = float("inf")
+    marks = [(2, 9, 0, 5, inf), (2, 9, 1, 6, -inf), (2, 1290, 1, 7, inf), (0, 0, 0, 8, inf), (0, 699, 0, 8, inf), (0, 350, 1, 9, -inf),
+             (0, 351, 1, 10, inf), (0, 13, 1, 10, -inf), (2, 640, 1, 11, float("nan"))]
+    for b, t, h, d, x in marks:
+        for pool in (s.v, v):
+            pool.view(-1, 2, D)[s.slots(b)[t], h, d] = x
+    if not fused:
+        s.k, s.v = k.clone(), v.clone()
+    if workspace:
+        out = s.run(fused)
+    else:
+        s.k_new, s.v_new = (s.k_new, s.v_new) if fused else (None, None)
+        out = _whole(s, D ** -0.5)
+    hit = {(0, 0, 8): inf, (0, 1, 9): -inf, (0, 1, 10): None, (2, 0, 5): inf, (2, 1, 6): -inf, (2, 1, 7): inf, (2, 1, 11): None}
+    o = out.clone()
+    for (b, h, d), x in hit.items():
+        rows = slice(s.qo[b], s.qo[b + 1])
+        got = out[rows, 4 * h:4 * h + 4, d]
+        assert (got == x).all() if x else got.isnan().all(), (b, h, d, got)
+        o[rows, 4 * h:4 * h + 4, d] = want[rows, 4 * h:4 * h + 4, d].to(dtype)
+    assert o.isfinite().all()
+    s.n_rows = s.T
+    s.check(o, *s.clean)
+
+
+def _formula(s, k, v):
+    """The outputs in 64 bits over pools k and v, which the setup keeps for check()."""
+    from oracle import tree_oracle as O
+    s.clean = (k.clone(), v.clone())
+    return torch.cat([O.attention(s.q[s.qo[b]:s.qo[b + 1]], k.view(-1, s.Hkv, s.D)[s.slots(b)], v.view(-1, s.Hkv, s.D)[s.slots(b)], s.see[b])[0]
+                      for b in range(s.B)])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bits", [0, 12, 24, 31, 40, 90])
+@pytest.mark.parametrize("ctx", [40, 600])
+def test_infinite_values_of_weak_keys(dtype, bits, ctx):
+    """One cached key 2^bits times as heavy as all others, one of which has an infinite value: the result is infinite there and
+    the heavy key's elsewhere, off by the others' N 2^-bits and what tests/test_gpu_tree_exact.py counts."""
+    s = Setup(2, [ctx], [chain(3)], dtype, 4, 1, 128)
+    s.k.zero_(), s.k_new.zero_(), s.v.zero_(), s.v_new.zero_(), s.q.zero_()
+    at = s.slots(0)
+    s.k.view(-1, 1, 128)[at[3], 0, 0], s.q[:, :, 0] = 1, 1
+    s.v.view(-1, 1, 128)[at[3]] = 1
+    s.v.view(-1, 1, 128)[at[33], 0, 17] = float("inf")
+    out = s.run(sm_scale=max(bits, 1e-6) * math.log(2))
+    assert (out[:, :, 17] == float("inf")).all()
+    rest = torch.cat([out[:, :, :17], out[:, :, 18:]], 2).double()
+    for t in range(3):
+        want = 1 / (1 + (ctx + t) * 2.0 ** -bits)  # (node t sees ctx tokens and t + 1 nodes)
+        tol = U[dtype] * want + 2.0 ** -15 * want + (ctx + 3) * 2.0 ** -24
+        assert ((rest[t] - want).abs() <= tol).all()
