@@ -50,6 +50,7 @@ constexpr int kTreeMaxNodes = 1024;
 constexpr int kTreeWin = 1024;          // pages whose place is in LDS
 constexpr int kTreeBlockBytes = 16384;  // K, or V, of a block of keys
 constexpr int kTreeSlots = 4;           // blocks in LDS: 128 KB, one workgroup a CU
+constexpr int64_t kTreeStream = 256 << 20;  // bytes of K/V, read once, from which on they are loaded past the caches, which they exceed
 constexpr int kTreeTurn = 3;            // blocks' time that a workgroup takes to begin a row tile
 constexpr float kTreeSlack = 8.0f;  // how far (log2) scores may rise above the running maximum that P is taken at
 constexpr float kTreeHalfUp = 7.0f;  // log2 of what half's P are taken times: with the slack 2^15 at most, and half a step of half's smallest
@@ -102,7 +103,7 @@ struct TreeParams {
   int32_t spans;       // workgroups per KV head
   int32_t tile_waves;  // waves of 16 rows of a row tile
   int32_t whole;       // no partials: a workgroup takes a whole row tile
-  int32_t stream;      // the call's K/V exceed the caches and are read once: loaded past them
+  int32_t one_tile;    // trees are one row tile each: K/V are read once
   int32_t num_work;    // workgroups that attend (spans a KV head); the others write the new rows
   uint64_t* ws_tag;    // the workspace's first word: a decode call's record in the same memory is void
   int4* meta;          // per sequence: its first unit of work, its blocks, units a workgroup, units before a row tile's blocks
@@ -319,18 +320,21 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
   auto units_of = [&](const SeqOf& x) { return tiles_of(x) * (p.whole ? 1 : blocks_of(x) + turn); };
   int group0 = 0, before = 0;  // the first of the sequences in seq_lds, the units before it
   int total;
+  bool stream;
   {
     const SeqOf s = tree_seq(p, lane);
     int u = units_of(s), tiles = tiles_of(s);
-    int incl = wave_scan_i32(u), incl_tiles = wave_scan_i32(tiles);
+    int incl = wave_scan_i32(u), incl_tiles = wave_scan_i32(p.whole ? tiles * blocks_of(s) : tiles);
     total = __builtin_amdgcn_readlane(incl, 63);
-    int all_tiles = __builtin_amdgcn_readlane(incl_tiles, 63);
+    int all_tiles = __builtin_amdgcn_readlane(incl_tiles, 63);  // (whole: blocks)
     for (int s0 = 64; s0 < p.batch; s0 += 64) {
       const SeqOf x = tree_seq(p, s0 + lane);
       total += wave_sum_i32(units_of(x));
-      all_tiles += wave_sum_i32(tiles_of(x));
+      all_tiles += wave_sum_i32(p.whole ? tiles_of(x) * blocks_of(x) : tiles_of(x));
     }
     total = __builtin_amdgcn_readfirstlane(total);
+    // (by the lengths: a page may be far larger than what a sequence has of it)
+    stream = p.one_tile && (int64_t)__builtin_amdgcn_readfirstlane(p.whole ? all_tiles : total) * p.num_kv_heads * 2 * kTreeBlockBytes > kTreeStream;
     if (!p.whole && total >= kTreeTurn * p.spans) {  // uniform
       turn = kTreeTurn;
       total += turn * __builtin_amdgcn_readfirstlane(all_tiles);
@@ -460,7 +464,7 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
           kp = p.k_new + at * p.k_new_stride + k_piece;
           vp = p.v_new + at * p.v_new_stride + v_piece;
         }
-        if (p.stream) {  // uniform
+        if (stream) {  // uniform
           load_lds16<true>(kp, ks + 1024 * kWaves * i);
           load_lds16<true>(vp, vs + 1024 * kWaves * i);
         } else {
@@ -1080,7 +1084,7 @@ extern "C" int nslg_paged_tree_attention(const void* q, int64_t q_stride, const 
   p.spans = (int32_t)spans;
   const int64_t work = total_q > 0 ? spans * num_kv_heads : 0;
   p.num_work = (int32_t)work;
-  p.stream = tree_tiles(rows, head_dim, dtype) == 1 && total_pages * page_size * num_kv_heads * head_dim * 2 * eb > ((int64_t)256 << 20);
+  p.one_tile = tree_tiles(rows, head_dim, dtype) == 1;
   hipStream_t s = as_stream(stream);
   if (dtype == NSLG_F16) return launch_tree_dim<F16>(p, head_dim, s);
   if (dtype == NSLG_BF16) return launch_tree_dim<BF16>(p, head_dim, s);

@@ -107,3 +107,17 @@ def test_infinite_values_of_weak_keys(dtype, bits, ctx):
         want = 1 / (1 + (ctx + t) * 2.0 ** -bits)  # (node t sees ctx tokens and t + 1 nodes)
         tol = U[dtype] * want + 2.0 ** -15 * want + (ctx + 3) * 2.0 ** -24
         assert ((rest[t] - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("workspace", [True, False])
+@pytest.mark.parametrize("ctx,ps", [(4000, 16), (4000, 5000), (4400, 5000)])
+def test_keys_on_both_sides_of_what_the_caches_hold(ctx, ps, workspace):
+    """16 sequences of 4000 tokens are 246 MiB of K and V, of 4400 271, on both sides of 256: the longer ones' are loaded past the caches, by their lengths
+    and not by the pages that they have."""
+    from test_gpu_tree_exact import _whole
+    s = Setup(ctx, [ctx - 9 * b for b in range(16)], [random_tree(random.Random(b), 8) for b in range(16)], torch.float16, 8, 8, 128, ps)
+    s.k, s.v = s.written()
+    if not workspace:
+        s.k_new = s.v_new = None
+    out = s.run(False) if workspace else _whole(s, 128 ** -0.5)
+    s.check(out, s.k, s.v)
