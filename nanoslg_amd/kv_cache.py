@@ -259,6 +259,10 @@ class KVCacheManager(ABC):
             if live:
                 live[0] = False
 
+    def _begin_nodes(self, seq_ids, counts):
+        """begin_forward of trees of so many nodes."""
+        return self.begin_forward(seq_ids, counts)
+
     def begin_tree(self, seq_ids: List[str], parents):
         """A forward over a tree of drafted tokens for each sequence (a tree_cache.TreeCacheContext). parents: for each
         sequence its nodes' parents (node 0 the root: -1; each other one's lies before it), or an int32 tensor [B, nodes] on
@@ -1881,6 +1885,11 @@ class PagedKVCache(KVCacheManager):
     @property
     def _states(self):
         return self.seqs
+
+    def _begin_nodes(self, seq_ids, counts):
+        # (a steady decode step's plan lies in a ring of buffers that later steps write; a tree's is its context's own)
+        self._dev_plan = None
+        return self.begin_forward(seq_ids, counts)
 
     def _end_tree(self, st, accepted, nodes):
         """End a forward of `nodes` tokens behind st's with the first `accepted` of them. The pages stay with the

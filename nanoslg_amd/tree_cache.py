@@ -22,7 +22,7 @@ from typing import List, Optional, Sequence, Union
 import numpy as np
 import torch
 
-from .kv_cache import CacheContext, _upload_i32
+from .kv_cache import CacheContext, _current_stream, _upload_i32
 
 Trees = Union[Sequence[Sequence[int]], torch.Tensor]
 
@@ -38,10 +38,15 @@ def _host_trees(parents: Sequence[Sequence[int]]):
     return counts, flat
 
 
+def _raw_stream(device: torch.device) -> int:
+    """The current stream's handle."""
+    return torch._C._cuda_getCurrentRawStream(device.index) if device.type == "cuda" else 0
+
+
 class TreeCacheContext(CacheContext):
     """The context of a forward over trees (a manager's begin_tree). Tensors are [B, S, ...] grids, S at least the largest
     tree's nodes, tree b's nodes the first columns of row b; outputs of the other columns are zero. A forward may run
-    on any stream that waits for the one begin_tree ran on."""
+    on any stream that waits for the one begin_tree ran on; the context may be dropped while it runs there."""
 
     is_tree = True
 
@@ -63,7 +68,7 @@ class TreeCacheContext(CacheContext):
         if len(counts) != len(seq_ids) or min(counts) < 1 or max(counts) > kern.MAX_TREE_NODES:
             raise ValueError(f"begin_tree: a tree of 1 to {kern.MAX_TREE_NODES} nodes for each of {len(seq_ids)} sequences")
 
-        ctx = cache.begin_forward(seq_ids, counts)  # pages, copy-on-write, block table
+        ctx = cache._begin_nodes(seq_ids, counts)  # pages, copy-on-write, block table
         self.cache = cache
         self.seq_ids, self.new_token_counts, self.input_offsets = ctx.seq_ids, counts, [0] * len(counts)
         self.batch_size, self.seq_lens, self.start_positions = ctx.batch_size, ctx.seq_lens, ctx.start_positions
@@ -80,6 +85,7 @@ class TreeCacheContext(CacheContext):
         self._mask, pos = kern.tree_plan(self._parents, self._plan.qo_indptr, self._start, self._total, self._max_q,
                                          **self._rows(self._max_q))
         self._pos = {self._max_q: pos}  # by grid width
+        self._device, self._stream, self._used_on = device, _raw_stream(device), set()
         cache._open_trees.update(dict.fromkeys(seq_ids, self._live))
 
     def _rows(self, S: int):
@@ -120,13 +126,30 @@ class TreeCacheContext(CacheContext):
         if last >= limit:
             raise IndexError(f"position {last} is outside the rope tables ({limit} rows)")
 
+    def _hold(self, S: int) -> None:
+        """The memory of what an attend of this width reads is given back behind the current stream's work too, where that is not
+        the stream which it was made on."""
+        raw = _raw_stream(self._device)
+        if (raw == self._stream and not self._used_on) or (raw, S) in self._used_on:
+            return
+        self._used_on.add((raw, S))
+        stream, plan = _current_stream(self._device.index), vars(self._plan)
+        own = [self._mask, self._start, self._parents, *self._pos.values()]
+        for x in (*plan.values(), *(t for d in plan.values() if isinstance(d, dict) for t in d.values())):
+            if isinstance(x, torch.Tensor) and x.device == self._device:
+                own.append(x)
+        for t in own:
+            t.record_stream(stream)
+
     def _attend(self, q, k_layer, v_layer, **new):
         plan = self._plan
         B, S, Hq, D = q.shape
+        rows = self._rows(S)
+        self._hold(S)
         # (scratch from the allocator: forwards of one cache may run on several streams)
         out = self.cache.kernels.paged_tree_attention(q.reshape(B * S, Hq, D), self._mask, plan.qo_indptr, self._total, self._max_q,
                                                       k_layer, v_layer, plan.indptr, plan.indices, plan.lpl, plan.total_pages,
-                                                      **self._rows(S), **new)
+                                                      **rows, **new)
         return out.view(B, S, Hq * D)
 
     def attend(self, layer_idx, q, k_new, v_new, n_heads, n_kv_heads):
@@ -140,7 +163,9 @@ class TreeCacheContext(CacheContext):
         S = q.shape[1]
         self._rows(S)  # (refuses a grid that is too narrow)
         k_layer, v_layer = self.cache._kv_layer(layer_idx)
-        q = self.cache.kernels.rope_append(q, k_new, v_new, self._pos_for(S), self._plan.slots_for(S), cos, sin, k_layer, v_layer)
+        pos, slots = self._pos_for(S), self._plan.slots_for(S)
+        self._hold(S)
+        q = self.cache.kernels.rope_append(q, k_new, v_new, pos, slots, cos, sin, k_layer, v_layer)
         return self._attend(q, k_layer, v_layer)
 
 

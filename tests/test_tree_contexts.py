@@ -97,3 +97,84 @@ def test_forwards_that_do_not_begin_leave_a_tree_open(backend):
     with pytest.raises(ValueError):
         cache.begin_tree(ids[:1], [[-1, 5]])
     assert cache.end_tree(ctx, _i32([[0, 1, 2], [0, -1, -1]]), _i32([3, 1])) == [3, 1]
+
+
+@BACKENDS
+@pytest.mark.parametrize("rope", [True, False])
+def test_a_forward_on_another_stream_holds_what_it_reads(backend, rope, monkeypatch):
+    """Every tensor of the context that a kernel is given on another stream than begin_tree's is recorded there, once for each
+    stream and width; on begin_tree's own nothing is."""
+    from types import SimpleNamespace
+
+    from nanoslg_amd import tree_cache
+    given, held, now = [], [], [7]
+    calls = SimpleNamespace(**vars(CPU))
+    for name in ("paged_tree_attention", "rope_append"):
+        def call(*a, _f=getattr(CPU, name), **kw):
+            given.extend(t.data_ptr() for t in (*a, *kw.values()) if isinstance(t, torch.Tensor) and t.dtype == torch.int32)
+            return _f(*a, **kw)
+        setattr(calls, name, call)
+    monkeypatch.setattr(tree_cache, "_raw_stream", lambda device: now[0])
+    monkeypatch.setattr(tree_cache, "_current_stream", lambda index: now[0])
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, stream: held.append((t.data_ptr(), stream)))
+    cache, model = make(backend, "cpu", calls), Model("cpu")
+    ids, _ = prefill(cache, model, [[1, 2, 3], [4, 5]], "cpu")
+    ctx = cache.begin_tree(ids, [[-1, 0, 0], [-1]])
+    held.clear()
+
+    def forward(S):
+        given.clear()
+        model(torch.zeros(2, S, dtype=torch.long), ctx, rope)
+
+    forward(3)
+    assert not held
+    for now[0], S in ((8, 3), (8, 5), (9, 5), (7, 6), (8, 6)):
+        before = len(held)
+        forward(S)
+        assert given and {(p, now[0]) for p in given} <= set(held) and len(held) > before
+        before = len(held)
+        forward(S)
+        assert len(held) == before
+
+
+def test_trees_of_roots_have_a_plan_of_their_own():
+    """Later decode steps, of any sequences, do not write the plan of an open tree."""
+    cache, model = make("paged", "cpu", CPU), Model("cpu")
+    ids, _ = prefill(cache, model, [[1, 2, 3], [4, 5]], "cpu")
+    for _ in range(2):
+        step = cache.begin_forward(ids, [1, 1])
+        _write(cache, step, 1, 4.0)
+        cache.end_forward(step)
+    assert cache._dev_plan is not None
+    seen = []
+    begin = cache._begin_steady_decode
+    cache._begin_steady_decode = lambda *a: seen.append(a) or begin(*a)
+    ctx = cache.begin_tree(ids, [[-1], [-1]])
+    assert not seen
+    assert cache.end_tree(ctx, _i32([[0], [0]]), _i32([1, 1])) == [1, 1]
+
+
+@pytest.mark.gpu
+@BACKENDS
+def test_a_context_dropped_while_its_forward_runs_elsewhere(backend):
+    """What is allocated meanwhile does not take the memory that the waiting kernels will read."""
+    from nanoslg_amd import kernels
+    dev = "cuda:0"
+    g = torch.Generator(device=dev).manual_seed(0)
+    cache, model = make(backend, dev, kernels), Model(dev)
+    ids, _ = prefill(cache, model, [[1, 2, 3] * 9, [4, 5]], dev)
+    trees = [[-1, 0, 0, 1, 3, 3], [-1, 0]]
+    q, k, v = (torch.randn(2, 6, h, D, generator=g, device=dev) for h in (HQ, HKV, HKV))
+    ctx = cache.begin_tree(ids, trees)
+    want = ctx.attend(0, q, k, v, HQ, HKV).clone()
+    side = torch.cuda.Stream()
+    for _ in range(2):
+        ctx = cache.begin_tree(ids, trees)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)
+            got = ctx.attend(0, q, k, v, HQ, HKV)
+        del ctx
+        taken = [torch.zeros(n, dtype=torch.int32, device=dev) for n in (1, 60, 120, 500, 1000, 5000) for _ in range(20)]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and not any(t.any() for t in taken)
