@@ -121,3 +121,17 @@ def test_keys_on_both_sides_of_what_the_caches_hold(ctx, ps, workspace):
         s.k_new = s.v_new = None
     out = s.run(False) if workspace else _whole(s, 128 ** -0.5)
     s.check(out, s.k, s.v)
+
+
+@pytest.mark.parametrize("dtype,D,ps,ctx", [(torch.float16, 128, 1, 3000), (torch.bfloat16, 64, 1, 5200), (torch.float32, 128, 1, 2100),
+                                            (torch.float16, 256, 2, 4500), (torch.bfloat16, 128, 3, 7001)])
+@pytest.mark.parametrize("pages", [None, 1])  # no scratch: all keys by one workgroup; spans for a page: nearly so
+def test_more_pages_than_a_window(dtype, D, ps, ctx, pages):
+    """More than 1024 pages of a sequence in one workgroup's keys: their places are loaded anew on the way, in the plain blocks and
+    in those of the tree."""
+    from test_gpu_tree_exact import _whole
+    s = Setup(ctx, [ctx, 1023 * ps, 1024 * ps + 5], [random_tree(random.Random(n), n) for n in (33, 4, 70)], dtype, 4, 1, D, ps)
+    k, v = s.written()
+    out = _whole(s, D ** -0.5) if pages is None else s.run(total_pages=pages)
+    s.check(out, k, v)
+    assert torch.equal(s.k, k) and torch.equal(s.v, v)
