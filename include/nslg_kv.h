@@ -739,7 +739,9 @@ int nslg_paged_tree_attention(const void* q, int64_t q_stride, const uint32_t* m
  *   draft_probs given (children drawn, independently, from the node's draft row q):
  *       accepted if u_accept[j] q(x) W < r(x); once rejected, r becomes max(r / W - q, 0) and W its sum.
  * The accepted child is the next node. Where none is, the next token is drawn from r: the first one at which the
- * running sum of r exceeds u_next[b] times its sum. Tokens so accepted and drawn have the target's distribution.
+ * running sum of r exceeds u_next[b] times its sum. Rows are to sum to 1, up to their type's roundings, one filtered (top-k,
+ * top-p) once it is normalised again: tokens so accepted and drawn then have the target's distribution. A row of another sum is taken
+ * as it is: with p = (1/4, 1/4) a given token is accepted with 1/4, not 1/2.
  * Tests and sums are in 64 bits. Negative weights and those that are not finite count as 0; where nothing is left
  * of r the token is drawn from p, and next_token is -1 where p holds nothing either (or the sequence has no nodes).
  * A drafted token without weight, or outside the vocabulary, is rejected whatever its number. Probabilities of exactly one token (p(x) = 1) make

@@ -178,7 +178,8 @@ def verify_tree(tokens: torch.Tensor, parents: torch.Tensor, qo_indptr: torch.Te
     or q_rows[t]; u_accept float32 [total_q], u_next float32 [B]. draft_probs, like target_probs: a node's row is the
     distribution that its children were drawn from, independently; without it the drafted tokens are taken as given.
     Returns (path, count, next): int32 [B, max_q] accepted nodes, the root first, -1 behind them; their number
-    [B]; the token that follows [B]. Accepted and next tokens have the target's distribution. Rows with the
+    [B]; the token that follows [B]. Accepted and next tokens have the target's distribution where rows sum to 1 (a row
+    filtered by top-k or top-p is normalised again first; nothing here does it). Rows with the
     probability of one token 1 make this greedy verification. `workspace`: with it, kept from call to call and used by one call
     at a time, several workgroups take a sequence."""
     dev = _one_device(tokens, parents, qo_indptr, target_probs, u_accept, u_next)

@@ -273,7 +273,7 @@ class KVCacheManager(ABC):
     def accept_tree(self, ctx, tokens, target_probs, u_accept, u_next, draft_probs=None):
         """Verify a tree forward's drafted tokens and end it with the accepted nodes. tokens and u_accept [B, S] on the
         forward's grid (numbers in [0, 1); the roots' are not read), target_probs and draft_probs [B, S, vocabulary] (kernels.
-        verify_tree), u_next [B]. Returns a tree_cache.TreeResult; waits for the GPU."""
+        verify_tree: rows that sum to 1), u_next [B]. Returns a tree_cache.TreeResult; waits for the GPU."""
         from . import tree_cache
         return tree_cache.accept_tree(self, ctx, tokens, target_probs, u_accept, u_next, draft_probs)
 
