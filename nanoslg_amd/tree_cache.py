@@ -188,12 +188,12 @@ def _check_open(cache, ctx, what: str) -> None:
 
 
 def _nodes(ctx: TreeCacheContext, t: torch.Tensor, name: str) -> torch.Tensor:
-    """A [B, S] grid's entries of the nodes, ragged."""
+    """A [B, S] grid's entries of the nodes, ragged and one behind the other (a column of a wider tensor is neither)."""
     B = ctx.batch_size
     if t.dim() != 2 or t.shape[0] != B or t.shape[1] < ctx._max_q:
         raise ValueError(f"accept_tree: {name} must be [{B}, S], S at least {ctx._max_q}")
     rows = ctx._rows(t.shape[1])
-    return t.reshape(-1)[rows["q_rows"][:ctx._total].long()] if rows else t.reshape(-1)
+    return t.reshape(-1)[rows["q_rows"][:ctx._total].long()] if rows else t.reshape(-1).contiguous()
 
 
 def accept_tree(cache, ctx: TreeCacheContext, tokens: torch.Tensor, target_probs: torch.Tensor, u_accept: torch.Tensor,
@@ -208,7 +208,7 @@ def accept_tree(cache, ctx: TreeCacheContext, tokens: torch.Tensor, target_probs
     S, V = target_probs.shape[1:]
     path, count, token = cache.kernels.verify_tree(
         _nodes(ctx, tokens, "tokens").to(torch.int32), ctx._parents, ctx._plan.qo_indptr, ctx._total, ctx._max_q,
-        target_probs.reshape(B * S, V), _nodes(ctx, u_accept, "u_accept"), u_next.reshape(-1),
+        target_probs.reshape(B * S, V), _nodes(ctx, u_accept, "u_accept"), u_next.reshape(-1).contiguous(),
         draft_probs=None if draft_probs is None else draft_probs.reshape(B * S, V), q_rows=ctx._rows(S).get("q_rows"),
         workspace=cache.workspace)
     _move(cache, ctx, path, count)

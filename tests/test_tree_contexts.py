@@ -178,3 +178,33 @@ def test_a_context_dropped_while_its_forward_runs_elsewhere(backend):
         taken = [torch.zeros(n, dtype=torch.int32, device=dev) for n in (1, 60, 120, 500, 1000, 5000) for _ in range(20)]
         torch.cuda.synchronize()
         assert torch.equal(got, want) and not any(t.any() for t in taken)
+
+
+@BACKENDS
+@pytest.mark.parametrize("nodes", [1, 3])
+def test_numbers_and_tokens_as_parts_of_wider_tensors(backend, nodes):
+    """A column of one tensor of uniform numbers, tokens of a longer buffer: the call takes them as their values."""
+    from types import SimpleNamespace
+    V, B = 60, 2
+    calls, strided = SimpleNamespace(**vars(CPU)), []
+
+    def verify(tokens, parents, qo, total, max_q, probs, u_accept, u_next, **kw):
+        strided.extend(not t.is_contiguous() for t in (tokens, parents, u_accept, u_next))
+        return CPU.verify_tree(tokens, parents, qo, total, max_q, probs, u_accept, u_next, **kw)
+
+    calls.verify_tree = verify
+    done = []
+    for parts in (False, True):
+        cache, model = make(backend, "cpu", calls), Model("cpu")
+        ids, _ = prefill(cache, model, [[1, 2, 3], [4, 5]], "cpu")
+        g = torch.Generator().manual_seed(1)
+        u = torch.rand(B, 2 * nodes + 2, generator=g)
+        tokens = torch.randint(0, 3, (B, 2 * nodes), generator=g, dtype=torch.int32)
+        probs = torch.zeros(B, nodes, V)
+        probs[:, :, :3] = 1 / 3
+        ctx = cache.begin_tree(ids, [[-1] + [0] * (nodes - 1)] * B)
+        args = (tokens[:, ::2], u[:, :2 * nodes:2], u[:, -1])
+        tok, ua, un = args if parts else (a.clone(memory_format=torch.contiguous_format) for a in args)
+        done.append(cache.accept_tree(ctx, tok, probs, ua, un))
+    assert not any(strided)
+    assert torch.equal(done[0].path, done[1].path) and torch.equal(done[0].next_tokens, done[1].next_tokens)
