@@ -451,7 +451,8 @@ __global__ void __launch_bounds__(256) tree_move_kernel(MoveParams p) {
   const int b = blockIdx.y, tid = threadIdx.x;
   const int layer = blockIdx.x >> 1;
   const int n = max(p.qo_indptr[b + 1] - p.qo_indptr[b], 0);
-  const int count = min(p.count[b], min(n, p.path_stride));
+  const int count = p.count[b];
+  if (count > min(n, p.path_stride)) return;
   const int32_t* path = p.path + (int64_t)b * p.path_stride;
   // a path: rising nodes of the tree
   bool ok = true;

@@ -135,3 +135,18 @@ def test_more_pages_than_a_window(dtype, D, ps, ctx, pages):
     out = _whole(s, D ** -0.5) if pages is None else s.run(total_pages=pages)
     s.check(out, k, v)
     assert torch.equal(s.k, k) and torch.equal(s.v, v)
+
+
+def test_counts_past_a_tree_or_a_path_move_nothing():
+    """The first count entries of such a path are not rising nodes of the tree: the sequence is left as it is."""
+    from nanoslg_amd import kernels
+    s = Setup(7, [10, 20, 30, 5], [chain(3), chain(6), chain(6), chain(4)], torch.float16, 2, 2, 64, 16, layers=2)
+    k, v = s.k.clone(), s.v.clone()
+    path = _i32([[1, 2, -1, -1], [1, 3, 4, 5], [1, 3, 4, 5], [-1] * 4])
+    kernels.move_accepted(s.k, s.v, path, _i32([4, 5, 3, -2]), s.qo, s.indptr, s.indices, s.last)
+    at = s.slots(2)[30:].tolist()
+    for pool in (k, v):
+        flat = pool.view(2, -1, 2, 64)
+        for i, node in enumerate((1, 3, 4)):
+            flat[:, at[i]] = flat[:, at[node]].clone()
+    assert torch.equal(s.k, k) and torch.equal(s.v, v)
