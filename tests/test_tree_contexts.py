@@ -208,3 +208,26 @@ def test_numbers_and_tokens_as_parts_of_wider_tensors(backend, nodes):
         done.append(cache.accept_tree(ctx, tok, probs, ua, un))
     assert not any(strided)
     assert torch.equal(done[0].path, done[1].path) and torch.equal(done[0].next_tokens, done[1].next_tokens)
+
+
+@BACKENDS
+@pytest.mark.parametrize("uniform,wide", [(True, 0), (True, 2), (False, 0), (False, 3)])
+def test_what_the_attention_call_is_told(backend, uniform, wide):
+    """The pages of the call's block table, always; with q_rows the rows of a grid, without them the ragged rows alone."""
+    from types import SimpleNamespace
+    calls, seen = SimpleNamespace(**vars(CPU)), []
+
+    def attention(q, mask, qo, total, max_q, k, v, indptr, indices, lpl, pages, **kw):
+        seen.append(kw.get("q_rows") is not None)
+        assert pages == int(indptr[-1]) == indices[:pages].numel() and total == int(qo[-1])
+        rows = (len(qo) - 1) * kw["grid_width"] if seen[-1] else total
+        assert q.shape[0] == rows and (kw.get("k_new") is None or kw["k_new"].shape[:-2].numel() == rows)
+        return CPU.paged_tree_attention(q, mask, qo, total, max_q, k, v, indptr, indices, lpl, pages, **kw)
+
+    calls.paged_tree_attention = attention
+    cache, model = make(backend, "cpu", calls), Model("cpu")
+    ids, _ = prefill(cache, model, [list(range(9)), [4, 5]], "cpu")
+    ctx = cache.begin_tree(ids, [[-1, 0, 0], [-1, 0, 1] if uniform else [-1]])
+    for rope in (True, False):
+        model(torch.zeros(2, 3 + wide, dtype=torch.long), ctx, rope)
+    assert len(seen) == 2 * L and all(s == (wide > 0 or not uniform) for s in seen)
