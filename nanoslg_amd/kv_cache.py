@@ -2487,6 +2487,8 @@ class DecodeGraph:
         ctx = self.ctxs[i]
         ctx.start_positions = start.tolist()
         ctx.seq_lens = (start + 1).tolist()
+        if cache._open_trees:
+            cache._drop_trees(self.seq_ids)
         self.graphs[i].replay()
         self.done[i].record(_current_stream(self.dev_index))
         self.used[i] = True

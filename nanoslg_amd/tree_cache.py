@@ -12,7 +12,7 @@ behind the sequence's tokens; each node sees those tokens, its ancestors and its
 ancestors. accept_tree verifies the drafted tokens (``kernels.verify_tree``), moves the accepted nodes' K/V together in
 every layer and advances the sequences by them; the token that follows them is the next step's root. end_tree ends a
 forward with paths that the caller has found. A context that is dropped leaves its sequences as they were; it is dropped by
-the next forward of any of its sequences (begin_forward, begin_tree) and by a sequence's release, if not before.
+the next forward of any of its sequences (begin_forward, begin_tree, a DecodeGraph's step) and by a sequence's release, if not before.
 """
 from __future__ import annotations
 

@@ -231,3 +231,56 @@ def test_what_the_attention_call_is_told(backend, uniform, wide):
     for rope in (True, False):
         model(torch.zeros(2, 3 + wide, dtype=torch.long), ctx, rope)
     assert len(seen) == 2 * L and all(s == (wide > 0 or not uniform) for s in seen)
+
+
+@pytest.mark.gpu
+def test_a_graph_step_drops_an_open_tree():
+    from nanoslg_amd import kernels
+    from nanoslg_amd import kv_cache as KC
+    dev = "cuda:0"
+    cache, model = make("paged", dev, kernels), Model(dev)
+    ids, _ = prefill(cache, model, [[1, 2, 3], [4, 5]], dev)
+    q, k, v = (torch.zeros(2, 1, h, D, device=dev) for h in (HQ, HKV, HKV))
+    graph = KC.DecodeGraph(cache, ids, lambda ctx: [ctx.attend(i, q, k, v, HQ, HKV) for i in range(L)])
+    ctx = cache.begin_tree(ids[:1], [[-1, 0]])
+    graph.step()
+    torch.cuda.synchronize()
+    x = torch.zeros(1, 2, HQ, D, device=dev)
+    with pytest.raises(ValueError, match="have changed"):
+        ctx.attend(0, x, x[:, :, :HKV], x[:, :, :HKV], HQ, HKV)
+    with pytest.raises(ValueError, match="has changed"):
+        cache.end_tree(ctx, torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev))
+
+
+@pytest.mark.gpu
+@BACKENDS
+def test_a_tree_forward_in_a_graph(backend):
+    """Captured on the capture's own stream, replayed over other rows, the context dropped behind the last replay."""
+    from nanoslg_amd import kernels
+    dev = "cuda:0"
+    g = torch.Generator(device=dev).manual_seed(0)
+    cache, model = make(backend, dev, kernels), Model(dev)
+    ids, _ = prefill(cache, model, [[1, 2, 3] * 9, [4, 5]], dev)
+    ctx = cache.begin_tree(ids, [[-1, 0, 0, 1, 3, 3], [-1, 0]])
+    q, k, v = (torch.randn(2, 6, h, D, generator=g, device=dev) for h in (HQ, HKV, HKV))
+
+    def forward():
+        return [ctx.attend_rope(i, q, k, v, model.cos, model.sin, HQ, HKV) for i in range(L)]
+
+    forward()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = forward()
+    for _ in range(3):
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=g, device=dev))
+        want = [o.clone() for o in forward()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+    counts = cache.end_tree(ctx, _i32([[0, 2, -1], [0, 1, -1]]).to(dev), _i32([2, 2]).to(dev))
+    assert counts == [2, 2]
+    del ctx, graph
+    torch.cuda.synchronize()
