@@ -709,7 +709,7 @@ int nslg_tree_plan(const int32_t* parents, const int32_t* qo_indptr, const int32
 /*
  * Attention of a batch of trees over one layer of a paged cache: node t of sequence b sees the start_b tokens before its
  * tree and the nodes whose bits its mask row has (nslg_tree_plan's, or any other). A row that sees no token is zero.
- * What an unseen token holds (infinities and NaN too) does not reach a row.
+ * What an unseen token holds (infinities and NaN too) does not reach a row; an infinite value of a seen one comes out as it is.
  *   k_new, v_new    null: the nodes' K/V rows are in the pool; else rows of Hkv*D elements at element
  *                   strides, 16-byte aligned, laid out as q's rows: they are written to the nodes' slots and read from
  *                   there, in the same launch. No other sequence of the call may read a page written.

@@ -22,14 +22,16 @@
 //   O^T[d x row] += V^T P^T     (MFMA; 16-bit V^T operands by transposing LDS reads; P in two terms)
 //
 // What bounds it (a call among others; 32/8 heads, D = 128 but in the fourth):
-//   32 trees of 32 over 2k-16k, fp16      259 us: the keys' way from HBM into LDS, 1.13 GB at 4.65 TB/s in the kernel (a 2 GiB
-//                                                 copy: 4.96)
+//   32 trees of 32 over 2k-16k, fp16      302 us: 2.2 us a block of 16 KB and 128 rows: its way from HBM (1.8 at a 2 GiB
+//                                                 copy's 4.96 TB/s), LDS, products and softmax of waves in step with each
+//                                                 other; matrix units busy for 39 %, vector units 63 % (259 us, and 1.4 times
+//                                                 the error, with P in one term)
 //   8 trees of 24-60 over 256-8k, bf16     55 us: products and softmax of the same waves in turn, 2.9 us a block and 256
 //                                                 rows (2.5 at the rate of an 8192^3 product), and about 8 us a row tile (its
 //                                                 pages, rows, first block, partial). Over the call the vector units are
 //                                                 busy for 50 %, the matrix units 29 %, LDS 20 %, without conflicts
 //   4 trees of 128 over 1k-6k, D = 256     62 us: the same, 1.5 us a block and 128 rows (1.3); 4 row tiles a tree read its keys
-//   1 tree of 16 over 2k, fp16             17 us: a chain of dependent reads (lengths, pages, keys, partials) and two launches
+//   1 tree of 16 over 2k, fp16             18 us: a chain of dependent reads (lengths, pages, keys, partials) and two launches
 //   4 chains of 5-9 over 700-3k, fp32      27 us: the same, and products at a ninth of bf16's rate
 //
 // A key that a row does not see counts nothing, whatever it holds: its score is replaced, and since a
@@ -53,8 +55,8 @@ constexpr int kTreeSlots = 4;           // blocks in LDS: 128 KB, one workgroup 
 constexpr int64_t kTreeStream = 256 << 20;  // bytes of K/V, read once, from which on they are loaded past the caches, which they exceed
 constexpr int kTreeTurn = 3;            // blocks' time that a workgroup takes to begin a row tile
 constexpr float kTreeSlack = 8.0f;  // how far (log2) scores may rise above the running maximum that P is taken at
-constexpr float kTreeHalfUp = 7.0f;  // log2 of what half's P are taken times: with the slack 2^15 at most, and half a step of half's smallest
-                                     // numbers is 2^-32 of a row's largest weight (2^-25 without; 128k weak keys beside a strong one then lost 4e-3)
+constexpr float kTreeHalfUp = 7.0f;  // log2 of what half's P are taken times: with the slack 2^15 at most; half's smallest number is then 2^-31
+                                     // of a row's largest weight (2^-24 without: 131072 weak keys beside a strong one lost 2e-3)
 
 // Division of 0 .. 2^31 - 1 by a number that the host knows: with 2^l >= d, m = floor(2^(31 + l) / d) + 1 exceeds
 // 2^(31 + l) / d by at most 2^l / d of what a quotient's floor allows.
@@ -586,7 +588,7 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
         __builtin_amdgcn_sched_barrier(0);
       }
       // A later block's loads go out here: at the block's start the waves waited to get rid of theirs, all at once, before any
-      // product (265 us with 32 trees of 32 nodes over 2k-16k tokens, 308 from there).
+      // product (265 us with 32 trees of 32 nodes over 2k-16k tokens and P in one term, 308 from there).
       if (u == 0 && blk + kSlots - 1 < n_blk) issue(blk + kSlots - 1);
       __builtin_amdgcn_sched_barrier(0);
       uint32_t vis = 0;
@@ -619,7 +621,7 @@ __global__ void __launch_bounds__((TreeTile<T, D, kRW>::kThreads), (TreeTile<T, 
         const float x = fast_exp2(fmaf(s[j >> 2][j & 3], p.scale_log2, neg_m));
         s[j >> 2][j & 3] = x;
         // (the rows' sums take the probabilities before they are rounded, a lane's keys at a time; as a product with a row of ones
-        // they cost a matrix instruction in 13 to 17: 250 us with 32 trees over 2k-16k tokens, now 243)
+        // they cost a matrix instruction in 13 to 17: 250 us with 32 trees over 2k-16k tokens and P in one term, then 243)
         lsum[j & 3] += x;
       }
       // A probability goes into the product in two terms: 16 bits of bfloat16, 21 of half (one term, of 11, was seen in the outputs:
